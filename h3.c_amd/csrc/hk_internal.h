@@ -29,7 +29,16 @@ struct h3_gpu_tensor {
      * output_dim, problems) it was built and validated for; all zero for
      * every other tensor */
     uint32_t group_shape[4];
+    /* host-side record of an adapter table or an attention plan: what kind
+     * it is (0 for every other tensor) and what it was made for */
+    struct hk_record {
+        uint32_t kind;
+        uint32_t n[15];
+    } record;
 };
+
+/* kinds of records */
+enum { HK_RECORD_LORA = 1, HK_RECORD_PACKED = 2 };
 
 struct hk_cache_block;
 struct hk_timing;

@@ -146,6 +146,15 @@ def lib():
                                                  _U32, _U32, _F]),
         "h3_hip_linear_group_bf16": (_I, [_P, _P, _U32, _U32, _P, _U32, _U32,
                                           _U32]),
+        "h3_hip_lora_table": (_P, [_P, _P, _P, _P, _P, _U32, _U32, _U32]),
+        "h3_hip_linear_lora_bf16": (_I, [_P, _P, _P, _P, _P, _P, _P, _U32,
+                                         _U32, _U32]),
+        "h3_hip_linear_lora_gelu_bf16": (_I, [_P, _P, _P, _P, _P, _P, _P,
+                                              _U32, _U32, _U32]),
+        "h3_hip_sdpa_packed_plan": (_P, [_P, _P, _P, _P, _P, _U32, _U32,
+                                         _U32, _U32]),
+        "h3_hip_sdpa_packed_bf16": (_I, [_P, _P, _P, _SZ, _U32, _P, _SZ, _P,
+                                         _SZ, _U32, _P, _F]),
         "h3_gpu_layer_adaln_bf16": (_I, [_P, _P, _P, _P, _P, _P, _P, _U32,
                                          _U32, _U32, _U32, _U32, _F]),
         "h3_gpu_gate_layer_adaln_bf16": (_I, [_P, _P, _P, _P, _P, _P, _P,
@@ -412,6 +421,28 @@ class Gpu:
     def new_f32(self, n):
         t = self.L.h3_gpu_tensor_new_f32(self.h, n)
         self.check(t, "f32 alloc")
+        self._owned.append(t)
+        return t
+
+    def lora_table(self, down, up, ranks, scales, input_dim, output_dim):
+        """h3_hip_lora_table of lists of handles, ranks and scales."""
+        n = len(ranks)
+        t = self.L.h3_hip_lora_table(
+            self.h, (_P * n)(*down), (_P * n)(*up), (_U32 * n)(*ranks),
+            (_F * n)(*scales), n, input_dim, output_dim)
+        self.check(t, "adapter table")
+        self._owned.append(t)
+        return t
+
+    def sdpa_packed_plan(self, q_first, q_rows, kv_first, kv_rows, heads,
+                         kv_heads, head_dim):
+        """h3_hip_sdpa_packed_plan of lists of row numbers."""
+        n = len(q_rows)
+        t = self.L.h3_hip_sdpa_packed_plan(
+            self.h, *((_U32 * n)(*v) for v in (q_first, q_rows, kv_first,
+                                               kv_rows)),
+            n, heads, kv_heads, head_dim)
+        self.check(t, "attention plan")
         self._owned.append(t)
         return t
 

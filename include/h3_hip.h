@@ -255,6 +255,84 @@ int h3_gpu_linear_gelu_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
                             const h3_gpu_tensor *bias, uint32_t rows,
                             uint32_t input_dim, uint32_t output_dim);
 
+/* Low-rank adapters of several requests beside one projection:
+ *   y[r] = bf16(x[r] . weight^T + bias + s_a (x[r] . down_a^T) . up_a^T)
+ * with a = adapter_map[r] (U32 [rows], in any order); a row whose entry is
+ * not below the table's count has no adapter.  down_a is [rank_a][input_dim],
+ * up_a [output_dim][rank_a], both bf16; ranks go from 0 (no adapter) to 1024
+ * and may differ.
+ *
+ * h3_hip_lora_table copies the adapters, laid out for the kernels, so the
+ * given tensors may be freed or changed once it returns (change an adapter by
+ * building another table); free the table with h3_gpu_tensor_free.  Adapters
+ * and scales have to be finite: rows of several requests share a matrix
+ * product, where one adapter's infinity would reach the others' rows.  NULL
+ * entries of down and up are allowed at rank 0.
+ *
+ * h3_hip_linear_lora_bf16 runs the projection; input_dim and output_dim have
+ * to be the table's.  Sums are F32 and the result is rounded once: x . down^T
+ * is held as two bf16 halves, 16 significant bits, between the products.
+ * h3_hip_linear_lora_gelu_bf16 applies the GELU of h3_gpu_linear_gelu_bf16 to
+ * the sum, rounded to bf16 first as there.
+ * bias may be NULL; output must be a tensor of its own.  No reference
+ * counterpart: the reference serves one request at a time. */
+h3_gpu_tensor *h3_hip_lora_table(h3_gpu *gpu,
+                                 const h3_gpu_tensor *const *down,
+                                 const h3_gpu_tensor *const *up,
+                                 const uint32_t *ranks, const float *scales,
+                                 uint32_t count, uint32_t input_dim,
+                                 uint32_t output_dim);
+int h3_hip_linear_lora_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
+                            const h3_gpu_tensor *input,
+                            const h3_gpu_tensor *weight,
+                            const h3_gpu_tensor *bias,
+                            const h3_gpu_tensor *table,
+                            const h3_gpu_tensor *adapter_map, uint32_t rows,
+                            uint32_t input_dim, uint32_t output_dim);
+int h3_hip_linear_lora_gelu_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
+                                 const h3_gpu_tensor *input,
+                                 const h3_gpu_tensor *weight,
+                                 const h3_gpu_tensor *bias,
+                                 const h3_gpu_tensor *table,
+                                 const h3_gpu_tensor *adapter_map,
+                                 uint32_t rows, uint32_t input_dim,
+                                 uint32_t output_dim);
+
+/* Attention of several requests packed in one call: the query rows
+ * [q_first[i], + q_rows[i]) of request i attend to the key rows
+ * [kv_first[i], + kv_rows[i]), each range counted in rows of the query and of
+ * the key and value tensors.  Query head h reads key head
+ * h / (heads / kv_heads).  Self-attention has the same ranges on both sides;
+ * cross-attention reads each request's own text, or one text that requests
+ * share.  Query ranges must not overlap, key ranges may.  A request without
+ * key rows gets zeros; output rows of no request are left as they were.
+ *
+ * h3_hip_sdpa_packed_plan validates the ranges and lays the work out once for
+ * a set of requests (free it with h3_gpu_tensor_free); the call takes any
+ * tensors that hold the plan's rows.  heads has to be a multiple of kv_heads
+ * and head_dim 1 to 256; multiples of 8 up to 128, with offsets and strides
+ * in multiples of 8, run on the matrix cores.
+ *
+ * Head h of query row r starts at element query_offset + r query_stride +
+ * h head_dim of `query` (likewise key and value, with kv_stride), so Q, K and
+ * V may lie in the fused rows of one projection.  The output is
+ * [row][heads][head_dim], a tensor of its own.  Numerics as in
+ * h3_gpu_sdpa_bf16: F32 online softmax, P rounded to bf16 before P.V.  The
+ * scale has to be finite and not negative.  No reference counterpart: the
+ * reference serves one request at a time. */
+h3_gpu_tensor *h3_hip_sdpa_packed_plan(h3_gpu *gpu, const uint32_t *q_first,
+                                       const uint32_t *q_rows,
+                                       const uint32_t *kv_first,
+                                       const uint32_t *kv_rows,
+                                       uint32_t requests, uint32_t heads,
+                                       uint32_t kv_heads, uint32_t head_dim);
+int h3_hip_sdpa_packed_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
+                            const h3_gpu_tensor *query, size_t query_offset,
+                            uint32_t query_stride, const h3_gpu_tensor *key,
+                            size_t key_offset, const h3_gpu_tensor *value,
+                            size_t value_offset, uint32_t kv_stride,
+                            const h3_gpu_tensor *plan, float scale);
+
 /* h3_gpu_patch_linear_bf16_offset / _map (h3_gpu.h:116-135) without the
  * reference's fixed checkpoint shape (5376 outputs from 32 or 96 inputs):
  * any output width and up to 4096 inputs, for reduced-width test models.
