@@ -3,12 +3,20 @@
  *   o = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q . k_j),
  * over request i's key rows j and key head h / (heads / kv_heads).
  *
- * The plan is laid out on the host, once for a set of requests, and uploaded.
+ * The plan is laid out on the host, once for a set of requests, and uploaded:
+ * work items of HK_PACKED_QB query rows of one request and key head, over all
+ * of its key tiles or a piece of them.
+ *
+ * The query heads that share a key head are rows of one item: "virtual row"
+ * r * group + g is head g of the group of the request's row r, so single rows
+ * with shared heads fill an item's columns and K and V are read once for the
+ * group.
  *
  * The simple kernel here (one wave per query row and head) serves
  * H3_HIP_REFERENCE=1 and the head sizes, offsets and strides that the
  * matrix-core kernel does not take.
  */
+#include "hk_attn.h"
 #include "hk_common.h"
 #include "hk_internal.h"
 
@@ -17,9 +25,12 @@
 
 #include <algorithm>
 #include <new>
+#include <type_traits>
 #include <vector>
 
 #define HK_PACKED_MAX_DIM 256u
+#define HK_PACKED_WAVES 4u
+#define HK_PACKED_QB (HK_PACKED_WAVES * 32u) /* virtual rows of an item */
 
 /* a request with query rows, in device memory */
 struct hk_packed_request {
@@ -27,21 +38,47 @@ struct hk_packed_request {
     uint32_t before; /* query rows of the requests before it in the plan */
 };
 
+/* A work item: virtual rows [row, + HK_PACKED_QB) of a request's `rows`, of
+ * one key head, over key tiles [tile, tile_end) of the request's keys.  Whole
+ * items store their rows; a piece leaves its sums in part `part`.  An item of
+ * no rows fills a place in the launch. */
+struct hk_packed_item {
+    uint32_t q_first, rows, row, kv_head;
+    uint32_t kv_first, kv_rows, tile, tile_end;
+    uint32_t part;
+};
+#define HK_PACKED_WHOLE 0xffffffffu
+
+/* The pieces [part, + pieces) of one item's rows. */
+struct hk_packed_join {
+    uint32_t q_first, rows, row, kv_head;
+    uint32_t part, pieces;
+};
+
 /* hk_record.n of a plan */
 enum { HK_PACKED_HEADS, HK_PACKED_KV_HEADS, HK_PACKED_DIM,
        HK_PACKED_REQUESTS, /* those with query rows */
        HK_PACKED_ROWS,     /* query rows of all requests */
        HK_PACKED_Q_END,    /* rows that the query and output tensors hold */
-       HK_PACKED_KV_END };
+       HK_PACKED_KV_END,
+       HK_PACKED_ITEMS,    /* entries of each list, which follow each other: */
+       HK_PACKED_JOINS,    /* requests, items, joins */
+       HK_PACKED_PARTS };
 
 struct hk_packed_args {
     const uint16_t *q, *k, *v;
     uint16_t *o;
     uint64_t q_stride, kv_stride; /* elements from a row to the next */
-    uint32_t heads, kv_heads, dim;
-    float scale;
+    uint32_t heads, kv_heads, dim, group;
+    float scale, scale_log2;
     const hk_packed_request *requests;
     uint32_t request_count, rows;
+    const hk_packed_item *items;
+    const hk_packed_join *joins;
+    /* pieces' sums: F32 O [part][HK_PACKED_QB][padded dim], not divided, and
+     * (running maximum in the exp2 domain, sum) [part][HK_PACKED_QB] */
+    float *part_o;
+    float2 *part_ml;
 };
 
 /* One wave per (query row, head), 64 keys at a time: lane j scores key j of
@@ -102,6 +139,523 @@ __global__ void __launch_bounds__(256) hk_packed_simple(hk_packed_args a) {
             out[d * 64u + lane] = hk_f2bf(sum == 0.0f ? 0.0f : o[d] / sum);
 }
 
+/* ------------------------------------------------- the matrix-core kernel
+ *
+ * The scheme of hk_flash_fwd (hk_attn.hip) on a list of items: S^T = K . Q^T
+ * with the Q fragments in registers, the softmax in the lanes that hold a
+ * query's scores, O^T = V^T . P^T with P straight from the score accumulators
+ * and V^T from transposing LDS reads, and two LDS stages of 64 keys filled by
+ * direct-to-LDS loads.  What differs:
+ *   - rows of K and V come through buffer resources that end with the
+ *     request's keys, so what lies behind them (other requests' rows) reads
+ *     as zeros and P = 0 meets no infinity or NaN there;
+ *   - DP = 64 or 128 dims, smaller heads padded: a lane whose piece lies past
+ *     the head's dims loads from beyond the resource, zeros;
+ *   - tile addresses are 64-bit, so a context may pass 4 GiB;
+ *   - NaN scores stay NaN (this file is compiled without the flag that lets
+ *     hk_attn.hip assume none). */
+
+/* The swizzles of LDS tiles with rows of DP bf16: 16-byte chunk c of row r
+ * lies at chunk c ^ key(r).  K's fragment reads take one chunk of 16
+ * consecutive rows per 16 lanes, V's transposing reads 64 bytes of 4
+ * consecutive rows per 32 lanes; with 256-byte rows each row fills all banks
+ * once (keys as in hk_attn.h), 128-byte rows lie two to a turn of the
+ * banks. */
+template <int DP>
+__device__ __forceinline__ uint32_t hk_packed_k_key(uint32_t row) {
+    return DP == 128 ? row & 15u : (row >> 1) & 7u;
+}
+
+template <int DP>
+__device__ __forceinline__ uint32_t hk_packed_v_key(uint32_t row) {
+    return DP == 128 ? (row & 3u) << 2 : ((row >> 1) & 1u) << 2;
+}
+
+/* hk_vt_read and hk_vt_wait (hk_attn.h) for ND blocks of 32 dims and rows of
+ * 64 ND bytes. */
+template <int ND>
+__device__ __forceinline__ void hk_packed_vt_read(hk_v2i (&vt)[ND][2],
+                                                  const uint32_t (&frag)[ND],
+                                                  uint32_t off) {
+#pragma unroll
+    for (int d = 0; d < ND; d++)
+        asm volatile("ds_read_b64_tr_b16 %0, %2 offset:%3\n\t"
+                     "ds_read_b64_tr_b16 %1, %2 offset:%4"
+                     : "=v"(vt[d][0]), "=v"(vt[d][1])
+                     : "v"(frag[d]), "i"(off), "i"(off + 8u * 64u * ND));
+}
+
+template <int N>
+__device__ __forceinline__ void hk_packed_vt_wait(hk_v2i (&vt)[4][2]) {
+    hk_vt_wait<N>(vt);
+}
+
+template <int N>
+__device__ __forceinline__ void hk_packed_vt_wait(hk_v2i (&vt)[2][2]) {
+    asm volatile("s_waitcnt lgkmcnt(%4)"
+                 : "+v"(vt[0][0]), "+v"(vt[0][1]), "+v"(vt[1][0]),
+                   "+v"(vt[1][1])
+                 : "i"(N));
+}
+
+/* A wave's direct-to-LDS load of 16 bytes per lane.  A function of its own:
+ * in a lambda of a kernel template, the cast to LDS keeps the host pass from
+ * emitting the kernel's launch stub when it depends on the template's
+ * parameters. */
+__device__ __forceinline__ void hk_packed_dma16(__amdgpu_buffer_rsrc_t r,
+                                                uint8_t *lds,
+                                                uint32_t offset) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (hk_lds_void *)lds, 16, offset,
+                                             0, 0, 0);
+}
+
+template <int DP>
+__global__ void __launch_bounds__(HK_PACKED_WAVES * 64, 2)
+hk_packed_flash(hk_packed_args a) {
+    constexpr int NK = DP / 16, ND = DP / 32, CHUNKS = DP / 8;
+    constexpr uint32_t ROW = DP * 2u, TILE = HK_KT * ROW, STAGE = 2u * TILE;
+    /* 1-KiB loads per wave, tile and operand */
+    constexpr int DMA = TILE / 1024 / HK_PACKED_WAVES;
+    extern __shared__ __attribute__((aligned(16))) uint8_t hk_lds[];
+    const uint32_t tid = threadIdx.x, lane = tid & 63u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t col = lane & 31u, half = lane >> 5;
+
+    const hk_packed_item it = a.items[blockIdx.x];
+    if (it.row >= it.rows) return;
+    const uint32_t dim_chunks = a.dim >> 3;
+
+    /* wave w fills rows of a tile with DMA loads of 64 / CHUNKS rows each,
+     * lane l physical chunk l % CHUNKS of row l / CHUNKS; the swizzle is
+     * applied on the global side */
+    const uint32_t stride = (uint32_t)a.kv_stride * 2u; /* bytes */
+    uint32_t k_off[DMA], v_off[DMA];
+#pragma unroll
+    for (int i = 0; i < DMA; i++) {
+        const uint32_t row =
+            (wave * DMA + i) * (64u / CHUNKS) + lane / CHUNKS;
+        const uint32_t kc = (lane % CHUNKS) ^ hk_packed_k_key<DP>(row);
+        const uint32_t vc = (lane % CHUNKS) ^ hk_packed_v_key<DP>(row);
+        k_off[i] = kc < dim_chunks ? row * stride + kc * 16u : 0x80000000u;
+        v_off[i] = vc < dim_chunks ? row * stride + vc * 16u : 0x80000000u;
+    }
+    const uint64_t kv_base =
+        (uint64_t)it.kv_first * a.kv_stride + (uint64_t)it.kv_head * a.dim;
+    auto issue_tile = [&](uint32_t tile, uint32_t stage) {
+        const uint32_t kv0 = tile * HK_KT;
+        const uint64_t base = kv_base + kv0 * a.kv_stride;
+        /* the rows of this tile that the request has end the resource: 64
+         * rows stay below 2^31 bytes (hk_packed_takes) */
+        const uint32_t rows = min(it.kv_rows - kv0, (uint32_t)HK_KT);
+        const uint32_t bytes = (rows - 1u) * stride + a.dim * 2u;
+        const __amdgpu_buffer_rsrc_t vr = hk_attn_rsrc(a.v + base, bytes);
+        const __amdgpu_buffer_rsrc_t kr = hk_attn_rsrc(a.k + base, bytes);
+        uint8_t *st = hk_lds + stage * STAGE;
+#pragma unroll
+        for (int i = 0; i < DMA; i++)
+            hk_packed_dma16(vr, st + TILE + (wave * DMA + i) * 1024u,
+                            v_off[i]);
+#pragma unroll
+        for (int i = 0; i < DMA; i++)
+            hk_packed_dma16(kr, st + (wave * DMA + i) * 1024u, k_off[i]);
+    };
+    const uint32_t n = it.tile_end - it.tile;
+    if (n) issue_tile(it.tile, 0);
+
+    /* Q fragments, the B operand of S^T = K . Q^T: k-step ks of this lane's
+     * virtual row, dims 16 ks + 8 half .. + 8 */
+    const uint32_t vrow0 = it.row + wave * 32u, vrow = vrow0 + col;
+    hk_bf16x8 qf[NK];
+    {
+        const uint32_t r = vrow / a.group, g = vrow - r * a.group;
+        const uint16_t *q = a.q + ((uint64_t)it.q_first + r) * a.q_stride +
+                            (uint64_t)(it.kv_head * a.group + g) * a.dim;
+#pragma unroll
+        for (int ks = 0; ks < NK; ks++) {
+            hk_v4i x = {0, 0, 0, 0};
+            if (vrow < it.rows && 2u * ks + half < dim_chunks)
+                x = *(const hk_v4i *)(q + ks * 16u + half * 8u);
+            qf[ks] = __builtin_bit_cast(hk_bf16x8, x);
+        }
+    }
+
+    const uint32_t lds_base =
+        (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)
+            hk_lds;
+    uint32_t k_frag[NK];
+#pragma unroll
+    for (int kk = 0; kk < NK; kk++)
+        k_frag[kk] =
+            lds_base + col * ROW +
+            (((kk * 2u + half) ^ hk_packed_k_key<DP>(col)) << 4);
+    /* the transposing reads' source lanes, as in hk_flash_fwd */
+    uint32_t v_frag[ND];
+    {
+        const uint32_t j = lane & 15u, g1 = (lane >> 4) & 1u;
+        const uint32_t row = 4u * half + (j >> 2);
+        const uint32_t low = 2u * g1 + ((j & 3u) >> 1);
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+            v_frag[d] =
+                lds_base + TILE + row * ROW +
+                (((d * 4u + low) ^ hk_packed_v_key<DP>(row)) << 4) +
+                8u * (j & 1u);
+    }
+
+    hk_f32x16 o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; d++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) o[d][r] = 0.0f;
+    float m_run = -INFINITY, l_part = 0.0f;
+    /* a wave whose rows all lie past the request's stages its share of every
+     * tile and meets every barrier, and computes nothing */
+    const bool live = vrow0 < it.rows;
+
+    auto tile_step = [&](auto stage_tag, uint32_t tile, bool more,
+                         auto tail_tag) {
+        constexpr uint32_t stage = decltype(stage_tag)::value;
+        constexpr bool tail = decltype(tail_tag)::value;
+        if (more) issue_tile(tile + 1u, stage ^ 1u);
+        if (live) {
+        hk_f32x16 s[2];
+#pragma unroll
+        for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[kt][r] = 0.0f;
+#pragma unroll
+        for (int kk = 0; kk < NK; kk++)
+#pragma unroll
+            for (int kt = 0; kt < 2; kt++) {
+                const hk_bf16x8 kf = *(const hk_bf16x8 *)(
+                    (__attribute__((address_space(3))) uint8_t *)(uintptr_t)
+                        (k_frag[kk] + stage * STAGE + kt * 32u * ROW));
+                s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                    kf, qf[kk], s[kt], 0, 0, 0);
+            }
+        const uint32_t kv0 = tile * HK_KT;
+        if (tail && it.kv_rows - kv0 < HK_KT) {
+#pragma unroll
+            for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const uint32_t key = kv0 + kt * 32u + (r >> 2) * 8u +
+                                         half * 4u + (r & 3);
+                    if (key >= it.kv_rows) s[kt][r] = -INFINITY;
+                }
+        }
+        /* The softmax of hk_flash_fwd: P = exp2(s - m_run) against the
+         * running maximum as it stands, which moves (O and l rescaled) only
+         * when it is unset or a lane's P sum passes 2^32.  P <= 2^32 keeps O
+         * and l far from overflow; P rounds to bf16 for the product, l sums
+         * the unrounded P. */
+        hk_bf16x8 pf[2][2];
+        auto exps = [&]() -> float {
+            const float neg = -m_run;
+            float sum = 0.0f;
+#pragma unroll
+            for (int kt = 0; kt < 2; kt++) {
+                float p[16];
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    p[r] = __builtin_amdgcn_exp2f(
+                        __builtin_fmaf(s[kt][r], a.scale_log2, neg));
+                    /* -inf times a scale of zero is not what a key past the
+                     * end weighs */
+                    if (tail && s[kt][r] == -INFINITY) p[r] = 0.0f;
+                    sum += p[r];
+                }
+#pragma unroll
+                for (int st = 0; st < 2; st++) {
+                    hk_bf16x8 v;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) v[e] = (__bf16)p[st * 8 + e];
+                    pf[kt][st] = v;
+                }
+            }
+            return sum;
+        };
+        const bool unset = m_run == -INFINITY;
+        float sum = unset ? 0.0f : exps();
+        if (__builtin_amdgcn_ballot_w64(unset || sum > 0x1p32f)) {
+            float mx = -INFINITY;
+#pragma unroll
+            for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) mx = fmaxf(mx, s[kt][r]);
+            const auto sw = __builtin_amdgcn_permlane32_swap(
+                __float_as_uint(mx), __float_as_uint(mx), false, false);
+            mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) *
+                 a.scale_log2;
+            const float m_new = fmaxf(m_run, mx);
+            const float ref = m_new == -INFINITY ? 0.0f : m_new;
+            const float c = __builtin_amdgcn_exp2f(m_run - ref);
+            m_run = ref;
+            l_part *= c;
+#pragma unroll
+            for (int d = 0; d < ND; d++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) o[d][r] *= c;
+            sum = exps();
+        }
+        l_part += sum;
+
+        hk_v2i vt[2][ND][2];
+        hk_packed_vt_read<ND>(vt[0], v_frag, stage * STAGE);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int kt = i >> 1, st = i & 1;
+            if (i < 3) {
+                hk_packed_vt_read<ND>(vt[(i + 1) & 1], v_frag,
+                                      stage * STAGE + (i + 1) * 16u * ROW);
+                hk_packed_vt_wait<2 * ND>(vt[i & 1]);
+            } else {
+                hk_packed_vt_wait<0>(vt[i & 1]);
+            }
+#pragma unroll
+            for (int d = 0; d < ND; d++) {
+                const hk_v4i both = {vt[i & 1][d][0][0], vt[i & 1][d][0][1],
+                                     vt[i & 1][d][1][0], vt[i & 1][d][1][1]};
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                    __builtin_bit_cast(hk_bf16x8, both), pf[kt][st], o[d], 0,
+                    0, 0);
+            }
+        }
+        } /* live */
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+    };
+    using S0 = std::integral_constant<uint32_t, 0>;
+    using S1 = std::integral_constant<uint32_t, 1>;
+    using NT = std::integral_constant<bool, false>;
+    using TT = std::integral_constant<bool, true>;
+    if (n) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        uint32_t i = 0;
+        for (; i + 2 < n; i += 2) {
+            tile_step(S0(), it.tile + i, true, NT());
+            tile_step(S1(), it.tile + i + 1, true, NT());
+        }
+        if (i + 2 == n) {
+            tile_step(S0(), it.tile + i, true, NT());
+            tile_step(S1(), it.tile + i + 1, false, TT());
+        } else {
+            tile_step(S0(), it.tile + i, false, TT());
+        }
+    }
+
+    /* The lane holds query column `col`, dims 32 d + 8 (r / 4) + 4 half +
+     * r % 4.  The wave's rows go through LDS of its own (free after the last
+     * barrier), 16-byte chunk c of row r at c ^ key, and leave as whole
+     * rows. */
+    const float l = l_part + __shfl_xor(l_part, 32, 64);
+    if (it.part != HK_PACKED_WHOLE) {
+        float *pw = (float *)(hk_lds + wave * (32u * 64u * 4u));
+        float *part = a.part_o + (size_t)it.part * HK_PACKED_QB * DP;
+#pragma unroll
+        for (int hd = 0; hd < DP / 64; hd++) {
+#pragma unroll
+            for (int dd = 0; dd < 2; dd++)
+#pragma unroll
+                for (int blk = 0; blk < 4; blk++) {
+                    const int d = 2 * hd + dd;
+                    const uint32_t c = dd * 8u + blk * 2u + half;
+                    *(float4 *)(pw + col * 64u + ((c ^ (col & 15u)) << 2)) =
+                        make_float4(o[d][blk * 4 + 0], o[d][blk * 4 + 1],
+                                    o[d][blk * 4 + 2], o[d][blk * 4 + 3]);
+                }
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const uint32_t r = i * 4u + (lane >> 4), c = lane & 15u;
+                const float4 v =
+                    *(const float4 *)(pw + r * 64u + ((c ^ (r & 15u)) << 2));
+                if (vrow0 + r < it.rows)
+                    *(float4 *)(part + (size_t)(wave * 32u + r) * DP +
+                                hd * 64u + c * 4u) = v;
+            }
+        }
+        if (half == 0 && vrow < it.rows)
+            a.part_ml[(size_t)it.part * HK_PACKED_QB + wave * 32u + col] =
+                make_float2(m_run, l);
+        return;
+    }
+    /* no keys, or none with weight: zeros (a NaN sum gives NaN) */
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    uint8_t *ow = hk_lds + wave * (32u * ROW);
+#pragma unroll
+    for (int d = 0; d < ND; d++)
+#pragma unroll
+        for (int blk = 0; blk < 4; blk++) {
+            const uint32_t chunk = d * 4u + blk;
+            *(uint2 *)(ow + col * ROW +
+                       ((chunk ^ hk_packed_k_key<DP>(col)) << 4) + half * 8u) =
+                make_uint2(hk_pack2(o[d][blk * 4 + 0] * inv,
+                                    o[d][blk * 4 + 1] * inv),
+                           hk_pack2(o[d][blk * 4 + 2] * inv,
+                                    o[d][blk * 4 + 3] * inv));
+        }
+#pragma unroll
+    for (int i = 0; i < 32 * CHUNKS / 64; i++) {
+        const uint32_t r = i * (64u / CHUNKS) + lane / CHUNKS;
+        const uint32_t c = lane % CHUNKS, vr = vrow0 + r;
+        const uint4 v = *(const uint4 *)(
+            ow + r * ROW + ((c ^ hk_packed_k_key<DP>(r)) << 4));
+        if (vr >= it.rows || c >= dim_chunks) continue;
+        const uint32_t qr = vr / a.group, g = vr - qr * a.group;
+        *(uint4 *)(a.o +
+                   (((uint64_t)it.q_first + qr) * a.heads +
+                    it.kv_head * a.group + g) * a.dim + c * 8u) = v;
+    }
+}
+
+/* Joins the pieces of an item's rows: with the pieces' maxima m_p, sums l_p
+ * and undivided O_p, O = sum_p 2^(m_p - M) O_p / sum_p 2^(m_p - M) l_p, M =
+ * max_p m_p, in piece order.  A wave per row; a lane holds DP / 64 dims. */
+template <int DP>
+__global__ void __launch_bounds__(256) hk_packed_joined(hk_packed_args a) {
+    const hk_packed_join j = a.joins[blockIdx.x];
+    const uint32_t ql = blockIdx.y * 4u + (threadIdx.x >> 6);
+    const uint32_t lane = threadIdx.x & 63u, vr = j.row + ql;
+    if (vr >= j.rows) return;
+    constexpr int PER = DP / 64;
+    const float2 *ml = a.part_ml + (size_t)j.part * HK_PACKED_QB + ql;
+    const float *po = a.part_o + ((size_t)j.part * HK_PACKED_QB + ql) * DP +
+                      lane * PER;
+    float top = -INFINITY;
+    for (uint32_t p = 0; p < j.pieces; p++)
+        top = fmaxf(top, ml[(size_t)p * HK_PACKED_QB].x);
+    float sum[PER] = {}, l = 0.0f;
+    for (uint32_t p = 0; p < j.pieces; p++) {
+        const float2 mine = ml[(size_t)p * HK_PACKED_QB];
+        const float w = __builtin_amdgcn_exp2f(mine.x - top);
+        l += w * mine.y;
+#pragma unroll
+        for (int e = 0; e < PER; e++)
+            sum[e] += w * po[(size_t)p * HK_PACKED_QB * DP + e];
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const uint32_t qr = vr / a.group, g = vr - qr * a.group;
+    uint16_t *out = a.o + (((uint64_t)j.q_first + qr) * a.heads +
+                           j.kv_head * a.group + g) * a.dim;
+#pragma unroll
+    for (int e = 0; e < PER; e++)
+        if (lane * PER + e < a.dim) out[lane * PER + e] = hk_f2bf(sum[e] * inv);
+}
+
+template <int DP>
+static void hk_packed_launch(struct h3_gpu *gpu, const hk_packed_args &a,
+                             uint32_t items, uint32_t joins) {
+    constexpr uint32_t lds = 2u * 2u * HK_KT * DP * 2u;
+    hipLaunchKernelGGL(hk_packed_flash<DP>, dim3(items),
+                       dim3(HK_PACKED_WAVES * 64u), lds, gpu->stream, a);
+    if (joins)
+        hipLaunchKernelGGL(hk_packed_joined<DP>,
+                           dim3(joins, HK_PACKED_QB / 4u), dim3(256), 0,
+                           gpu->stream, a);
+}
+
+/* Whether the matrix-core kernel takes these rows: whole 16-byte pieces, and
+ * 64 key rows below 2^31 bytes, the reach of a tile's lane offsets. */
+static bool hk_packed_takes(const struct h3_gpu *gpu,
+                            const hk_packed_args &a) {
+    return !gpu->reference_kernels && a.dim % 8u == 0 && a.dim <= 128u &&
+           a.q_stride % 8u == 0 && a.kv_stride % 8u == 0 &&
+           a.kv_stride < (1u << 24) &&
+           (((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v |
+             (uintptr_t)a.o) & 15u) == 0;
+}
+
+/* How a plan's items are dealt out.  An item costs its key tiles and about
+ * three tiles' time for its start and end.  Where the longest item takes
+ * longer than an even share of all work (two workgroups a CU), items are cut
+ * into pieces of about that share.
+ *
+ * Workgroups go to the 8 XCDs in turn.  The items of one request and key head
+ * share K and V, so they go to one XCD's queue (in runs of at most 1/64 of
+ * all work, so that the queues come out level), longest first; items of no
+ * rows fill the shorter queues. */
+struct hk_packed_work {
+    std::vector<hk_packed_item> items;
+    std::vector<hk_packed_join> joins;
+    uint32_t parts;
+};
+
+static void hk_packed_lay_out(const std::vector<hk_packed_request> &list,
+                              uint32_t group, uint32_t kv_heads, uint32_t cus,
+                              hk_packed_work &work) {
+    const double own = 3.0; /* an item's start and end, in tiles */
+    struct sized { uint32_t request, tiles, rows, blocks; };
+    std::vector<sized> order;
+    double total = 0.0;
+    for (uint32_t i = 0; i < list.size(); i++) {
+        const uint32_t rows = list[i].q_rows * group;
+        const sized s = {i, (uint32_t)(((uint64_t)list[i].kv_rows + HK_KT - 1) /
+                                       HK_KT),
+                         rows, (uint32_t)(((uint64_t)rows + HK_PACKED_QB - 1) /
+                                          HK_PACKED_QB)};
+        order.push_back(s);
+        total += (double)s.blocks * kv_heads * (s.tiles + own);
+    }
+    std::stable_sort(order.begin(), order.end(),
+                     [](const sized &x, const sized &y) {
+                         return x.tiles > y.tiles;
+                     });
+    const double share = total / (2.0 * cus);
+    /* a cut costs a join: worth it only where the longest item stands out */
+    const double longest = order.empty() ? 0.0 : order[0].tiles + own;
+    const uint32_t most = longest > share + 8.0
+                              ? (uint32_t)std::max(4.0, share)
+                              : UINT32_MAX;
+    std::vector<hk_packed_item> queue[8];
+    double load[8] = {};
+    const double run = total / 64.0;
+    work.parts = 0;
+    for (const sized &s : order) {
+        const hk_packed_request &r = list[s.request];
+        const uint32_t pieces =
+            s.tiles > most ? (s.tiles + most - 1) / most : 1;
+        const uint32_t per = pieces > 1 ? (s.tiles + pieces - 1) / pieces
+                                        : s.tiles;
+        int at = -1;
+        double here = 0.0;
+        for (uint32_t h = 0; h < kv_heads; h++) {
+            at = -1;
+            for (uint32_t b = 0; b < s.blocks; b++) {
+                if (at < 0 || here > run) {
+                    at = (int)(std::min_element(load, load + 8) - load);
+                    here = 0.0;
+                }
+                hk_packed_item item = {r.q_first, s.rows, b * HK_PACKED_QB, h,
+                                       r.kv_first, r.kv_rows, 0, s.tiles,
+                                       HK_PACKED_WHOLE};
+                if (pieces == 1) {
+                    queue[at].push_back(item);
+                } else {
+                    uint32_t made = 0;
+                    const uint32_t first = work.parts;
+                    for (uint32_t t = 0; t < s.tiles; t += per, made++) {
+                        item.tile = t;
+                        item.tile_end = std::min(s.tiles, t + per);
+                        item.part = work.parts++;
+                        queue[at].push_back(item);
+                    }
+                    work.joins.push_back({r.q_first, s.rows, item.row, h,
+                                          first, made});
+                }
+                const double cost = s.tiles + own * pieces;
+                load[at] += cost;
+                here += cost;
+            }
+        }
+    }
+    size_t longest_queue = 0;
+    for (const auto &q : queue) longest_queue = std::max(longest_queue, q.size());
+    for (size_t j = 0; j < longest_queue; j++)
+        for (const auto &q : queue)
+            work.items.push_back(j < q.size() ? q[j] : hk_packed_item{});
+}
+
 extern "C" {
 
 h3_gpu_tensor *h3_hip_sdpa_packed_plan(h3_gpu *gpu, const uint32_t *q_first,
@@ -151,24 +705,38 @@ h3_gpu_tensor *h3_hip_sdpa_packed_plan(h3_gpu *gpu, const uint32_t *q_first,
                              "overlap at row %u", ranges[i].first);
                 return NULL;
             }
-        if (rows * heads > 0x7fffffffull) {
+        /* (an item for every 128 of them: 4 million items) */
+        if (rows * heads >= 1ull << 29) {
             hk_fail(gpu, "attention plan: too many query rows and heads");
             return NULL;
         }
-        const size_t count = list.size();
-        if (list.empty()) list.push_back({0, 0, 0, 0, 0});
-        h3_gpu_tensor *plan = h3_gpu_tensor_from_u32(
-            gpu, (const uint32_t *)list.data(),
-            list.size() * sizeof(hk_packed_request) / 4);
+        hk_packed_work work;
+        hk_packed_lay_out(list, heads / kv_heads, kv_heads,
+                          gpu->num_cus > 0 ? (uint32_t)gpu->num_cus : 256u,
+                          work);
+        std::vector<uint32_t> words;
+        auto add = [&](const void *data, size_t bytes) {
+            const uint32_t *w = (const uint32_t *)data;
+            words.insert(words.end(), w, w + bytes / 4);
+        };
+        add(list.data(), list.size() * sizeof(list[0]));
+        add(work.items.data(), work.items.size() * sizeof(work.items[0]));
+        add(work.joins.data(), work.joins.size() * sizeof(work.joins[0]));
+        if (words.empty()) words.push_back(0);
+        h3_gpu_tensor *plan =
+            h3_gpu_tensor_from_u32(gpu, words.data(), words.size());
         if (!plan) return NULL;
         plan->record.kind = HK_RECORD_PACKED;
         plan->record.n[HK_PACKED_HEADS] = heads;
         plan->record.n[HK_PACKED_KV_HEADS] = kv_heads;
         plan->record.n[HK_PACKED_DIM] = head_dim;
-        plan->record.n[HK_PACKED_REQUESTS] = (uint32_t)count;
+        plan->record.n[HK_PACKED_REQUESTS] = (uint32_t)list.size();
         plan->record.n[HK_PACKED_ROWS] = (uint32_t)rows;
         plan->record.n[HK_PACKED_Q_END] = (uint32_t)q_end;
         plan->record.n[HK_PACKED_KV_END] = (uint32_t)kv_end;
+        plan->record.n[HK_PACKED_ITEMS] = (uint32_t)work.items.size();
+        plan->record.n[HK_PACKED_JOINS] = (uint32_t)work.joins.size();
+        plan->record.n[HK_PACKED_PARTS] = work.parts;
         return plan;
     } catch (const std::bad_alloc &) {
         hk_fail(gpu, "out of host memory");
@@ -233,10 +801,31 @@ int h3_hip_sdpa_packed_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
     a.kv_heads = kv_heads;
     a.dim = dim;
     a.scale = scale;
+    a.group = heads / kv_heads;
+    a.scale_log2 = scale * 1.4426950408889634f;
     a.requests = (const hk_packed_request *)plan->data;
     a.request_count = n[HK_PACKED_REQUESTS];
     a.rows = n[HK_PACKED_ROWS];
+    a.items = (const hk_packed_item *)(a.requests + a.request_count);
+    a.joins = (const hk_packed_join *)(a.items + n[HK_PACKED_ITEMS]);
     hk_op_begin(gpu, "attention_packed");
+    if (hk_packed_takes(gpu, a)) {
+        const size_t padded = dim <= 64 ? 64 : 128;
+        const size_t rows = (size_t)n[HK_PACKED_PARTS] * HK_PACKED_QB;
+        if (rows) {
+            a.part_o = (float *)hk_splitk_space(
+                gpu, rows * (padded * sizeof(float) + sizeof(float2)));
+            if (!a.part_o) return 0;
+            a.part_ml = (float2 *)(a.part_o + rows * padded);
+        }
+        if (padded == 64)
+            hk_packed_launch<64>(gpu, a, n[HK_PACKED_ITEMS],
+                                 n[HK_PACKED_JOINS]);
+        else
+            hk_packed_launch<128>(gpu, a, n[HK_PACKED_ITEMS],
+                                  n[HK_PACKED_JOINS]);
+        return hk_op_end(gpu, "attention_packed", HK_KIND_SDPA);
+    }
     const uint64_t waves = (uint64_t)a.rows * heads;
     hipLaunchKernelGGL(hk_packed_simple, dim3((unsigned)((waves + 3) / 4)),
                        dim3(256), 0, gpu->stream, a);
