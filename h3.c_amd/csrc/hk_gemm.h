@@ -149,4 +149,43 @@ __device__ __forceinline__ void hk_tile_coords(uint32_t tile, uint32_t tiles_m,
     tile_n = in_band / band_rows;
 }
 
+/* Dynamic LDS of a kernel with 32 jb rows per tile. */
+static inline uint32_t hk_gemm_lds(uint32_t jb) {
+    return HK_STAGES * (32u * jb * HK_BK * 2u + HK_TILE_BYTES) + 256u;
+}
+
+/* ------------------------------------------------ low-rank adapters */
+
+/* one adapter of a table (hk_lora.hip), in device memory; the kernels read it
+ * as four 8-byte words */
+struct hk_lora_entry {
+    const uint16_t *down; /* A: [rank][K] */
+    const uint16_t *up;   /* B twice: [N][2 padded], zeros past the rank */
+    uint32_t rank, padded; /* the rank, and as a multiple of 32 */
+    float scale;
+    uint32_t bad; /* set by hk_lora_pack: an element is not finite */
+};
+
+#define HK_LORA_NONE 0xffffffffu
+
+/* What the GEMM with adapters adds to its K loop: for row r of adapter a =
+ * map[r] < count, s_a x[r] . A_a^T as bf16 halves low[r][0, padded) and
+ * [padded, 2 padded) (their sum is the F32 value to 16 bits), against the row
+ * of B twice. */
+struct hk_lora_ext {
+    const hk_lora_entry *entries;
+    uint32_t count;
+    const uint32_t *map;
+    const uint16_t *low;
+    uint32_t pitch; /* elements of a row of `low`: twice the largest padded */
+    uint32_t low_bytes;
+};
+
+struct h3_gpu;
+/* Launches hk_gemm_lora with 32 jb rows per tile on g; epilogue HK_EPI_STORE,
+ * HK_EPI_GELU or HK_EPI_PARTIAL. */
+void hk_gemm_lora_launch(struct h3_gpu *gpu, int epilogue, uint32_t jb,
+                         uint32_t workgroups, const hk_gemm_args &g,
+                         const hk_lora_ext &lora);
+
 #endif

@@ -319,10 +319,9 @@ static uint32_t hk_gemm_grid(uint32_t tiles, uint32_t cus) {
     return wgs < cus ? wgs : cus;
 }
 
-/* Whether the MFMA kernels take this shape and these pointers. */
-static bool hk_gemm_mfma_ok(const struct h3_gpu *gpu, const void *x,
-                            const void *w, const void *bias, const void *c,
-                            uint32_t m, uint32_t n, uint32_t k, int epilogue) {
+bool hk_gemm_mfma_ok(const struct h3_gpu *gpu, const void *x, const void *w,
+                     const void *bias, const void *c, uint32_t m, uint32_t n,
+                     uint32_t k, int epilogue) {
     const uint64_t w_rows = epilogue == HK_EPI_SWIGLU ? 2ull * n : n;
     const uint64_t x_bytes = (uint64_t)m * k * 2, w_bytes = w_rows * k * 2;
     /* operand buffers must leave room for a row offset plus a k offset
@@ -367,10 +366,6 @@ static hk_gemm_kernel hk_gemm_pick_epi(int epilogue, uint32_t jb) {
     }
 }
 
-static uint32_t hk_gemm_lds(uint32_t jb) {
-    return HK_STAGES * (32u * jb * HK_BK * 2u + HK_TILE_BYTES) + 256u;
-}
-
 static void hk_gemm_lds_setup(const struct h3_gpu *gpu) {
     const uint64_t bit = 1ull << (gpu->device & 63);
     if (hk_gemm_lds_ready & bit) return;
@@ -388,11 +383,15 @@ static void hk_gemm_lds_setup(const struct h3_gpu *gpu) {
     hk_gemm_lds_ready |= bit;
 }
 
-static void hk_gemm_launch(struct h3_gpu *gpu, hk_gemm_kernel kernel,
-                           uint32_t jb, uint32_t workgroups,
-                           const hk_gemm_args &g) {
-    hipLaunchKernelGGL(kernel, dim3(workgroups), dim3(HK_GEMM_THREADS),
-                       hk_gemm_lds(jb), gpu->stream, g);
+static void hk_gemm_launch(struct h3_gpu *gpu, int epilogue, uint32_t jb,
+                           uint32_t workgroups, const hk_gemm_args &g,
+                           const hk_lora_ext *lora) {
+    if (lora)
+        hk_gemm_lora_launch(gpu, epilogue, jb, workgroups, g, *lora);
+    else
+        hipLaunchKernelGGL(hk_gemm_pick_epi(epilogue, jb), dim3(workgroups),
+                           dim3(HK_GEMM_THREADS), hk_gemm_lds(jb),
+                           gpu->stream, g);
 }
 
 /* How the tiles of a launch run: `full` tiles in rounds of one per CU, then
@@ -586,13 +585,14 @@ static int hk_gemm_skinny_run(struct h3_gpu *gpu, hk_skinny_args &g,
 int hk_gemm_bf16(struct h3_gpu *gpu, const uint16_t *x, const uint16_t *w,
                  const uint16_t *bias, uint16_t *c, uint32_t m, uint32_t n,
                  uint32_t k, int epilogue, float *scratch,
-                 size_t scratch_bytes) {
+                 size_t scratch_bytes, const hk_lora_ext *lora) {
     if (!m || !n) return 1;
     const uint64_t w_rows = epilogue == HK_EPI_SWIGLU ? 2ull * n : n;
     const uint64_t x_bytes = (uint64_t)m * k * 2, w_bytes = w_rows * k * 2;
     const bool mfma = hk_gemm_mfma_ok(gpu, x, w, bias, c, m, n, k, epilogue);
     const uint32_t cus = gpu->num_cus > 0 ? (uint32_t)gpu->num_cus : 256u;
-    if (mfma && epilogue == HK_EPI_STORE && hk_skinny_takes(m, n, k, cus)) {
+    if (mfma && epilogue == HK_EPI_STORE && !lora &&
+        hk_skinny_takes(m, n, k, cus)) {
         hk_skinny_args g = {};
         g.x = x; g.w = w; g.bias = bias; g.c = c;
         g.m = m; g.n = n; g.k = k;
@@ -649,19 +649,17 @@ int hk_gemm_bf16(struct h3_gpu *gpu, const uint16_t *x, const uint16_t *w,
             const uint32_t splits = r.splits, steps = r.steps;
             if (full) {
                 g.tile_count = full;
-                hk_gemm_launch(gpu, hk_gemm_pick_epi(epilogue, jb), jb,
-                               hk_gemm_grid(full, cus), g);
+                hk_gemm_launch(gpu, epilogue, jb, hk_gemm_grid(full, cus), g,
+                               lora);
             }
             g.partial = partial;
             g.split_steps = steps;
             g.tile_base = full;
             g.part_tiles = tail;
             hk_gemm_launch(gpu,
-                           hk_gemm_pick_epi(epilogue == HK_EPI_SWIGLU
-                                                ? HK_EPI_PARTIAL_SWIGLU
-                                                : HK_EPI_PARTIAL,
-                                            jb),
-                           jb, tail * splits, g);
+                           epilogue == HK_EPI_SWIGLU ? HK_EPI_PARTIAL_SWIGLU
+                                                     : HK_EPI_PARTIAL,
+                           jb, tail * splits, g, lora);
             if (epilogue == HK_EPI_SWIGLU)
                 hipLaunchKernelGGL(hk_splitk_reduce<HK_EPI_SWIGLU>,
                                    dim3(tail * (g.tile_rows / 8)), dim3(256),
@@ -676,10 +674,12 @@ int hk_gemm_bf16(struct h3_gpu *gpu, const uint16_t *x, const uint16_t *w,
                                    0, gpu->stream, g, splits);
             return 1;
         }
-        hk_gemm_launch(gpu, hk_gemm_pick_epi(epilogue, jb), jb,
-                       hk_gemm_grid(g.tile_count, cus), g);
+        hk_gemm_launch(gpu, epilogue, jb, hk_gemm_grid(g.tile_count, cus), g,
+                       lora);
         return 1;
     }
+    if (lora) return hk_fail(gpu, "linear with adapters: not a shape for the "
+                                  "matrix cores");
     if (epilogue == HK_EPI_SWIGLU) {
         uint16_t *fused = (uint16_t *)hk_workspace(gpu, (size_t)m * n * 4);
         if (!fused) return 0;
@@ -793,8 +793,9 @@ static int hk_gemm_bf16_group(struct h3_gpu *gpu, const uint16_t *x,
     g.group_tiles = g.tiles_m * g.tiles_n;
     g.group = table;
     g.tile_count = count * g.group_tiles;
-    hk_gemm_launch(gpu, hk_gemm_pick<HK_EPI_STORE, true>(jb), jb,
-                   hk_gemm_grid(g.tile_count, cus), g);
+    hipLaunchKernelGGL((hk_gemm_pick<HK_EPI_STORE, true>(jb)),
+                       dim3(hk_gemm_grid(g.tile_count, cus)),
+                       dim3(HK_GEMM_THREADS), hk_gemm_lds(jb), gpu->stream, g);
     return 1;
 }
 

@@ -159,11 +159,18 @@ enum { HK_EPI_STORE = 0, HK_EPI_SWIGLU = 1, HK_EPI_GELU = 2,
  * Split-K partials go to the context's scratch (grown on demand), or, when
  * `scratch` is given, to that caller-owned device buffer of scratch_bytes:
  * then nothing is allocated, and a split that needs more fails (launches of
- * at most 128 rows use what the context has, and need no buffer). */
+ * at most 128 rows use what the context has, and need no buffer).  `lora`
+ * (plain and GELU epilogue, over 128 rows, hk_gemm_mfma_ok): the adapters'
+ * part is added to the sums. */
 int hk_gemm_bf16(struct h3_gpu *gpu, const uint16_t *a, const uint16_t *w,
                  const uint16_t *bias, uint16_t *c, uint32_t m, uint32_t n,
                  uint32_t k, int epilogue, float *scratch = nullptr,
-                 size_t scratch_bytes = 0);
+                 size_t scratch_bytes = 0,
+                 const struct hk_lora_ext *lora = nullptr);
+/* Whether the MFMA kernels take this shape and these pointers. */
+bool hk_gemm_mfma_ok(const struct h3_gpu *gpu, const void *x, const void *w,
+                     const void *bias, const void *c, uint32_t m, uint32_t n,
+                     uint32_t k, int epilogue);
 int hk_gemm_bf16_pair(struct h3_gpu *gpu, const uint16_t *x,
                       const uint16_t *w0, const uint16_t *b0, uint16_t *c0,
                       const uint16_t *w1, const uint16_t *b1, uint16_t *c1,
