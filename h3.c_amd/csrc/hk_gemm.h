@@ -156,14 +156,17 @@ static inline uint32_t hk_gemm_lds(uint32_t jb) {
 
 /* ------------------------------------------------ low-rank adapters */
 
-/* one adapter of a table (hk_lora.hip), in device memory; the kernels read it
- * as four 8-byte words */
+/* one adapter of a table (hk_lora.hip), in device memory; the kernels read
+ * its first words as 8-byte ones */
 struct hk_lora_entry {
     const uint16_t *down; /* A: [rank][K] */
     const uint16_t *up;   /* B twice: [N][2 padded], zeros past the rank */
     uint32_t rank, padded; /* the rank, and as a multiple of 32 */
     float scale;
     uint32_t bad; /* set by hk_lora_pack: an element is not finite */
+    /* B as MFMA fragments: lane l of 32 columns and 16 ranks has column l % 32,
+     * ranks 8 (l / 32) .. + 8: [N / 32][rank / 16][64][8], rounded up */
+    const uint16_t *fragments;
 };
 
 #define HK_LORA_NONE 0xffffffffu
@@ -179,6 +182,9 @@ struct hk_lora_ext {
     const uint16_t *low;
     uint32_t pitch; /* elements of a row of `low`: twice the largest padded */
     uint32_t low_bytes;
+    /* the adapters of each row tile's rows, in rising order: 256 entries a
+     * tile, (adapter, 2 padded, address of B), HK_LORA_NONE behind the last */
+    uint4 *lists;
 };
 
 struct h3_gpu;

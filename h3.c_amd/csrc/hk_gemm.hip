@@ -582,6 +582,13 @@ static int hk_gemm_skinny_run(struct h3_gpu *gpu, hk_skinny_args &g,
     return 1;
 }
 
+uint32_t hk_gemm_tile_rows(const struct h3_gpu *gpu, uint32_t m, uint32_t n,
+                           uint32_t k) {
+    const uint32_t cus = gpu->num_cus > 0 ? (uint32_t)gpu->num_cus : 256u;
+    return 32u * hk_gemm_row_blocks(m, (n + HK_BN - 1) / HK_BN, k / HK_BK, cus,
+                                    true);
+}
+
 int hk_gemm_bf16(struct h3_gpu *gpu, const uint16_t *x, const uint16_t *w,
                  const uint16_t *bias, uint16_t *c, uint32_t m, uint32_t n,
                  uint32_t k, int epilogue, float *scratch,

@@ -6,11 +6,14 @@
  * (the down projection, [rank][K]) and B (the up projection) as [N][2 padded],
  * with the rank padded by zeros to a multiple of 32 and each row twice, so
  * that a row against the two halves below is whole 64-deep steps of the GEMM
- * for any rank.
+ * for any rank; and B once more in the order in which the sum of few rows
+ * takes it (as rows of 128 bytes it read four times the lines at rank 16).
  *
- * The products run in two parts.  s_a x . A_a^T goes to scratch as two bf16
- * halves (hk_lora_low); then the projection's own GEMM takes it as a few more
- * steps of K against B_a.  Two halves because the matrix cores take bf16: one
+ * The products run in two parts.  x . A_a^T goes to scratch in F32, in pieces
+ * of K (hk_lora_low_unit).  Their sum times s_a, as two bf16 halves, meets
+ * B_a: as a few more steps of K of the projection's own GEMM over 128 rows
+ * (hk_lora_halves, hk_gemm_lora), in the sum of the skinny GEMM's pieces up to
+ * 128 (hk_lora_join).  Two halves because the matrix cores take bf16: one
  * would round the adapters' part to 8 bits before it is added, two keep 16,
  * below what F32 sums of that length keep.
  *
@@ -29,7 +32,8 @@
 #define HK_LORA_MAX_RANK 1024u
 
 /* hk_record.n of a table */
-enum { HK_LORA_IN, HK_LORA_OUT, HK_LORA_COUNT, HK_LORA_PADDED /* largest */ };
+enum { HK_LORA_IN, HK_LORA_OUT, HK_LORA_COUNT,
+       HK_LORA_RANK, HK_LORA_PADDED /* the largest */ };
 
 struct hk_lora_args {
     const uint16_t *x, *w, *bias;
@@ -40,18 +44,34 @@ struct hk_lora_args {
     const uint32_t *map;
     /* s_a x . A_a^T: F32 [rows][pitch] for the simple kernels */
     float *low;
-    uint32_t pitch;
+    uint32_t pitch; /* largest padded rank */
+    uint32_t rank;  /* largest rank */
     int gelu;
 };
 
-/* The matrix-core kernels' first product and the joining of the second. */
+/* The matrix-core kernels' first product. */
 struct hk_lora_low_args {
     const uint16_t *x;
     uint32_t m, k, x_bytes;
     hk_lora_ext ext;
-    uint32_t row_groups; /* of 32 rows */
-    uint32_t chunks;     /* of ranks, each a workgroup's */
-    uint32_t slots;      /* workgroups that share a row group's adapters */
+    /* x . A^T of K's pieces: F32 [piece][row][sum_pitch] */
+    float *sums;
+    uint32_t sum_pitch;
+    uint32_t pieces, piece_steps; /* of K, in 64-deep steps */
+    uint32_t row_groups;          /* of 16 J rows */
+    uint32_t chunks;              /* of 16 RB ranks */
+    uint32_t slots; /* workgroups that share a row group's adapters */
+    uint32_t units; /* workgroups in all of them */
+    struct hk_lora_row *rows; /* up to 128 rows: what each one's adapter is */
+};
+
+/* A row's adapter, found once for all of hk_lora_join's waves; rank 0 without
+ * one. */
+struct hk_lora_row {
+    const uint16_t *fragments;
+    uint32_t rank;
+    float scale;
+    uint32_t adapter, unused[3];
 };
 
 /* Copies a [rows][cols] matrix, `count` elements with zeros behind each row up
@@ -67,6 +87,21 @@ hk_lora_pack(const uint16_t *src, uint16_t *dst, uint32_t cols, uint32_t pitch,
     for (uint32_t t = 0; t < times; t++)
         dst[(r * times + t) * pitch + c] = v;
     if ((v & 0x7f80u) == 0x7f80u) entry->bad = 1; /* every writer writes 1 */
+}
+
+/* B ([N][rank]) as hk_lora_entry's fragments. */
+__global__ void __launch_bounds__(256)
+hk_lora_pack_fragments(const uint16_t *src, uint16_t *dst, uint32_t n,
+                       uint32_t rank, uint64_t count) {
+    const uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x;
+    if (i >= count) return;
+    const uint32_t at = (uint32_t)(i % 512u), lane = at >> 3;
+    const uint64_t block = i / 512u;
+    const uint32_t chunks = (rank + 15u) / 16u;
+    const uint64_t col = block / chunks * 32u + (lane & 31u);
+    const uint32_t k =
+        (uint32_t)(block % chunks) * 16u + (lane >> 5) * 8u + (at & 7u);
+    dst[i] = col < n && k < rank ? src[col * rank + k] : (uint16_t)0;
 }
 
 /* low[r][j] = s_a x[r] . A_a[j]: one wave an element. */
@@ -129,131 +164,152 @@ static int hk_lora_run_simple(struct h3_gpu *gpu, hk_lora_args &g) {
 
 /* --------------------------------------------- the matrix-core kernels */
 
-/* The least of the workgroup's 256 `ids` over `last` (any, where `last` is
- * none), the same for its four waves; `words` is 4 words of LDS. */
-__device__ __forceinline__ uint32_t hk_lora_next(const uint32_t *ids,
-                                                 uint32_t last,
-                                                 uint32_t *words) {
-    __syncthreads(); /* ids written, the words of the call before read */
-    uint32_t value = ids[threadIdx.x];
-    if (last != HK_LORA_NONE && value <= last) value = HK_LORA_NONE;
-#pragma unroll
-    for (int offset = 32; offset; offset >>= 1)
-        value = min(value, (uint32_t)__shfl_xor((int)value, offset, 64));
-    if ((threadIdx.x & 63u) == 0) words[threadIdx.x >> 6] = value;
-    __syncthreads();
-    value = min(min(words[0], words[1]), min(words[2], words[3]));
-    return (uint32_t)__builtin_amdgcn_readfirstlane((int)value);
-}
-
-/* hk_lora_low's workgroup: rows [32 group, + 32), ranks [16 RB chunk, + 16 RB)
- * of the row group's adapters slot, slot + slots, ... (in rising order).
+/* A workgroup of the first product: 16 J rows from row0 on, ranks [16 RB chunk,
+ * + 16 RB) of the rows' adapters slot, slot + slots, ... (in rising order),
+ * piece `piece` of K.
  *
  * v_mfma_f32_16x16x32_bf16 with A's rows against X's: RB blocks of 16 ranks,
- * two of 16 rows.  The four waves split K (64-deep steps w, w + 4, ...) and
- * add their sums in LDS.  Fragments come straight from global memory, two
- * 32-deep halves of a step so that every 128-byte line is used whole, and two
- * turns of two steps are in flight.  The kernel is bound by reading X once;
- * A is read by every row group, from L2. */
-#define HK_LORA_LOW_LDS(RB) (4u * 2u * (RB) * 1024u)
+ * J of 16 rows.  The waves split K (64-deep steps wave, wave + WAVES, ...) and
+ * add their sums in LDS.  A workgroup is bound by the latency of its loads and
+ * by how fast a CU takes them, so two turns of DEEP steps are in flight (about
+ * 190 registers), and a load takes 8 whole 128-byte lines: loaded as fragments
+ * (16 half lines each), 197 rows x 5120 took 13.0 us for 16 ranks and 27 for
+ * 64, and 6144 rows 34 for 64; as whole lines 6.9, 12.3 and 18.5.  The lines
+ * turn into fragments in LDS of the wave's own, with the GEMM's swizzle; a
+ * wave's LDS operations run in order, so one step's room is enough. */
+#define HK_LORA_WAVES 4
 
-template <int RB>
+template <int RB, int J>
+struct hk_lora_low_shape {
+    static constexpr int DEEP = 24 / (2 * (RB + J)); /* steps of a turn */
+    static constexpr uint32_t STEP = (RB + J) * 16u * 128u; /* bytes */
+    /* the waves' lines, or their sums and the rows' adapters */
+    static constexpr uint32_t SUMS = HK_LORA_WAVES * J * RB * 1024u;
+    static constexpr uint32_t LDS =
+        HK_LORA_WAVES * STEP > SUMS + 64u * J ? HK_LORA_WAVES * STEP
+                                              : SUMS + 64u * J;
+};
+
+template <int RB, int J>
 __device__ __forceinline__ void hk_lora_low_unit(const hk_lora_low_args &g,
-                                                 uint32_t group,
+                                                 uint32_t row0,
                                                  uint32_t chunk,
                                                  uint32_t slot,
+                                                 uint32_t piece,
                                                  uint8_t *lds) {
+    constexpr int DEEP = hk_lora_low_shape<RB, J>::DEEP;
+    constexpr uint32_t STEP = hk_lora_low_shape<RB, J>::STEP;
+    constexpr uint32_t WAVES = HK_LORA_WAVES;
+    constexpr uint32_t ROWS = 16u * J;
     const uint32_t tid = threadIdx.x, lane = tid & 63u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t r16 = lane & 15u, quad = lane >> 4;
-    const uint32_t row0 = group * 32u, rank0 = chunk * (16u * RB);
-    const uint32_t steps = g.k / HK_BK;
-    /* lane l of every wave has row l % 32's adapter */
-    uint32_t mine = HK_LORA_NONE;
-    if (row0 + (lane & 31u) < g.m) mine = g.ext.map[row0 + (lane & 31u)];
-    if (mine >= g.ext.count) mine = HK_LORA_NONE;
+    const uint32_t rank0 = chunk * (16u * RB);
+    const uint32_t first_step = piece * g.piece_steps;
+    const uint32_t steps = min(g.piece_steps, g.k / HK_BK - first_step);
+    /* lane l of every wave has row l % ROWS's adapter */
+    uint32_t left = HK_LORA_NONE;
+    if (row0 + (lane & (ROWS - 1u)) < g.m)
+        left = g.ext.map[row0 + (lane & (ROWS - 1u))];
+    if (left >= g.ext.count) left = HK_LORA_NONE;
+    const uint32_t mine = left;
 
+    /* lane l loads chunk l % 8 of row l / 8 of every 8 */
+    const uint32_t line = lane >> 3, chunk_off = (lane & 7u) * 16u;
     const __amdgpu_buffer_rsrc_t xr = hk_rsrc(g.x, g.x_bytes);
-    uint32_t x_off[2];
+    uint32_t x_off[2 * J];
 #pragma unroll
-    for (int j = 0; j < 2; j++)
-        x_off[j] = min(row0 + j * 16u + r16, g.m) * g.k * 2u + quad * 16u;
+    for (int j = 0; j < 2 * J; j++)
+        x_off[j] = min(row0 + j * 8u + line, g.m) * g.k * 2u + chunk_off;
+    /* and puts it into the wave's LDS at the swizzled place: A's rows, then
+     * X's; the key of 8 q + line depends on the parity of q */
+    uint8_t *own = lds + wave * STEP;
+    uint32_t put[2], get[2];
+#pragma unroll
+    for (int p = 0; p < 2; p++)
+        put[p] = line * 128u + (((lane & 7u) ^ hk_swz_key(p * 8u + line)) << 4);
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+        get[h] = r16 * 128u + (((h * 4u + quad) ^ hk_swz_key(r16)) << 4);
 
-    uint32_t turn = 0;
-    uint32_t left = mine;
-    for (;;) {
+    for (uint32_t turn = 0;; turn++) {
         uint32_t adapter = left;
 #pragma unroll
-        for (int offset = 16; offset; offset >>= 1)
+        for (int offset = (int)ROWS / 2; offset; offset >>= 1)
             adapter = min(adapter,
                           (uint32_t)__shfl_xor((int)adapter, offset, 64));
         adapter = (uint32_t)__builtin_amdgcn_readfirstlane((int)adapter);
         if (adapter == HK_LORA_NONE) break;
         left = left > adapter ? left : HK_LORA_NONE;
-        const bool taken = turn++ % g.slots == slot;
-        if (!taken) continue;
+        if (turn % g.slots != slot) continue;
         const uint64_t *entry = (const uint64_t *)(g.ext.entries + adapter);
         const uint16_t *down = (const uint16_t *)hk_group_word(entry, 0);
-        const uint64_t sizes = hk_group_word(entry, 2);
-        const uint32_t rank = (uint32_t)sizes;
-        const uint32_t padded = (uint32_t)(sizes >> 32);
-        const float scale =
-            __uint_as_float((uint32_t)hk_group_word(entry, 3));
-        if (rank0 >= padded) continue;
+        const uint32_t rank = (uint32_t)hk_group_word(entry, 2);
+        if (rank0 >= rank) continue;
         /* ranks past the last load, and come out, as zeros */
         const __amdgpu_buffer_rsrc_t ar = hk_rsrc(down, rank * g.k * 2u);
-        uint32_t a_off[RB];
+        uint32_t a_off[2 * RB];
 #pragma unroll
-        for (int i = 0; i < RB; i++)
-            a_off[i] = min(rank0 + i * 16u + r16, rank) * g.k * 2u +
-                       quad * 16u;
+        for (int i = 0; i < 2 * RB; i++)
+            a_off[i] = min(rank0 + i * 8u + line, rank) * g.k * 2u + chunk_off;
 
-        hk_f32x4 acc[RB][2];
+        hk_f32x4 acc[RB][J];
 #pragma unroll
         for (int i = 0; i < RB; i++)
 #pragma unroll
-            for (int j = 0; j < 2; j++) acc[i][j] = hk_f32x4{0, 0, 0, 0};
-        /* a turn: steps 8 t + wave and 8 t + 4 + wave; past the end of K the
-         * lane offset lies beyond the buffers and loads zeros */
-        hk_v4i fx[2][2][2][2], fa[2][2][2][RB];
+            for (int j = 0; j < J; j++) acc[i][j] = hk_f32x4{0, 0, 0, 0};
+        /* turn t: steps (DEEP t + u) WAVES + wave, u < DEEP; past the end of
+         * K the lane offset lies beyond the buffers and loads zeros */
+        hk_v4i lx[2][DEEP][2 * J], la[2][DEEP][2 * RB];
         auto load = [&](int buf, uint32_t t) {
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const uint32_t step = t * 8u + u * 4u + wave;
+            for (int u = 0; u < DEEP; u++) {
+                const uint32_t step = (t * DEEP + u) * WAVES + wave;
                 const bool live = step < steps;
-                const uint32_t kb = live ? step * (HK_BK * 2u) : 0u;
+                const uint32_t kb =
+                    live ? (first_step + step) * (HK_BK * 2u) : 0u;
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
+                for (int j = 0; j < 2 * J; j++)
+                    lx[buf][u][j] = __builtin_amdgcn_raw_buffer_load_b128(
+                        xr, live ? x_off[j] : 0xfffff000u, kb, 0);
 #pragma unroll
-                    for (int j = 0; j < 2; j++)
-                        fx[buf][u][h][j] = __builtin_amdgcn_raw_buffer_load_b128(
-                            xr, live ? x_off[j] + h * 64u : 0xfffff000u, kb,
-                            0);
-#pragma unroll
-                    for (int i = 0; i < RB; i++)
-                        fa[buf][u][h][i] = __builtin_amdgcn_raw_buffer_load_b128(
-                            ar, live ? a_off[i] + h * 64u : 0xfffff000u, kb,
-                            0);
-                }
+                for (int i = 0; i < 2 * RB; i++)
+                    la[buf][u][i] = __builtin_amdgcn_raw_buffer_load_b128(
+                        ar, live ? a_off[i] : 0xfffff000u, kb, 0);
             }
         };
         auto compute = [&](int buf) {
 #pragma unroll
-            for (int u = 0; u < 2; u++)
+            for (int u = 0; u < DEEP; u++) {
 #pragma unroll
-                for (int h = 0; h < 2; h++)
+                for (int i = 0; i < 2 * RB; i++)
+                    *(hk_v4i *)(own + i * 1024 + put[i & 1]) = la[buf][u][i];
+#pragma unroll
+                for (int j = 0; j < 2 * J; j++)
+                    *(hk_v4i *)(own + (2 * RB + j) * 1024 + put[j & 1]) =
+                        lx[buf][u][j];
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    hk_v4i fa[RB], fx[J];
+#pragma unroll
+                    for (int i = 0; i < RB; i++)
+                        fa[i] = *(const hk_v4i *)(own + i * 2048 + get[h]);
+#pragma unroll
+                    for (int j = 0; j < J; j++)
+                        fx[j] = *(const hk_v4i *)(own + (RB + j) * 2048 +
+                                                  get[h]);
 #pragma unroll
                     for (int i = 0; i < RB; i++)
 #pragma unroll
-                        for (int j = 0; j < 2; j++)
+                        for (int j = 0; j < J; j++)
                             acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                                __builtin_bit_cast(hk_bf16x8,
-                                                   fa[buf][u][h][i]),
-                                __builtin_bit_cast(hk_bf16x8,
-                                                   fx[buf][u][h][j]),
+                                __builtin_bit_cast(hk_bf16x8, fa[i]),
+                                __builtin_bit_cast(hk_bf16x8, fx[j]),
                                 acc[i][j], 0, 0, 0);
+                }
+            }
         };
-        const uint32_t turns = (steps + 7u) / 8u;
+        const uint32_t turns = (steps + DEEP * WAVES - 1u) / (DEEP * WAVES);
         load(0, 0);
         for (uint32_t t = 0; t < turns; t += 2u) {
             load(1, t + 1u);
@@ -265,53 +321,151 @@ __device__ __forceinline__ void hk_lora_low_unit(const hk_lora_low_args &g,
          * The waves' sums meet in LDS, [wave][row][rank]; a thread adds up 8
          * ranks of a row. */
         float *sums = (float *)lds;
+        uint32_t *has_of =
+            (uint32_t *)(lds + hk_lora_low_shape<RB, J>::SUMS);
+        __syncthreads(); /* the sums lie where other waves had their lines */
+        if (tid < ROWS) has_of[tid] = mine; /* rows' adapters, none past m */
 #pragma unroll
         for (int i = 0; i < RB; i++)
 #pragma unroll
-            for (int j = 0; j < 2; j++)
-                *(hk_f32x4 *)(sums + ((wave * 32u + j * 16u + r16) * RB + i) *
+            for (int j = 0; j < J; j++)
+                *(hk_f32x4 *)(sums + ((wave * ROWS + j * 16u + r16) * RB + i) *
                                          16u + quad * 4u) = acc[i][j];
         __syncthreads();
-        if (tid < 64u * RB) {
-            const uint32_t row = tid / (2u * RB), part = tid % (2u * RB);
-            float u[8] = {};
+        for (uint32_t at = tid; at < ROWS * 2u * RB; at += WAVES * 64u) {
+            const uint32_t row = at / (2u * RB), part = at % (2u * RB);
+            if (has_of[row] != adapter) continue;
+            hk_f32x4 u[2] = {};
 #pragma unroll
-            for (int w = 0; w < 4; w++)
+            for (int w = 0; w < (int)WAVES; w++)
 #pragma unroll
-                for (int e = 0; e < 8; e++)
-                    u[e] += sums[(w * 32u + row) * (RB * 16u) + part * 8u + e];
-            float low[8];
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                u[e] *= scale;
-                const float high = hk_bf2f(hk_f2bf(u[e]));
-                /* past bf16's range the first half is infinite and stays so */
-                low[e] = fabsf(high) == INFINITY ? 0.0f : u[e] - high;
-            }
+                for (int e = 0; e < 2; e++)
+                    u[e] += *(const hk_f32x4 *)(
+                        sums + (w * ROWS + row) * (RB * 16u) + part * 8u +
+                        e * 4u);
             const uint32_t first = rank0 + part * 8u;
-            if (row0 + row < g.m && g.ext.map[row0 + row] == adapter &&
-                first < padded) {
-                uint16_t *out = (uint16_t *)g.ext.low +
-                                (size_t)(row0 + row) * g.ext.pitch + first;
-                *(uint4 *)out = hk_pack8(u);
-                *(uint4 *)(out + padded) = hk_pack8(low);
-            }
+            if (first >= g.sum_pitch) continue;
+            hk_f32x4 *out = (hk_f32x4 *)(
+                g.sums + ((size_t)piece * g.m + row0 + row) * g.sum_pitch +
+                first);
+            out[0] = u[0];
+            out[1] = u[1];
         }
         __syncthreads();
     }
 }
 
-/* Over 128 rows: a workgroup per (row group, rank chunk).  The chunks of a row
- * group read the same X, so they go to one XCD: workgroups are dealt to the 8
- * XCDs in turn. */
-template <int RB>
-__global__ void __launch_bounds__(256, 2) hk_lora_low(hk_lora_low_args g) {
-    __shared__ __attribute__((aligned(16))) uint8_t lds[HK_LORA_LOW_LDS(RB)];
+/* Over 128 rows: a workgroup per (row group, rank chunk, piece of K).  The
+ * chunks of a row group read the same X, so they go to one XCD: workgroups are
+ * dealt to the 8 XCDs in turn. */
+template <int RB, int J>
+__global__ void __launch_bounds__(HK_LORA_WAVES * 64, 2)
+hk_lora_low(hk_lora_low_args g) {
+    __shared__ __attribute__((aligned(16)))
+    uint8_t lds[hk_lora_low_shape<RB, J>::LDS];
     const uint32_t eight = blockIdx.x / (8u * g.chunks);
     const uint32_t in = blockIdx.x - eight * 8u * g.chunks;
-    const uint32_t group = eight * 8u + (in & 7u);
-    if (group < g.row_groups)
-        hk_lora_low_unit<RB>(g, group, in >> 3, 0, lds);
+    const uint32_t at = eight * 8u + (in & 7u);
+    const uint32_t group = at % g.row_groups, piece = at / g.row_groups;
+    if (piece < g.pieces)
+        hk_lora_low_unit<RB, J>(g, group * 16u * J, in >> 3, 0, piece, lds);
+}
+
+/* 8 ranks of a row: the sums of K's pieces, four on their way at a time. */
+__device__ __forceinline__ void hk_lora_add_up(const float *sums,
+                                               size_t stride, uint32_t pieces,
+                                               hk_f32x4 (&u)[2]) {
+    u[0] = u[1] = hk_f32x4{0, 0, 0, 0};
+    for (uint32_t first = 0; first < pieces; first += 4u) {
+        hk_f32x4 v[4][2] = {};
+#pragma unroll
+        for (uint32_t p = 0; p < 4; p++)
+            if (first + p < pieces) {
+                v[p][0] = *(const hk_f32x4 *)(sums + (first + p) * stride);
+                v[p][1] = *(const hk_f32x4 *)(sums + (first + p) * stride + 4);
+            }
+#pragma unroll
+        for (uint32_t p = 0; p < 4; p++) {
+            u[0] += v[p][0];
+            u[1] += v[p][1];
+        }
+    }
+}
+
+/* The sums times the scale, as bf16 halves. */
+__device__ __forceinline__ void hk_lora_split(const hk_f32x4 (&u)[2],
+                                              float scale, uint4 &high,
+                                              uint4 &rest) {
+    float v[8], low[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        v[e] = scale * u[e >> 2][e & 3];
+        const float h = hk_bf2f(hk_f2bf(v[e]));
+        /* past bf16's range the first half is infinite and stays so */
+        low[e] = fabsf(h) == INFINITY ? 0.0f : v[e] - h;
+    }
+    high = hk_pack8(v);
+    rest = hk_pack8(low);
+}
+
+/* The halves that the GEMM takes (hk_lora_ext), zeros up to the padded rank:
+ * workgroups [0, units) of 256 threads, a thread 8 ranks of a row.  The others
+ * list the adapters of a row tile each: the least that is left, over and
+ * over. */
+__global__ void __launch_bounds__(256)
+hk_lora_halves(hk_lora_low_args g, uint32_t units, uint32_t tile_rows) {
+    const hk_lora_ext &x = g.ext;
+    const uint32_t tid = threadIdx.x;
+    if (blockIdx.x < units) {
+        const uint32_t eights = x.pitch / 16u;
+        const uint64_t at = (uint64_t)blockIdx.x * 256u + tid;
+        const uint32_t row = (uint32_t)(at / eights);
+        const uint32_t first = (uint32_t)(at - (uint64_t)row * eights) * 8u;
+        if (row >= g.m) return;
+        const uint32_t a = x.map[row];
+        if (a >= x.count) return;
+        const hk_lora_entry e = x.entries[a];
+        if (first >= e.padded) return;
+        uint4 high = make_uint4(0, 0, 0, 0), rest = high;
+        if (first < e.rank) {
+            hk_f32x4 u[2];
+            hk_lora_add_up(g.sums + (size_t)row * g.sum_pitch + first,
+                           (size_t)g.m * g.sum_pitch, g.pieces, u);
+            hk_lora_split(u, e.scale, high, rest);
+        }
+        uint16_t *out = (uint16_t *)x.low + (size_t)row * x.pitch + first;
+        *(uint4 *)out = high;
+        *(uint4 *)(out + e.padded) = rest;
+        return;
+    }
+    __shared__ uint32_t words[4];
+    const uint32_t tile = blockIdx.x - units, row = tile * tile_rows + tid;
+    uint32_t left = HK_LORA_NONE;
+    if (tid < tile_rows && row < g.m) left = x.map[row];
+    if (left >= x.count) left = HK_LORA_NONE;
+    uint32_t count = 0, listed = HK_LORA_NONE;
+    for (;;) {
+        uint32_t value = left;
+#pragma unroll
+        for (int offset = 32; offset; offset >>= 1)
+            value = min(value, (uint32_t)__shfl_xor((int)value, offset, 64));
+        __syncthreads(); /* the words of the turn before have been read */
+        if ((tid & 63u) == 0) words[tid >> 6] = value;
+        __syncthreads();
+        value = min(min(words[0], words[1]), min(words[2], words[3]));
+        if (value == HK_LORA_NONE) break;
+        if (tid == count) listed = value;
+        count++;
+        if (left == value) left = HK_LORA_NONE;
+    }
+    uint4 entry = make_uint4(listed, 0, 0, 0);
+    if (listed != HK_LORA_NONE) {
+        const hk_lora_entry e = x.entries[listed];
+        const uint64_t up = (uint64_t)(uintptr_t)e.up;
+        entry = make_uint4(listed, 2u * e.padded, (uint32_t)up,
+                           (uint32_t)(up >> 32));
+    }
+    x.lists[(size_t)tile * 256u + tid] = entry;
 }
 
 /* The GEMM with adapters; trace points are hk_gemm.hip's alone. */
@@ -349,9 +503,9 @@ static hk_gemm_lora_kernel hk_gemm_lora_pick_epi(int epilogue, uint32_t jb) {
                                       : hk_gemm_lora_pick<HK_EPI_STORE>(jb);
 }
 
-/* the GEMM's LDS, then the rows' adapters and hk_lora_least's words */
+/* the GEMM's LDS, then a tile's adapters by row and its list */
 static uint32_t hk_gemm_lora_lds(uint32_t jb) {
-    return hk_gemm_lds(jb) + 1024u + 32u;
+    return hk_gemm_lds(jb) + 1024u + 4096u;
 }
 
 void hk_gemm_lora_launch(struct h3_gpu *gpu, int epilogue, uint32_t jb,
@@ -380,113 +534,145 @@ void hk_gemm_lora_launch(struct h3_gpu *gpu, int epilogue, uint32_t jb,
  * first product share one launch: the former stream W for the whole launch,
  * the latter end under them.  The former always leave F32 pieces, which
  * hk_lora_join adds up with the adapters' second product. */
-template <int MB, int XA>
-__global__ void __launch_bounds__(256)
+template <int MB, int J>
+__global__ void __launch_bounds__(256, 2)
 hk_lora_skinny(hk_skinny_args s, hk_lora_low_args g, uint32_t columns,
-               uint32_t pieces, uint32_t units) {
+               uint32_t pieces) {
     extern __shared__ __attribute__((aligned(16))) uint8_t hk_xs[];
-    if (blockIdx.x < units) {
+    if (blockIdx.x < g.units) {
         uint32_t unit = blockIdx.x;
+        const uint32_t piece = unit % g.pieces;
+        unit /= g.pieces;
         const uint32_t chunk = unit % g.chunks;
         unit /= g.chunks;
-        hk_lora_low_unit<1>(g, unit % g.row_groups, chunk,
-                            unit / g.row_groups, hk_xs);
+        const uint32_t group = unit % g.row_groups;
+        hk_lora_low_unit<1, J>(g, group * 16u * J, chunk,
+                               unit / g.row_groups, piece, hk_xs);
+    } else if (blockIdx.x == g.units) {
+        if (threadIdx.x >= g.m) return;
+        const uint32_t a = g.ext.map[threadIdx.x];
+        hk_lora_row r = {};
+        r.adapter = HK_LORA_NONE;
+        if (a < g.ext.count) {
+            const hk_lora_entry e = g.ext.entries[a];
+            r.fragments = e.fragments;
+            r.rank = e.rank;
+            r.scale = e.scale;
+            r.adapter = a;
+        }
+        g.rows[threadIdx.x] = r;
     } else {
-        const uint32_t at = blockIdx.x - units;
-        hk_skinny_tile<MB, XA>(s, at % columns, at / columns, 0, columns,
-                               pieces);
+        const uint32_t at = blockIdx.x - g.units - 1u;
+        hk_skinny_tile<MB, 3>(s, at % columns, at / columns, 0, columns,
+                              pieces);
     }
 }
 
-/* C = act(pieces' sums + bias + low . B^T) for 32 columns and 32 rows: wave w
- * takes pieces w, w + 4, ... and the rows' adapters w, w + 4, ..., so that
- * their loads overlap, and the four waves' sums meet in LDS.  32x32x16 MFMAs
- * with B's rows against the rows of `low`, in the layout of the pieces
- * (hk_gemm_skinny). */
-__global__ void __launch_bounds__(256)
-hk_lora_join(hk_skinny_args g, hk_lora_ext lora, uint32_t mbs, uint32_t tiles,
-             uint32_t pieces, int gelu) {
-    __shared__ hk_f32x4 lds[4][4][64];
-    const uint32_t tid = threadIdx.x, lane = tid & 63u;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+/* C = act(pieces' sums + bias + s_a (x . A^T) . B^T) for 32 columns and 32
+ * rows, a wave: lane l has row l % 32 and its adapter, so that what an adapter
+ * takes in turn is B alone: 32x32x16 MFMAs of B's rows against the rows'
+ * halves, zeros in rows of others, onto the pieces' sums (the layout of
+ * hk_gemm_skinny's).  A wave waits for two loads in sequence, its row and B;
+ * the first 16 ranks' products are on their way with the row, and the next B
+ * while one is multiplied. */
+__global__ void __launch_bounds__(64)
+hk_lora_join(hk_skinny_args s, hk_lora_low_args g, uint32_t mbs,
+             uint32_t tiles, uint32_t pieces, int gelu) {
+    const uint32_t lane = threadIdx.x, half = lane >> 5;
     const uint32_t tile = blockIdx.x / mbs, mb = blockIdx.x % mbs;
-    const uint32_t row = mb * 32u + (lane & 31u), half = lane >> 5;
-    const uint32_t n0 = tile * 32u;
+    const uint32_t row = mb * 32u + (lane & 31u), n0 = tile * 32u;
+    const bool live = row < s.m;
+    const size_t low_stride = (size_t)s.m * g.sum_pitch;
+    const float *low = g.sums + (size_t)row * g.sum_pitch + half * 8u;
+    hk_lora_row mine = {};
+    hk_f32x4 u[2] = {};
     hk_f32x16 acc;
 #pragma unroll
     for (int r = 0; r < 16; r++) acc[r] = 0.0f;
-    const size_t stride = (size_t)tiles * mbs * 256u;
-    const hk_f32x4 *p =
-        (const hk_f32x4 *)g.partial + (size_t)blockIdx.x * 256u + lane;
-    if (row < g.m && n0 < g.n)
-        for (uint32_t s = wave; s < pieces; s += 4u)
+    if (live) {
+        mine = g.rows[row];
+        /* (what a row without an adapter reads here is not used) */
+        if (g.sum_pitch) hk_lora_add_up(low, low_stride, g.pieces, u);
+        const size_t stride = (size_t)tiles * mbs * 256u;
+        const hk_f32x4 *p =
+            (const hk_f32x4 *)s.partial + (size_t)blockIdx.x * 256u + lane;
+        for (uint32_t i = 0; i < pieces; i++)
 #pragma unroll
             for (int q = 0; q < 4; q++) {
-                const hk_f32x4 v = p[s * stride + q * 64u];
+                const hk_f32x4 v = p[i * stride + q * 64u];
 #pragma unroll
                 for (int e = 0; e < 4; e++) acc[q * 4 + e] += v[e];
             }
-    uint32_t left = HK_LORA_NONE;
-    if (row < g.m) left = lora.map[row];
-    if (left >= lora.count) left = HK_LORA_NONE;
-    const uint32_t mine = left;
-    for (uint32_t turn = 0;; turn++) {
-        uint32_t adapter = left;
-#pragma unroll
-        for (int offset = 16; offset; offset >>= 1)
-            adapter = min(adapter,
-                          (uint32_t)__shfl_xor((int)adapter, offset, 64));
-        adapter = (uint32_t)__builtin_amdgcn_readfirstlane((int)adapter);
-        if (adapter == HK_LORA_NONE) break;
-        left = left > adapter ? left : HK_LORA_NONE;
-        if ((turn & 3u) != wave) continue;
-        const uint64_t *entry = (const uint64_t *)(lora.entries + adapter);
-        const uint16_t *up = (const uint16_t *)hk_group_word(entry, 1);
-        const uint64_t sizes = hk_group_word(entry, 2);
-        const uint32_t rank = (uint32_t)sizes;
-        const uint32_t padded = (uint32_t)(sizes >> 32);
-        const uint32_t col = n0 + (lane & 31u);
-        const uint16_t *low = lora.low + (size_t)row * lora.pitch;
-        for (uint32_t k = half * 8u; k - half * 8u < rank; k += 16u) {
-            hk_v4i b = {0, 0, 0, 0}, high = {0, 0, 0, 0}, rest = {0, 0, 0, 0};
-            if (col < g.n)
-                b = *(const hk_v4i *)(up + (size_t)col * 2u * padded + k);
-            if (mine == adapter) {
-                high = *(const hk_v4i *)(low + k);
-                rest = *(const hk_v4i *)(low + padded + k);
-            }
+    }
+    for (uint32_t k = 0;; k += 16u) {
+        /* rows with ranks from k on */
+        bool left = k < mine.rank;
+        if (!__builtin_amdgcn_ballot_w64(left)) break;
+        uint4 high = make_uint4(0, 0, 0, 0), rest = high;
+        if (left) {
+            if (k) hk_lora_add_up(low + k, low_stride, g.pieces, u);
+            hk_lora_split(u, mine.scale, high, rest);
+        }
+        uint32_t adapter = HK_LORA_NONE;
+        hk_v4i b = {0, 0, 0, 0};
+        /* the next adapter of the rows that are left, and its B */
+        auto take = [&](uint32_t &which, hk_v4i &into) {
+            const uint64_t with = __builtin_amdgcn_ballot_w64(left);
+            which = HK_LORA_NONE;
+            if (!with) return;
+            const int lead = __builtin_ctzll(with);
+            auto of = [&](uint32_t v) {
+                return (uint32_t)__builtin_amdgcn_readlane((int)v, lead);
+            };
+            which = of(mine.adapter);
+            const uint64_t at = (uint64_t)(uintptr_t)mine.fragments;
+            const hk_v4i *fragments = (const hk_v4i *)(
+                (uint64_t)of((uint32_t)at) |
+                ((uint64_t)of((uint32_t)(at >> 32)) << 32));
+            const uint32_t chunks = (of(mine.rank) + 15u) / 16u;
+            left = left && mine.adapter != which;
+            into = fragments[((size_t)tile * chunks + k / 16u) * 64u + lane];
+        };
+        take(adapter, b);
+        while (adapter != HK_LORA_NONE) {
+            uint32_t next;
+            hk_v4i after = {0, 0, 0, 0};
+            take(next, after);
+            const hk_v4i none = {0, 0, 0, 0};
+            const bool its = mine.adapter == adapter;
+            const hk_v4i h = its ? __builtin_bit_cast(hk_v4i, high) : none;
+            const hk_v4i r = its ? __builtin_bit_cast(hk_v4i, rest) : none;
             acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
                 __builtin_bit_cast(hk_bf16x8, b),
-                __builtin_bit_cast(hk_bf16x8, high), acc, 0, 0, 0);
+                __builtin_bit_cast(hk_bf16x8, h), acc, 0, 0, 0);
             acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
                 __builtin_bit_cast(hk_bf16x8, b),
-                __builtin_bit_cast(hk_bf16x8, rest), acc, 0, 0, 0);
+                __builtin_bit_cast(hk_bf16x8, r), acc, 0, 0, 0);
+            adapter = next;
+            b = after;
         }
     }
+    if (!live) return;
 #pragma unroll
-    for (int q = 0; q < 4; q++)
-        lds[wave][q][lane] = hk_f32x4{acc[q * 4], acc[q * 4 + 1],
-                                      acc[q * 4 + 2], acc[q * 4 + 3]};
-    __syncthreads();
-    /* thread (q, lane): row as above, columns 8 q + 4 half .. + 4 */
-    const uint32_t q = wave, col = n0 + q * 8u + half * 4u;
-    if (row >= g.m || col >= g.n) return;
-    hk_f32x4 sum = lds[0][q][lane];
+    for (int q = 0; q < 4; q++) {
+        const uint32_t c = n0 + q * 8u + half * 4u;
+        if (c >= s.n) continue;
+        float out[4] = {acc[q * 4], acc[q * 4 + 1], acc[q * 4 + 2],
+                        acc[q * 4 + 3]};
+        if (s.bias) {
+            const uint2 bias = *(const uint2 *)(s.bias + c);
+            out[0] += hk_bf2f(bias.x & 0xffffu);
+            out[1] += hk_bf2f(bias.x >> 16);
+            out[2] += hk_bf2f(bias.y & 0xffffu);
+            out[3] += hk_bf2f(bias.y >> 16);
+        }
+        if (gelu)
 #pragma unroll
-    for (int w = 1; w < 4; w++) sum += lds[w][q][lane];
-    if (g.bias) {
-        const uint2 b = *(const uint2 *)(g.bias + col);
-        sum[0] += hk_bf2f(b.x & 0xffffu);
-        sum[1] += hk_bf2f(b.x >> 16);
-        sum[2] += hk_bf2f(b.y & 0xffffu);
-        sum[3] += hk_bf2f(b.y >> 16);
+            for (int i = 0; i < 4; i++)
+                out[i] = hk_gelu_tanh_f(hk_bf2f(hk_f2bf(out[i])));
+        *(uint2 *)(s.c + (size_t)row * s.n + c) =
+            make_uint2(hk_pack2(out[0], out[1]), hk_pack2(out[2], out[3]));
     }
-    if (gelu)
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-            sum[e] = hk_gelu_tanh_f(hk_bf2f(hk_f2bf(sum[e])));
-    *(uint2 *)(g.c + (size_t)row * g.n + col) =
-        make_uint2(hk_pack2(sum[0], sum[1]), hk_pack2(sum[2], sum[3]));
 }
 
 /* Whether the matrix-core kernels take the call: what the GEMM takes, and the
@@ -501,7 +687,37 @@ static bool hk_lora_takes(const struct h3_gpu *gpu, const hk_lora_args &g) {
            a + 2ull * g.k < most && b < most && low < most;
 }
 
+/* How the first product runs over 128 rows: 16 J rows a workgroup, K in
+ * `pieces`.  A workgroup takes about 4 us and 20 KB a us of X's and A's rows;
+ * two share a CU. */
+struct hk_lora_plan {
+    uint32_t j, pieces, steps;
+};
+
+static hk_lora_plan hk_lora_plan_of(uint32_t m, uint32_t k_steps, uint32_t rb,
+                                    uint32_t chunks, uint32_t cus) {
+    hk_lora_plan best = {2, 1, k_steps};
+    float least = INFINITY;
+    for (uint32_t j = 2; j <= 4; j += 2)
+        for (uint32_t p = 1; p <= 16 && p <= k_steps; p++) {
+            const uint32_t steps = (k_steps + p - 1) / p;
+            const uint32_t pieces = (k_steps + steps - 1) / steps;
+            const uint32_t wgs = (m + 16 * j - 1) / (16 * j) * chunks * pieces;
+            const float kb = (float)(steps * (j + rb)) * 2.0f;
+            const float us = (float)((wgs + 2 * cus - 1) / (2 * cus)) *
+                             (4.0f + kb / 20.0f);
+            if (us < least) {
+                least = us;
+                best = {j, pieces, steps};
+            }
+        }
+    return best;
+}
+
 static int hk_lora_run(struct h3_gpu *gpu, const hk_lora_args &a) {
+    const uint32_t cus = gpu->num_cus > 0 ? (uint32_t)gpu->num_cus : 256u;
+    const uint32_t k_steps = a.k / HK_BK;
+    const bool tall = a.m > 128u;
     hk_lora_low_args g = {};
     g.x = a.x;
     g.m = a.m; g.k = a.k;
@@ -510,29 +726,71 @@ static int hk_lora_run(struct h3_gpu *gpu, const hk_lora_args &a) {
     g.ext.count = a.count;
     g.ext.map = a.map;
     g.ext.pitch = 2u * a.pitch;
-    g.ext.low_bytes = (uint32_t)((uint64_t)a.m * a.pitch * 4);
-    uint16_t *low = (uint16_t *)hk_workspace(gpu, g.ext.low_bytes);
-    if (!low) return 0;
-    g.ext.low = low;
-    g.row_groups = (a.m + 31u) / 32u;
+    g.ext.low_bytes = tall ? (uint32_t)((uint64_t)a.m * a.pitch * 4) : 0u;
+    g.sum_pitch = (a.rank + 15u) & ~15u;
     g.slots = 1;
-    if (a.m > 128u) {
-        const uint32_t rb = a.pitch <= 16 ? 1 : a.pitch <= 32 ? 2 : 4;
-        g.chunks = (a.pitch + 16u * rb - 1) / (16u * rb);
-        if (a.pitch) {
-            const uint32_t grid = (g.row_groups + 7u) / 8u * 8u * g.chunks;
-            hipLaunchKernelGGL(rb == 1   ? hk_lora_low<1>
-                               : rb == 2 ? hk_lora_low<2>
-                                         : hk_lora_low<4>,
-                               dim3(grid), dim3(256), 0, gpu->stream, g);
-        }
+    uint32_t rb = 1;
+    if (tall) {
+        rb = a.rank <= 16 ? 1 : a.rank <= 32 ? 2 : 4;
+        g.chunks = (a.rank + 16u * rb - 1) / (16u * rb);
+        const hk_lora_plan plan =
+            hk_lora_plan_of(a.m, k_steps, rb, g.chunks, cus);
+        g.pieces = plan.pieces;
+        g.piece_steps = plan.steps;
+        g.row_groups = (a.m + 16u * plan.j - 1) / (16u * plan.j);
+        rb |= plan.j << 8;
+    } else {
+        /* beside W's stream: a quarter of K each, while the pieces stay few
+         * against what the join reads for every 32 columns */
+        g.chunks = g.sum_pitch / 16u;
+        const uint32_t group = a.m <= 16u ? 16u : 32u;
+        g.row_groups = (a.m + group - 1u) / group;
+        g.slots = a.count < group ? a.count : group;
+        g.piece_steps = (k_steps + 3u) / 4u;
+        g.pieces = (k_steps + g.piece_steps - 1) / g.piece_steps;
+        g.units = g.row_groups * g.chunks * g.slots * g.pieces;
+    }
+    /* the tiles' lists (at most one for every 128 rows) or the rows' adapters,
+     * the halves, the sums of K's pieces */
+    const size_t list_bytes =
+        tall ? ((size_t)a.m + 127) / 128 * 256 * sizeof(uint4)
+             : 128 * sizeof(hk_lora_row);
+    const size_t low_bytes = ((size_t)g.ext.low_bytes + 255) & ~(size_t)255;
+    const size_t sum_bytes =
+        (size_t)g.pieces * a.m * g.sum_pitch * sizeof(float);
+    uint8_t *space =
+        (uint8_t *)hk_workspace(gpu, list_bytes + low_bytes + sum_bytes);
+    if (!space) return 0;
+    g.ext.lists = (uint4 *)space;
+    g.rows = (hk_lora_row *)space;
+    g.ext.low = (const uint16_t *)(space + list_bytes);
+    g.sums = (float *)(space + list_bytes + low_bytes);
+
+    if (tall) {
+        void (*kernel)(hk_lora_low_args) =
+            rb == 0x201   ? hk_lora_low<1, 2>
+            : rb == 0x202 ? hk_lora_low<2, 2>
+            : rb == 0x204 ? hk_lora_low<4, 2>
+            : rb == 0x401 ? hk_lora_low<1, 4>
+            : rb == 0x402 ? hk_lora_low<2, 4>
+                          : hk_lora_low<4, 4>;
+        if (g.chunks)
+            hipLaunchKernelGGL(
+                kernel,
+                dim3((g.row_groups * g.pieces + 7u) / 8u * 8u * g.chunks),
+                dim3(HK_LORA_WAVES * 64), 0, gpu->stream, g);
+        const uint32_t tile_rows = hk_gemm_tile_rows(gpu, a.m, a.n, a.k);
+        const uint32_t units =
+            (uint32_t)(((uint64_t)a.m * (a.pitch / 8u) + 255) / 256);
+        hipLaunchKernelGGL(hk_lora_halves,
+                           dim3(units + (a.m + tile_rows - 1) / tile_rows),
+                           dim3(256), 0, gpu->stream, g, units, tile_rows);
         return hk_gemm_bf16(gpu, a.x, a.w, a.bias, a.c, a.m, a.n, a.k,
                             a.gelu ? HK_EPI_GELU : HK_EPI_STORE, NULL, 0,
                             &g.ext);
     }
-    const uint32_t mbs = g.row_groups, columns = (a.n + 127u) / 128u;
-    const uint32_t k_steps = a.k / HK_BK;
-    const uint32_t cus = gpu->num_cus > 0 ? (uint32_t)gpu->num_cus : 256u;
+
+    const uint32_t mbs = (a.m + 31u) / 32u, columns = (a.n + 127u) / 128u;
     hk_skinny_args s = {};
     s.x = a.x; s.w = a.w; s.bias = a.bias; s.c = a.c;
     s.m = a.m; s.n = a.n; s.k = a.k;
@@ -550,30 +808,32 @@ static int hk_lora_run(struct h3_gpu *gpu, const hk_lora_args &a) {
     s.partial = (float *)hk_splitk_space(
         gpu, (size_t)pieces * columns * 4 * mbs * 4096);
     if (!s.partial) return 0;
-    g.chunks = (a.pitch + 15u) / 16u;
-    /* a row group has at most 32 adapters */
-    g.slots = a.count < 32u ? a.count : 32u;
-    const uint32_t units = g.row_groups * g.chunks * g.slots;
     const size_t lds = mbs * 4096 * 4 + 16384;
-    void (*kernel)(hk_skinny_args, hk_lora_low_args, uint32_t, uint32_t,
-                   uint32_t) = mbs == 1   ? hk_lora_skinny<1, 3>
-                               : mbs == 2 ? hk_lora_skinny<2, 3>
-                               : mbs == 3 ? hk_lora_skinny<3, 3>
-                                          : hk_lora_skinny<4, 3>;
+    void (*kernel)(hk_skinny_args, hk_lora_low_args, uint32_t, uint32_t) =
+        a.m <= 16  ? hk_lora_skinny<1, 1>
+        : mbs == 1 ? hk_lora_skinny<1, 2>
+        : mbs == 2 ? hk_lora_skinny<2, 2>
+        : mbs == 3 ? hk_lora_skinny<3, 2>
+                   : hk_lora_skinny<4, 2>;
+    /* devices (bit = ordinal) whose kernel has its LDS limit raised */
     static uint64_t ready = 0;
     const uint64_t bit = 1ull << (gpu->device & 63);
     if (mbs == 4 && !(ready & bit)) {
-        (void)hipFuncSetAttribute((const void *)hk_lora_skinny<4, 3>,
+        (void)hipFuncSetAttribute((const void *)hk_lora_skinny<4, 2>,
                                   hipFuncAttributeMaxDynamicSharedMemorySize,
                                   (int)lds);
         ready |= bit;
     }
-    hipLaunchKernelGGL(kernel, dim3(units + columns * pieces), dim3(256), lds,
-                       gpu->stream, s, g, columns, pieces, units);
-    hipLaunchKernelGGL(hk_lora_join, dim3((a.n + 31) / 32 * mbs), dim3(256), 0,
-                       gpu->stream, s, g.ext, mbs, columns * 4, pieces,
-                       a.gelu);
+    hipLaunchKernelGGL(kernel, dim3(g.units + 1 + columns * pieces), dim3(256),
+                       lds, gpu->stream, s, g, columns, pieces);
+    hipLaunchKernelGGL(hk_lora_join, dim3((a.n + 31) / 32 * mbs), dim3(64), 0,
+                       gpu->stream, s, g, mbs, columns * 4, pieces, a.gelu);
     return 1;
+}
+
+/* elements of an adapter's fragments, a multiple of 512 */
+static size_t hk_lora_fragment_count(uint32_t n, uint32_t rank) {
+    return ((size_t)n + 31) / 32 * ((rank + 15) / 16) * 512;
 }
 
 extern "C" {
@@ -594,7 +854,7 @@ h3_gpu_tensor *h3_hip_lora_table(h3_gpu *gpu,
     const size_t head = ((size_t)count * sizeof(hk_lora_entry) + 255) &
                         ~(size_t)255;
     size_t bytes = head;
-    uint32_t largest = 0;
+    uint32_t largest = 0, largest_rank = 0;
     for (uint32_t a = 0; a < count; a++) {
         if (ranks[a] > HK_LORA_MAX_RANK) {
             hk_fail(gpu, "adapter %u: rank %u is over %u", a, ranks[a],
@@ -613,9 +873,11 @@ h3_gpu_tensor *h3_hip_lora_table(h3_gpu *gpu,
             return NULL;
         const uint32_t padded = (ranks[a] + 31u) & ~31u;
         if (padded > largest) largest = padded;
+        if (ranks[a] > largest_rank) largest_rank = ranks[a];
         bytes += ((size_t)ranks[a] * input_dim * 2 + 255) & ~(size_t)255;
         bytes += (size_t)padded * output_dim * 4;
         bytes = (bytes + 255) & ~(size_t)255;
+        bytes += hk_lora_fragment_count(output_dim, ranks[a]) * 2;
     }
     hk_lora_entry *entries =
         (hk_lora_entry *)calloc(count, sizeof(hk_lora_entry));
@@ -640,6 +902,8 @@ h3_gpu_tensor *h3_hip_lora_table(h3_gpu *gpu,
         at += ((size_t)e.rank * input_dim * 2 + 255) & ~(size_t)255;
         e.up = (const uint16_t *)at;
         at += ((size_t)e.padded * output_dim * 4 + 255) & ~(size_t)255;
+        e.fragments = (const uint16_t *)at;
+        at += hk_lora_fragment_count(output_dim, e.rank) * 2;
     }
     const size_t entry_bytes = (size_t)count * sizeof(hk_lora_entry);
     hipError_t status = hipMemcpyAsync(device, entries, entry_bytes,
@@ -657,6 +921,11 @@ h3_gpu_tensor *h3_hip_lora_table(h3_gpu *gpu,
                            dim3(256), 0, gpu->stream, HK_CBF16(up[a]),
                            (uint16_t *)e.up, e.rank, e.padded, 2u, u,
                            device + a);
+        const uint64_t f = hk_lora_fragment_count(output_dim, e.rank);
+        hipLaunchKernelGGL(hk_lora_pack_fragments,
+                           dim3((unsigned)((f + 255) / 256)), dim3(256), 0,
+                           gpu->stream, HK_CBF16(up[a]),
+                           (uint16_t *)e.fragments, output_dim, e.rank, f);
         status = hipGetLastError();
     }
     if (status == hipSuccess)
@@ -681,6 +950,7 @@ h3_gpu_tensor *h3_hip_lora_table(h3_gpu *gpu,
     table->record.n[HK_LORA_IN] = input_dim;
     table->record.n[HK_LORA_OUT] = output_dim;
     table->record.n[HK_LORA_COUNT] = count;
+    table->record.n[HK_LORA_RANK] = largest_rank;
     table->record.n[HK_LORA_PADDED] = largest;
     return table;
 }
@@ -726,6 +996,7 @@ static int hk_linear_lora(h3_gpu *gpu, h3_gpu_tensor *output,
     g.entries = (const hk_lora_entry *)table->data;
     g.count = table->record.n[HK_LORA_COUNT];
     g.pitch = table->record.n[HK_LORA_PADDED];
+    g.rank = table->record.n[HK_LORA_RANK];
     g.map = HK_CU32(adapter_map);
     g.gelu = gelu;
     const char *name = gelu ? "gemm_lora_gelu" : "gemm_lora";

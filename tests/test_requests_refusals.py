@@ -20,7 +20,7 @@ def call(**more):
     a = dict(y=y, x=x, w=w, b=b, table=table(), ids=ids, rows=rows, k=k, n=n)
     a.update(more)
     ok = gpu.L.h3_hip_linear_lora_bf16(gpu.h, *a.values())
-    made = [l for l in launches() if l[0] != "hk_lora_pack"]
+    made = [l for l in launches() if not l[0].startswith("hk_lora_pack")]
     return ["" if ok else gpu.error(), len(made)]
 """
 
