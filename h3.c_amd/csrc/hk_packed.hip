@@ -24,7 +24,9 @@
 #include <stdlib.h>
 
 #include <algorithm>
+#include <functional>
 #include <new>
+#include <queue>
 #include <type_traits>
 #include <vector>
 
@@ -63,6 +65,7 @@ enum { HK_PACKED_HEADS, HK_PACKED_KV_HEADS, HK_PACKED_DIM,
        HK_PACKED_KV_END,
        HK_PACKED_ITEMS,    /* entries of each list, which follow each other: */
        HK_PACKED_JOINS,    /* requests, items, joins */
+       HK_PACKED_JOIN_ROWS, /* the most virtual rows of a join */
        HK_PACKED_PARTS };
 
 struct hk_packed_args {
@@ -263,20 +266,30 @@ hk_packed_flash(hk_packed_args a) {
     if (n) issue_tile(it.tile, 0);
 
     /* Q fragments, the B operand of S^T = K . Q^T: k-step ks of this lane's
-     * virtual row, dims 16 ks + 8 half .. + 8 */
+     * virtual row, dims 16 ks + 8 half .. + 8.  Offsets from the item's first
+     * row (hk_packed_takes); rows past the request's and dims past the head's
+     * load from beyond the resource, zeros. */
     const uint32_t vrow0 = it.row + wave * 32u, vrow = vrow0 + col;
+    const uint32_t r0 = it.row / a.group;
     hk_bf16x8 qf[NK];
     {
         const uint32_t r = vrow / a.group, g = vrow - r * a.group;
-        const uint16_t *q = a.q + ((uint64_t)it.q_first + r) * a.q_stride +
-                            (uint64_t)(it.kv_head * a.group + g) * a.dim;
+        const __amdgpu_buffer_rsrc_t qr = hk_attn_rsrc(
+            a.q + ((uint64_t)it.q_first + r0) * a.q_stride +
+                (uint64_t)it.kv_head * a.group * a.dim,
+            0x7ffffff0u);
+        const uint32_t off =
+            n && vrow < it.rows ? (r - r0) * (uint32_t)a.q_stride * 2u +
+                                      g * a.dim * 2u + half * 16u
+                                : 0x80000000u;
 #pragma unroll
-        for (int ks = 0; ks < NK; ks++) {
-            hk_v4i x = {0, 0, 0, 0};
-            if (vrow < it.rows && 2u * ks + half < dim_chunks)
-                x = *(const hk_v4i *)(q + ks * 16u + half * 8u);
-            qf[ks] = __builtin_bit_cast(hk_bf16x8, x);
-        }
+        for (int ks = 0; ks < NK; ks++)
+            qf[ks] = __builtin_bit_cast(
+                hk_bf16x8,
+                __builtin_amdgcn_raw_buffer_load_b128(
+                    qr,
+                    2u * ks + half < dim_chunks ? off + ks * 32u : 0x80000000u,
+                    0, 0));
     }
 
     const uint32_t lds_base =
@@ -360,9 +373,6 @@ hk_packed_flash(hk_packed_args a) {
                 for (int r = 0; r < 16; r++) {
                     p[r] = __builtin_amdgcn_exp2f(
                         __builtin_fmaf(s[kt][r], a.scale_log2, neg));
-                    /* -inf times a scale of zero is not what a key past the
-                     * end weighs */
-                    if (tail && s[kt][r] == -INFINITY) p[r] = 0.0f;
                     sum += p[r];
                 }
 #pragma unroll
@@ -451,28 +461,26 @@ hk_packed_flash(hk_packed_args a) {
      * rows. */
     const float l = l_part + __shfl_xor(l_part, 32, 64);
     if (it.part != HK_PACKED_WHOLE) {
-        float *pw = (float *)(hk_lds + wave * (32u * 64u * 4u));
+        /* 32 dims at a time, rows of 128 bytes */
+        float *pw = (float *)(hk_lds + wave * (32u * 32u * 4u));
         float *part = a.part_o + (size_t)it.part * HK_PACKED_QB * DP;
 #pragma unroll
-        for (int hd = 0; hd < DP / 64; hd++) {
+        for (int d = 0; d < ND; d++) {
 #pragma unroll
-            for (int dd = 0; dd < 2; dd++)
+            for (int blk = 0; blk < 4; blk++) {
+                const uint32_t c = blk * 2u + half;
+                *(float4 *)(pw + col * 32u + ((c ^ (col & 7u)) << 2)) =
+                    make_float4(o[d][blk * 4 + 0], o[d][blk * 4 + 1],
+                                o[d][blk * 4 + 2], o[d][blk * 4 + 3]);
+            }
 #pragma unroll
-                for (int blk = 0; blk < 4; blk++) {
-                    const int d = 2 * hd + dd;
-                    const uint32_t c = dd * 8u + blk * 2u + half;
-                    *(float4 *)(pw + col * 64u + ((c ^ (col & 15u)) << 2)) =
-                        make_float4(o[d][blk * 4 + 0], o[d][blk * 4 + 1],
-                                    o[d][blk * 4 + 2], o[d][blk * 4 + 3]);
-                }
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const uint32_t r = i * 4u + (lane >> 4), c = lane & 15u;
+            for (int i = 0; i < 4; i++) {
+                const uint32_t r = i * 8u + (lane >> 3), c = lane & 7u;
                 const float4 v =
-                    *(const float4 *)(pw + r * 64u + ((c ^ (r & 15u)) << 2));
+                    *(const float4 *)(pw + r * 32u + ((c ^ (r & 7u)) << 2));
                 if (vrow0 + r < it.rows)
                     *(float4 *)(part + (size_t)(wave * 32u + r) * DP +
-                                hd * 64u + c * 4u) = v;
+                                d * 32u + c * 4u) = v;
             }
         }
         if (half == 0 && vrow < it.rows)
@@ -495,23 +503,30 @@ hk_packed_flash(hk_packed_args a) {
                            hk_pack2(o[d][blk * 4 + 2] * inv,
                                     o[d][blk * 4 + 3] * inv));
         }
+    const __amdgpu_buffer_rsrc_t outr =
+        hk_attn_rsrc(a.o + (((uint64_t)it.q_first + r0) * a.heads +
+                            it.kv_head * a.group) * a.dim,
+                     0x7ffffff0u);
 #pragma unroll
     for (int i = 0; i < 32 * CHUNKS / 64; i++) {
         const uint32_t r = i * (64u / CHUNKS) + lane / CHUNKS;
         const uint32_t c = lane % CHUNKS, vr = vrow0 + r;
-        const uint4 v = *(const uint4 *)(
+        const hk_v4i v = *(const hk_v4i *)(
             ow + r * ROW + ((c ^ hk_packed_k_key<DP>(r)) << 4));
-        if (vr >= it.rows || c >= dim_chunks) continue;
         const uint32_t qr = vr / a.group, g = vr - qr * a.group;
-        *(uint4 *)(a.o +
-                   (((uint64_t)it.q_first + qr) * a.heads +
-                    it.kv_head * a.group + g) * a.dim + c * 8u) = v;
+        __builtin_amdgcn_raw_buffer_store_b128(
+            v, outr,
+            vr < it.rows && c < dim_chunks
+                ? (((qr - r0) * a.heads + g) * a.dim + c * 8u) * 2u
+                : 0x80000000u,
+            0, 0);
     }
 }
 
 /* Joins the pieces of an item's rows: with the pieces' maxima m_p, sums l_p
  * and undivided O_p, O = sum_p 2^(m_p - M) O_p / sum_p 2^(m_p - M) l_p, M =
- * max_p m_p, in piece order.  A wave per row; a lane holds DP / 64 dims. */
+ * max_p m_p, in piece order.  A wave per row; a lane holds DP / 64 dims and
+ * has four pieces on their way. */
 template <int DP>
 __global__ void __launch_bounds__(256) hk_packed_joined(hk_packed_args a) {
     const hk_packed_join j = a.joins[blockIdx.x];
@@ -519,20 +534,35 @@ __global__ void __launch_bounds__(256) hk_packed_joined(hk_packed_args a) {
     const uint32_t lane = threadIdx.x & 63u, vr = j.row + ql;
     if (vr >= j.rows) return;
     constexpr int PER = DP / 64;
+    typedef float per __attribute__((ext_vector_type(PER)));
     const float2 *ml = a.part_ml + (size_t)j.part * HK_PACKED_QB + ql;
     const float *po = a.part_o + ((size_t)j.part * HK_PACKED_QB + ql) * DP +
                       lane * PER;
+    /* the maximum over all pieces, 64 at a time */
     float top = -INFINITY;
-    for (uint32_t p = 0; p < j.pieces; p++)
+    for (uint32_t p = lane; p < j.pieces; p += 64u)
         top = fmaxf(top, ml[(size_t)p * HK_PACKED_QB].x);
-    float sum[PER] = {}, l = 0.0f;
-    for (uint32_t p = 0; p < j.pieces; p++) {
-        const float2 mine = ml[(size_t)p * HK_PACKED_QB];
-        const float w = __builtin_amdgcn_exp2f(mine.x - top);
-        l += w * mine.y;
+    top = hk_wave_max(top);
+    per sum = {};
+    float l = 0.0f;
+    for (uint32_t first = 0; first < j.pieces; first += 4u) {
+        float2 mine[4];
+        per op[4];
 #pragma unroll
-        for (int e = 0; e < PER; e++)
-            sum[e] += w * po[(size_t)p * HK_PACKED_QB * DP + e];
+        for (uint32_t p = 0; p < 4; p++) {
+            const size_t at =
+                (size_t)min(first + p, j.pieces - 1u) * HK_PACKED_QB;
+            mine[p] = ml[at];
+            op[p] = *(const per *)(po + at * DP);
+        }
+#pragma unroll
+        for (uint32_t p = 0; p < 4; p++) {
+            const float w = first + p < j.pieces
+                                ? __builtin_amdgcn_exp2f(mine[p].x - top)
+                                : 0.0f;
+            l += first + p < j.pieces ? w * mine[p].y : 0.0f;
+            sum += first + p < j.pieces ? op[p] * w : per{};
+        }
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     const uint32_t qr = vr / a.group, g = vr - qr * a.group;
@@ -545,113 +575,167 @@ __global__ void __launch_bounds__(256) hk_packed_joined(hk_packed_args a) {
 
 template <int DP>
 static void hk_packed_launch(struct h3_gpu *gpu, const hk_packed_args &a,
-                             uint32_t items, uint32_t joins) {
+                             const uint32_t *n) {
     constexpr uint32_t lds = 2u * 2u * HK_KT * DP * 2u;
-    hipLaunchKernelGGL(hk_packed_flash<DP>, dim3(items),
+    hipLaunchKernelGGL(hk_packed_flash<DP>, dim3(n[HK_PACKED_ITEMS]),
                        dim3(HK_PACKED_WAVES * 64u), lds, gpu->stream, a);
-    if (joins)
+    if (n[HK_PACKED_JOINS])
         hipLaunchKernelGGL(hk_packed_joined<DP>,
-                           dim3(joins, HK_PACKED_QB / 4u), dim3(256), 0,
-                           gpu->stream, a);
+                           dim3(n[HK_PACKED_JOINS],
+                                (n[HK_PACKED_JOIN_ROWS] + 3u) / 4u),
+                           dim3(256), 0, gpu->stream, a);
 }
 
-/* Whether the matrix-core kernel takes these rows: whole 16-byte pieces, and
- * 64 key rows below 2^31 bytes, the reach of a tile's lane offsets. */
+/* Whether the matrix-core kernel takes these rows: whole 16-byte pieces, 64
+ * key rows and 128 query and output rows below 2^31 bytes (the reach of lane
+ * offsets), and a scale that -inf times it is -inf, what keys past the end are
+ * set to. */
 static bool hk_packed_takes(const struct h3_gpu *gpu,
                             const hk_packed_args &a) {
     return !gpu->reference_kernels && a.dim % 8u == 0 && a.dim <= 128u &&
            a.q_stride % 8u == 0 && a.kv_stride % 8u == 0 &&
-           a.kv_stride < (1u << 24) &&
+           a.kv_stride < (1u << 24) && a.q_stride < (1u << 23) &&
+           (uint64_t)a.heads * a.dim < (1u << 23) && a.scale_log2 > 0x1p-100f &&
            (((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v |
              (uintptr_t)a.o) & 15u) == 0;
 }
 
-/* How a plan's items are dealt out.  An item costs its key tiles and about
- * three tiles' time for its start and end.  Where the longest item takes
- * longer than an even share of all work (two workgroups a CU), items are cut
- * into pieces of about that share.
+/* How a plan's items are dealt out.  An item costs its key tiles and, for its
+ * start and end, about three tiles' time (`own`).
  *
- * Workgroups go to the 8 XCDs in turn.  The items of one request and key head
- * share K and V, so they go to one XCD's queue (in runs of at most 1/64 of
- * all work, so that the queues come out level), longest first; items of no
- * rows fill the shorter queues. */
+ * Workgroups go to the 8 XCDs in turn.  A request's items, head by head, go to
+ * the XCDs' queues in 8 even runs, so that items that share K and V mostly
+ * share an L2 and every XCD has its part of the long and of the short ones (a
+ * run to the least filled queue each time: 512 items of equal length dealt out
+ * less evenly took a second round, 50 us for 43).  Longest first; items of no
+ * rows fill the shorter queues.
+ *
+ * Where items are few and long, they are cut into pieces of at most `most`
+ * tiles: the length with which the last of the CUs' places (two workgroups a
+ * CU) ends first, each taking the next item when it is free, with 8 tiles'
+ * time for the join. */
 struct hk_packed_work {
     std::vector<hk_packed_item> items;
     std::vector<hk_packed_join> joins;
-    uint32_t parts;
+    uint32_t parts, join_rows;
 };
+
+struct hk_packed_sized {
+    uint32_t request, tiles, rows, blocks;
+};
+
+static const float hk_packed_own = 3.0f;
+
+/* The pieces of an item of `tiles` tiles, and each one's length. */
+static uint32_t hk_packed_pieces(uint32_t tiles, uint32_t most,
+                                 uint32_t &per) {
+    uint32_t pieces = tiles > most ? (tiles + most - 1) / most : 1;
+    per = pieces > 1 ? (tiles + pieces - 1) / pieces : tiles;
+    return pieces > 1 ? (tiles + per - 1) / per : 1;
+}
+
+/* When the last place ends, in tiles. */
+static float hk_packed_end(const std::vector<hk_packed_sized> &order,
+                           uint32_t kv_heads, uint32_t places, uint32_t most) {
+    std::priority_queue<float, std::vector<float>, std::greater<float>> free;
+    for (uint32_t i = 0; i < places; i++) free.push(0.0f);
+    float end = 0.0f;
+    bool cut = false;
+    for (const hk_packed_sized &s : order) {
+        uint32_t per;
+        const uint32_t pieces = hk_packed_pieces(s.tiles, most, per);
+        cut |= pieces > 1;
+        const uint64_t count = (uint64_t)s.blocks * kv_heads * pieces;
+        for (uint64_t i = 0; i < count; i++) {
+            const float t = free.top() + (float)per + hk_packed_own;
+            free.pop();
+            free.push(t);
+            end = std::max(end, t);
+        }
+    }
+    return end + (cut ? 8.0f : 0.0f);
+}
 
 static void hk_packed_lay_out(const std::vector<hk_packed_request> &list,
                               uint32_t group, uint32_t kv_heads, uint32_t cus,
                               hk_packed_work &work) {
-    const double own = 3.0; /* an item's start and end, in tiles */
-    struct sized { uint32_t request, tiles, rows, blocks; };
-    std::vector<sized> order;
+    const uint32_t qb = HK_PACKED_QB, places = cus * 2u;
+    std::vector<hk_packed_sized> order;
     double total = 0.0;
+    uint64_t items = 0;
     for (uint32_t i = 0; i < list.size(); i++) {
         const uint32_t rows = list[i].q_rows * group;
-        const sized s = {i, (uint32_t)(((uint64_t)list[i].kv_rows + HK_KT - 1) /
-                                       HK_KT),
-                         rows, (uint32_t)(((uint64_t)rows + HK_PACKED_QB - 1) /
-                                          HK_PACKED_QB)};
+        const hk_packed_sized s = {
+            i, (uint32_t)(((uint64_t)list[i].kv_rows + HK_KT - 1) / HK_KT),
+            rows, (uint32_t)(((uint64_t)rows + qb - 1) / qb)};
         order.push_back(s);
-        total += (double)s.blocks * kv_heads * (s.tiles + own);
+        items += (uint64_t)s.blocks * kv_heads;
+        total += (double)s.blocks * kv_heads * (s.tiles + hk_packed_own);
     }
     std::stable_sort(order.begin(), order.end(),
-                     [](const sized &x, const sized &y) {
+                     [](const hk_packed_sized &x, const hk_packed_sized &y) {
                          return x.tiles > y.tiles;
                      });
-    const double share = total / (2.0 * cus);
-    /* a cut costs a join: worth it only where the longest item stands out */
-    const double longest = order.empty() ? 0.0 : order[0].tiles + own;
-    const uint32_t most = longest > share + 8.0
-                              ? (uint32_t)std::max(4.0, share)
-                              : UINT32_MAX;
-    std::vector<hk_packed_item> queue[8];
-    double load[8] = {};
-    const double run = total / 64.0;
-    work.parts = 0;
-    for (const sized &s : order) {
-        const hk_packed_request &r = list[s.request];
-        const uint32_t pieces =
-            s.tiles > most ? (s.tiles + most - 1) / most : 1;
-        const uint32_t per = pieces > 1 ? (s.tiles + pieces - 1) / pieces
-                                        : s.tiles;
-        int at = -1;
-        double here = 0.0;
-        for (uint32_t h = 0; h < kv_heads; h++) {
-            at = -1;
-            for (uint32_t b = 0; b < s.blocks; b++) {
-                if (at < 0 || here > run) {
-                    at = (int)(std::min_element(load, load + 8) - load);
-                    here = 0.0;
-                }
-                hk_packed_item item = {r.q_first, s.rows, b * HK_PACKED_QB, h,
-                                       r.kv_first, r.kv_rows, 0, s.tiles,
-                                       HK_PACKED_WHOLE};
-                if (pieces == 1) {
-                    queue[at].push_back(item);
-                } else {
-                    uint32_t made = 0;
-                    const uint32_t first = work.parts;
-                    for (uint32_t t = 0; t < s.tiles; t += per, made++) {
-                        item.tile = t;
-                        item.tile_end = std::min(s.tiles, t + per);
-                        item.part = work.parts++;
-                        queue[at].push_back(item);
-                    }
-                    work.joins.push_back({r.q_first, s.rows, item.row, h,
-                                          first, made});
-                }
-                const double cost = s.tiles + own * pieces;
-                load[at] += cost;
-                here += cost;
+    uint32_t most = UINT32_MAX;
+    /* (many items come out level whole) */
+    if (!order.empty() && items <= 8ull * places &&
+        order[0].tiles > total / places) {
+        float best = hk_packed_end(order, kv_heads, places, most);
+        const uint32_t share = (uint32_t)(total / places) + 1u;
+        uint32_t tried = 0;
+        for (uint32_t i = 4; i <= 24; i++) { /* half to three times a share */
+            const uint32_t length = std::max(4u, share * i / 8u);
+            if (length == tried || length >= order[0].tiles) continue;
+            tried = length;
+            const float end = hk_packed_end(order, kv_heads, places, length);
+            if (end < best) {
+                best = end;
+                most = length;
             }
         }
     }
-    size_t longest_queue = 0;
-    for (const auto &q : queue) longest_queue = std::max(longest_queue, q.size());
-    for (size_t j = 0; j < longest_queue; j++)
+    std::vector<hk_packed_item> queue[8];
+    double load[8] = {};
+    work.parts = work.join_rows = 0;
+    for (const hk_packed_sized &s : order) {
+        const hk_packed_request &r = list[s.request];
+        uint32_t per;
+        const uint32_t pieces = hk_packed_pieces(s.tiles, most, per);
+        const uint64_t count = (uint64_t)s.blocks * kv_heads;
+        for (uint64_t run = 0; run < 8; run++) {
+            /* the longer runs are the last ones */
+            const uint64_t end = count * (run + 1) / 8;
+            uint64_t i = count * run / 8;
+            auto &q = *std::min_element(
+                queue, queue + 8, [&](const auto &x, const auto &y) {
+                    return load[&x - queue] < load[&y - queue];
+                });
+            load[&q - queue] +=
+                (double)(end - i) * (s.tiles + hk_packed_own * pieces);
+            for (; i < end; i++) {
+                hk_packed_item item = {r.q_first, s.rows,
+                                       (uint32_t)(i % s.blocks) * qb,
+                                       (uint32_t)(i / s.blocks), r.kv_first,
+                                       r.kv_rows, 0, s.tiles,
+                                       HK_PACKED_WHOLE};
+                if (pieces > 1) {
+                    work.joins.push_back({r.q_first, s.rows, item.row,
+                                          item.kv_head, work.parts, pieces});
+                    work.join_rows = std::max(
+                        work.join_rows, std::min(s.rows - item.row, qb));
+                }
+                for (uint32_t p = 0; p < pieces; p++) {
+                    item.tile = p * per;
+                    item.tile_end = std::min(s.tiles, item.tile + per);
+                    if (pieces > 1) item.part = work.parts++;
+                    q.push_back(item);
+                }
+            }
+        }
+    }
+    size_t longest = 0;
+    for (const auto &q : queue) longest = std::max(longest, q.size());
+    for (size_t j = 0; j < longest; j++)
         for (const auto &q : queue)
             work.items.push_back(j < q.size() ? q[j] : hk_packed_item{});
 }
@@ -736,6 +820,7 @@ h3_gpu_tensor *h3_hip_sdpa_packed_plan(h3_gpu *gpu, const uint32_t *q_first,
         plan->record.n[HK_PACKED_KV_END] = (uint32_t)kv_end;
         plan->record.n[HK_PACKED_ITEMS] = (uint32_t)work.items.size();
         plan->record.n[HK_PACKED_JOINS] = (uint32_t)work.joins.size();
+        plan->record.n[HK_PACKED_JOIN_ROWS] = work.join_rows;
         plan->record.n[HK_PACKED_PARTS] = work.parts;
         return plan;
     } catch (const std::bad_alloc &) {
@@ -819,11 +904,9 @@ int h3_hip_sdpa_packed_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
             a.part_ml = (float2 *)(a.part_o + rows * padded);
         }
         if (padded == 64)
-            hk_packed_launch<64>(gpu, a, n[HK_PACKED_ITEMS],
-                                 n[HK_PACKED_JOINS]);
+            hk_packed_launch<64>(gpu, a, n);
         else
-            hk_packed_launch<128>(gpu, a, n[HK_PACKED_ITEMS],
-                                  n[HK_PACKED_JOINS]);
+            hk_packed_launch<128>(gpu, a, n);
         return hk_op_end(gpu, "attention_packed", HK_KIND_SDPA);
     }
     const uint64_t waves = (uint64_t)a.rows * heads;

@@ -109,11 +109,11 @@ def test_every_tile_once_at_random():
                group * kv, kv, rng.choice([64, 128])))
 
 
-def test_rows_share_no_output():
-    """Launches of plans whose rows or heads differ launch as many items."""
+def test_long_items_are_cut():
     made, items, joins = cover(([1] * 8, [6144] * 8, 64, 8, 128))
-    # 64 long items on 512 places: cut, and joined
-    assert len(joins) == 64 and len(made) == 2
+    # 64 long items on 512 places: cut, each place at most one, and joined
+    assert len(joins) == 64 and len(made) == 2 and len(items) == 512
+    assert made[1][2] == 2  # 8 rows each, four a workgroup
     assert made[0][0] == "hk_packed_flash<128>"
     made, items, joins = cover(([6144] * 2, [512] * 2, 40, 40, 128))
     assert not len(joins) and len(made) == 1
