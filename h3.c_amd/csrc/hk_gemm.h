@@ -189,7 +189,7 @@ struct hk_lora_ext {
 
 struct h3_gpu;
 /* Launches hk_gemm_lora with 32 jb rows per tile on g; epilogue HK_EPI_STORE,
- * HK_EPI_GELU or HK_EPI_PARTIAL. */
+ * HK_EPI_GELU_F32 or HK_EPI_PARTIAL. */
 void hk_gemm_lora_launch(struct h3_gpu *gpu, int epilogue, uint32_t jb,
                          uint32_t workgroups, const hk_gemm_args &g,
                          const hk_lora_ext &lora);

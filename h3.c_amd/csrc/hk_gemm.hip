@@ -224,7 +224,8 @@ static uint64_t hk_gemm_lds_ready = 0;
 
 /* Split-K reduction over the tile-local partials: 4 tile rows per
  * workgroup, 4 columns per thread; C = epilogue(bf16 rounding of
- * sum_s partial + bias), GELU after the reference's bf16 rounding. */
+ * sum_s partial + bias), GELU after the reference's bf16 rounding, or
+ * (HK_EPI_GELU_F32, beside adapters) of the F32 sum. */
 template <int EPI>
 __global__ void __launch_bounds__(256)
 hk_splitk_reduce(hk_gemm_args g, uint32_t splits) {
@@ -296,6 +297,9 @@ hk_splitk_reduce(hk_gemm_args g, uint32_t splits) {
 #pragma unroll
         for (int e = 0; e < 4; e++)
             out[e] = hk_gelu_tanh_f(hk_bf2f(hk_f2bf(out[e])));
+    } else if (EPI == HK_EPI_GELU_F32) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) out[e] = hk_gelu_tanh_f(out[e]);
     }
     *(uint2 *)(c + (size_t)m * g.n + n) =
         make_uint2(hk_pack2(out[0], out[1]), hk_pack2(out[2], out[3]));
@@ -673,6 +677,10 @@ int hk_gemm_bf16(struct h3_gpu *gpu, const uint16_t *x, const uint16_t *w,
                                    0, gpu->stream, g, splits);
             else if (epilogue == HK_EPI_GELU)
                 hipLaunchKernelGGL(hk_splitk_reduce<HK_EPI_GELU>,
+                                   dim3(tail * (g.tile_rows / 4)), dim3(256),
+                                   0, gpu->stream, g, splits);
+            else if (epilogue == HK_EPI_GELU_F32)
+                hipLaunchKernelGGL(hk_splitk_reduce<HK_EPI_GELU_F32>,
                                    dim3(tail * (g.tile_rows / 4)), dim3(256),
                                    0, gpu->stream, g, splits);
             else

@@ -152,7 +152,8 @@ double hk_now(void);
 /* GEMM epilogues */
 enum { HK_EPI_STORE = 0, HK_EPI_SWIGLU = 1, HK_EPI_GELU = 2,
        HK_EPI_PARTIAL = 3, /* internal: f32 split-K partial tiles */
-       HK_EPI_PARTIAL_SWIGLU = 4 /* internal: the same, SwiGLU W rows */ };
+       HK_EPI_PARTIAL_SWIGLU = 4, /* internal: the same, SwiGLU W rows */
+       HK_EPI_GELU_F32 = 5 /* beside adapters: no rounding before the GELU */ };
 
 /* C[M,N] = epi(A[M,K] . W[N,K]^T + bias).  For HK_EPI_SWIGLU the weight has
  * 2*N rows (gate rows [0,N), up rows [N,2N)) and C is the [M,N] activation.
@@ -160,7 +161,7 @@ enum { HK_EPI_STORE = 0, HK_EPI_SWIGLU = 1, HK_EPI_GELU = 2,
  * `scratch` is given, to that caller-owned device buffer of scratch_bytes:
  * then nothing is allocated, and a split that needs more fails (launches of
  * at most 128 rows use what the context has, and need no buffer).  `lora`
- * (plain and GELU epilogue, over 128 rows, hk_gemm_mfma_ok): the adapters'
+ * (HK_EPI_STORE or HK_EPI_GELU_F32, over 128 rows, hk_gemm_mfma_ok): the adapters'
  * part is added to the sums. */
 int hk_gemm_bf16(struct h3_gpu *gpu, const uint16_t *a, const uint16_t *w,
                  const uint16_t *bias, uint16_t *c, uint32_t m, uint32_t n,

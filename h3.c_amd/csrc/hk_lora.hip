@@ -104,23 +104,25 @@ hk_lora_pack_fragments(const uint16_t *src, uint16_t *dst, uint32_t n,
     dst[i] = col < n && k < rank ? src[col * rank + k] : (uint16_t)0;
 }
 
-/* low[r][j] = s_a x[r] . A_a[j]: one wave an element. */
+/* low[r][j] = s_a x[r] . A_a[j]: one wave an element at a time. */
 __global__ void __launch_bounds__(256) hk_lora_low_simple(hk_lora_args g) {
-    const uint64_t i = (uint64_t)blockIdx.x * 4u + (threadIdx.x >> 6);
-    const uint32_t row = (uint32_t)(i / g.pitch);
-    const uint32_t j = (uint32_t)(i - (uint64_t)row * g.pitch);
-    if (row >= g.m) return;
-    const uint32_t a = g.map[row];
-    if (a >= g.count) return;
-    const hk_lora_entry e = g.entries[a];
-    if (j >= e.rank) return;
-    const uint16_t *x = g.x + (size_t)row * g.k;
-    const uint16_t *down = e.down + (size_t)j * g.k;
-    float sum = 0.0f;
-    for (uint32_t k = threadIdx.x & 63u; k < g.k; k += 64u)
-        sum = fmaf(hk_bf2f(x[k]), hk_bf2f(down[k]), sum);
-    sum = hk_wave_sum(sum);
-    if ((threadIdx.x & 63u) == 0) g.low[i] = e.scale * sum;
+    const uint64_t count = (uint64_t)g.m * g.pitch;
+    for (uint64_t i = (uint64_t)blockIdx.x * 4u + (threadIdx.x >> 6);
+         i < count; i += (uint64_t)gridDim.x * 4u) {
+        const uint32_t row = (uint32_t)(i / g.pitch);
+        const uint32_t j = (uint32_t)(i - (uint64_t)row * g.pitch);
+        const uint32_t a = g.map[row];
+        if (a >= g.count) continue;
+        const hk_lora_entry e = g.entries[a];
+        if (j >= e.rank) continue;
+        const uint16_t *x = g.x + (size_t)row * g.k;
+        const uint16_t *down = e.down + (size_t)j * g.k;
+        float sum = 0.0f;
+        for (uint32_t k = threadIdx.x & 63u; k < g.k; k += 64u)
+            sum = fmaf(hk_bf2f(x[k]), hk_bf2f(down[k]), sum);
+        sum = hk_wave_sum(sum);
+        if ((threadIdx.x & 63u) == 0) g.low[i] = e.scale * sum;
+    }
 }
 
 /* One thread an output: the shared product, then the adapter's. */
@@ -141,7 +143,7 @@ __global__ void __launch_bounds__(256) hk_lora_simple(hk_lora_args g) {
         for (uint32_t j = 0; j < e.rank; j++)
             sum = fmaf(low[j], hk_bf2f(up[j]), sum);
     }
-    if (g.gelu) sum = hk_gelu_tanh_f(hk_bf2f(hk_f2bf(sum)));
+    if (g.gelu) sum = hk_gelu_tanh_f(sum);
     g.c[(size_t)row * g.n + col] = hk_f2bf(sum);
 }
 
@@ -149,11 +151,11 @@ static int hk_lora_run_simple(struct h3_gpu *gpu, hk_lora_args &g) {
     if (g.pitch) {
         g.low = (float *)hk_workspace(gpu, (size_t)g.m * g.pitch * 4);
         if (!g.low) return 0;
-        const uint64_t waves = (uint64_t)g.m * g.pitch;
-        if ((waves + 3) / 4 > 0x7fffffffull)
-            return hk_fail(gpu, "linear with adapters: too many rows");
-        hipLaunchKernelGGL(hk_lora_low_simple, dim3((waves + 3) / 4),
-                           dim3(256), 0, gpu->stream, g);
+        const uint64_t blocks = ((uint64_t)g.m * g.pitch + 3) / 4;
+        hipLaunchKernelGGL(
+            hk_lora_low_simple,
+            dim3((unsigned)(blocks < 1u << 20 ? blocks : 1u << 20)),
+            dim3(256), 0, gpu->stream, g);
     }
     hipLaunchKernelGGL(hk_lora_simple,
                        dim3((g.n + 255) / 256, g.m < 65535u ? g.m : 65535u,
@@ -392,14 +394,15 @@ __device__ __forceinline__ void hk_lora_add_up(const float *sums,
     }
 }
 
-/* The sums times the scale, as bf16 halves. */
+/* The sums of `ranks` ranks times the scale, as bf16 halves; zeros past them,
+ * where an infinity in the row has met A's padding. */
 __device__ __forceinline__ void hk_lora_split(const hk_f32x4 (&u)[2],
-                                              float scale, uint4 &high,
-                                              uint4 &rest) {
+                                              float scale, uint32_t ranks,
+                                              uint4 &high, uint4 &rest) {
     float v[8], low[8];
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-        v[e] = scale * u[e >> 2][e & 3];
+    for (uint32_t e = 0; e < 8; e++) {
+        v[e] = e < ranks ? scale * u[e >> 2][e & 3] : 0.0f;
         const float h = hk_bf2f(hk_f2bf(v[e]));
         /* past bf16's range the first half is infinite and stays so */
         low[e] = fabsf(h) == INFINITY ? 0.0f : v[e] - h;
@@ -431,7 +434,7 @@ hk_lora_halves(hk_lora_low_args g, uint32_t units, uint32_t tile_rows) {
             hk_f32x4 u[2];
             hk_lora_add_up(g.sums + (size_t)row * g.sum_pitch + first,
                            (size_t)g.m * g.sum_pitch, g.pieces, u);
-            hk_lora_split(u, e.scale, high, rest);
+            hk_lora_split(u, e.scale, e.rank - first, high, rest);
         }
         uint16_t *out = (uint16_t *)x.low + (size_t)row * x.pitch + first;
         *(uint4 *)out = high;
@@ -499,8 +502,9 @@ static hk_gemm_lora_kernel hk_gemm_lora_pick(uint32_t jb) {
 
 static hk_gemm_lora_kernel hk_gemm_lora_pick_epi(int epilogue, uint32_t jb) {
     return epilogue == HK_EPI_PARTIAL ? hk_gemm_lora_pick<HK_EPI_PARTIAL>(jb)
-           : epilogue == HK_EPI_GELU  ? hk_gemm_lora_pick<HK_EPI_GELU>(jb)
-                                      : hk_gemm_lora_pick<HK_EPI_STORE>(jb);
+           : epilogue == HK_EPI_GELU_F32
+               ? hk_gemm_lora_pick<HK_EPI_GELU_F32>(jb)
+               : hk_gemm_lora_pick<HK_EPI_STORE>(jb);
 }
 
 /* the GEMM's LDS, then a tile's adapters by row and its list */
@@ -516,7 +520,7 @@ void hk_gemm_lora_launch(struct h3_gpu *gpu, int epilogue, uint32_t jb,
     const uint64_t bit = 1ull << (gpu->device & 63);
     if (!(ready & bit)) {
         for (uint32_t j = 4; j <= 8; j++)
-            for (int epi : {HK_EPI_STORE, HK_EPI_GELU, HK_EPI_PARTIAL})
+            for (int epi : {HK_EPI_STORE, HK_EPI_GELU_F32, HK_EPI_PARTIAL})
                 if (const hk_gemm_lora_kernel kernel =
                         hk_gemm_lora_pick_epi(epi, j))
                     (void)hipFuncSetAttribute(
@@ -611,7 +615,10 @@ hk_lora_join(hk_skinny_args s, hk_lora_low_args g, uint32_t mbs,
         uint4 high = make_uint4(0, 0, 0, 0), rest = high;
         if (left) {
             if (k) hk_lora_add_up(low + k, low_stride, g.pieces, u);
-            hk_lora_split(u, mine.scale, high, rest);
+            const uint32_t from = k + half * 8u;
+            hk_lora_split(u, mine.scale,
+                          mine.rank > from ? mine.rank - from : 0u, high,
+                          rest);
         }
         uint32_t adapter = HK_LORA_NONE;
         hk_v4i b = {0, 0, 0, 0};
@@ -669,7 +676,7 @@ hk_lora_join(hk_skinny_args s, hk_lora_low_args g, uint32_t mbs,
         if (gelu)
 #pragma unroll
             for (int i = 0; i < 4; i++)
-                out[i] = hk_gelu_tanh_f(hk_bf2f(hk_f2bf(out[i])));
+                out[i] = hk_gelu_tanh_f(out[i]);
         *(uint2 *)(s.c + (size_t)row * s.n + c) =
             make_uint2(hk_pack2(out[0], out[1]), hk_pack2(out[2], out[3]));
     }
@@ -786,7 +793,7 @@ static int hk_lora_run(struct h3_gpu *gpu, const hk_lora_args &a) {
                            dim3(units + (a.m + tile_rows - 1) / tile_rows),
                            dim3(256), 0, gpu->stream, g, units, tile_rows);
         return hk_gemm_bf16(gpu, a.x, a.w, a.bias, a.c, a.m, a.n, a.k,
-                            a.gelu ? HK_EPI_GELU : HK_EPI_STORE, NULL, 0,
+                            a.gelu ? HK_EPI_GELU_F32 : HK_EPI_STORE, NULL, 0,
                             &g.ext);
     }
 

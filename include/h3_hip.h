@@ -272,8 +272,9 @@ int h3_gpu_linear_gelu_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
  * h3_hip_linear_lora_bf16 runs the projection; input_dim and output_dim have
  * to be the table's.  Sums are F32 and the result is rounded once: x . down^T
  * is held as two bf16 halves, 16 significant bits, between the products.
- * h3_hip_linear_lora_gelu_bf16 applies the GELU of h3_gpu_linear_gelu_bf16 to
- * the sum, rounded to bf16 first as there.
+ * h3_hip_linear_lora_gelu_bf16 applies the tanh GELU to the F32 sum, also in
+ * rows without an adapter: the rounding to bf16 that h3_gpu_linear_gelu_bf16
+ * puts before it, for the reference's sake, is not made here.
  * bias may be NULL; output must be a tensor of its own.  No reference
  * counterpart: the reference serves one request at a time. */
 h3_gpu_tensor *h3_hip_lora_table(h3_gpu *gpu,

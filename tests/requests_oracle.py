@@ -57,10 +57,9 @@ def lora(x, w, b, down, up, ranks, scales, ids, k, n, act=False):
     # every half of the low products is a term
     bound += (k + 2 * most + 1) * F32 * size
     if act:
-        # the sum rounds to bf16 first; the derivative of gelu is under 1.13;
-        # the activation's own F32 arithmetic is under 2^-20 of the argument
-        bound = 1.13 * (bound + BF16 * np.abs(y)) * (1 + BF16) + \
-            2.0 ** -20 * np.abs(y)
+        # the derivative of gelu is under 1.13; the activation's own F32
+        # arithmetic is under 2^-20 of the argument
+        bound = 1.13 * bound + 2.0 ** -20 * np.abs(y)
         y = gelu(y)
     return y, bound * (1 + BF16) + BF16 * np.abs(y) + 1e-37
 

@@ -150,6 +150,34 @@ def test_products_past_the_types_range_are_infinite(gpu, rows):
     assert (got == np.inf).all()
 
 
+@pytest.mark.parametrize("rows", [9, 200])
+@pytest.mark.parametrize("rank", [1, 4, 20, 40])
+def test_an_infinity_against_positive_adapters_is_one(gpu, rows, rank):
+    """It meets the ranks there are, not their padding (0 times it is NaN)."""
+    a = make(16, np.zeros(rows), [rank], 64, 64)
+    x = np.ones((rows, 64))
+    x[::3, 5] = np.inf
+    a.update(x=ro_bits(x.reshape(-1)), w=ro_bits(np.ones(64 * 64)),
+             down=[ro_bits(np.ones(rank * 64))],
+             up=[ro_bits(np.ones(rank * 64))])
+    got = to_f32(run(gpu, a)).reshape(rows, 64)
+    assert (got[::3] == np.inf).all()
+    assert np.isfinite(np.delete(got, np.s_[::3], 0)).all()
+
+
+@pytest.mark.parametrize("rows", [12, 300])
+def test_gelu_of_the_sum_itself(gpu, rows):
+    """One rounding.  From -2 up F32 leaves an error under 2^-16 of the result,
+    so that under one result in 2^7 lies so near a border between two bf16
+    values that it may fall to the other; rounded twice, many would."""
+    a = make(17, np.zeros(rows), [16], 256, 512)
+    got = to_f32(run(gpu, a, True)).astype(np.float64)
+    sums, _ = ro.lora(**a)
+    nearest = to_f32(ro_bits(ro.gelu(sums))).reshape(-1)
+    up = sums.reshape(-1) > -2
+    assert up.sum() > 1000 and (got != nearest)[up].mean() < 2.0 ** -7
+
+
 def ro_bits(values):
     import oracle
     return oracle.bf16(np.asarray(values, np.float32))
