@@ -84,15 +84,12 @@ struct hk_packed_args {
     float2 *part_ml;
 };
 
-/* One wave per (query row, head), 64 keys at a time: lane j scores key j of
- * the turn, then lane l adds up dims l, l + 64, ... of the turn's values.
+/* One wave per (query row, head) at a time, 64 keys a turn: lane j scores key
+ * j of the turn, then lane l adds up dims l, l + 64, ... of the turn's values.
  * Running maximum and sum in F32; P stays F32. */
-__global__ void __launch_bounds__(256) hk_packed_simple(hk_packed_args a) {
-    const uint64_t i = (uint64_t)blockIdx.x * 4u + (threadIdx.x >> 6);
+__device__ void hk_packed_simple_row(const hk_packed_args &a, uint32_t nth,
+                                     uint32_t head) {
     const uint32_t lane = threadIdx.x & 63u;
-    const uint32_t nth = (uint32_t)(i / a.heads);
-    const uint32_t head = (uint32_t)(i - (uint64_t)nth * a.heads);
-    if (nth >= a.rows) return;
     /* the last request that begins at or before the nth query row */
     uint32_t low = 0, high = a.request_count;
     while (high - low > 1) {
@@ -140,6 +137,14 @@ __global__ void __launch_bounds__(256) hk_packed_simple(hk_packed_args a) {
     for (uint32_t d = 0; d < HK_PACKED_MAX_DIM / 64; d++)
         if (d * 64u + lane < a.dim)
             out[d * 64u + lane] = hk_f2bf(sum == 0.0f ? 0.0f : o[d] / sum);
+}
+
+__global__ void __launch_bounds__(256) hk_packed_simple(hk_packed_args a) {
+    for (uint64_t i = (uint64_t)blockIdx.x * 4u + (threadIdx.x >> 6);
+         i < (uint64_t)a.rows * a.heads; i += (uint64_t)gridDim.x * 4u) {
+        const uint32_t nth = (uint32_t)(i / a.heads);
+        hk_packed_simple_row(a, nth, (uint32_t)(i - (uint64_t)nth * a.heads));
+    }
 }
 
 /* ------------------------------------------------- the matrix-core kernel
@@ -359,7 +364,7 @@ hk_packed_flash(hk_packed_args a) {
         }
         /* The softmax of hk_flash_fwd: P = exp2(s - m_run) against the
          * running maximum as it stands, which moves (O and l rescaled) only
-         * when it is unset or a lane's P sum passes 2^32.  P <= 2^32 keeps O
+         * when it is unset or one of its P sums passes 2^32.  P <= 2^32 keeps O
          * and l far from overflow; P rounds to bf16 for the product, l sums
          * the unrounded P. */
         hk_bf16x8 pf[2][2];
@@ -387,7 +392,13 @@ hk_packed_flash(hk_packed_args a) {
         };
         const bool unset = m_run == -INFINITY;
         float sum = unset ? 0.0f : exps();
-        if (__builtin_amdgcn_ballot_w64(unset || sum > 0x1p32f)) {
+        uint32_t move = unset || sum > 0x1p32f;
+        if (__builtin_amdgcn_ballot_w64(move)) {
+            /* a row's other half's too, but no other row's: what a row comes
+             * to does not depend on the rows beside it */
+            const auto mv =
+                __builtin_amdgcn_permlane32_swap(move, move, false, false);
+            move = mv[0] | mv[1];
             float mx = -INFINITY;
 #pragma unroll
             for (int kt = 0; kt < 2; kt++)
@@ -397,9 +408,10 @@ hk_packed_flash(hk_packed_args a) {
                 __float_as_uint(mx), __float_as_uint(mx), false, false);
             mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) *
                  a.scale_log2;
-            const float m_new = fmaxf(m_run, mx);
+            const float m_new = move ? fmaxf(m_run, mx) : m_run;
             const float ref = m_new == -INFINITY ? 0.0f : m_new;
-            const float c = __builtin_amdgcn_exp2f(m_run - ref);
+            const float c =
+                move ? __builtin_amdgcn_exp2f(m_run - ref) : 1.0f;
             m_run = ref;
             l_part *= c;
 #pragma unroll
@@ -407,6 +419,8 @@ hk_packed_flash(hk_packed_args a) {
 #pragma unroll
                 for (int r = 0; r < 16; r++) o[d][r] *= c;
             sum = exps();
+            /* every score so far -inf: the maximum stays unset */
+            m_run = m_new;
         }
         l_part += sum;
 
@@ -543,6 +557,7 @@ __global__ void __launch_bounds__(256) hk_packed_joined(hk_packed_args a) {
     for (uint32_t p = lane; p < j.pieces; p += 64u)
         top = fmaxf(top, ml[(size_t)p * HK_PACKED_QB].x);
     top = hk_wave_max(top);
+    if (top == -INFINITY) top = 0.0f; /* no piece has a weight */
     per sum = {};
     float l = 0.0f;
     for (uint32_t first = 0; first < j.pieces; first += 4u) {
@@ -909,9 +924,11 @@ int h3_hip_sdpa_packed_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
             hk_packed_launch<128>(gpu, a, n);
         return hk_op_end(gpu, "attention_packed", HK_KIND_SDPA);
     }
-    const uint64_t waves = (uint64_t)a.rows * heads;
-    hipLaunchKernelGGL(hk_packed_simple, dim3((unsigned)((waves + 3) / 4)),
-                       dim3(256), 0, gpu->stream, a);
+    const uint64_t blocks = ((uint64_t)a.rows * heads + 3) / 4;
+    hipLaunchKernelGGL(
+        hk_packed_simple,
+        dim3((unsigned)(blocks < 1u << 20 ? blocks : 1u << 20)), dim3(256), 0,
+        gpu->stream, a);
     return hk_op_end(gpu, "attention_packed", HK_KIND_SDPA);
 }
 

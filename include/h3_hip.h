@@ -306,7 +306,8 @@ int h3_hip_linear_lora_gelu_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
  * h / (heads / kv_heads).  Self-attention has the same ranges on both sides;
  * cross-attention reads each request's own text, or one text that requests
  * share.  Query ranges must not overlap, key ranges may.  A request without
- * key rows gets zeros; output rows of no request are left as they were.
+ * key rows gets zeros, as does a row all of whose scores are -inf; output rows
+ * of no request are left as they were.
  *
  * h3_hip_sdpa_packed_plan validates the ranges and lays the work out once for
  * a set of requests (free it with h3_gpu_tensor_free); the call takes any

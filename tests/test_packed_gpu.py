@@ -214,6 +214,20 @@ def test_a_query_row_that_is_nan(gpu, dim):
 
 
 @pytest.mark.parametrize("dim", [64, 128])
+def test_a_row_is_the_same_beside_any_others(gpu, dim):
+    """Its bits, with rows beside it whose maximum moves at other keys."""
+    a = Case(19, [64, 9], [700, 300], 4, 2, dim)
+    want = a.run(gpu)
+    q = to_f32(a.q).reshape(a.rows, -1).copy()
+    other = np.arange(a.rows) % 3 > 0
+    q[other] *= 200 * np.random.default_rng(1).uniform(-1, 1, (other.sum(), 1))
+    a.q = ro_bits(q)
+    got = a.run(gpu)
+    assert (got[~other] == want[~other]).all()
+    assert (got[other] != want[other]).any()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
 def test_a_key_that_is_nan_or_infinite(gpu, dim):
     """A NaN key makes its request's rows NaN; an infinite one as well, where
     its score is (inf - inf)."""
@@ -232,6 +246,33 @@ def test_a_key_that_is_nan_or_infinite(gpu, dim):
         assert np.isfinite(to_f32(got[:40, :2][~lost])).all()
         assert (got[40:] == want[40:]).all()
         assert (got[:, 2:] == want[:, 2:]).all()
+
+
+@pytest.mark.parametrize("dim", [64, 80, 100, 128])
+def test_keys_of_no_weight_before_far_lower_ones(gpu, dim):
+    """Scores of -inf for the first tiles, or all of a piece, and then scores
+    whose weights against a maximum of 0 would all be 0; the last request has
+    no others and gets zeros."""
+    for qn, kn, out in (([40, 2, 3], [200, 331, 70], [70, 129, 70]),
+                        ([1, 1], [9720, 500], [5000, 500])):
+        a = Case(18, qn, kn, 4, 2, dim)
+        q = to_f32(a.q).reshape(a.rows, -1)
+        a.q = ro_bits(1 + np.abs(q) / 4)
+        kv = to_f32(a.kvs).reshape(a.kv, -1).copy()
+        kv[:, :2 * dim] = kv[:, :2 * dim] / 4 - 18
+        bits = ro_bits(kv).reshape(a.kv, -1)
+        for f, n in zip(a.kf, out):
+            bits[f:f + n, 0] = bits[f:f + n, dim] = 0xFF80
+        a.kvs = bits.reshape(-1)
+        got = a.run(gpu)
+        # the oracle is not shown the keys of no weight
+        whole = a.kf, a.kn
+        a.kf = [f + n for f, n in zip(a.kf, out)]
+        a.kn = [k - n for k, n in zip(a.kn, out)]
+        want, bound, _ = a.want()
+        a.kf, a.kn = whole
+        assert np.abs(want[0]).max() > 0
+        ro.check(got, want, bound)
 
 
 def test_the_same_call_gives_the_same_bits(gpu):
