@@ -587,10 +587,13 @@ static int hk_gemm_skinny_run(struct h3_gpu *gpu, hk_skinny_args &g,
 }
 
 uint32_t hk_gemm_tile_rows(const struct h3_gpu *gpu, uint32_t m, uint32_t n,
-                           uint32_t k) {
+                           uint32_t k, float *us) {
     const uint32_t cus = gpu->num_cus > 0 ? (uint32_t)gpu->num_cus : 256u;
-    return 32u * hk_gemm_row_blocks(m, (n + HK_BN - 1) / HK_BN, k / HK_BK, cus,
-                                    true);
+    const uint32_t columns = (n + HK_BN - 1) / HK_BN, k_steps = k / HK_BK;
+    const uint32_t jb = hk_gemm_row_blocks(m, columns, k_steps, cus, true);
+    *us = hk_gemm_estimate(jb, (m + 32u * jb - 1) / (32u * jb) * columns,
+                           k_steps, cus, true);
+    return 32u * jb;
 }
 
 int hk_gemm_bf16(struct h3_gpu *gpu, const uint16_t *x, const uint16_t *w,

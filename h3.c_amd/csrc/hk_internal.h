@@ -168,9 +168,10 @@ int hk_gemm_bf16(struct h3_gpu *gpu, const uint16_t *a, const uint16_t *w,
                  uint32_t k, int epilogue, float *scratch = nullptr,
                  size_t scratch_bytes = 0,
                  const struct hk_lora_ext *lora = nullptr);
-/* The rows of a tile of such a launch. */
+/* The rows of a tile of such a launch over tiles (not the skinny kernel), and
+ * the estimated time of one without adapters. */
 uint32_t hk_gemm_tile_rows(const struct h3_gpu *gpu, uint32_t m, uint32_t n,
-                           uint32_t k);
+                           uint32_t k, float *us);
 /* Whether the MFMA kernels take this shape and these pointers. */
 bool hk_gemm_mfma_ok(const struct h3_gpu *gpu, const void *x, const void *w,
                      const void *bias, const void *c, uint32_t m, uint32_t n,

@@ -29,6 +29,8 @@
 #include <math.h>
 #include <stdlib.h>
 
+#include <algorithm>
+
 #define HK_LORA_MAX_RANK 1024u
 
 /* hk_record.n of a table */
@@ -62,7 +64,7 @@ struct hk_lora_low_args {
     uint32_t chunks;              /* of 16 RB ranks */
     uint32_t slots; /* workgroups that share a row group's adapters */
     uint32_t units; /* workgroups in all of them */
-    struct hk_lora_row *rows; /* up to 128 rows: what each one's adapter is */
+    struct hk_lora_row *rows; /* for hk_lora_join: each row's adapter */
 };
 
 /* A row's adapter, found once for all of hk_lora_join's waves; rank 0 without
@@ -209,12 +211,17 @@ __device__ __forceinline__ void hk_lora_low_unit(const hk_lora_low_args &g,
     const uint32_t rank0 = chunk * (16u * RB);
     const uint32_t first_step = piece * g.piece_steps;
     const uint32_t steps = min(g.piece_steps, g.k / HK_BK - first_step);
-    /* lane l of every wave has row l % ROWS's adapter */
+    /* lane l of every wave has row l % ROWS's adapter, and of the first 64
+     * adapters the entry of number l: not one more wait for each */
     uint32_t left = HK_LORA_NONE;
     if (row0 + (lane & (ROWS - 1u)) < g.m)
         left = g.ext.map[row0 + (lane & (ROWS - 1u))];
-    if (left >= g.ext.count) left = HK_LORA_NONE;
-    const uint32_t mine = left;
+    uint64_t down_of = 0;
+    uint32_t rank_of = 0;
+    if (lane < g.ext.count) {
+        down_of = (uint64_t)(uintptr_t)g.ext.entries[lane].down;
+        rank_of = g.ext.entries[lane].rank;
+    }
 
     /* lane l loads chunk l % 8 of row l / 8 of every 8 */
     const uint32_t line = lane >> 3, chunk_off = (lane & 7u) * 16u;
@@ -234,6 +241,30 @@ __device__ __forceinline__ void hk_lora_low_unit(const hk_lora_low_args &g,
     for (int h = 0; h < 2; h++)
         get[h] = r16 * 128u + (((h * 4u + quad) ^ hk_swz_key(r16)) << 4);
 
+    /* turn t of K: steps (DEEP t + u) WAVES + wave, u < DEEP; past the end of
+     * K the lane offset lies beyond the buffers and loads zeros */
+    hk_v4i lx[2][DEEP][2 * J];
+    auto step_of = [&](uint32_t t, int u) {
+        return (t * DEEP + u) * WAVES + wave;
+    };
+    auto load_x = [&](int buf, uint32_t t) {
+#pragma unroll
+        for (int u = 0; u < DEEP; u++) {
+            const uint32_t step = step_of(t, u);
+            const bool live = step < steps;
+            const uint32_t kb = live ? (first_step + step) * (HK_BK * 2u) : 0u;
+#pragma unroll
+            for (int j = 0; j < 2 * J; j++)
+                lx[buf][u][j] = __builtin_amdgcn_raw_buffer_load_b128(
+                    xr, live ? x_off[j] : 0xfffff000u, kb, 0);
+        }
+    };
+    /* X does not wait for the adapter */
+    load_x(0, 0);
+    bool have_x = true;
+    if (left >= g.ext.count) left = HK_LORA_NONE;
+    const uint32_t mine = left;
+
     for (uint32_t turn = 0;; turn++) {
         uint32_t adapter = left;
 #pragma unroll
@@ -244,12 +275,26 @@ __device__ __forceinline__ void hk_lora_low_unit(const hk_lora_low_args &g,
         if (adapter == HK_LORA_NONE) break;
         left = left > adapter ? left : HK_LORA_NONE;
         if (turn % g.slots != slot) continue;
-        const uint64_t *entry = (const uint64_t *)(g.ext.entries + adapter);
-        const uint16_t *down = (const uint16_t *)hk_group_word(entry, 0);
-        const uint32_t rank = (uint32_t)hk_group_word(entry, 2);
+        uint64_t down;
+        uint32_t rank;
+        if (adapter < 64u) {
+            auto of = [&](uint32_t v) {
+                return (uint32_t)__builtin_amdgcn_readlane((int)v,
+                                                           (int)adapter);
+            };
+            down = (uint64_t)of((uint32_t)down_of) |
+                   ((uint64_t)of((uint32_t)(down_of >> 32)) << 32);
+            rank = of(rank_of);
+        } else {
+            const uint64_t *entry =
+                (const uint64_t *)(g.ext.entries + adapter);
+            down = hk_group_word(entry, 0);
+            rank = (uint32_t)hk_group_word(entry, 2);
+        }
         if (rank0 >= rank) continue;
         /* ranks past the last load, and come out, as zeros */
-        const __amdgpu_buffer_rsrc_t ar = hk_rsrc(down, rank * g.k * 2u);
+        const __amdgpu_buffer_rsrc_t ar =
+            hk_rsrc((const uint16_t *)down, rank * g.k * 2u);
         uint32_t a_off[2 * RB];
 #pragma unroll
         for (int i = 0; i < 2 * RB; i++)
@@ -260,20 +305,14 @@ __device__ __forceinline__ void hk_lora_low_unit(const hk_lora_low_args &g,
         for (int i = 0; i < RB; i++)
 #pragma unroll
             for (int j = 0; j < J; j++) acc[i][j] = hk_f32x4{0, 0, 0, 0};
-        /* turn t: steps (DEEP t + u) WAVES + wave, u < DEEP; past the end of
-         * K the lane offset lies beyond the buffers and loads zeros */
-        hk_v4i lx[2][DEEP][2 * J], la[2][DEEP][2 * RB];
-        auto load = [&](int buf, uint32_t t) {
+        hk_v4i la[2][DEEP][2 * RB];
+        auto load_a = [&](int buf, uint32_t t) {
 #pragma unroll
             for (int u = 0; u < DEEP; u++) {
-                const uint32_t step = (t * DEEP + u) * WAVES + wave;
+                const uint32_t step = step_of(t, u);
                 const bool live = step < steps;
                 const uint32_t kb =
                     live ? (first_step + step) * (HK_BK * 2u) : 0u;
-#pragma unroll
-                for (int j = 0; j < 2 * J; j++)
-                    lx[buf][u][j] = __builtin_amdgcn_raw_buffer_load_b128(
-                        xr, live ? x_off[j] : 0xfffff000u, kb, 0);
 #pragma unroll
                 for (int i = 0; i < 2 * RB; i++)
                     la[buf][u][i] = __builtin_amdgcn_raw_buffer_load_b128(
@@ -312,11 +351,15 @@ __device__ __forceinline__ void hk_lora_low_unit(const hk_lora_low_args &g,
             }
         };
         const uint32_t turns = (steps + DEEP * WAVES - 1u) / (DEEP * WAVES);
-        load(0, 0);
+        if (!have_x) load_x(0, 0);
+        have_x = false;
+        load_a(0, 0);
         for (uint32_t t = 0; t < turns; t += 2u) {
-            load(1, t + 1u);
+            load_x(1, t + 1u);
+            load_a(1, t + 1u);
             compute(0);
-            load(0, t + 2u);
+            load_x(0, t + 2u);
+            load_a(0, t + 2u);
             compute(1);
         }
         /* acc[i][j][e]: rank rank0 + 16 i + 4 quad + e, row row0 + 16 j + r16.
@@ -357,9 +400,26 @@ __device__ __forceinline__ void hk_lora_low_unit(const hk_lora_low_args &g,
     }
 }
 
-/* Over 128 rows: a workgroup per (row group, rank chunk, piece of K).  The
- * chunks of a row group read the same X, so they go to one XCD: workgroups are
- * dealt to the 8 XCDs in turn. */
+/* A row's adapter, for hk_lora_second. */
+__device__ __forceinline__ void hk_lora_find_row(const hk_lora_low_args &g,
+                                                 uint32_t row) {
+    if (row >= g.m) return;
+    const uint32_t a = g.ext.map[row];
+    hk_lora_row r = {};
+    r.adapter = HK_LORA_NONE;
+    if (a < g.ext.count) {
+        const hk_lora_entry e = g.ext.entries[a];
+        r.fragments = e.fragments;
+        r.rank = e.rank;
+        r.scale = e.scale;
+        r.adapter = a;
+    }
+    g.rows[row] = r;
+}
+
+/* The first product by itself: a workgroup per (row group, rank chunk, piece
+ * of K, slot).  The chunks of a row group read the same X, so they go to one
+ * XCD: workgroups are dealt to the 8 XCDs in turn. */
 template <int RB, int J>
 __global__ void __launch_bounds__(HK_LORA_WAVES * 64, 2)
 hk_lora_low(hk_lora_low_args g) {
@@ -368,9 +428,10 @@ hk_lora_low(hk_lora_low_args g) {
     const uint32_t eight = blockIdx.x / (8u * g.chunks);
     const uint32_t in = blockIdx.x - eight * 8u * g.chunks;
     const uint32_t at = eight * 8u + (in & 7u);
-    const uint32_t group = at % g.row_groups, piece = at / g.row_groups;
-    if (piece < g.pieces)
-        hk_lora_low_unit<RB, J>(g, group * 16u * J, in >> 3, 0, piece, lds);
+    const uint32_t group = at % g.row_groups, rest = at / g.row_groups;
+    if (rest < g.pieces * g.slots)
+        hk_lora_low_unit<RB, J>(g, group * 16u * J, in >> 3, rest / g.pieces,
+                                rest % g.pieces, lds);
 }
 
 /* 8 ranks of a row: the sums of K's pieces, four on their way at a time. */
@@ -534,132 +595,93 @@ void hk_gemm_lora_launch(struct h3_gpu *gpu, int epilogue, uint32_t jb,
                        gpu->stream, g, lora);
 }
 
-/* Up to 128 rows.  The skinny GEMM's workgroups and those of the adapters'
- * first product share one launch: the former stream W for the whole launch,
- * the latter end under them.  The former always leave F32 pieces, which
- * hk_lora_join adds up with the adapters' second product. */
-template <int MB, int J>
-__global__ void __launch_bounds__(256, 2)
-hk_lora_skinny(hk_skinny_args s, hk_lora_low_args g, uint32_t columns,
-               uint32_t pieces) {
-    extern __shared__ __attribute__((aligned(16))) uint8_t hk_xs[];
-    if (blockIdx.x < g.units) {
-        uint32_t unit = blockIdx.x;
-        const uint32_t piece = unit % g.pieces;
-        unit /= g.pieces;
-        const uint32_t chunk = unit % g.chunks;
-        unit /= g.chunks;
-        const uint32_t group = unit % g.row_groups;
-        hk_lora_low_unit<1, J>(g, group * 16u * J, chunk,
-                               unit / g.row_groups, piece, hk_xs);
-    } else if (blockIdx.x == g.units) {
-        if (threadIdx.x >= g.m) return;
-        const uint32_t a = g.ext.map[threadIdx.x];
-        hk_lora_row r = {};
-        r.adapter = HK_LORA_NONE;
-        if (a < g.ext.count) {
-            const hk_lora_entry e = g.ext.entries[a];
-            r.fragments = e.fragments;
-            r.rank = e.rank;
-            r.scale = e.scale;
-            r.adapter = a;
-        }
-        g.rows[threadIdx.x] = r;
-    } else {
-        const uint32_t at = blockIdx.x - g.units - 1u;
-        hk_skinny_tile<MB, 3>(s, at % columns, at / columns, 0, columns,
-                              pieces);
-    }
-}
-
-/* C = act(pieces' sums + bias + s_a (x . A^T) . B^T) for 32 columns and 32
- * rows, a wave: lane l has row l % 32 and its adapter, so that what an adapter
- * takes in turn is B alone: 32x32x16 MFMAs of B's rows against the rows'
- * halves, zeros in rows of others, onto the pieces' sums (the layout of
- * hk_gemm_skinny's).  A wave waits for two loads in sequence, its row and B;
- * the first 16 ranks' products are on their way with the row, and the next B
- * while one is multiplied. */
-__global__ void __launch_bounds__(64)
-hk_lora_join(hk_skinny_args s, hk_lora_low_args g, uint32_t mbs,
-             uint32_t tiles, uint32_t pieces, int gelu) {
-    const uint32_t lane = threadIdx.x, half = lane >> 5;
-    const uint32_t tile = blockIdx.x / mbs, mb = blockIdx.x % mbs;
-    const uint32_t row = mb * 32u + (lane & 31u), n0 = tile * 32u;
-    const bool live = row < s.m;
-    const size_t low_stride = (size_t)s.m * g.sum_pitch;
-    const float *low = g.sums + (size_t)row * g.sum_pitch + half * 8u;
-    hk_lora_row mine = {};
-    hk_f32x4 u[2] = {};
-    hk_f32x16 acc;
-#pragma unroll
-    for (int r = 0; r < 16; r++) acc[r] = 0.0f;
-    if (live) {
-        mine = g.rows[row];
-        /* (what a row without an adapter reads here is not used) */
-        if (g.sum_pitch) hk_lora_add_up(low, low_stride, g.pieces, u);
-        const size_t stride = (size_t)tiles * mbs * 256u;
-        const hk_f32x4 *p =
-            (const hk_f32x4 *)s.partial + (size_t)blockIdx.x * 256u + lane;
-        for (uint32_t i = 0; i < pieces; i++)
-#pragma unroll
-            for (int q = 0; q < 4; q++) {
-                const hk_f32x4 v = p[i * stride + q * 64u];
-#pragma unroll
-                for (int e = 0; e < 4; e++) acc[q * 4 + e] += v[e];
-            }
-    }
+/* Adds s_a (x . A^T) . B^T to acc, the sums of 32 columns and 32 rows of a
+ * wave in the layout of hk_skinny_tile: lane l has row l % 32 and its adapter
+ * `mine` (rank 0 without one), so that what an adapter takes in turn is B
+ * alone: 32x32x16 MFMAs of B's rows against the rows' halves, zeros in rows of
+ * others.  16 ranks at a time, with the next 16 on their way: `u` holds the
+ * lane's 8 of the first (add_up of `low`).  Each B is a wait, but where the
+ * rows have several adapters four of them are one. */
+__device__ __forceinline__ void hk_lora_second(const hk_lora_low_args &g,
+                                               const hk_lora_row &mine,
+                                               const float *low,
+                                               hk_f32x4 (&u)[2], uint32_t tile,
+                                               hk_f32x16 &acc) {
+    const uint32_t lane = threadIdx.x & 63u, half = lane >> 5;
     for (uint32_t k = 0;; k += 16u) {
         /* rows with ranks from k on */
         bool left = k < mine.rank;
-        if (!__builtin_amdgcn_ballot_w64(left)) break;
-        uint4 high = make_uint4(0, 0, 0, 0), rest = high;
-        if (left) {
-            if (k) hk_lora_add_up(low + k, low_stride, g.pieces, u);
-            const uint32_t from = k + half * 8u;
-            hk_lora_split(u, mine.scale,
-                          mine.rank > from ? mine.rank - from : 0u, high,
-                          rest);
-        }
-        uint32_t adapter = HK_LORA_NONE;
-        hk_v4i b = {0, 0, 0, 0};
-        /* the next adapter of the rows that are left, and its B */
-        auto take = [&](uint32_t &which, hk_v4i &into) {
-            const uint64_t with = __builtin_amdgcn_ballot_w64(left);
-            which = HK_LORA_NONE;
-            if (!with) return;
-            const int lead = __builtin_ctzll(with);
+        uint64_t with = __builtin_amdgcn_ballot_w64(left);
+        if (!with) return;
+        const uint32_t from = k + half * 8u;
+        uint4 high, rest;
+        hk_lora_split(u, mine.scale, mine.rank > from ? mine.rank - from : 0u,
+                      high, rest);
+        if (k + 16u < mine.rank)
+            hk_lora_add_up(low + k + 16u, (size_t)g.m * g.sum_pitch, g.pieces,
+                           u);
+        /* the next adapter of the rows that are left (of none: the last one
+         * again, for no rows), and its B */
+        int lead = 0;
+        bool its = false;
+        auto take = [&]() {
+            if (with) lead = __builtin_ctzll(with);
             auto of = [&](uint32_t v) {
                 return (uint32_t)__builtin_amdgcn_readlane((int)v, lead);
             };
-            which = of(mine.adapter);
             const uint64_t at = (uint64_t)(uintptr_t)mine.fragments;
-            const hk_v4i *fragments = (const hk_v4i *)(
-                (uint64_t)of((uint32_t)at) |
-                ((uint64_t)of((uint32_t)(at >> 32)) << 32));
+            const hk_v4i *fragments =
+                (const hk_v4i *)((uint64_t)of((uint32_t)at) |
+                                 ((uint64_t)of((uint32_t)(at >> 32)) << 32));
             const uint32_t chunks = (of(mine.rank) + 15u) / 16u;
-            left = left && mine.adapter != which;
-            into = fragments[((size_t)tile * chunks + k / 16u) * 64u + lane];
+            its = left && mine.adapter == of(mine.adapter);
+            left = left && !its;
+            with = __builtin_amdgcn_ballot_w64(left);
+            return fragments[((size_t)tile * chunks + k / 16u) * 64u + lane];
         };
-        take(adapter, b);
-        while (adapter != HK_LORA_NONE) {
-            uint32_t next;
-            hk_v4i after = {0, 0, 0, 0};
-            take(next, after);
+        auto multiply = [&](const hk_v4i &b, bool rows) {
             const hk_v4i none = {0, 0, 0, 0};
-            const bool its = mine.adapter == adapter;
-            const hk_v4i h = its ? __builtin_bit_cast(hk_v4i, high) : none;
-            const hk_v4i r = its ? __builtin_bit_cast(hk_v4i, rest) : none;
+            const hk_v4i h = rows ? __builtin_bit_cast(hk_v4i, high) : none;
+            const hk_v4i r = rows ? __builtin_bit_cast(hk_v4i, rest) : none;
             acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
                 __builtin_bit_cast(hk_bf16x8, b),
                 __builtin_bit_cast(hk_bf16x8, h), acc, 0, 0, 0);
             acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
                 __builtin_bit_cast(hk_bf16x8, b),
                 __builtin_bit_cast(hk_bf16x8, r), acc, 0, 0, 0);
-            adapter = next;
-            b = after;
+        };
+        const hk_v4i first = take();
+        const bool firsts = its;
+        if (!with) {
+            multiply(first, firsts);
+            continue;
+        }
+        hk_v4i b[3];
+        bool rows[3];
+        auto three = [&]() {
+#pragma unroll
+            for (int i = 0; i < 3; i++) {
+                b[i] = take();
+                rows[i] = its;
+            }
+        };
+        three();
+        multiply(first, firsts);
+        for (;;) {
+#pragma unroll
+            for (int i = 0; i < 3; i++) multiply(b[i], rows[i]);
+            if (!with) break;
+            three();
         }
     }
-    if (!live) return;
+}
+
+/* C = act(acc + bias) for the lane's columns of `row`. */
+__device__ __forceinline__ void hk_lora_store(const hk_skinny_args &s,
+                                              const hk_f32x16 &acc,
+                                              uint32_t row, uint32_t n0,
+                                              int gelu) {
+    const uint32_t half = (threadIdx.x & 63u) >> 5;
 #pragma unroll
     for (int q = 0; q < 4; q++) {
         const uint32_t c = n0 + q * 8u + half * 4u;
@@ -675,11 +697,100 @@ hk_lora_join(hk_skinny_args s, hk_lora_low_args g, uint32_t mbs,
         }
         if (gelu)
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                out[i] = hk_gelu_tanh_f(out[i]);
+            for (int i = 0; i < 4; i++) out[i] = hk_gelu_tanh_f(out[i]);
         *(uint2 *)(s.c + (size_t)row * s.n + c) =
             make_uint2(hk_pack2(out[0], out[1]), hk_pack2(out[2], out[3]));
     }
+}
+
+/* The skinny GEMM and the adapters' first product in one launch: `tiles`
+ * workgroups of the former, which stream W and leave F32 sums, in one piece
+ * of K or more, and the latter's units (32 rows, 16 ranks).  hk_lora_join adds
+ * both up.  Tiles that are all resident at once go first and the units beside
+ * them (the other order kept CUs from W's stream: 160 rows x 5120 -> 5120 with
+ * ranks up to 64 took 34 us against 29), several rounds of tiles behind the
+ * units.
+ *
+ * Over 128 rows there are `groups` of 32 MB rows.  Those of one part of W
+ * (column and piece) follow each other on one XCD and find it in its L2:
+ * workgroups go to the 8 XCDs in turn, each XCD takes a run of (part, group). */
+template <int MB, int J, bool GROUPS>
+__global__ void __launch_bounds__(256, 2)
+hk_lora_skinny(hk_skinny_args s, hk_lora_low_args g, uint32_t columns,
+               uint32_t pieces, uint32_t groups, uint32_t first_tile,
+               uint32_t tiles) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t hk_xs[];
+    const uint32_t at = blockIdx.x - first_tile;
+    if (at < tiles) {
+        const uint32_t turn =
+            GROUPS ? at % 8u * (tiles / 8u) + at / 8u : at;
+        const uint32_t part = GROUPS ? turn / groups : turn;
+        if (part >= columns * pieces) return;
+        hk_skinny_args own = s;
+        if constexpr (GROUPS) {
+            const uint32_t group = turn - part * groups;
+            own.x += (size_t)group * 32u * MB * s.k;
+            own.m = min(s.m - group * 32u * MB, 32u * MB);
+            own.x_bytes = own.m * s.k * 2u;
+            own.partial += (size_t)group * pieces * columns * 4u * MB * 1024u;
+        }
+        hk_skinny_tile<MB, 3, GROUPS ? HK_LOAD_SHARED : HK_LOAD_ONCE>(
+            own, part % columns, part / columns, 0, columns, pieces);
+        return;
+    }
+    uint32_t unit = blockIdx.x < first_tile ? blockIdx.x
+                                            : blockIdx.x - tiles;
+    if (unit >= g.units) {
+        hk_lora_find_row(g, (unit - g.units) * 256u + threadIdx.x);
+        return;
+    }
+    const uint32_t piece = unit % g.pieces;
+    unit /= g.pieces;
+    const uint32_t chunk = unit % g.chunks;
+    unit /= g.chunks;
+    const uint32_t group = unit % g.row_groups;
+    hk_lora_low_unit<1, J>(g, group * 16u * J, chunk, unit / g.row_groups,
+                           piece, hk_xs);
+}
+
+/* C = act(pieces' sums + bias + s_a (x . A^T) . B^T) for 32 columns and 32
+ * rows, a wave; blockIdx.y is the row group. */
+__global__ void __launch_bounds__(256, 5)
+hk_lora_join(hk_skinny_args s, hk_lora_low_args g, uint32_t mbs,
+             uint32_t tiles, uint32_t pieces, int gelu) {
+    const uint32_t lane = threadIdx.x & 63u, half = lane >> 5;
+    const uint32_t at =
+        blockIdx.x * 4u + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t tile = at / mbs;
+    const uint32_t mb = blockIdx.y * mbs + at % mbs;
+    if (tile * 32u >= s.n) return;
+    const uint32_t row = mb * 32u + (lane & 31u);
+    const bool live = row < s.m;
+    const float *low = g.sums + (size_t)row * g.sum_pitch + half * 8u;
+    hk_lora_row mine = {};
+    hk_f32x4 u[2] = {};
+    hk_f32x16 acc;
+#pragma unroll
+    for (int r = 0; r < 16; r++) acc[r] = 0.0f;
+    if (live) {
+        mine = g.rows[row];
+        /* (what a row without an adapter reads here is not used) */
+        if (g.sum_pitch)
+            hk_lora_add_up(low, (size_t)s.m * g.sum_pitch, g.pieces, u);
+        const size_t stride = (size_t)tiles * mbs * 256u;
+        const hk_f32x4 *p = (const hk_f32x4 *)s.partial +
+                            blockIdx.y * pieces * stride +
+                            (size_t)at * 256u + lane;
+        for (uint32_t i = 0; i < pieces; i++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const hk_f32x4 v = p[i * stride + q * 64u];
+#pragma unroll
+                for (int e = 0; e < 4; e++) acc[q * 4 + e] += v[e];
+            }
+    }
+    hk_lora_second(g, mine, low, u, tile, acc);
+    if (live) hk_lora_store(s, acc, row, tile * 32u, gelu);
 }
 
 /* Whether the matrix-core kernels take the call: what the GEMM takes, and the
@@ -694,37 +805,192 @@ static bool hk_lora_takes(const struct h3_gpu *gpu, const hk_lora_args &g) {
            a + 2ull * g.k < most && b < most && low < most;
 }
 
-/* How the first product runs over 128 rows: 16 J rows a workgroup, K in
- * `pieces`.  A workgroup takes about 4 us and 20 KB a us of X's and A's rows;
- * two share a CU. */
-struct hk_lora_plan {
-    uint32_t j, pieces, steps;
-};
-
-static hk_lora_plan hk_lora_plan_of(uint32_t m, uint32_t k_steps, uint32_t rb,
-                                    uint32_t chunks, uint32_t cus) {
-    hk_lora_plan best = {2, 1, k_steps};
+/* The projection's own GEMM, with the halves as more steps of its K.
+ *
+ * The first product by itself: 16 RB ranks and 16 J rows a workgroup, K in
+ * pieces, the adapters of a row group over slots (of several requests' rows
+ * some groups have two or three).  A turn takes about 4 us and 20 KB a us of
+ * X's and A's rows; two workgroups share a CU. */
+static int hk_lora_run_tiles(struct h3_gpu *gpu, const hk_lora_args &a,
+                             hk_lora_low_args &g, uint32_t cus,
+                             uint32_t tile_rows) {
+    const uint32_t k_steps = a.k / HK_BK;
+    const uint32_t rb = a.rank <= 16 ? 1 : a.rank <= 32 ? 2 : 4;
+    const uint32_t turns = std::min(a.count, 3u);
+    g.chunks = (a.rank + 16u * rb - 1) / (16u * rb);
+    uint32_t rows = 2;
     float least = INFINITY;
     for (uint32_t j = 2; j <= 4; j += 2)
-        for (uint32_t p = 1; p <= 16 && p <= k_steps; p++) {
-            const uint32_t steps = (k_steps + p - 1) / p;
-            const uint32_t pieces = (k_steps + steps - 1) / steps;
-            const uint32_t wgs = (m + 16 * j - 1) / (16 * j) * chunks * pieces;
-            const float kb = (float)(steps * (j + rb)) * 2.0f;
-            const float us = (float)((wgs + 2 * cus - 1) / (2 * cus)) *
-                             (4.0f + kb / 20.0f);
-            if (us < least) {
-                least = us;
-                best = {j, pieces, steps};
+        for (uint32_t slots = 1; slots <= turns; slots++)
+            for (uint32_t p = 1; p <= 16 && p <= k_steps; p++) {
+                const uint32_t steps = (k_steps + p - 1) / p;
+                const uint32_t pieces = (k_steps + steps - 1) / steps;
+                const uint32_t groups = (a.m + 16 * j - 1) / (16 * j);
+                const uint32_t wgs = groups * g.chunks * pieces * slots;
+                const float kb = (float)(steps * (j + rb)) * 2.0f;
+                const float us = (float)((wgs + 2 * cus - 1) / (2 * cus)) *
+                                 (float)((turns + slots - 1) / slots) *
+                                 (4.0f + kb / 20.0f);
+                if (us < least) {
+                    least = us;
+                    rows = j;
+                    g.pieces = pieces;
+                    g.piece_steps = steps;
+                    g.slots = slots;
+                    g.row_groups = groups;
+                }
             }
-        }
-    return best;
+    /* the tiles' lists (at most one for every 128 rows), the halves, the sums
+     * of K's pieces */
+    g.ext.low_bytes = (uint32_t)((uint64_t)a.m * a.pitch * 4);
+    const size_t list_bytes = ((size_t)a.m + 127) / 128 * 256 * sizeof(uint4);
+    const size_t low_bytes = ((size_t)g.ext.low_bytes + 255) & ~(size_t)255;
+    uint8_t *space = (uint8_t *)hk_workspace(
+        gpu, list_bytes + low_bytes +
+                 (size_t)g.pieces * a.m * g.sum_pitch * sizeof(float));
+    if (!space) return 0;
+    g.ext.lists = (uint4 *)space;
+    g.ext.low = (const uint16_t *)(space + list_bytes);
+    g.sums = (float *)(space + list_bytes + low_bytes);
+    void (*kernel)(hk_lora_low_args) =
+        rb == 1   ? (rows == 2 ? hk_lora_low<1, 2> : hk_lora_low<1, 4>)
+        : rb == 2 ? (rows == 2 ? hk_lora_low<2, 2> : hk_lora_low<2, 4>)
+                  : (rows == 2 ? hk_lora_low<4, 2> : hk_lora_low<4, 4>);
+    if (g.chunks)
+        hipLaunchKernelGGL(kernel,
+                           dim3((g.row_groups * g.pieces * g.slots + 7u) / 8u *
+                                8u * g.chunks),
+                           dim3(HK_LORA_WAVES * 64), 0, gpu->stream, g);
+    const uint32_t units =
+        (uint32_t)(((uint64_t)a.m * (a.pitch / 8u) + 255) / 256);
+    hipLaunchKernelGGL(hk_lora_halves,
+                       dim3(units + (a.m + tile_rows - 1) / tile_rows),
+                       dim3(256), 0, gpu->stream, g, units, tile_rows);
+    return hk_gemm_bf16(gpu, a.x, a.w, a.bias, a.c, a.m, a.n, a.k,
+                        a.gelu ? HK_EPI_GELU_F32 : HK_EPI_STORE, NULL, 0,
+                        &g.ext);
+}
+
+/* How the skinny GEMM's workgroups run: groups of 32 mbs rows, K in pieces of
+ * `steps` 64-deep steps as the plain skinny GEMM cuts it, while there is one
+ * workgroup a CU. */
+struct hk_lora_cut {
+    uint32_t groups, mbs, columns, pieces, steps, tiles;
+};
+
+static hk_lora_cut hk_lora_cut_of(uint32_t m, uint32_t n, uint32_t k_steps,
+                                  uint32_t cus) {
+    hk_lora_cut c;
+    const uint32_t blocks = (m + 31u) / 32u;
+    c.groups = (blocks + 3u) / 4u;
+    c.mbs = (blocks + c.groups - 1u) / c.groups;
+    c.columns = (n + 127u) / 128u;
+    c.pieces = std::min(cus / (c.columns * c.groups), k_steps / 8u);
+    c.steps = k_steps;
+    if (c.pieces > 1) {
+        c.steps = ((k_steps + c.pieces - 1) / c.pieces + 3u) & ~3u;
+        c.pieces = (k_steps + c.steps - 1) / c.steps;
+    } else {
+        c.pieces = 1;
+    }
+    c.tiles = c.columns * c.pieces * c.groups;
+    if (c.groups > 1) c.tiles = (c.tiles + 7u) & ~7u;
+    return c;
+}
+
+/* The skinny GEMM's workgroups over groups of at most 128 rows. */
+static int hk_lora_run_skinny(struct h3_gpu *gpu, const hk_lora_args &a,
+                              hk_lora_low_args &g, uint32_t cus,
+                              const hk_lora_cut &cut) {
+    const uint32_t k_steps = a.k / HK_BK;
+    g.chunks = g.sum_pitch / 16u;
+    const uint32_t unit_rows = a.m <= 16u ? 16u : 32u;
+    g.row_groups = (a.m + unit_rows - 1u) / unit_rows;
+    /* the adapters of some rows side by side, and a quarter of K each (more
+     * pieces the join would read for every 32 columns).  Over 128 rows there
+     * are no more units than the CUs have places beside W's stream, and pieces
+     * only of a long K: the join of 573 rows x 1280 -> 3420 with ranks of 128
+     * took 25 us with four, 16 with one. */
+    const uint32_t room =
+        cut.groups == 1 ? UINT32_MAX
+                        : 3u * cus / (g.row_groups * std::max(1u, g.chunks));
+    g.slots = std::max(1u, std::min({a.count, unit_rows, room}));
+    const uint32_t most =
+        cut.groups == 1 ? 4u : std::min({4u, room / g.slots, k_steps / 16u});
+    const uint32_t quarters = std::max(1u, most);
+    g.piece_steps = (k_steps + quarters - 1u) / quarters;
+    g.pieces = (k_steps + g.piece_steps - 1) / g.piece_steps;
+    g.units = g.row_groups * g.chunks * g.slots * g.pieces;
+    uint32_t others = g.units + (a.m + 255u) / 256u;
+    if (cut.groups > 1) others = (others + 7u) & ~7u;
+    /* the rows' adapters, the sums of K's pieces */
+    const size_t row_bytes = (size_t)a.m * sizeof(hk_lora_row);
+    uint8_t *space = (uint8_t *)hk_workspace(
+        gpu, row_bytes +
+                 (size_t)g.pieces * a.m * g.sum_pitch * sizeof(float));
+    if (!space) return 0;
+    g.rows = (hk_lora_row *)space;
+    g.sums = (float *)(space + row_bytes);
+
+    hk_skinny_args s = {};
+    s.x = a.x; s.w = a.w; s.bias = a.bias; s.c = a.c;
+    s.m = a.m; s.n = a.n; s.k = a.k;
+    s.x_bytes = g.x_bytes;
+    s.w_bytes = (uint32_t)((uint64_t)a.n * a.k * 2);
+    s.split_steps = cut.steps;
+    s.partial = (float *)hk_splitk_space(
+        gpu, (size_t)cut.groups * cut.pieces * cut.columns * 4 * cut.mbs *
+                 4096);
+    if (!s.partial) return 0;
+    const size_t lds = cut.mbs * 4096 * 4 + 16384;
+    void (*kernel)(hk_skinny_args, hk_lora_low_args, uint32_t, uint32_t,
+                   uint32_t, uint32_t, uint32_t) =
+        cut.groups > 1 ? (cut.mbs == 3 ? hk_lora_skinny<3, 2, true>
+                                       : hk_lora_skinny<4, 2, true>)
+        : a.m <= 16    ? hk_lora_skinny<1, 1, false>
+        : cut.mbs == 1 ? hk_lora_skinny<1, 2, false>
+        : cut.mbs == 2 ? hk_lora_skinny<2, 2, false>
+        : cut.mbs == 3 ? hk_lora_skinny<3, 2, false>
+                       : hk_lora_skinny<4, 2, false>;
+    /* devices (bit = ordinal) whose kernels have their LDS limit raised */
+    static uint64_t ready = 0;
+    const uint64_t bit = 1ull << (gpu->device & 63);
+    if (cut.mbs == 4 && !(ready & bit)) {
+        (void)hipFuncSetAttribute((const void *)hk_lora_skinny<4, 2, false>,
+                                  hipFuncAttributeMaxDynamicSharedMemorySize,
+                                  (int)lds);
+        (void)hipFuncSetAttribute((const void *)hk_lora_skinny<4, 2, true>,
+                                  hipFuncAttributeMaxDynamicSharedMemorySize,
+                                  (int)lds);
+        ready |= bit;
+    }
+    hipLaunchKernelGGL(kernel, dim3(cut.tiles + others), dim3(256), lds,
+                       gpu->stream, s, g, cut.columns, cut.pieces, cut.groups,
+                       cut.tiles <= 2u * cus ? 0u : others, cut.tiles);
+    hipLaunchKernelGGL(hk_lora_join,
+                       dim3(((a.n + 31) / 32 * cut.mbs + 3) / 4, cut.groups),
+                       dim3(256), 0, gpu->stream, s, g, cut.mbs,
+                       cut.columns * 4, cut.pieces, a.gelu);
+    return 1;
+}
+
+/* Estimated microseconds over 128 rows: a step takes 0.65 us with one
+ * workgroup on a CU and 1.1 with two, the pieces' sums go both ways at 4.5
+ * TB/s (160 to 4000 rows of eight K x N: within 20%).  Skinny workgroups and
+ * tiles, measured with one adapter of rank 16 (us): 160 x 320 -> 5120 12.5 and
+ * 24.6, 1200 rows 28.3 and 26.2; 512 x 512 -> 1536 14.2 and 31.1, 4000 rows
+ * 32.4 and 43.5; 160 x 5120 -> 5120 25.6 and 39.1, 384 38.4 and 46.0, 512 58.8
+ * and 54.2; 160 x 5120 -> 13824 56.0 and 72.2, 384 109 and 84. */
+static float hk_lora_skinny_us(const hk_lora_cut &c, uint32_t m, uint32_t n,
+                               uint32_t cus) {
+    const uint32_t rounds = (c.tiles + 2 * cus - 1) / (2 * cus);
+    return (float)rounds * (float)c.steps * (c.tiles <= cus ? 0.65f : 1.1f) +
+           6.0f +
+           (float)m * (float)n * (float)(8 * c.pieces + 2) / 4.5e6f;
 }
 
 static int hk_lora_run(struct h3_gpu *gpu, const hk_lora_args &a) {
     const uint32_t cus = gpu->num_cus > 0 ? (uint32_t)gpu->num_cus : 256u;
-    const uint32_t k_steps = a.k / HK_BK;
-    const bool tall = a.m > 128u;
     hk_lora_low_args g = {};
     g.x = a.x;
     g.m = a.m; g.k = a.k;
@@ -733,109 +999,17 @@ static int hk_lora_run(struct h3_gpu *gpu, const hk_lora_args &a) {
     g.ext.count = a.count;
     g.ext.map = a.map;
     g.ext.pitch = 2u * a.pitch;
-    g.ext.low_bytes = tall ? (uint32_t)((uint64_t)a.m * a.pitch * 4) : 0u;
     g.sum_pitch = (a.rank + 15u) & ~15u;
-    g.slots = 1;
-    uint32_t rb = 1;
-    if (tall) {
-        rb = a.rank <= 16 ? 1 : a.rank <= 32 ? 2 : 4;
-        g.chunks = (a.rank + 16u * rb - 1) / (16u * rb);
-        const hk_lora_plan plan =
-            hk_lora_plan_of(a.m, k_steps, rb, g.chunks, cus);
-        g.pieces = plan.pieces;
-        g.piece_steps = plan.steps;
-        g.row_groups = (a.m + 16u * plan.j - 1) / (16u * plan.j);
-        rb |= plan.j << 8;
-    } else {
-        /* beside W's stream: a quarter of K each, while the pieces stay few
-         * against what the join reads for every 32 columns */
-        g.chunks = g.sum_pitch / 16u;
-        const uint32_t group = a.m <= 16u ? 16u : 32u;
-        g.row_groups = (a.m + group - 1u) / group;
-        g.slots = a.count < group ? a.count : group;
-        g.piece_steps = (k_steps + 3u) / 4u;
-        g.pieces = (k_steps + g.piece_steps - 1) / g.piece_steps;
-        g.units = g.row_groups * g.chunks * g.slots * g.pieces;
-    }
-    /* the tiles' lists (at most one for every 128 rows) or the rows' adapters,
-     * the halves, the sums of K's pieces */
-    const size_t list_bytes =
-        tall ? ((size_t)a.m + 127) / 128 * 256 * sizeof(uint4)
-             : 128 * sizeof(hk_lora_row);
-    const size_t low_bytes = ((size_t)g.ext.low_bytes + 255) & ~(size_t)255;
-    const size_t sum_bytes =
-        (size_t)g.pieces * a.m * g.sum_pitch * sizeof(float);
-    uint8_t *space =
-        (uint8_t *)hk_workspace(gpu, list_bytes + low_bytes + sum_bytes);
-    if (!space) return 0;
-    g.ext.lists = (uint4 *)space;
-    g.rows = (hk_lora_row *)space;
-    g.ext.low = (const uint16_t *)(space + list_bytes);
-    g.sums = (float *)(space + list_bytes + low_bytes);
-
-    if (tall) {
-        void (*kernel)(hk_lora_low_args) =
-            rb == 0x201   ? hk_lora_low<1, 2>
-            : rb == 0x202 ? hk_lora_low<2, 2>
-            : rb == 0x204 ? hk_lora_low<4, 2>
-            : rb == 0x401 ? hk_lora_low<1, 4>
-            : rb == 0x402 ? hk_lora_low<2, 4>
-                          : hk_lora_low<4, 4>;
-        if (g.chunks)
-            hipLaunchKernelGGL(
-                kernel,
-                dim3((g.row_groups * g.pieces + 7u) / 8u * 8u * g.chunks),
-                dim3(HK_LORA_WAVES * 64), 0, gpu->stream, g);
-        const uint32_t tile_rows = hk_gemm_tile_rows(gpu, a.m, a.n, a.k);
-        const uint32_t units =
-            (uint32_t)(((uint64_t)a.m * (a.pitch / 8u) + 255) / 256);
-        hipLaunchKernelGGL(hk_lora_halves,
-                           dim3(units + (a.m + tile_rows - 1) / tile_rows),
-                           dim3(256), 0, gpu->stream, g, units, tile_rows);
-        return hk_gemm_bf16(gpu, a.x, a.w, a.bias, a.c, a.m, a.n, a.k,
-                            a.gelu ? HK_EPI_GELU_F32 : HK_EPI_STORE, NULL, 0,
-                            &g.ext);
-    }
-
-    const uint32_t mbs = (a.m + 31u) / 32u, columns = (a.n + 127u) / 128u;
-    hk_skinny_args s = {};
-    s.x = a.x; s.w = a.w; s.bias = a.bias; s.c = a.c;
-    s.m = a.m; s.n = a.n; s.k = a.k;
-    s.x_bytes = g.x_bytes;
-    s.w_bytes = (uint32_t)((uint64_t)a.n * a.k * 2);
-    /* pieces as the plain skinny GEMM cuts them */
-    uint32_t pieces = min(cus / columns, k_steps / 8u);
-    s.split_steps = k_steps;
-    if (pieces > 1) {
-        s.split_steps = ((k_steps + pieces - 1) / pieces + 3u) & ~3u;
-        pieces = (k_steps + s.split_steps - 1) / s.split_steps;
-    } else {
-        pieces = 1;
-    }
-    s.partial = (float *)hk_splitk_space(
-        gpu, (size_t)pieces * columns * 4 * mbs * 4096);
-    if (!s.partial) return 0;
-    const size_t lds = mbs * 4096 * 4 + 16384;
-    void (*kernel)(hk_skinny_args, hk_lora_low_args, uint32_t, uint32_t) =
-        a.m <= 16  ? hk_lora_skinny<1, 1>
-        : mbs == 1 ? hk_lora_skinny<1, 2>
-        : mbs == 2 ? hk_lora_skinny<2, 2>
-        : mbs == 3 ? hk_lora_skinny<3, 2>
-                   : hk_lora_skinny<4, 2>;
-    /* devices (bit = ordinal) whose kernel has its LDS limit raised */
-    static uint64_t ready = 0;
-    const uint64_t bit = 1ull << (gpu->device & 63);
-    if (mbs == 4 && !(ready & bit)) {
-        (void)hipFuncSetAttribute((const void *)hk_lora_skinny<4, 2>,
-                                  hipFuncAttributeMaxDynamicSharedMemorySize,
-                                  (int)lds);
-        ready |= bit;
-    }
-    hipLaunchKernelGGL(kernel, dim3(g.units + 1 + columns * pieces), dim3(256),
-                       lds, gpu->stream, s, g, columns, pieces);
-    hipLaunchKernelGGL(hk_lora_join, dim3((a.n + 31) / 32 * mbs), dim3(64), 0,
-                       gpu->stream, s, g, mbs, columns * 4, pieces, a.gelu);
-    return 1;
+    const hk_lora_cut cut = hk_lora_cut_of(a.m, a.n, a.k / HK_BK, cus);
+    if (cut.groups == 1) return hk_lora_run_skinny(gpu, a, g, cus, cut);
+    float us;
+    const uint32_t tile_rows = hk_gemm_tile_rows(gpu, a.m, a.n, a.k, &us);
+    /* over tiles, the first product and the halves come before the GEMM, and
+     * several adapters to a tile are more steps of it */
+    us += a.count > 1 ? 18.0f : 14.0f;
+    return hk_lora_skinny_us(cut, a.m, a.n, cus) < us
+               ? hk_lora_run_skinny(gpu, a, g, cus, cut)
+               : hk_lora_run_tiles(gpu, a, g, cus, tile_rows);
 }
 
 /* elements of an adapter's fragments, a multiple of 512 */

@@ -46,8 +46,8 @@
  * is a register result the compiler waits for), synchronises, stages
  * X(s + XA) into the buffer every wave finished reading in step s - 1, issues
  * W(s + 3) and computes. */
-/* the non-temporal (streaming) cache policy of a buffer load */
-enum { HK_LOAD_ONCE = 2 };
+/* cache policies of W's loads: non-temporal (streaming), and as usual */
+enum { HK_LOAD_ONCE = 2, HK_LOAD_SHARED = 0 };
 
 struct hk_skinny_args {
     const uint16_t *x, *w, *bias;
@@ -66,7 +66,7 @@ struct hk_skinny_args {
 };
 
 /* Workgroup (x, y, z) of `columns` x `pieces` ones a problem. */
-template <int MB, int XA>
+template <int MB, int XA, int W_POLICY = HK_LOAD_ONCE>
 __device__ __forceinline__ void hk_skinny_tile(const hk_skinny_args &g,
                                                uint32_t x, uint32_t y,
                                                uint32_t z, uint32_t columns,
@@ -126,7 +126,7 @@ __device__ __forceinline__ void hk_skinny_tile(const hk_skinny_args &g,
         for (int q = 0; q < 4; q++)
             wf[slot][q] = __builtin_amdgcn_raw_buffer_load_b128(
                 wr, hk_skinny_lane(wo[q], step, steps),
-                hk_skinny_k_bytes(base + step, k / 64u), HK_LOAD_ONCE);
+                hk_skinny_k_bytes(base + step, k / 64u), W_POLICY);
     };
     /* fragment of X rows mb*32 + row, logical chunk 2q + half */
     auto read_x = [&](int buf, int mb, int q) {

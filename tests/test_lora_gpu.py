@@ -109,6 +109,19 @@ def test_long_and_wide(gpu, rows, k, n):
                     scale=0.02))
 
 
+@pytest.mark.parametrize("rows,k,n", [
+    (129, 64, 132), (200, 64, 4), (300, 192, 4100), (417, 448, 1004),
+    (545, 2688, 260), (641, 320, 5120), (1800, 512, 388), (259, 1280, 12900)])
+def test_groups_of_rows(gpu, rows, k, n):
+    """Over 128 rows of few steps of K: groups of 96 and 128 rows, a last one
+    of few, whole sums and pieces, one round of workgroups and more."""
+    check(gpu, make(rows + n, blocks((rows // 2, 1), (rows // 4, NONE),
+                                     (rows - rows // 2 - rows // 4, 0)),
+                    [64, 16], k, n))
+    check(gpu, make(rows + k, spread(rows, 4, 2), [16, 40, 8, 100], k, n,
+                    bias=False), True)
+
+
 def test_no_row_has_an_adapter(gpu):
     """The same as the projection alone, to its own rounding."""
     for rows in (7, 128, 300):
