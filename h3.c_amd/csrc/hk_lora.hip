@@ -810,7 +810,10 @@ static bool hk_lora_takes(const struct h3_gpu *gpu, const hk_lora_args &g) {
  * The first product by itself: 16 RB ranks and 16 J rows a workgroup, K in
  * pieces, the adapters of a row group over slots (of several requests' rows
  * some groups have two or three).  A turn takes about 4 us and 20 KB a us of
- * X's and A's rows; two workgroups share a CU. */
+ * X's and A's rows, a piece 0.35 us for its sums; two workgroups share a CU.
+ * Within a third of the best of 14 shapes of launch: 778 rows x 7168, rank 16,
+ * 8.4 us (in one piece 20), 4756 x 5376, ranks up to 64, 25 (44), 6144 x 5120,
+ * up to 128, 36 (34 to 55). */
 static int hk_lora_run_tiles(struct h3_gpu *gpu, const hk_lora_args &a,
                              hk_lora_low_args &g, uint32_t cus,
                              uint32_t tile_rows) {
@@ -826,11 +829,15 @@ static int hk_lora_run_tiles(struct h3_gpu *gpu, const hk_lora_args &a,
                 const uint32_t steps = (k_steps + p - 1) / p;
                 const uint32_t pieces = (k_steps + steps - 1) / steps;
                 const uint32_t groups = (a.m + 16 * j - 1) / (16 * j);
-                const uint32_t wgs = groups * g.chunks * pieces * slots;
+                /* four workgroups that find no adapter in a turn's time; a
+                 * group's further turns come once, at the end */
+                const uint32_t wgs =
+                    groups * g.chunks * pieces * (3 + slots) / 4;
                 const float kb = (float)(steps * (j + rb)) * 2.0f;
-                const float us = (float)((wgs + 2 * cus - 1) / (2 * cus)) *
-                                 (float)((turns + slots - 1) / slots) *
-                                 (4.0f + kb / 20.0f);
+                const float us = (float)((wgs + 2 * cus - 1) / (2 * cus) +
+                                         (turns + slots - 1) / slots - 1) *
+                                     (4.0f + kb / 20.0f) +
+                                 0.35f * (float)pieces;
                 if (us < least) {
                     least = us;
                     rows = j;
