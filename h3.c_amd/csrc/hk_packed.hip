@@ -625,124 +625,172 @@ static bool hk_packed_takes(const struct h3_gpu *gpu,
  * less evenly took a second round, 50 us for 43).  Longest first; items of no
  * rows fill the shorter queues.
  *
- * Where items are few and long, they are cut into pieces of at most `most`
- * tiles: the length with which the last of the CUs' places (two workgroups a
- * CU) ends first, each taking the next item when it is free, with 8 tiles'
- * time for the join. */
+ * Items are cut into pieces by when the last of the places that take one after
+ * the other would end, the join's time included:
+ * - all items, where they are few and long (the longest over a place's share of
+ *   the work), so that two workgroups a CU keep its loads going;
+ * - those behind the last full round of one item a CU, where that promises 5%
+ *   (two workgroups of matrix products share what one alone would get, so a
+ *   CU is one place; self-attention in us, uncut and cut: 1200 rows x 56
+ *   heads, 2.2 rounds, 62.8 and 54.8; 2378 x 56, 4.2, 189 and 173; 2560 x 40,
+ *   3.1, 158 and 148; counted as two places a CU, 2185 x 40, 2.8 rounds, was
+ *   cut and took 129 for 113). */
 struct hk_packed_work {
     std::vector<hk_packed_item> items;
     std::vector<hk_packed_join> joins;
     uint32_t parts, join_rows;
 };
 
-struct hk_packed_sized {
+/* Items [first, first + count) of a request: kv_head * blocks + block of its
+ * rows. */
+struct hk_packed_run {
     uint32_t request, tiles, rows, blocks;
+    uint64_t first, count;
+    uint32_t pieces, per; /* of each item, in tiles */
 };
 
-static const float hk_packed_own = 3.0f;
+static const float hk_packed_own = 3.0f, hk_packed_join_time = 8.0f;
 
-/* The pieces of an item of `tiles` tiles, and each one's length. */
-static uint32_t hk_packed_pieces(uint32_t tiles, uint32_t most,
-                                 uint32_t &per) {
-    uint32_t pieces = tiles > most ? (tiles + most - 1) / most : 1;
-    per = pieces > 1 ? (tiles + pieces - 1) / pieces : tiles;
-    return pieces > 1 ? (tiles + per - 1) / per : 1;
+/* Cuts the run's items into pieces of at most `most` tiles. */
+static void hk_packed_cut(hk_packed_run &r, uint32_t most) {
+    r.pieces = r.tiles > most ? (r.tiles + most - 1) / most : 1;
+    r.per = r.pieces > 1 ? (r.tiles + r.pieces - 1) / r.pieces : r.tiles;
+    r.pieces = r.pieces > 1 ? (r.tiles + r.per - 1) / r.per : 1;
 }
 
-/* When the last place ends, in tiles. */
-static float hk_packed_end(const std::vector<hk_packed_sized> &order,
-                           uint32_t kv_heads, uint32_t places, uint32_t most) {
-    std::priority_queue<float, std::vector<float>, std::greater<float>> free;
-    for (uint32_t i = 0; i < places; i++) free.push(0.0f);
-    float end = 0.0f;
+/* When the last place ends, in tiles.  `end` is sorted: the places before the
+ * first one's end after an item of length t take one each, in order, before
+ * any takes its second. */
+static float hk_packed_end(const std::vector<hk_packed_run> &runs,
+                           uint32_t places) {
+    std::vector<float> end(places, 0.0f);
     bool cut = false;
-    for (const hk_packed_sized &s : order) {
-        uint32_t per;
-        const uint32_t pieces = hk_packed_pieces(s.tiles, most, per);
-        cut |= pieces > 1;
-        const uint64_t count = (uint64_t)s.blocks * kv_heads * pieces;
-        for (uint64_t i = 0; i < count; i++) {
-            const float t = free.top() + (float)per + hk_packed_own;
-            free.pop();
-            free.push(t);
-            end = std::max(end, t);
+    for (size_t i = 0; i < runs.size();) {
+        const float t = (float)runs[i].per + hk_packed_own;
+        uint64_t left = 0;
+        for (const uint32_t per = runs[i].per;
+             i < runs.size() && runs[i].per == per; i++) {
+            cut |= runs[i].pieces > 1;
+            left += runs[i].count * runs[i].pieces;
+        }
+        while (left) {
+            const auto until = std::upper_bound(end.begin(), end.end(),
+                                                end.front() + t);
+            const uint64_t n =
+                std::min<uint64_t>(left, (uint64_t)(until - end.begin()));
+            for (uint64_t j = 0; j < n; j++) end[j] += t;
+            std::inplace_merge(end.begin(), end.begin() + (ptrdiff_t)n,
+                               end.end());
+            left -= n;
         }
     }
-    return end + (cut ? 8.0f : 0.0f);
+    return end.back() + (cut ? hk_packed_join_time : 0.0f);
 }
 
 static void hk_packed_lay_out(const std::vector<hk_packed_request> &list,
                               uint32_t group, uint32_t kv_heads, uint32_t cus,
                               hk_packed_work &work) {
     const uint32_t qb = HK_PACKED_QB, places = cus * 2u;
-    std::vector<hk_packed_sized> order;
+    std::vector<hk_packed_run> runs;
     double total = 0.0;
     uint64_t items = 0;
     for (uint32_t i = 0; i < list.size(); i++) {
         const uint32_t rows = list[i].q_rows * group;
-        const hk_packed_sized s = {
-            i, (uint32_t)(((uint64_t)list[i].kv_rows + HK_KT - 1) / HK_KT),
-            rows, (uint32_t)(((uint64_t)rows + qb - 1) / qb)};
-        order.push_back(s);
-        items += (uint64_t)s.blocks * kv_heads;
-        total += (double)s.blocks * kv_heads * (s.tiles + hk_packed_own);
+        const uint32_t tiles =
+            (uint32_t)(((uint64_t)list[i].kv_rows + HK_KT - 1) / HK_KT);
+        const uint32_t blocks = (uint32_t)(((uint64_t)rows + qb - 1) / qb);
+        const uint64_t count = (uint64_t)blocks * kv_heads;
+        runs.push_back({i, tiles, rows, blocks, 0, count, 1, tiles});
+        items += count;
+        total += (double)count * (tiles + hk_packed_own);
     }
-    std::stable_sort(order.begin(), order.end(),
-                     [](const hk_packed_sized &x, const hk_packed_sized &y) {
+    std::stable_sort(runs.begin(), runs.end(),
+                     [](const hk_packed_run &x, const hk_packed_run &y) {
                          return x.tiles > y.tiles;
                      });
-    uint32_t most = UINT32_MAX;
     /* (many items come out level whole) */
-    if (!order.empty() && items <= 8ull * places &&
-        order[0].tiles > total / places) {
-        float best = hk_packed_end(order, kv_heads, places, most);
+    if (!runs.empty() && items <= 16ull * places) {
+        std::vector<hk_packed_run> chosen = runs;
         const uint32_t share = (uint32_t)(total / places) + 1u;
-        uint32_t tried = 0;
-        for (uint32_t i = 4; i <= 24; i++) { /* half to three times a share */
-            const uint32_t length = std::max(4u, share * i / 8u);
-            if (length == tried || length >= order[0].tiles) continue;
-            tried = length;
-            const float end = hk_packed_end(order, kv_heads, places, length);
-            if (end < best) {
-                best = end;
-                most = length;
+        if (runs[0].tiles >= share) { /* few and long */
+            float best = hk_packed_end(runs, places);
+            uint32_t tried = 0;
+            for (uint32_t i = 4; i <= 24; i++) { /* half to three shares */
+                const uint32_t length = std::max(4u, share * i / 8u);
+                if (length == tried || length >= runs[0].tiles) continue;
+                tried = length;
+                std::vector<hk_packed_run> cut = runs;
+                for (hk_packed_run &r : cut) hk_packed_cut(r, length);
+                const float end = hk_packed_end(cut, places);
+                if (end < best) {
+                    best = end;
+                    chosen = cut;
+                }
+            }
+        } else if (items % cus) {
+            std::vector<hk_packed_run> head, tail;
+            uint64_t whole = items - items % cus;
+            double rest = 0.0;
+            for (const hk_packed_run &r : runs) {
+                hk_packed_run h = r, t = r;
+                h.count = std::min(whole, r.count);
+                t.first = h.count;
+                t.count = r.count - h.count;
+                whole -= h.count;
+                rest += (double)t.count * t.tiles;
+                if (h.count) head.push_back(h);
+                if (t.count) tail.push_back(t);
+            }
+            float best = 0.95f * hk_packed_end(runs, cus);
+            for (uint32_t i = 4; i <= 8; i++) { /* one to two shares */
+                const uint32_t length =
+                    std::max(4u, (uint32_t)(rest / cus * i / 4) + 1u);
+                std::vector<hk_packed_run> cut = head;
+                for (hk_packed_run r : tail) {
+                    hk_packed_cut(r, length);
+                    cut.push_back(r);
+                }
+                const float end = hk_packed_end(cut, cus);
+                if (end < best) {
+                    best = end;
+                    chosen = cut;
+                }
             }
         }
+        runs = chosen;
     }
     std::vector<hk_packed_item> queue[8];
     double load[8] = {};
     work.parts = work.join_rows = 0;
-    for (const hk_packed_sized &s : order) {
+    for (const hk_packed_run &s : runs) {
         const hk_packed_request &r = list[s.request];
-        uint32_t per;
-        const uint32_t pieces = hk_packed_pieces(s.tiles, most, per);
-        const uint64_t count = (uint64_t)s.blocks * kv_heads;
         for (uint64_t run = 0; run < 8; run++) {
             /* the longer runs are the last ones */
-            const uint64_t end = count * (run + 1) / 8;
-            uint64_t i = count * run / 8;
+            const uint64_t end = s.first + s.count * (run + 1) / 8;
+            uint64_t i = s.first + s.count * run / 8;
             auto &q = *std::min_element(
                 queue, queue + 8, [&](const auto &x, const auto &y) {
                     return load[&x - queue] < load[&y - queue];
                 });
             load[&q - queue] +=
-                (double)(end - i) * (s.tiles + hk_packed_own * pieces);
+                (double)(end - i) * (s.tiles + hk_packed_own * s.pieces);
             for (; i < end; i++) {
                 hk_packed_item item = {r.q_first, s.rows,
                                        (uint32_t)(i % s.blocks) * qb,
                                        (uint32_t)(i / s.blocks), r.kv_first,
                                        r.kv_rows, 0, s.tiles,
                                        HK_PACKED_WHOLE};
-                if (pieces > 1) {
+                if (s.pieces > 1) {
                     work.joins.push_back({r.q_first, s.rows, item.row,
-                                          item.kv_head, work.parts, pieces});
+                                          item.kv_head, work.parts,
+                                          s.pieces});
                     work.join_rows = std::max(
                         work.join_rows, std::min(s.rows - item.row, qb));
                 }
-                for (uint32_t p = 0; p < pieces; p++) {
-                    item.tile = p * per;
-                    item.tile_end = std::min(s.tiles, item.tile + per);
-                    if (pieces > 1) item.part = work.parts++;
+                for (uint32_t p = 0; p < s.pieces; p++) {
+                    item.tile = p * s.per;
+                    item.tile_end = std::min(s.tiles, item.tile + s.per);
+                    if (s.pieces > 1) item.part = work.parts++;
                     q.push_back(item);
                 }
             }

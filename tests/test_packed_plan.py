@@ -161,3 +161,16 @@ def test_flash_kernels_wait_for_their_transposed_reads():
     for name, body in found.items():
         assert any("ds_read_b64_tr_b16" in l for l in body), name
         assert not _offenders(body), (name, _offenders(body)[:3])
+
+
+def test_items_behind_the_last_full_round_are_cut():
+    # 1064 items on 256 CUs: the last 40 in pieces, the others whole
+    made, items, joins = cover(([2378], [2378], 56, 56, 128))
+    assert len(joins) == 40 and len(made) == 2
+    assert sum(items[:, 8] == WHOLE) == 1024
+    made, items, joins = cover(([77, 1200], [77, 1200], 56, 56, 128))
+    assert len(joins) and len(made) == 2
+    # five rounds, and 2.8
+    for rows in (4096, 2185):
+        made, items, joins = cover(([rows], [rows], 40, 40, 128))
+        assert not len(joins) and len(made) == 1
