@@ -249,6 +249,42 @@ def test_calls_queued_one_after_the_other(gpu):
         ro.check(gpu.read_bf16(y), want, bound)
 
 
+@pytest.mark.parametrize("rows,adapters,k,n", [
+    (100, 100, 256, 320), (128, 70, 64, 132), (300, 280, 192, 260),
+    (2000, 300, 320, 5120)])
+def test_more_adapters_than_lanes_or_rows_of_a_tile(gpu, rows, adapters, k, n):
+    check(gpu, make(20, np.arange(rows) * 7 % adapters, [2] * adapters, k, n))
+
+
+def test_two_contexts_at_once(gpu):
+    """Each with its own scratch; a table serves both."""
+    import h3hip
+    with h3hip.Gpu() as other:
+        a = make(21, spread(500, 3, 1), [16, 8, 40], 512, 768)
+        b = make(22, spread(90, 3, 2), [64, 4, 20], 1024, 512)
+        shared = table_of(gpu, a)
+        made = []
+        for g, c, table in ((gpu, a, shared), (other, a, shared),
+                            (gpu, b, None), (other, b, None)):
+            made.append((g, c, table or table_of(g, c),
+                         [g.new_bf16(len(c["ids"]) * c["n"]) for _ in "123"],
+                         g.bf16(c["x"]), g.bf16(c["w"]), g.bf16(c["b"]),
+                         g.u32(c["ids"])))
+        gpu.begin()
+        other.begin()
+        for turn in range(3):
+            for g, c, table, y, x, w, bias, ids in made:
+                g.check(g.L.h3_hip_linear_lora_bf16(
+                    g.h, y[turn], x, w, bias, table, ids, len(c["ids"]),
+                    c["k"], c["n"]))
+        other.submit()
+        gpu.submit()
+        for g, c, table, y, *_ in made:
+            want, bound = ro.lora(**c)
+            for t in y:
+                ro.check(g.read_bf16(t), want, bound)
+
+
 def test_simple_kernels(gpu):
     """H3_HIP_REFERENCE=1 takes the sequential kernels, at the same bounds."""
     code = """

@@ -275,6 +275,53 @@ def test_keys_of_no_weight_before_far_lower_ones(gpu, dim):
         ro.check(got, want, bound)
 
 
+@pytest.mark.parametrize("dim", [64, 72, 128])
+def test_rows_that_lie_past_four_gigabytes(gpu, dim):
+    """Row strides of 16 MB: 330 key rows over 5 GB."""
+    a = Case(23, [3, 2], [129, 201], 1, 1, dim)
+    compact = gpu.bf16(a.kvs)
+    stride = (1 << 23) + 8
+    q, kv = gpu.bf16(a.q), gpu.new_bf16((a.kv - 1) * stride + 2 * dim)
+    gpu.begin()
+    for r in range(a.kv):
+        gpu.check(gpu.L.h3_gpu_copy_bf16(gpu.h, kv, r * stride, compact,
+                                         r * 2 * dim, 2 * dim))
+    gpu.submit()
+    plan = gpu.sdpa_packed_plan(a.qf, a.qn, a.kf, a.kn, 1, 1, dim)
+    y = gpu.new_bf16(a.rows * dim)
+    gpu.run("h3_hip_sdpa_packed_bf16", y, q, 0, a.qs, kv, 0, kv, dim, stride,
+            plan, a.scale)
+    got = gpu.read_bf16(y).reshape(a.rows, 1, dim)
+    gpu.free(kv)
+    want, bound, _ = a.want()
+    ro.check(got, want, bound)
+    assert (got == a.run(gpu)).all()
+
+
+def test_two_contexts_at_once(gpu):
+    """Each with its own sums of pieces; a plan serves both."""
+    import h3hip
+    with h3hip.Gpu() as other:
+        a = Case(24, [1, 2], [9720, 5000], 8, 2, 128)
+        plan = gpu.sdpa_packed_plan(a.qf, a.qn, a.kf, a.kn, 8, 2, 128)
+        n = a.rows * 8 * 128
+        made = [(g, [g.new_bf16(n) for _ in range(4)], g.bf16(a.q),
+                 g.bf16(a.kvs)) for g in (gpu, other)]
+        gpu.begin()
+        other.begin()
+        for turn in range(4):
+            for g, y, q, kv in made:
+                g.check(g.L.h3_hip_sdpa_packed_bf16(
+                    g.h, y[turn], q, 0, a.qs, kv, 0, kv, 256, a.ks, plan,
+                    a.scale))
+        other.submit()
+        gpu.submit()
+        want, bound, _ = a.want()
+        for g, y, *_ in made:
+            for t in y:
+                ro.check(g.read_bf16(t).reshape(a.rows, 8, 128), want, bound)
+
+
 def test_the_same_call_gives_the_same_bits(gpu):
     for a in (Case(13, [1, 1, 2], [9000, 33, 700], 8, 1, 128),
               Case(14, [300, 40], [400, 1300], 4, 4, 64)):
