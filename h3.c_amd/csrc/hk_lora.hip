@@ -11,11 +11,20 @@
  *
  * The products run in two parts.  x . A_a^T goes to scratch in F32, in pieces
  * of K (hk_lora_low_unit).  Their sum times s_a, as two bf16 halves, meets
- * B_a: as a few more steps of K of the projection's own GEMM over 128 rows
- * (hk_lora_halves, hk_gemm_lora), in the sum of the skinny GEMM's pieces up to
- * 128 (hk_lora_join).  Two halves because the matrix cores take bf16: one
- * would round the adapters' part to 8 bits before it is added, two keep 16,
- * below what F32 sums of that length keep.
+ * B_a: up to 128 rows, and where the projection has few tiles or steps of K,
+ * in the sum of the skinny GEMM's pieces (hk_lora_skinny, hk_lora_join), else
+ * as a few more steps of K of the projection's own GEMM (hk_lora_halves,
+ * hk_gemm_lora).  Two halves because the matrix cores take bf16: one would
+ * round the adapters' part to 8 bits before it is added, two keep 16, below
+ * what F32 sums of that length keep.  The activation takes the F32 sum.
+ *
+ * Measured, in brackets the projection alone in the same run (us): 8 rows x
+ * 5120 -> 5120, eight adapters of rank 16, 16.8 (13.7); 39 x 2688 -> 96768
+ * 101 (87), 5.3 TB/s; 197 x 5120 -> 5376 32 (36); 778 x 7168 -> 5376 90 (84);
+ * 4756 x 5376 -> 21504, ranks 64 and 4, 828 (805), 1.34 PFLOP/s; 6144 x 5120
+ * -> 13824 with GELU, ranks up to 128, 690 (667).  W's bytes bound the first
+ * two, launches and the chains of dependent loads in them beside that, the
+ * matrix cores at the package's power limit the last two.
  *
  * The simple kernels here (one wave per element of x . A^T, one thread per
  * output, sums in sequence) serve H3_HIP_REFERENCE=1 and the shapes that the
@@ -178,7 +187,8 @@ static int hk_lora_run_simple(struct h3_gpu *gpu, hk_lora_args &g) {
  * by how fast a CU takes them, so two turns of DEEP steps are in flight (about
  * 190 registers), and a load takes 8 whole 128-byte lines: loaded as fragments
  * (16 half lines each), 197 rows x 5120 took 13.0 us for 16 ranks and 27 for
- * 64, and 6144 rows 34 for 64; as whole lines 6.9, 12.3 and 18.5.  The lines
+ * 64, and 6144 rows 34 for 64; as whole lines 6.9, 12.3 and 18.5 (one adapter,
+ * one piece, by itself).  The lines
  * turn into fragments in LDS of the wave's own, with the GEMM's swizzle; a
  * wave's LDS operations run in order, so one step's room is enough. */
 #define HK_LORA_WAVES 4
@@ -474,8 +484,8 @@ __device__ __forceinline__ void hk_lora_split(const hk_f32x4 (&u)[2],
 
 /* The halves that the GEMM takes (hk_lora_ext), zeros up to the padded rank:
  * workgroups [0, units) of 256 threads, a thread 8 ranks of a row.  The others
- * list the adapters of a row tile each: the least that is left, over and
- * over. */
+ * list the adapters of a row tile each: the least that is left, over and over.
+ * 5 us, whatever the rows: the launch and three loads in sequence. */
 __global__ void __launch_bounds__(256)
 hk_lora_halves(hk_lora_low_args g, uint32_t units, uint32_t tile_rows) {
     const hk_lora_ext &x = g.ext;
@@ -754,7 +764,14 @@ hk_lora_skinny(hk_skinny_args s, hk_lora_low_args g, uint32_t columns,
 }
 
 /* C = act(pieces' sums + bias + s_a (x . A^T) . B^T) for 32 columns and 32
- * rows, a wave; blockIdx.y is the row group. */
+ * rows, a wave; blockIdx.y is the row group.  Bound by its chain of loads (the
+ * row, its first ranks and the pieces; B; 7 us at 8 rows x 5120) and by how
+ * many waves a CU holds: five workgroups (994 rows x 5120 took 16.3 us with
+ * four, 14.4 with five; 39 rows x 96768 13.8).  Tried and slower: 32 ranks at
+ * a time, all ranks of an adapter in sequence (8 rows with an adapter each 15
+ * us), and the same in the skinny workgroups behind whole sums, where the
+ * chain has one wave to hide in (160 rows x 320 -> 5120 32 us against 15 with
+ * four adapters of up to 64). */
 __global__ void __launch_bounds__(256, 5)
 hk_lora_join(hk_skinny_args s, hk_lora_low_args g, uint32_t mbs,
              uint32_t tiles, uint32_t pieces, int gelu) {
@@ -1014,7 +1031,8 @@ static int hk_lora_run(struct h3_gpu *gpu, const hk_lora_args &a) {
     /* over tiles, the first product and the halves come before the GEMM, and
      * several adapters to a tile are more steps of it */
     us += a.count > 1 ? 18.0f : 14.0f;
-    return hk_lora_skinny_us(cut, a.m, a.n, cus) < us
+    return cut.groups <= 65535u && /* a grid's second dimension */
+                   hk_lora_skinny_us(cut, a.m, a.n, cus) < us
                ? hk_lora_run_skinny(gpu, a, g, cus, cut)
                : hk_lora_run_tiles(gpu, a, g, cus, tile_rows);
 }

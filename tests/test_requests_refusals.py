@@ -157,3 +157,25 @@ out.append(call(plan=plan(qn=[0, 0])))
 """)
     assert all(not error and launched for error, launched in out[:-1]), out
     assert out[-1] == ["", 0]
+
+
+@pytest.mark.parametrize("m,k,n", [(8_400_000, 64, 4), (129, 64, 1 << 22),
+                                   (70_000, 64, 4096), (128, 64, 1 << 24)])
+def test_adapter_launches_stay_within_a_grid(m, k, n):
+    """Threads of a launch below 2^32 and its second dimension below 2^16, for
+    the most rows and columns too."""
+    made = on_fake("""
+x, w = gpu.new_bf16(m * k), gpu.new_bf16(n * k)
+y, ids = gpu.new_bf16(m * n), gpu.L.h3_gpu_tensor_from_u32(gpu.h, None, m)
+tables = []
+for rank in (4, 64):
+    d, u = gpu.new_bf16(rank * k), gpu.new_bf16(rank * n)
+    tables.append(gpu.lora_table([d] * 3, [u] * 3, [rank] * 3, [1.0] * 3, k, n))
+gpu.begin(); fake.fake_clear()
+for t in tables:
+    assert gpu.L.h3_hip_linear_lora_bf16(gpu.h, y, x, w, None, t, ids, m, k, n)
+out = launches()
+""", m=m, k=k, n=n)
+    assert made
+    for kernel, x, y, z, threads, _ in made:
+        assert x * threads < 1 << 32 and y < 1 << 16 and z < 1 << 16, kernel
