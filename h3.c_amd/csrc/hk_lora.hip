@@ -725,7 +725,7 @@ __device__ __forceinline__ void hk_lora_store(const hk_skinny_args &s,
  * (column and piece) follow each other on one XCD and find it in its L2:
  * workgroups go to the 8 XCDs in turn, each XCD takes a run of (part, group). */
 template <int MB, int J, bool GROUPS>
-__global__ void __launch_bounds__(256, 2)
+__global__ void __launch_bounds__(256, MB > 4 ? 1 : 2)
 hk_lora_skinny(hk_skinny_args s, hk_lora_low_args g, uint32_t columns,
                uint32_t pieces, uint32_t groups, uint32_t first_tile,
                uint32_t tiles) {
@@ -903,10 +903,10 @@ struct hk_lora_cut {
 };
 
 static hk_lora_cut hk_lora_cut_of(uint32_t m, uint32_t n, uint32_t k_steps,
-                                  uint32_t cus) {
+                                  uint32_t cus, uint32_t most) {
     hk_lora_cut c;
     const uint32_t blocks = (m + 31u) / 32u;
-    c.groups = (blocks + 3u) / 4u;
+    c.groups = (blocks + most - 1u) / most;
     c.mbs = (blocks + c.groups - 1u) / c.groups;
     c.columns = (n + 127u) / 128u;
     c.pieces = std::min(cus / (c.columns * c.groups), k_steps / 8u);
@@ -922,7 +922,30 @@ static hk_lora_cut hk_lora_cut_of(uint32_t m, uint32_t n, uint32_t k_steps,
     return c;
 }
 
-/* The skinny GEMM's workgroups over groups of at most 128 rows. */
+typedef void (*hk_lora_skinny_kernel)(hk_skinny_args, hk_lora_low_args,
+                                      uint32_t, uint32_t, uint32_t, uint32_t,
+                                      uint32_t);
+
+static hk_lora_skinny_kernel hk_lora_skinny_pick(uint32_t m,
+                                                 const hk_lora_cut &c) {
+    if (c.groups > 1)
+        return c.mbs == 3 ? hk_lora_skinny<3, 2, true>
+                          : hk_lora_skinny<4, 2, true>;
+    switch (c.mbs) {
+    case 1:
+        return m <= 16 ? hk_lora_skinny<1, 1, false>
+                       : hk_lora_skinny<1, 2, false>;
+    case 2: return hk_lora_skinny<2, 2, false>;
+    case 3: return hk_lora_skinny<3, 2, false>;
+    case 4: return hk_lora_skinny<4, 2, false>;
+    case 5: return hk_lora_skinny<5, 2, false>;
+    case 6: return hk_lora_skinny<6, 2, false>;
+    default: return hk_lora_skinny<7, 2, false>;
+    }
+}
+
+/* The skinny GEMM's workgroups over groups of at most 128 rows, or one of at
+ * most 224. */
 static int hk_lora_run_skinny(struct h3_gpu *gpu, const hk_lora_args &a,
                               hk_lora_low_args &g, uint32_t cus,
                               const hk_lora_cut &cut) {
@@ -936,11 +959,11 @@ static int hk_lora_run_skinny(struct h3_gpu *gpu, const hk_lora_args &a,
      * only of a long K: the join of 573 rows x 1280 -> 3420 with ranks of 128
      * took 25 us with four, 16 with one. */
     const uint32_t room =
-        cut.groups == 1 ? UINT32_MAX
+        a.m <= 128u ? UINT32_MAX
                         : 3u * cus / (g.row_groups * std::max(1u, g.chunks));
     g.slots = std::max(1u, std::min({a.count, unit_rows, room}));
     const uint32_t most =
-        cut.groups == 1 ? 4u : std::min({4u, room / g.slots, k_steps / 16u});
+        a.m <= 128u ? 4u : std::min({4u, room / g.slots, k_steps / 16u});
     const uint32_t quarters = std::max(1u, most);
     g.piece_steps = (k_steps + quarters - 1u) / quarters;
     g.pieces = (k_steps + g.piece_steps - 1) / g.piece_steps;
@@ -967,30 +990,23 @@ static int hk_lora_run_skinny(struct h3_gpu *gpu, const hk_lora_args &a,
                  4096);
     if (!s.partial) return 0;
     const size_t lds = cut.mbs * 4096 * 4 + 16384;
-    void (*kernel)(hk_skinny_args, hk_lora_low_args, uint32_t, uint32_t,
-                   uint32_t, uint32_t, uint32_t) =
-        cut.groups > 1 ? (cut.mbs == 3 ? hk_lora_skinny<3, 2, true>
-                                       : hk_lora_skinny<4, 2, true>)
-        : a.m <= 16    ? hk_lora_skinny<1, 1, false>
-        : cut.mbs == 1 ? hk_lora_skinny<1, 2, false>
-        : cut.mbs == 2 ? hk_lora_skinny<2, 2, false>
-        : cut.mbs == 3 ? hk_lora_skinny<3, 2, false>
-                       : hk_lora_skinny<4, 2, false>;
-    /* devices (bit = ordinal) whose kernels have their LDS limit raised */
-    static uint64_t ready = 0;
-    const uint64_t bit = 1ull << (gpu->device & 63);
-    if (cut.mbs == 4 && !(ready & bit)) {
-        (void)hipFuncSetAttribute((const void *)hk_lora_skinny<4, 2, false>,
-                                  hipFuncAttributeMaxDynamicSharedMemorySize,
-                                  (int)lds);
-        (void)hipFuncSetAttribute((const void *)hk_lora_skinny<4, 2, true>,
-                                  hipFuncAttributeMaxDynamicSharedMemorySize,
-                                  (int)lds);
-        ready |= bit;
+    const hk_lora_skinny_kernel kernel = hk_lora_skinny_pick(a.m, cut);
+    if (cut.mbs >= 4) {
+        /* the limit raised, once per device (bit = ordinal) and kernel */
+        static uint64_t ready[2][8];
+        const uint64_t bit = 1ull << (gpu->device & 63);
+        uint64_t &done = ready[cut.groups > 1][cut.mbs];
+        if (!(done & bit))
+            (void)hipFuncSetAttribute(
+                (const void *)kernel,
+                hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        done |= bit;
     }
+    /* tiles that are all resident at once start first */
+    const bool tiles_first = cut.tiles <= (cut.mbs > 4 ? cus : 2u * cus);
     hipLaunchKernelGGL(kernel, dim3(cut.tiles + others), dim3(256), lds,
                        gpu->stream, s, g, cut.columns, cut.pieces, cut.groups,
-                       cut.tiles <= 2u * cus ? 0u : others, cut.tiles);
+                       tiles_first ? 0u : others, cut.tiles);
     hipLaunchKernelGGL(hk_lora_join,
                        dim3(((a.n + 31) / 32 * cut.mbs + 3) / 4, cut.groups),
                        dim3(256), 0, gpu->stream, s, g, cut.mbs,
@@ -999,17 +1015,25 @@ static int hk_lora_run_skinny(struct h3_gpu *gpu, const hk_lora_args &a,
 }
 
 /* Estimated microseconds over 128 rows: a step takes 0.65 us with one
- * workgroup on a CU and 1.1 with two, the pieces' sums go both ways at 4.5
- * TB/s (160 to 4000 rows of eight K x N: within 20%).  Skinny workgroups and
- * tiles, measured with one adapter of rank 16 (us): 160 x 320 -> 5120 12.5 and
- * 24.6, 1200 rows 28.3 and 26.2; 512 x 512 -> 1536 14.2 and 31.1, 4000 rows
- * 32.4 and 43.5; 160 x 5120 -> 5120 25.6 and 39.1, 384 38.4 and 46.0, 512 58.8
- * and 54.2; 160 x 5120 -> 13824 56.0 and 72.2, 384 109 and 84. */
+ * workgroup of up to 128 rows on a CU and 1.1 with two, more with more rows,
+ * the pieces' sums go both ways at 4.5 TB/s; with more rows the first
+ * product's units find no room on the CUs that have a workgroup, which a short
+ * piece does not hide (133 to 4000 rows of eight K x N: within 20%).  Groups of 128 rows and tiles, measured
+ * with one adapter of rank 16 (us): 160 x 320 -> 5120 12.5 and 24.6, 1200 rows
+ * 28.3 and 26.2; 512 x 512 -> 1536 14.2 and 31.1, 4000 rows 32.4 and 43.5; 160
+ * x 5120 -> 5120 25.6 and 39.1, 384 38.4 and 46.0, 512 58.8 and 54.2; 384 x
+ * 5120 -> 13824 109 and 84.  Those and one group: 133 x 5120 -> 13824 69 and
+ * 45, 197 rows 63 and 56; 133 x 5376 -> 21504 95 (tiles) and 72; 197 x 5120 ->
+ * 5120 30.4 and 31.5. */
 static float hk_lora_skinny_us(const hk_lora_cut &c, uint32_t m, uint32_t n,
                                uint32_t cus) {
-    const uint32_t rounds = (c.tiles + 2 * cus - 1) / (2 * cus);
-    return (float)rounds * (float)c.steps * (c.tiles <= cus ? 0.65f : 1.1f) +
-           6.0f +
+    static const float step_us[8] = {0.65f, 0.65f, 0.65f, 0.65f,
+                                     0.65f, 0.75f, 0.78f, 0.95f};
+    const uint32_t places = c.mbs > 4 || c.tiles <= cus ? cus : 2 * cus;
+    const float step = places > cus ? 1.1f : step_us[c.mbs];
+    const uint32_t rounds = (c.tiles + places - 1) / places;
+    const float start = c.mbs <= 4 ? 6.0f : c.pieces > 1 ? 14.0f : 8.0f;
+    return (float)rounds * (float)c.steps * step + start +
            (float)m * (float)n * (float)(8 * c.pieces + 2) / 4.5e6f;
 }
 
@@ -1024,17 +1048,27 @@ static int hk_lora_run(struct h3_gpu *gpu, const hk_lora_args &a) {
     g.ext.map = a.map;
     g.ext.pitch = 2u * a.pitch;
     g.sum_pitch = (a.rank + 15u) & ~15u;
-    const hk_lora_cut cut = hk_lora_cut_of(a.m, a.n, a.k / HK_BK, cus);
+    hk_lora_cut cut = hk_lora_cut_of(a.m, a.n, a.k / HK_BK, cus, 4);
     if (cut.groups == 1) return hk_lora_run_skinny(gpu, a, g, cus, cut);
-    float us;
-    const uint32_t tile_rows = hk_gemm_tile_rows(gpu, a.m, a.n, a.k, &us);
-    /* over tiles, the first product and the halves come before the GEMM, and
-     * several adapters to a tile are more steps of it */
-    us += a.count > 1 ? 18.0f : 14.0f;
-    return cut.groups <= 65535u && /* a grid's second dimension */
-                   hk_lora_skinny_us(cut, a.m, a.n, cus) < us
-               ? hk_lora_run_skinny(gpu, a, g, cus, cut)
-               : hk_lora_run_tiles(gpu, a, g, cus, tile_rows);
+    float skinny = cut.groups <= 65535u /* a grid's second dimension */
+                       ? hk_lora_skinny_us(cut, a.m, a.n, cus)
+                       : INFINITY;
+    if (a.m <= 224u) {
+        const hk_lora_cut one = hk_lora_cut_of(a.m, a.n, a.k / HK_BK, cus, 7);
+        const float us = hk_lora_skinny_us(one, a.m, a.n, cus);
+        if (us < skinny) {
+            skinny = us;
+            cut = one;
+        }
+    }
+    float tiles;
+    const uint32_t tile_rows = hk_gemm_tile_rows(gpu, a.m, a.n, a.k, &tiles);
+    /* over tiles W streams at 3 TB/s at most, the first product and the halves
+     * come before the GEMM, and several adapters to a tile are more steps */
+    tiles = std::max(tiles, (float)a.n * (float)a.k * 2.0f / 3e6f) +
+            (a.count > 1 ? 18.0f : 14.0f);
+    return skinny < tiles ? hk_lora_run_skinny(gpu, a, g, cus, cut)
+                          : hk_lora_run_tiles(gpu, a, g, cus, tile_rows);
 }
 
 /* elements of an adapter's fragments, a multiple of 512 */

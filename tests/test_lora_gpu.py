@@ -111,10 +111,13 @@ def test_long_and_wide(gpu, rows, k, n):
 
 @pytest.mark.parametrize("rows,k,n", [
     (129, 64, 132), (200, 64, 4), (300, 192, 4100), (417, 448, 1004),
-    (545, 2688, 260), (641, 320, 5120), (1800, 512, 388), (259, 1280, 12900)])
+    (545, 2688, 260), (641, 320, 5120), (1800, 512, 388), (259, 1280, 12900),
+    (130, 5120, 13700), (161, 5120, 13824), (224, 5120, 13600),
+    (150, 1024, 34000)])
 def test_groups_of_rows(gpu, rows, k, n):
-    """Over 128 rows of few steps of K: groups of 96 and 128 rows, a last one
-    of few, whole sums and pieces, one round of workgroups and more."""
+    """Over 128 rows of few steps of K or many columns: groups of 96 and 128
+    rows, a last one of few, one of 160, 192 and 224, whole sums and pieces,
+    one round of workgroups and more."""
     check(gpu, make(rows + n, blocks((rows // 2, 1), (rows // 4, NONE),
                                      (rows - rows // 2 - rows // 4, 0)),
                     [64, 16], k, n))
