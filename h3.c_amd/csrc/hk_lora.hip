@@ -269,9 +269,9 @@ __device__ __forceinline__ void hk_lora_low_unit(const hk_lora_low_args &g,
                     xr, live ? x_off[j] : 0xfffff000u, kb, 0);
         }
     };
-    /* X does not wait for the adapter */
-    load_x(0, 0);
-    bool have_x = true;
+    /* X does not wait for the adapter, where there will mostly be one */
+    bool have_x = slot == 0 && chunk == 0;
+    if (have_x) load_x(0, 0);
     if (left >= g.ext.count) left = HK_LORA_NONE;
     const uint32_t mine = left;
 
