@@ -157,8 +157,10 @@ __global__ void __launch_bounds__(256) hk_packed_simple(hk_packed_args a) {
  *   - rows of K and V come through buffer resources that end with the
  *     request's keys, so what lies behind them (other requests' rows) reads
  *     as zeros and P = 0 meets no infinity or NaN there;
- *   - DP = 64 or 128 dims, smaller heads padded: a lane whose piece lies past
- *     the head's dims loads from beyond the resource, zeros;
+ *   - DIMS = 64, 96 or 128 dims in LDS rows of 64 or 128 (4000 rows, 24 heads
+ *     of 96 over 4: 193 us, computed as 128 dims 222), smaller heads padded: a
+ *     lane whose piece lies past the head's dims loads from beyond the
+ *     resource, zeros;
  *   - tile addresses are 64-bit, so a context may pass 4 GiB;
  *   - NaN scores stay NaN (this file is compiled without the flag that lets
  *     hk_attn.hip assume none).
@@ -193,8 +195,8 @@ __device__ __forceinline__ uint32_t hk_packed_v_key(uint32_t row) {
 }
 
 /* hk_vt_read and hk_vt_wait (hk_attn.h) for ND blocks of 32 dims and rows of
- * 64 ND bytes. */
-template <int ND>
+ * ROW bytes. */
+template <int ND, uint32_t ROW>
 __device__ __forceinline__ void hk_packed_vt_read(hk_v2i (&vt)[ND][2],
                                                   const uint32_t (&frag)[ND],
                                                   uint32_t off) {
@@ -203,12 +205,20 @@ __device__ __forceinline__ void hk_packed_vt_read(hk_v2i (&vt)[ND][2],
         asm volatile("ds_read_b64_tr_b16 %0, %2 offset:%3\n\t"
                      "ds_read_b64_tr_b16 %1, %2 offset:%4"
                      : "=v"(vt[d][0]), "=v"(vt[d][1])
-                     : "v"(frag[d]), "i"(off), "i"(off + 8u * 64u * ND));
+                     : "v"(frag[d]), "i"(off), "i"(off + 8u * ROW));
 }
 
 template <int N>
 __device__ __forceinline__ void hk_packed_vt_wait(hk_v2i (&vt)[4][2]) {
     hk_vt_wait<N>(vt);
+}
+
+template <int N>
+__device__ __forceinline__ void hk_packed_vt_wait(hk_v2i (&vt)[3][2]) {
+    asm volatile("s_waitcnt lgkmcnt(%6)"
+                 : "+v"(vt[0][0]), "+v"(vt[0][1]), "+v"(vt[1][0]),
+                   "+v"(vt[1][1]), "+v"(vt[2][0]), "+v"(vt[2][1])
+                 : "i"(N));
 }
 
 template <int N>
@@ -230,10 +240,11 @@ __device__ __forceinline__ void hk_packed_dma16(__amdgpu_buffer_rsrc_t r,
                                              0, 0, 0);
 }
 
-template <int DP>
+template <int DIMS>
 __global__ void __launch_bounds__(HK_PACKED_WAVES * 64, 2)
 hk_packed_flash(hk_packed_args a) {
-    constexpr int NK = DP / 16, ND = DP / 32, CHUNKS = DP / 8;
+    constexpr int DP = DIMS <= 64 ? 64 : 128;
+    constexpr int NK = DIMS / 16, ND = DIMS / 32, CHUNKS = DP / 8;
     constexpr uint32_t ROW = DP * 2u, TILE = HK_KT * ROW, STAGE = 2u * TILE;
     /* 1-KiB loads per wave, tile and operand */
     constexpr int DMA = TILE / 1024 / HK_PACKED_WAVES;
@@ -438,13 +449,14 @@ hk_packed_flash(hk_packed_args a) {
         l_part += sum;
 
         hk_v2i vt[2][ND][2];
-        hk_packed_vt_read<ND>(vt[0], v_frag, stage * STAGE);
+        hk_packed_vt_read<ND, ROW>(vt[0], v_frag, stage * STAGE);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int kt = i >> 1, st = i & 1;
             if (i < 3) {
-                hk_packed_vt_read<ND>(vt[(i + 1) & 1], v_frag,
-                                      stage * STAGE + (i + 1) * 16u * ROW);
+                hk_packed_vt_read<ND, ROW>(vt[(i + 1) & 1], v_frag,
+                                           stage * STAGE +
+                                               (i + 1) * 16u * ROW);
                 hk_packed_vt_wait<2 * ND>(vt[i & 1]);
             } else {
                 hk_packed_vt_wait<0>(vt[i & 1]);
@@ -602,11 +614,12 @@ __global__ void __launch_bounds__(256) hk_packed_joined(hk_packed_args a) {
         if (lane * PER + e < a.dim) out[lane * PER + e] = hk_f2bf(sum[e] * inv);
 }
 
-template <int DP>
+template <int DIMS>
 static void hk_packed_launch(struct h3_gpu *gpu, const hk_packed_args &a,
                              const uint32_t *n) {
+    constexpr int DP = DIMS <= 64 ? 64 : 128;
     constexpr uint32_t lds = 2u * 2u * HK_KT * DP * 2u;
-    hipLaunchKernelGGL(hk_packed_flash<DP>, dim3(n[HK_PACKED_ITEMS]),
+    hipLaunchKernelGGL(hk_packed_flash<DIMS>, dim3(n[HK_PACKED_ITEMS]),
                        dim3(HK_PACKED_WAVES * 64u), lds, gpu->stream, a);
     if (n[HK_PACKED_JOINS])
         hipLaunchKernelGGL(hk_packed_joined<DP>,
@@ -980,8 +993,10 @@ int h3_hip_sdpa_packed_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
             if (!a.part_o) return 0;
             a.part_ml = (float2 *)(a.part_o + rows * padded);
         }
-        if (padded == 64)
+        if (dim <= 64)
             hk_packed_launch<64>(gpu, a, n);
+        else if (dim <= 96)
+            hk_packed_launch<96>(gpu, a, n);
         else
             hk_packed_launch<128>(gpu, a, n);
         return hk_op_end(gpu, "attention_packed", HK_KIND_SDPA);

@@ -121,7 +121,8 @@ def test_long_items_are_cut():
 
 @pytest.mark.parametrize("dim,kernel", [
     (1, "hk_packed_simple"), (8, "hk_packed_flash<64>"),
-    (64, "hk_packed_flash<64>"), (72, "hk_packed_flash<128>"),
+    (64, "hk_packed_flash<64>"), (72, "hk_packed_flash<96>"),
+    (96, "hk_packed_flash<96>"), (104, "hk_packed_flash<128>"),
     (100, "hk_packed_simple"), (128, "hk_packed_flash<128>"),
     (136, "hk_packed_simple"), (256, "hk_packed_simple")])
 def test_kernel_by_head_size(dim, kernel):
@@ -157,7 +158,7 @@ def test_flash_kernels_wait_for_their_transposed_reads():
             name = None
         elif name:
             found[name].append(line)
-    assert len(found) >= 2
+    assert len(found) == 3
     for name, body in found.items():
         assert any("ds_read_b64_tr_b16" in l for l in body), name
         assert not _offenders(body), (name, _offenders(body)[:3])
