@@ -171,7 +171,7 @@ __global__ void __launch_bounds__(256) hk_packed_simple(hk_packed_args a) {
  * an item's start and end around eight tiles (four clips of 6144 rows 180 us,
  * 620 TFLOP/s and 2.9 TB/s); single rows the bytes of K and V (eight rows over
  * contexts of 4096 to 9720 49 us, 4.7 TB/s) or, with short contexts, the chain
- * item, first tile, last tile, store (sixteen rows 14 us, 3.5 TB/s).
+ * item, tiles, joining, store (sixteen rows 13 us, 3.8 TB/s).
  *
  * Four waves of 32 rows and two workgroups a CU: with eight waves 6144 rows of
  * self-attention took 720 us for 754, but 4096 rows 344 for 335, 2378 rows x
@@ -240,6 +240,238 @@ __device__ __forceinline__ void hk_packed_dma16(__amdgpu_buffer_rsrc_t r,
                                              0, 0, 0);
 }
 
+/* An item of at most 32 rows: the waves share its rows and split its keys, 32
+ * at a time, wave w every fourth from the wth on.  A wave's tiles are its own,
+ * so no wave waits for another before the end: K of its next one loads once S
+ * is computed, V once P . V is.  Bound by the chain of a step (scores, maximum,
+ * exponentials, product: about 1 us, whatever the loads do), of which there
+ * are a quarter as many as with the waves on rows: three rows, the longest
+ * context 473 keys, 64 heads over 8, 7.0 us instead of 12.6 (13.9 with four
+ * stages of tiles instead of two); sixteen rows x 40 heads 12.8 and 14.3; one
+ * row, 2566 keys, 24 heads of 96 over 4, 9.0 and 10.9.  Long contexts, bound
+ * by K's and V's bytes, are level. */
+template <int DIMS>
+__device__ __forceinline__ void hk_packed_few(const hk_packed_args &a,
+                                              const hk_packed_item &it,
+                                              uint8_t *lds) {
+    constexpr int DP = DIMS <= 64 ? 64 : 128;
+    constexpr int NK = DIMS / 16, ND = DIMS / 32, CHUNKS = DP / 8;
+    constexpr uint32_t KEYS = 32, ROW = DP * 2u, TILE = KEYS * ROW;
+    constexpr int LOADS = TILE / 1024; /* of K or V of a tile */
+    const uint32_t tid = threadIdx.x, lane = tid & 63u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t col = lane & 31u, half = lane >> 5;
+    const uint32_t dim_chunks = a.dim >> 3;
+    const uint32_t stride = (uint32_t)a.kv_stride * 2u;
+    uint8_t *own = lds + wave * (2u * TILE);
+    uint32_t k_off[LOADS], v_off[LOADS];
+#pragma unroll
+    for (int i = 0; i < LOADS; i++) {
+        const uint32_t row = i * (64u / CHUNKS) + lane / CHUNKS;
+        const uint32_t kc = (lane % CHUNKS) ^ hk_packed_k_key<DP>(row);
+        const uint32_t vc = (lane % CHUNKS) ^ hk_packed_v_key<DP>(row);
+        k_off[i] = kc < dim_chunks ? row * stride + kc * 16u : 0x80000000u;
+        v_off[i] = vc < dim_chunks ? row * stride + vc * 16u : 0x80000000u;
+    }
+    const uint64_t kv_base =
+        (uint64_t)it.kv_first * a.kv_stride + (uint64_t)it.kv_head * a.dim;
+    const uint32_t last =
+        min(it.tile_end * (HK_KT / KEYS), (it.kv_rows + KEYS - 1u) / KEYS);
+    /* K or V of a tile; past the last one, loads that touch no memory, so that
+     * the waits below count right */
+    auto load = [&](const uint16_t *from, uint32_t tile, uint8_t *to,
+                    const uint32_t (&off)[LOADS]) {
+        const uint32_t kv0 = tile * KEYS;
+        const uint32_t rows = min(it.kv_rows - kv0, KEYS);
+        const __amdgpu_buffer_rsrc_t r = hk_attn_rsrc(
+            from + kv_base + kv0 * a.kv_stride,
+            tile < last ? (rows - 1u) * stride + a.dim * 2u : 0u);
+#pragma unroll
+        for (int i = 0; i < LOADS; i++)
+            hk_packed_dma16(r, to + i * 1024u, off[i]);
+    };
+    uint32_t tile = it.tile * (HK_KT / KEYS) + wave;
+    load(a.k, tile, own, k_off);
+
+    const uint32_t vrow = it.row + col, r0 = it.row / a.group;
+    hk_bf16x8 qf[NK];
+    {
+        const uint32_t r = vrow / a.group, g = vrow - r * a.group;
+        const __amdgpu_buffer_rsrc_t qr = hk_attn_rsrc(
+            a.q + ((uint64_t)it.q_first + r0) * a.q_stride +
+                (uint64_t)it.kv_head * a.group * a.dim,
+            0x7ffffff0u);
+        const uint32_t off = vrow < it.rows
+                                 ? (r - r0) * (uint32_t)a.q_stride * 2u +
+                                       g * a.dim * 2u + half * 16u
+                                 : 0x80000000u;
+#pragma unroll
+        for (int ks = 0; ks < NK; ks++)
+            qf[ks] = __builtin_bit_cast(
+                hk_bf16x8,
+                __builtin_amdgcn_raw_buffer_load_b128(
+                    qr,
+                    2u * ks + half < dim_chunks ? off + ks * 32u : 0x80000000u,
+                    0, 0));
+    }
+    load(a.v, tile, own + TILE, v_off);
+
+    const uint32_t own_at =
+        (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)own;
+    uint32_t v_frag[ND];
+    {
+        const uint32_t j = lane & 15u, g1 = (lane >> 4) & 1u;
+        const uint32_t row = 4u * half + (j >> 2);
+        const uint32_t low = 2u * g1 + ((j & 3u) >> 1);
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+            v_frag[d] = own_at + TILE + row * ROW +
+                        (((d * 4u + low) ^ hk_packed_v_key<DP>(row)) << 4) +
+                        8u * (j & 1u);
+    }
+    hk_f32x16 o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; d++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) o[d][r] = 0.0f;
+    float m_run = -INFINITY, l_part = 0.0f;
+    for (; tile < last; tile += HK_PACKED_WAVES) {
+        /* K has landed; V, issued behind it, may be on its way */
+        asm volatile("s_waitcnt vmcnt(%0)" ::"i"(LOADS) : "memory");
+        hk_f32x16 s;
+#pragma unroll
+        for (int r = 0; r < 16; r++) s[r] = 0.0f;
+#pragma unroll
+        for (int kk = 0; kk < NK; kk++) {
+            const hk_bf16x8 kf = *(const hk_bf16x8 *)(
+                own + col * ROW +
+                (((kk * 2u + half) ^ hk_packed_k_key<DP>(col)) << 4));
+            s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[kk], s, 0, 0,
+                                                        0);
+        }
+        /* this tile's K has been read */
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        load(a.k, tile + HK_PACKED_WAVES, own, k_off);
+        const uint32_t kv0 = tile * KEYS;
+        if (it.kv_rows - kv0 < KEYS) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const uint32_t key = kv0 + (r >> 2) * 8u + half * 4u + (r & 3);
+                if (key >= it.kv_rows) s[r] = -INFINITY;
+            }
+        }
+        /* the softmax of hk_packed_flash, with the maximum itself */
+        float mx = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < 16; r++) mx = fmaxf(mx, s[r]);
+        const auto sw = __builtin_amdgcn_permlane32_swap(
+            __float_as_uint(mx), __float_as_uint(mx), false, false);
+        mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) *
+             a.scale_log2;
+        const float m_new = fmaxf(m_run, mx);
+        const float ref = m_new == -INFINITY ? 0.0f : m_new;
+        const float c = __builtin_amdgcn_exp2f(m_run - ref);
+        m_run = m_new;
+        float sum = 0.0f;
+        hk_bf16x8 pf[2];
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+            const float p = __builtin_amdgcn_exp2f(
+                __builtin_fmaf(s[r], a.scale_log2, -ref));
+            sum += p;
+            pf[r >> 3][r & 7] = (__bf16)p;
+        }
+        l_part = l_part * c + sum;
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) o[d][r] *= c;
+        /* V has landed; the next K may be on its way */
+        asm volatile("s_waitcnt vmcnt(%0)" ::"i"(LOADS) : "memory");
+        hk_v2i vt[2][ND][2];
+        hk_packed_vt_read<ND, ROW>(vt[0], v_frag, 0);
+        hk_packed_vt_read<ND, ROW>(vt[1], v_frag, 16u * ROW);
+        hk_packed_vt_wait<2 * ND>(vt[0]);
+#pragma unroll
+        for (int st = 0; st < 2; st++) {
+            if (st) hk_packed_vt_wait<0>(vt[1]);
+#pragma unroll
+            for (int d = 0; d < ND; d++) {
+                const hk_v4i both = {vt[st][d][0][0], vt[st][d][0][1],
+                                     vt[st][d][1][0], vt[st][d][1][1]};
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                    __builtin_bit_cast(hk_bf16x8, both), pf[st], o[d], 0, 0,
+                    0);
+            }
+        }
+        asm volatile("" ::: "memory");
+        load(a.v, tile + HK_PACKED_WAVES, own + TILE, v_off);
+    }
+    /* The waves' sums: M and L of each row over LDS, then O, scaled to M (and
+     * by 1 / L for a whole item), 32 dims at a time in rows of 128 bytes. */
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    float2 *ml = (float2 *)lds;
+    const float l_own = l_part + __shfl_xor(l_part, 32, 64);
+    if (half == 0) ml[wave * 32u + col] = make_float2(m_run, l_own);
+    __syncthreads();
+    float top = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (uint32_t w = 0; w < HK_PACKED_WAVES; w++)
+        top = fmaxf(top, ml[w * 32u + col].x);
+    const float ref = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+    for (uint32_t w = 0; w < HK_PACKED_WAVES; w++) {
+        const float2 v = ml[w * 32u + col];
+        l += __builtin_amdgcn_exp2f(v.x - ref) * v.y;
+    }
+    const bool whole = it.part == HK_PACKED_WHOLE;
+    float weight = __builtin_amdgcn_exp2f(m_run - ref);
+    if (whole) weight *= l == 0.0f ? 0.0f : 1.0f / l;
+    else if (wave == 0 && half == 0 && vrow < it.rows)
+        a.part_ml[(size_t)it.part * HK_PACKED_QB + col] = make_float2(top, l);
+    __syncthreads();
+#pragma unroll
+    for (int d = 0; d < ND; d++)
+#pragma unroll
+        for (int blk = 0; blk < 4; blk++) {
+            const uint32_t c = blk * 2u + half;
+            *(float4 *)(own + d * 4096u + col * 128u +
+                        ((c ^ (col & 7u)) << 4)) =
+                make_float4(o[d][blk * 4 + 0] * weight,
+                            o[d][blk * 4 + 1] * weight,
+                            o[d][blk * 4 + 2] * weight,
+                            o[d][blk * 4 + 3] * weight);
+        }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t i = 0; i < 32u * DIMS / 4u / (HK_PACKED_WAVES * 64u); i++) {
+        const uint32_t at = i * (HK_PACKED_WAVES * 64u) + tid;
+        const uint32_t r = at / (DIMS / 4u), dim4 = at % (DIMS / 4u);
+        const uint32_t c = dim4 & 7u;
+        hk_f32x4 sum = {0, 0, 0, 0};
+#pragma unroll
+        for (uint32_t w = 0; w < HK_PACKED_WAVES; w++)
+            sum += *(const hk_f32x4 *)(lds + w * (2u * TILE) +
+                                       (dim4 >> 3) * 4096u + r * 128u +
+                                       ((c ^ (r & 7u)) << 4));
+        const uint32_t vr = it.row + r;
+        if (vr >= it.rows || dim4 * 4u >= a.dim) continue;
+        if (!whole) {
+            *(hk_f32x4 *)(a.part_o +
+                          ((size_t)it.part * HK_PACKED_QB + r) * DP +
+                          dim4 * 4u) = sum;
+            continue;
+        }
+        const uint32_t qr = vr / a.group, g = vr - qr * a.group;
+        *(uint2 *)(a.o +
+                   (((uint64_t)it.q_first + qr) * a.heads +
+                    it.kv_head * a.group + g) * a.dim +
+                   dim4 * 4u) =
+            make_uint2(hk_pack2(sum[0], sum[1]), hk_pack2(sum[2], sum[3]));
+    }
+}
+
 template <int DIMS>
 __global__ void __launch_bounds__(HK_PACKED_WAVES * 64, 2)
 hk_packed_flash(hk_packed_args a) {
@@ -255,6 +487,10 @@ hk_packed_flash(hk_packed_args a) {
 
     const hk_packed_item it = a.items[blockIdx.x];
     if (it.row >= it.rows) return;
+    if (it.rows - it.row <= 32u) {
+        hk_packed_few<DIMS>(a, it, hk_lds);
+        return;
+    }
     const uint32_t dim_chunks = a.dim >> 3;
 
     /* wave w fills rows of a tile with DMA loads of 64 / CHUNKS rows each,

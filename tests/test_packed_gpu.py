@@ -89,6 +89,17 @@ def test_head_sizes(gpu, dim):
     Case(dim, [70, 1, 9], [33, 130, 64], 4, 2, dim).check(gpu)
 
 
+@pytest.mark.parametrize("dim", [8, 64, 72, 96, 128])
+@pytest.mark.parametrize("kn", [1, 31, 32, 33, 64, 65, 95, 97, 127, 128, 129, 161,
+                                256, 300, 1025])
+def test_few_rows_share_the_waves(gpu, dim, kn):
+    """Up to 32 virtual rows a key head: keys split over the waves, of which
+    some have none; and the 33rd."""
+    Case(25, [1, 4, 5, 32, 33], [kn, 33, kn, 0, kn], 1, 1, dim, gap=1,
+         pad=8).check(gpu)
+    Case(26, [4, 1, 3, 36], [kn, kn, 2, kn], 16, 2, dim).check(gpu)
+
+
 @pytest.mark.parametrize("heads,kv_heads", [(1, 1), (5, 5), (6, 3), (8, 1),
                                             (12, 4), (64, 8), (33, 1),
                                             (40, 1)])
