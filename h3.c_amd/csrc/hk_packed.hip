@@ -40,7 +40,7 @@ struct hk_packed_request {
     uint32_t before; /* query rows of the requests before it in the plan */
 };
 
-/* A work item: virtual rows [row, + HK_PACKED_QB) of a request's `rows`, of
+/* A work item: virtual rows [row, rows) of a request, at most HK_PACKED_QB, of
  * one key head, over key tiles [tile, tile_end) of the request's keys.  Whole
  * items store their rows; a piece leaves its sums in part `part`.  An item of
  * no rows fills a place in the launch. */
@@ -897,7 +897,16 @@ static bool hk_packed_takes(const struct h3_gpu *gpu,
  *   CU is one place; self-attention in us, uncut and cut: 1200 rows x 56
  *   heads, 2.2 rounds, 62.8 and 54.8; 2378 x 56, 4.2, 189 and 173; 2560 x 40,
  *   3.1, 158 and 148; counted as two places a CU, 2185 x 40, 2.8 rounds, was
- *   cut and took 129 for 113). */
+ *   cut and took 129 for 113).
+ *
+ * Where 128 rows make few items, items of 32 rows fill the CUs and have a
+ * quarter of the steps (hk_packed_few), at the price of K and V four times
+ * from L2: up to one a CU, and up to two if they are mostly full (measured with
+ * 128 and 32 rows, us: 700 rows of self-attention x 8 heads, 176 small items,
+ * 17.2 and 11.2; 537 x 16 over 2, 272, 15.5 and 13.4; 1200 x 12 of 64, 456,
+ * 22.3 and 13.1; 300 rows x 24 heads of 96, 512 keys, 240, 12.1 and 8.6; but
+ * 300 rows x 40, 400 and 5 tiles, 11.3 and 12.4; four times 50 rows x 40, 320
+ * half empty ones, 13.7 and 15.2). */
 struct hk_packed_work {
     std::vector<hk_packed_item> items;
     std::vector<hk_packed_join> joins;
@@ -950,13 +959,13 @@ static float hk_packed_end(const std::vector<hk_packed_run> &runs,
     return end.back() + (cut ? hk_packed_join_time : 0.0f);
 }
 
-static void hk_packed_lay_out(const std::vector<hk_packed_request> &list,
-                              uint32_t group, uint32_t kv_heads, uint32_t cus,
-                              hk_packed_work &work) {
-    const uint32_t qb = HK_PACKED_QB, places = cus * 2u;
+/* The requests' items of `qb` rows, whole, those with the most tiles first;
+ * their number in `items`. */
+static std::vector<hk_packed_run> hk_packed_whole(
+    const std::vector<hk_packed_request> &list, uint32_t group,
+    uint32_t kv_heads, uint32_t qb, uint64_t &items) {
     std::vector<hk_packed_run> runs;
-    double total = 0.0;
-    uint64_t items = 0;
+    items = 0;
     for (uint32_t i = 0; i < list.size(); i++) {
         const uint32_t rows = list[i].q_rows * group;
         const uint32_t tiles =
@@ -965,26 +974,49 @@ static void hk_packed_lay_out(const std::vector<hk_packed_request> &list,
         const uint64_t count = (uint64_t)blocks * kv_heads;
         runs.push_back({i, tiles, rows, blocks, 0, count, 1, tiles});
         items += count;
-        total += (double)count * (tiles + hk_packed_own);
     }
     std::stable_sort(runs.begin(), runs.end(),
                      [](const hk_packed_run &x, const hk_packed_run &y) {
                          return x.tiles > y.tiles;
                      });
+    return runs;
+}
+
+static void hk_packed_lay_out(const std::vector<hk_packed_request> &list,
+                              uint32_t group, uint32_t kv_heads,
+                              uint32_t dims, uint32_t cus,
+                              hk_packed_work &work) {
+    const uint32_t places = cus * 2u;
+    uint32_t qb = HK_PACKED_QB;
+    uint64_t items, small;
+    std::vector<hk_packed_run> runs =
+        hk_packed_whole(list, group, kv_heads, qb, items);
+    const std::vector<hk_packed_run> low =
+        hk_packed_whole(list, group, kv_heads, 32, small);
+    double total = 0.0;
+    for (const hk_packed_run &r : runs)
+        total += (double)r.count * (r.tiles + hk_packed_own);
     /* (many items come out level whole) */
     if (!runs.empty() && items <= 16ull * places) {
         std::vector<hk_packed_run> chosen = runs;
         const uint32_t share = (uint32_t)(total / places) + 1u;
+        float best = hk_packed_end(runs, places);
         if (runs[0].tiles >= share) { /* few and long */
-            float best = hk_packed_end(runs, places);
             uint32_t tried = 0;
             for (uint32_t i = 4; i <= 24; i++) { /* half to three shares */
                 const uint32_t length = std::max(4u, share * i / 8u);
                 if (length == tried || length >= runs[0].tiles) continue;
                 tried = length;
                 std::vector<hk_packed_run> cut = runs;
-                for (hk_packed_run &r : cut) hk_packed_cut(r, length);
-                const float end = hk_packed_end(cut, places);
+                double bytes = 0.0; /* of the pieces' sums, both ways */
+                for (hk_packed_run &r : cut) {
+                    hk_packed_cut(r, length);
+                    if (r.pieces > 1)
+                        bytes += (double)r.rows * kv_heads * r.pieces * dims *
+                                 8.0;
+                }
+                const float end = hk_packed_end(cut, places) +
+                                  (float)(bytes / 4.5e6);
                 if (end < best) {
                     best = end;
                     chosen = cut;
@@ -1004,7 +1036,7 @@ static void hk_packed_lay_out(const std::vector<hk_packed_request> &list,
                 if (h.count) head.push_back(h);
                 if (t.count) tail.push_back(t);
             }
-            float best = 0.95f * hk_packed_end(runs, cus);
+            float least = 0.95f * hk_packed_end(runs, cus);
             for (uint32_t i = 4; i <= 8; i++) { /* one to two shares */
                 const uint32_t length =
                     std::max(4u, (uint32_t)(rest / cus * i / 4) + 1u);
@@ -1014,11 +1046,18 @@ static void hk_packed_lay_out(const std::vector<hk_packed_request> &list,
                     cut.push_back(r);
                 }
                 const float end = hk_packed_end(cut, cus);
-                if (end < best) {
-                    best = end;
+                if (end < least) {
+                    least = end;
                     chosen = cut;
                 }
             }
+        }
+        const float step = small <= cus ? 0.6f : 0.85f;
+        if (small > items && small <= places &&
+            (small <= cus || small >= 3 * items) &&
+            hk_packed_own + 1.0f + step * (float)runs[0].tiles < best) {
+            qb = 32;
+            chosen = low;
         }
         runs = chosen;
     }
@@ -1038,17 +1077,18 @@ static void hk_packed_lay_out(const std::vector<hk_packed_request> &list,
             load[&q - queue] +=
                 (double)(end - i) * (s.tiles + hk_packed_own * s.pieces);
             for (; i < end; i++) {
-                hk_packed_item item = {r.q_first, s.rows,
-                                       (uint32_t)(i % s.blocks) * qb,
+                const uint32_t row = (uint32_t)(i % s.blocks) * qb;
+                hk_packed_item item = {r.q_first, std::min(s.rows, row + qb),
+                                       row,
                                        (uint32_t)(i / s.blocks), r.kv_first,
                                        r.kv_rows, 0, s.tiles,
                                        HK_PACKED_WHOLE};
                 if (s.pieces > 1) {
-                    work.joins.push_back({r.q_first, s.rows, item.row,
+                    work.joins.push_back({r.q_first, item.rows, row,
                                           item.kv_head, work.parts,
                                           s.pieces});
                     work.join_rows = std::max(
-                        work.join_rows, std::min(s.rows - item.row, qb));
+                        work.join_rows, item.rows - row);
                 }
                 for (uint32_t p = 0; p < s.pieces; p++) {
                     item.tile = p * s.per;
@@ -1121,7 +1161,7 @@ h3_gpu_tensor *h3_hip_sdpa_packed_plan(h3_gpu *gpu, const uint32_t *q_first,
             return NULL;
         }
         hk_packed_work work;
-        hk_packed_lay_out(list, heads / kv_heads, kv_heads,
+        hk_packed_lay_out(list, heads / kv_heads, kv_heads, head_dim,
                           gpu->num_cus > 0 ? (uint32_t)gpu->num_cus : 256u,
                           work);
         std::vector<uint32_t> words;

@@ -54,17 +54,21 @@ def cover(case):
     qn, kn, heads, kv, dim = case
     made, items, joins = lists(case)
     group = heads // kv
-    seen, parts = {}, {}
+    seen, ends = {}, {}
     for qf, rows, row, head, kf, kr, t0, t1, part in items.tolist():
         if rows == 0:
             continue
         seen.setdefault((qf, row, head), []).append((t0, t1, part))
         i = next(i for i in range(len(qn)) if sum(qn[:i]) == qf and qn[i])
-        assert rows == qn[i] * group and kr == kn[i] and row < rows
-        assert kf == sum(kn[:i])
-    want = {(sum(qn[:i]), b, h) for i in range(len(qn))
-            for b in range(0, qn[i] * group, QB) for h in range(kv)}
-    assert set(seen) == want
+        assert row < rows <= qn[i] * group and kr == kn[i]
+        assert kf == sum(kn[:i]) and ends.setdefault((qf, row, head),
+                                                     rows) == rows
+    # rows in blocks of one size, 128 or 32, whole but for a request's last
+    qb = 32 if any(row % QB for _, row, _ in seen) else QB
+    want = {(sum(qn[:i]), b, h): min(b + qb, qn[i] * group)
+            for i in range(len(qn))
+            for b in range(0, qn[i] * group, qb) for h in range(kv)}
+    assert ends == want
     joined = {(qf, row, head): (part, pieces)
               for qf, _, row, head, part, pieces in joins.tolist()}
     used = []
@@ -175,3 +179,16 @@ def test_items_behind_the_last_full_round_are_cut():
     for rows in (4096, 2185):
         made, items, joins = cover(([rows], [rows], 40, 40, 128))
         assert not len(joins) and len(made) == 1
+
+
+def test_few_items_are_of_few_rows():
+    # 48 items of 128 rows; 102 of which the small ones would be 400
+    for qn, heads, small in (([700], 8, 176), ([300], 40, 0), ([1], 8, 0)):
+        made, items, joins = cover((qn, qn, heads, heads, 128))
+        sizes = items[items[:, 1] > 0]
+        assert not len(joins)
+        assert (sizes[:, 1] - sizes[:, 2]).max() <= (32 if small else 128)
+        assert not small or len(sizes) == small
+    # long contexts are cut instead
+    made, items, joins = cover(([128], [9720], 8, 8, 128))
+    assert len(joins) == 8
