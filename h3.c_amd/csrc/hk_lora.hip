@@ -400,6 +400,11 @@ __device__ __forceinline__ void hk_lora_low_unit(const hk_lora_low_args &g,
                         e * 4u);
             const uint32_t first = rank0 + part * 8u;
             if (first >= g.sum_pitch) continue;
+            /* an infinity in the row has met A's padding: zeros there */
+            if (first + 8u > rank)
+#pragma unroll
+                for (uint32_t e = 0; e < 8; e++)
+                    if (first + e >= rank) u[e >> 2][e & 3] = 0.0f;
             hk_f32x4 *out = (hk_f32x4 *)(
                 g.sums + ((size_t)piece * g.m + row0 + row) * g.sum_pitch +
                 first);
@@ -444,10 +449,18 @@ hk_lora_low(hk_lora_low_args g) {
                                 rest % g.pieces, lds);
 }
 
-/* 8 ranks of a row: the sums of K's pieces, four on their way at a time. */
+/* 8 ranks of a row: the sums of K's pieces, four on their way at a time.  (One
+ * piece, as with a short K, is its own sum: with the general way's zeros and
+ * additions at every 16 ranks of every 32 columns, the join of 573 rows x 3420
+ * at rank 128 took 16.0 us for 12.8.) */
 __device__ __forceinline__ void hk_lora_add_up(const float *sums,
                                                size_t stride, uint32_t pieces,
                                                hk_f32x4 (&u)[2]) {
+    if (pieces == 1u) {
+        u[0] = *(const hk_f32x4 *)sums;
+        u[1] = *(const hk_f32x4 *)(sums + 4);
+        return;
+    }
     u[0] = u[1] = hk_f32x4{0, 0, 0, 0};
     for (uint32_t first = 0; first < pieces; first += 4u) {
         hk_f32x4 v[4][2] = {};
@@ -465,15 +478,14 @@ __device__ __forceinline__ void hk_lora_add_up(const float *sums,
     }
 }
 
-/* The sums of `ranks` ranks times the scale, as bf16 halves; zeros past them,
- * where an infinity in the row has met A's padding. */
+/* The sums times the scale, as bf16 halves. */
 __device__ __forceinline__ void hk_lora_split(const hk_f32x4 (&u)[2],
-                                              float scale, uint32_t ranks,
-                                              uint4 &high, uint4 &rest) {
+                                              float scale, uint4 &high,
+                                              uint4 &rest) {
     float v[8], low[8];
 #pragma unroll
     for (uint32_t e = 0; e < 8; e++) {
-        v[e] = e < ranks ? scale * u[e >> 2][e & 3] : 0.0f;
+        v[e] = scale * u[e >> 2][e & 3];
         const float h = hk_bf2f(hk_f2bf(v[e]));
         /* past bf16's range the first half is infinite and stays so */
         low[e] = fabsf(h) == INFINITY ? 0.0f : v[e] - h;
@@ -505,7 +517,7 @@ hk_lora_halves(hk_lora_low_args g, uint32_t units, uint32_t tile_rows) {
             hk_f32x4 u[2];
             hk_lora_add_up(g.sums + (size_t)row * g.sum_pitch + first,
                            (size_t)g.m * g.sum_pitch, g.pieces, u);
-            hk_lora_split(u, e.scale, e.rank - first, high, rest);
+            hk_lora_split(u, e.scale, high, rest);
         }
         uint16_t *out = (uint16_t *)x.low + (size_t)row * x.pitch + first;
         *(uint4 *)out = high;
@@ -609,9 +621,9 @@ void hk_gemm_lora_launch(struct h3_gpu *gpu, int epilogue, uint32_t jb,
  * wave in the layout of hk_skinny_tile: lane l has row l % 32 and its adapter
  * `mine` (rank 0 without one), so that what an adapter takes in turn is B
  * alone: 32x32x16 MFMAs of B's rows against the rows' halves, zeros in rows of
- * others.  16 ranks at a time, with the next 16 on their way: `u` holds the
- * lane's 8 of the first (add_up of `low`).  Each B is a wait, but where the
- * rows have several adapters four of them are one. */
+ * others.  16 ranks at a time: `u` holds the lane's 8 of the first (add_up of
+ * `low`), the next load beside B.  Each B is a wait, but where the rows have
+ * several adapters four of them are one. */
 __device__ __forceinline__ void hk_lora_second(const hk_lora_low_args &g,
                                                const hk_lora_row &mine,
                                                const float *low,
@@ -623,13 +635,8 @@ __device__ __forceinline__ void hk_lora_second(const hk_lora_low_args &g,
         bool left = k < mine.rank;
         uint64_t with = __builtin_amdgcn_ballot_w64(left);
         if (!with) return;
-        const uint32_t from = k + half * 8u;
         uint4 high, rest;
-        hk_lora_split(u, mine.scale, mine.rank > from ? mine.rank - from : 0u,
-                      high, rest);
-        if (k + 16u < mine.rank)
-            hk_lora_add_up(low + k + 16u, (size_t)g.m * g.sum_pitch, g.pieces,
-                           u);
+        hk_lora_split(u, mine.scale, high, rest);
         /* the next adapter of the rows that are left (of none: the last one
          * again, for no rows), and its B */
         int lead = 0;
@@ -662,6 +669,10 @@ __device__ __forceinline__ void hk_lora_second(const hk_lora_low_args &g,
         };
         const hk_v4i first = take();
         const bool firsts = its;
+        /* beside B's wait, the rows' next 16 ranks */
+        if (k + 16u < mine.rank)
+            hk_lora_add_up(low + k + 16u, (size_t)g.m * g.sum_pitch, g.pieces,
+                           u);
         if (!with) {
             multiply(first, firsts);
             continue;
@@ -765,7 +776,8 @@ hk_lora_skinny(hk_skinny_args s, hk_lora_low_args g, uint32_t columns,
 
 /* C = act(pieces' sums + bias + s_a (x . A^T) . B^T) for 32 columns and 32
  * rows, a wave; blockIdx.y is the row group.  Bound by its chain of loads (the
- * row, its first ranks and the pieces; B; 7 us at 8 rows x 5120) and by how
+ * row, its first ranks and the pieces; B; 7 us at 8 rows x 5120), at higher
+ * ranks by the halves' arithmetic, made anew for every 32 columns, and by how
  * many waves a CU holds: five workgroups (994 rows x 5120 took 16.3 us with
  * four, 14.4 with five; 39 rows x 96768 13.8).  Tried and slower: 32 ranks at
  * a time, all ranks of an adapter in sequence (8 rows with an adapter each 15
@@ -1064,10 +1076,13 @@ static int hk_lora_run(struct h3_gpu *gpu, const hk_lora_args &a) {
     float tiles;
     const uint32_t tile_rows = hk_gemm_tile_rows(gpu, a.m, a.n, a.k, &tiles);
     /* over tiles W streams at 3 TB/s at most, the first product and the halves
-     * come before the GEMM, and several adapters to a tile are more steps */
+     * come before the GEMM, and several adapters to a tile are more steps; in
+     * the skinny workgroups' launch several adapters are more units (551 rows
+     * x 5120 -> 5120 of eight, 64 us by the estimate, took 76) */
     tiles = std::max(tiles, (float)a.n * (float)a.k * 2.0f / 3e6f) +
             (a.count > 1 ? 18.0f : 14.0f);
-    return skinny < tiles ? hk_lora_run_skinny(gpu, a, g, cus, cut)
+    return skinny < (a.count > 1 ? 0.9f : 1.0f) * tiles
+               ? hk_lora_run_skinny(gpu, a, g, cus, cut)
                           : hk_lora_run_tiles(gpu, a, g, cus, tile_rows);
 }
 

@@ -4,7 +4,7 @@
  * over request i's key rows j and key head h / (heads / kv_heads).
  *
  * The plan is laid out on the host, once for a set of requests, and uploaded:
- * work items of HK_PACKED_QB query rows of one request and key head, over all
+ * work items of 128 or 32 query rows of one request and key head, over all
  * of its key tiles or a piece of them.
  *
  * The query heads that share a key head are rows of one item: "virtual row"
