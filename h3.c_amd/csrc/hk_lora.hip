@@ -20,7 +20,7 @@
  *
  * Measured, in brackets the projection alone in the same run (us): 8 rows x
  * 5120 -> 5120, eight adapters of rank 16, 16.8 (13.7); 39 x 2688 -> 96768
- * 101 (87), 5.3 TB/s; 197 x 5120 -> 5376 32 (36); 778 x 7168 -> 5376 90 (84);
+ * 101 (87), 5.3 TB/s; 197 x 5120 -> 5376 32 (36); 778 x 7168 -> 5376 88 (85);
  * 4756 x 5376 -> 21504, ranks 64 and 4, 828 (805), 1.34 PFLOP/s; 6144 x 5120
  * -> 13824 with GELU, ranks up to 128, 690 (667).  W's bytes bound the first
  * two, launches and the chains of dependent loads in them beside that, the
