@@ -160,7 +160,7 @@ out.append(call(plan=plan(qn=[0, 0])))
 
 
 @pytest.mark.parametrize("m,k,n", [(8_400_000, 64, 4), (129, 64, 1 << 22),
-                                   (70_000, 64, 4096), (128, 64, 1 << 24)])
+                                   (70_000, 64, 4096), (128, 64, 1 << 22)])
 def test_adapter_launches_stay_within_a_grid(m, k, n):
     """Threads of a launch below 2^32 and its second dimension below 2^16, for
     the most rows and columns too."""
