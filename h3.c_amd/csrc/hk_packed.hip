@@ -31,6 +31,7 @@
 #include <vector>
 
 #define HK_PACKED_MAX_DIM 256u
+#define HK_PACKED_MAX_KEYS 0xffffff00u /* of a request */
 #define HK_PACKED_WAVES 4u
 #define HK_PACKED_QB (HK_PACKED_WAVES * 32u) /* virtual rows of an item */
 
@@ -1136,6 +1137,13 @@ h3_gpu_tensor *h3_hip_sdpa_packed_plan(h3_gpu *gpu, const uint32_t *q_first,
             if (qe > UINT32_MAX || ke > UINT32_MAX) {
                 hk_fail(gpu, "attention plan: the rows of request %u pass "
                              "2^32", i);
+                return NULL;
+            }
+            /* the kernels count keys in 32 bits, up to the end of the last
+             * tile and a turn past it */
+            if (kv_rows[i] > HK_PACKED_MAX_KEYS) {
+                hk_fail(gpu, "attention plan: request %u has %u key rows, over "
+                             "%u", i, kv_rows[i], HK_PACKED_MAX_KEYS);
                 return NULL;
             }
             if (!q_rows[i]) continue;

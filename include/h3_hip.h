@@ -313,7 +313,8 @@ int h3_hip_linear_lora_gelu_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
  * a set of requests (free it with h3_gpu_tensor_free); the call takes any
  * tensors that hold the plan's rows.  heads has to be a multiple of kv_heads
  * and head_dim 1 to 256; multiples of 8 up to 128, with offsets and strides
- * in multiples of 8, run on the matrix cores.
+ * in multiples of 8, run on the matrix cores.  A request may have up to
+ * 2^32 - 256 key rows.
  *
  * Head h of query row r starts at element query_offset + r query_stride +
  * h head_dim of `query` (likewise key and value, with kv_stride), so Q, K and
