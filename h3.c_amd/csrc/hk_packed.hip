@@ -856,8 +856,16 @@ static void hk_packed_launch(struct h3_gpu *gpu, const hk_packed_args &a,
                              const uint32_t *n) {
     constexpr int DP = DIMS <= 64 ? 64 : 128;
     constexpr uint32_t lds = 2u * 2u * HK_KT * DP * 2u;
-    hipLaunchKernelGGL(hk_packed_flash<DIMS>, dim3(n[HK_PACKED_ITEMS]),
-                       dim3(HK_PACKED_WAVES * 64u), lds, gpu->stream, a);
+    /* a launch has fewer than 2^32 threads; whole turns of the XCDs */
+    const uint32_t most = 1u << 23;
+    for (uint32_t first = 0; first < n[HK_PACKED_ITEMS]; first += most) {
+        hk_packed_args part = a;
+        part.items = a.items + first;
+        hipLaunchKernelGGL(hk_packed_flash<DIMS>,
+                           dim3(std::min(n[HK_PACKED_ITEMS] - first, most)),
+                           dim3(HK_PACKED_WAVES * 64u), lds, gpu->stream,
+                           part);
+    }
     if (n[HK_PACKED_JOINS])
         hipLaunchKernelGGL(hk_packed_joined<DP>,
                            dim3(n[HK_PACKED_JOINS],
@@ -1163,7 +1171,7 @@ h3_gpu_tensor *h3_hip_sdpa_packed_plan(h3_gpu *gpu, const uint32_t *q_first,
                              "overlap at row %u", ranges[i].first);
                 return NULL;
             }
-        /* (an item for every 128 of them: 4 million items) */
+        /* (an item for every 128 of them, or, of single rows, each) */
         if (rows * heads >= 1ull << 29) {
             hk_fail(gpu, "attention plan: too many query rows and heads");
             return NULL;

@@ -28,3 +28,21 @@ def test_more_keys_than_the_kernels_count(qn, kn):
 
 def test_the_most_keys_that_they_count():
     assert on_fake(PLAN + "out = bool(plan([1], [0xFFFFFF00]))")
+
+
+@pytest.mark.parametrize("rows,heads", [(6000, 3000), (8000, 4)])
+def test_launches_of_many_items_stay_within_a_grid(rows, heads):
+    """A single row's key heads are an item each; a launch has fewer than 2^32
+    threads, and the launches together every item once."""
+    made = on_fake(PLAN + """
+h = plan([1] * rows, [64] * rows, heads, heads)
+y, q = gpu.new_bf16(rows * heads * 8), gpu.new_bf16(rows * heads * 8)
+k = gpu.new_bf16(64 * heads * 8)
+gpu.begin(); fake.fake_clear()
+assert gpu.L.h3_hip_sdpa_packed_bf16(gpu.h, y, q, 0, heads * 8, k, 0, k, 0,
+                                     heads * 8, h, 1.0), gpu.error()
+out = launches()
+""", rows=rows, heads=heads)
+    assert all(kernel == "hk_packed_flash<64>" for kernel, *_ in made)
+    assert all(x * threads < 1 << 32 for _, x, _, _, threads, _ in made)
+    assert sum(x for _, x, *_ in made) == rows * heads
