@@ -80,14 +80,16 @@ struct hk_packed_args {
     const hk_packed_item *items;
     const hk_packed_join *joins;
     /* pieces' sums: F32 O [part][HK_PACKED_QB][padded dim], not divided, and
-     * (running maximum in the exp2 domain, sum) [part][HK_PACKED_QB] */
+     * (reference, sum) [part][HK_PACKED_QB] */
     float *part_o;
     float2 *part_ml;
 };
 
 /* One wave per (query row, head) at a time, 64 keys a turn: lane j scores key
  * j of the turn, then lane l adds up dims l, l + 64, ... of the turn's values.
- * Running maximum and sum in F32; P stays F32. */
+ * Running maximum and sum in F32; P stays F32.  The scale multiplies the
+ * distance from the maximum, which F32 holds however far the scores lie from
+ * zero. */
 __device__ void hk_packed_simple_row(const hk_packed_args &a, uint32_t nth,
                                      uint32_t head) {
     const uint32_t lane = threadIdx.x & 63u;
@@ -117,12 +119,13 @@ __device__ void hk_packed_simple_row(const hk_packed_args &a, uint32_t nth,
             s = 0.0f;
             for (uint32_t d = 0; d < a.dim; d++)
                 s = fmaf(hk_bf2f(q[d]), hk_bf2f(key[d]), s);
-            s *= a.scale;
         }
         const float most = fmaxf(top, hk_wave_max(s));
         /* every score so far -inf: no weights yet */
         const float ref = most == -INFINITY ? 0.0f : most;
-        const float keep = expf(top - ref), p = expf(s - ref);
+        const float keep =
+            top == -INFINITY ? 0.0f : expf((top - ref) * a.scale);
+        const float p = lane < left ? expf((s - ref) * a.scale) : 0.0f;
         top = most;
         sum = sum * keep + hk_wave_sum(p);
         for (uint32_t d = 0; d < HK_PACKED_MAX_DIM / 64; d++) o[d] *= keep;
@@ -228,6 +231,21 @@ __device__ __forceinline__ void hk_packed_vt_wait(hk_v2i (&vt)[2][2]) {
                  : "+v"(vt[0][0]), "+v"(vt[0][1]), "+v"(vt[1][0]),
                    "+v"(vt[1][1])
                  : "i"(N));
+}
+
+/* P = exp2((s - m) L), L = scale log2(e), against a reference m, a score
+ * itself (not yet times L): maxima, references between tiles and the pieces'
+ * are compared as (m - m') L.  Near zero, |m L| < HK_PACKED_FAR, one fused
+ * multiply-add a score does it, fma(s, L, -(m L)): what rounding m L moves the
+ * reference by, up to 2^-15, is less than the rounding of a score there.  The
+ * rounding grows with the score (at 2^33 it is 2^9, and P of every key would be
+ * 0 or infinite), so that beyond it m is subtracted from the scores first,
+ * which is exact near the maximum. */
+#define HK_PACKED_FAR 0x1p10f
+
+/* Whether -(m L) is: also if it is infinite or NaN. */
+__device__ __forceinline__ bool hk_packed_far(float neg) {
+    return !(fabsf(neg) < HK_PACKED_FAR);
 }
 
 /* A wave's direct-to-LDS load of 16 bytes per lane.  A function of its own:
@@ -367,18 +385,24 @@ __device__ __forceinline__ void hk_packed_few(const hk_packed_args &a,
         for (int r = 0; r < 16; r++) mx = fmaxf(mx, s[r]);
         const auto sw = __builtin_amdgcn_permlane32_swap(
             __float_as_uint(mx), __float_as_uint(mx), false, false);
-        mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) *
-             a.scale_log2;
+        mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
         const float m_new = fmaxf(m_run, mx);
         const float ref = m_new == -INFINITY ? 0.0f : m_new;
-        const float c = __builtin_amdgcn_exp2f(m_run - ref);
+        const float c = __builtin_amdgcn_exp2f((m_run - ref) * a.scale_log2);
+        float neg = -(ref * a.scale_log2);
+        if (__builtin_amdgcn_ballot_w64(hk_packed_far(neg))) {
+            const float less = hk_packed_far(neg) ? ref : 0.0f;
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[r] -= less;
+            if (hk_packed_far(neg)) neg = 0.0f;
+        }
         m_run = m_new;
         float sum = 0.0f;
         hk_bf16x8 pf[2];
 #pragma unroll
         for (int r = 0; r < 16; r++) {
             const float p = __builtin_amdgcn_exp2f(
-                __builtin_fmaf(s[r], a.scale_log2, -ref));
+                __builtin_fmaf(s[r], a.scale_log2, neg));
             sum += p;
             pf[r >> 3][r & 7] = (__bf16)p;
         }
@@ -424,10 +448,10 @@ __device__ __forceinline__ void hk_packed_few(const hk_packed_args &a,
 #pragma unroll
     for (uint32_t w = 0; w < HK_PACKED_WAVES; w++) {
         const float2 v = ml[w * 32u + col];
-        l += __builtin_amdgcn_exp2f(v.x - ref) * v.y;
+        l += __builtin_amdgcn_exp2f((v.x - ref) * a.scale_log2) * v.y;
     }
     const bool whole = it.part == HK_PACKED_WHOLE;
-    float weight = __builtin_amdgcn_exp2f(m_run - ref);
+    float weight = __builtin_amdgcn_exp2f((m_run - ref) * a.scale_log2);
     if (whole) weight *= l == 0.0f ? 0.0f : 1.0f / l;
     else if (wave == 0 && half == 0 && vrow < it.rows)
         a.part_ml[(size_t)it.part * HK_PACKED_QB + col] = make_float2(top, l);
@@ -586,7 +610,8 @@ hk_packed_flash(hk_packed_args a) {
     for (int d = 0; d < ND; d++)
 #pragma unroll
         for (int r = 0; r < 16; r++) o[d][r] = 0.0f;
-    float m_run = -INFINITY, l_part = 0.0f;
+    /* the reference m and -(m L); unset (-infinity) until a score has weight */
+    float m_run = -INFINITY, neg = INFINITY, l_part = 0.0f;
     /* a wave whose rows all lie past the request's stages its share of every
      * tile and meets every barrier, and computes nothing */
     const bool live = vrow0 < it.rows;
@@ -623,14 +648,16 @@ hk_packed_flash(hk_packed_args a) {
                     if (key >= it.kv_rows) s[kt][r] = -INFINITY;
                 }
         }
-        /* The softmax of hk_flash_fwd: P = exp2(s - m_run) against the
-         * running maximum as it stands, which moves (O and l rescaled) only
-         * when it is unset or one of its P sums passes 2^32.  P <= 2^32 keeps O
-         * and l far from overflow; P rounds to bf16 for the product, l sums
-         * the unrounded P. */
+        /* The softmax of hk_flash_fwd: P against the running maximum as it
+         * stands, which moves (O and l rescaled) only when it is unset or far
+         * or one of its P sums passes 2^32.  P <= 2^32 keeps O and l far from
+         * overflow.  P rounds to bf16, which the matrix cores take (two halves
+         * as of the adapters would be half as many products again), l sums the
+         * unrounded P: the result is off by 2^-8 of a weight at most where F32
+         * weights would leave it at the rounding of the output, 0.0023 and
+         * 0.0017 of its norm for 1500 keys. */
         hk_bf16x8 pf[2][2];
-        auto exps = [&]() -> float {
-            const float neg = -m_run;
+        auto exps = [&](float less) -> float {
             float sum = 0.0f;
 #pragma unroll
             for (int kt = 0; kt < 2; kt++) {
@@ -638,7 +665,7 @@ hk_packed_flash(hk_packed_args a) {
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
                     p[r] = __builtin_amdgcn_exp2f(
-                        __builtin_fmaf(s[kt][r], a.scale_log2, neg));
+                        __builtin_fmaf(s[kt][r], a.scale_log2, less));
                     sum += p[r];
                 }
 #pragma unroll
@@ -651,9 +678,9 @@ hk_packed_flash(hk_packed_args a) {
             }
             return sum;
         };
-        const bool unset = m_run == -INFINITY;
-        float sum = unset ? 0.0f : exps();
-        uint32_t move = unset || sum > 0x1p32f;
+        const bool far = hk_packed_far(neg); /* or unset */
+        float sum = far ? 0.0f : exps(neg);
+        uint32_t move = far || sum > 0x1p32f;
         if (__builtin_amdgcn_ballot_w64(move)) {
             /* a row's other half's too, but no other row's: what a row comes
              * to does not depend on the rows beside it */
@@ -667,21 +694,30 @@ hk_packed_flash(hk_packed_args a) {
                 for (int r = 0; r < 16; r++) mx = fmaxf(mx, s[kt][r]);
             const auto sw = __builtin_amdgcn_permlane32_swap(
                 __float_as_uint(mx), __float_as_uint(mx), false, false);
-            mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) *
-                 a.scale_log2;
+            mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
             const float m_new = move ? fmaxf(m_run, mx) : m_run;
             const float ref = m_new == -INFINITY ? 0.0f : m_new;
             const float c =
-                move ? __builtin_amdgcn_exp2f(m_run - ref) : 1.0f;
-            m_run = ref;
+                move ? __builtin_amdgcn_exp2f((m_run - ref) * a.scale_log2)
+                     : 1.0f;
+            /* every score so far -inf: the maximum stays unset */
+            m_run = m_new;
+            neg = -(m_new * a.scale_log2);
+            float less = -(ref * a.scale_log2);
+            if (__builtin_amdgcn_ballot_w64(hk_packed_far(less))) {
+                const float by = hk_packed_far(less) ? ref : 0.0f;
+#pragma unroll
+                for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) s[kt][r] -= by;
+                if (hk_packed_far(less)) less = 0.0f;
+            }
             l_part *= c;
 #pragma unroll
             for (int d = 0; d < ND; d++)
 #pragma unroll
                 for (int r = 0; r < 16; r++) o[d][r] *= c;
-            sum = exps();
-            /* every score so far -inf: the maximum stays unset */
-            m_run = m_new;
+            sum = exps(less);
         }
         l_part += sum;
 
@@ -799,9 +835,9 @@ hk_packed_flash(hk_packed_args a) {
     }
 }
 
-/* Joins the pieces of an item's rows: with the pieces' maxima m_p, sums l_p
- * and undivided O_p, O = sum_p 2^(m_p - M) O_p / sum_p 2^(m_p - M) l_p, M =
- * max_p m_p, in piece order.  A wave per row; a lane holds DP / 64 dims and
+/* Joins the pieces of an item's rows: with the pieces' references m_p, sums
+ * l_p and undivided O_p, O = sum_p w_p O_p / sum_p w_p l_p with w_p =
+ * 2^((m_p - M) L), M = max_p m_p, in piece order.  A wave per row; a lane holds DP / 64 dims and
  * has four pieces on their way.  Bound by the launch and two loads in
  * sequence: 64 joins of 8 rows take 4.8 us. */
 template <int DP>
@@ -836,7 +872,8 @@ __global__ void __launch_bounds__(256) hk_packed_joined(hk_packed_args a) {
 #pragma unroll
         for (uint32_t p = 0; p < 4; p++) {
             const float w = first + p < j.pieces
-                                ? __builtin_amdgcn_exp2f(mine[p].x - top)
+                                ? __builtin_amdgcn_exp2f((mine[p].x - top) *
+                                                         a.scale_log2)
                                 : 0.0f;
             l += first + p < j.pieces ? w * mine[p].y : 0.0f;
             sum += first + p < j.pieces ? op[p] * w : per{};
@@ -876,13 +913,14 @@ static void hk_packed_launch(struct h3_gpu *gpu, const hk_packed_args &a,
 /* Whether the matrix-core kernel takes these rows: whole 16-byte pieces, 64
  * key rows and 128 query and output rows below 2^31 bytes (the reach of lane
  * offsets), and a scale that -inf times it is -inf, what keys past the end are
- * set to. */
+ * set to, and 0 times it 0. */
 static bool hk_packed_takes(const struct h3_gpu *gpu,
                             const hk_packed_args &a) {
     return !gpu->reference_kernels && a.dim % 8u == 0 && a.dim <= 128u &&
            a.q_stride % 8u == 0 && a.kv_stride % 8u == 0 &&
            a.kv_stride < (1u << 24) && a.q_stride < (1u << 23) &&
            (uint64_t)a.heads * a.dim < (1u << 23) && a.scale_log2 > 0x1p-100f &&
+           isfinite(a.scale_log2) &&
            (((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v |
              (uintptr_t)a.o) & 15u) == 0;
 }
