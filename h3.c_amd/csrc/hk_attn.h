@@ -41,7 +41,9 @@ __device__ __forceinline__ uint32_t hk_v_swz(uint32_t row, uint32_t chunk) {
  * ds_read_tr builtin as possibly aliasing the direct-to-LDS loads in
  * flight and waits for all of them (vmcnt(0)) first -- the next tile's
  * loads, which then no longer overlap the current tile.  Their completion
- * is the caller's to wait for, with hk_vt_wait. */
+ * is the caller's to wait for, with hk_vt_wait.  The outputs are early
+ * clobbers: the second read's address must not lie in what the first one
+ * fills. */
 __device__ __forceinline__ void hk_vt_read(hk_v2i (&vt)[4][2],
                                            const uint32_t (&v_frag)[4],
                                            uint32_t off) {
@@ -49,7 +51,7 @@ __device__ __forceinline__ void hk_vt_read(hk_v2i (&vt)[4][2],
     for (int d = 0; d < 4; d++)
         asm volatile("ds_read_b64_tr_b16 %0, %2 offset:%3\n\t"
                      "ds_read_b64_tr_b16 %1, %2 offset:%4"
-                     : "=v"(vt[d][0]), "=v"(vt[d][1])
+                     : "=&v"(vt[d][0]), "=&v"(vt[d][1])
                      : "v"(v_frag[d]), "i"(off), "i"(off + 8u * 256u));
 }
 

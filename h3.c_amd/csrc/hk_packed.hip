@@ -208,7 +208,7 @@ __device__ __forceinline__ void hk_packed_vt_read(hk_v2i (&vt)[ND][2],
     for (int d = 0; d < ND; d++)
         asm volatile("ds_read_b64_tr_b16 %0, %2 offset:%3\n\t"
                      "ds_read_b64_tr_b16 %1, %2 offset:%4"
-                     : "=v"(vt[d][0]), "=v"(vt[d][1])
+                     : "=&v"(vt[d][0]), "=&v"(vt[d][1])
                      : "v"(frag[d]), "i"(off), "i"(off + 8u * ROW));
 }
 
