@@ -510,8 +510,14 @@ hk_packed_flash(hk_packed_args a) {
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t col = lane & 31u, half = lane >> 5;
 
-    const hk_packed_item it = a.items[blockIdx.x];
+    hk_packed_item it = a.items[blockIdx.x];
     if (it.row >= it.rows) return;
+    if (!a.part_o && it.part != HK_PACKED_WHOLE) {
+        /* no room for pieces' sums: the first one takes all keys */
+        if (it.tile) return;
+        it.tile_end = (it.kv_rows + HK_KT - 1u) / HK_KT;
+        it.part = HK_PACKED_WHOLE;
+    }
     if (it.rows - it.row <= 32u) {
         hk_packed_few<DIMS>(a, it, hk_lds);
         return;
@@ -837,9 +843,9 @@ hk_packed_flash(hk_packed_args a) {
 
 /* Joins the pieces of an item's rows: with the pieces' references m_p, sums
  * l_p and undivided O_p, O = sum_p w_p O_p / sum_p w_p l_p with w_p =
- * 2^((m_p - M) L), M = max_p m_p, in piece order.  A wave per row; a lane holds DP / 64 dims and
- * has four pieces on their way.  Bound by the launch and two loads in
- * sequence: 64 joins of 8 rows take 4.8 us. */
+ * 2^((m_p - M) L), M = max_p m_p, in piece order.  A wave per row; a lane
+ * holds DP / 64 dims and has four pieces on their way.  Bound by the launch and
+ * two loads in sequence: 64 joins of 8 rows take 4.8 us. */
 template <int DP>
 __global__ void __launch_bounds__(256) hk_packed_joined(hk_packed_args a) {
     const hk_packed_join j = a.joins[blockIdx.x];
@@ -903,7 +909,7 @@ static void hk_packed_launch(struct h3_gpu *gpu, const hk_packed_args &a,
                            dim3(HK_PACKED_WAVES * 64u), lds, gpu->stream,
                            part);
     }
-    if (n[HK_PACKED_JOINS])
+    if (a.part_o)
         hipLaunchKernelGGL(hk_packed_joined<DP>,
                            dim3(n[HK_PACKED_JOINS],
                                 (n[HK_PACKED_JOIN_ROWS] + 3u) / 4u),
@@ -1317,12 +1323,11 @@ int h3_hip_sdpa_packed_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
     if (hk_packed_takes(gpu, a)) {
         const size_t padded = dim <= 64 ? 64 : 128;
         const size_t rows = (size_t)n[HK_PACKED_PARTS] * HK_PACKED_QB;
-        if (rows) {
-            a.part_o = (float *)hk_splitk_space(
+        if (rows)
+            a.part_o = (float *)hk_splitk_try(
                 gpu, rows * (padded * sizeof(float) + sizeof(float2)));
-            if (!a.part_o) return 0;
-            a.part_ml = (float2 *)(a.part_o + rows * padded);
-        }
+        /* without scratch, items run whole */
+        if (a.part_o) a.part_ml = (float2 *)(a.part_o + rows * padded);
         if (dim <= 64)
             hk_packed_launch<64>(gpu, a, n);
         else if (dim <= 96)

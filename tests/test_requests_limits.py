@@ -46,3 +46,25 @@ out = launches()
     assert all(kernel == "hk_packed_flash<64>" for kernel, *_ in made)
     assert all(x * threads < 1 << 32 for _, x, _, _, threads, _ in made)
     assert sum(x for _, x, *_ in made) == rows * heads
+
+
+@pytest.mark.parametrize("qn,kn,heads,kv,dim", [
+    ([1] * 8, [6144] * 8, 64, 8, 128), ([128, 40], [9720, 9000], 32, 32, 64),
+    ([300], [3000], 12, 4, 96)])
+def test_packed_attention_without_scratch(qn, kn, heads, kv, dim):
+    """It is taken, with no joins."""
+    made = on_fake(PLAN + """
+h = plan(qn, kn, heads, kv, dim)
+y, q = (gpu.new_bf16(sum(qn) * heads * dim) for _ in "yq")
+k = gpu.new_bf16(max(kn) * kv * dim)
+gpu.begin()
+out = []
+for size in (0, -1):
+    fake.fake_largest_block(C.c_size_t(size)); fake.fake_clear()
+    assert gpu.L.h3_hip_sdpa_packed_bf16(
+        gpu.h, y, q, 0, heads * dim, k, 0, k, 0, kv * dim, h, 1.0), gpu.error()
+    out.append([l[0] for l in launches()])
+""", qn=qn, kn=kn, heads=heads, kv=kv, dim=dim)
+    flash = f"hk_packed_flash<{dim}>"
+    joined = f"hk_packed_joined<{64 if dim <= 64 else 128}>"
+    assert made == [[flash], [flash, joined]]
