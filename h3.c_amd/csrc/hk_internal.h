@@ -161,8 +161,8 @@ enum { HK_EPI_STORE = 0, HK_EPI_SWIGLU = 1, HK_EPI_GELU = 2,
  * `scratch` is given, to that caller-owned device buffer of scratch_bytes:
  * then nothing is allocated, and a split that needs more fails (launches of
  * at most 128 rows use what the context has, and need no buffer).  `lora`
- * (HK_EPI_STORE or HK_EPI_GELU_F32, over 128 rows, hk_gemm_mfma_ok): the adapters'
- * part is added to the sums. */
+ * (HK_EPI_STORE or HK_EPI_GELU_F32, over tiles at any number of rows,
+ * hk_gemm_mfma_ok): the adapters' part is added to the sums. */
 int hk_gemm_bf16(struct h3_gpu *gpu, const uint16_t *a, const uint16_t *w,
                  const uint16_t *bias, uint16_t *c, uint32_t m, uint32_t n,
                  uint32_t k, int epilogue, float *scratch = nullptr,

@@ -844,9 +844,10 @@ static bool hk_lora_takes(const struct h3_gpu *gpu, const hk_lora_args &g) {
  * 8.4 us (in one piece 20), 4756 x 5376, ranks up to 64, 25 (44), 6144 x 5120,
  * up to 128, 36 (34 to 55). */
 static int hk_lora_run_tiles(struct h3_gpu *gpu, const hk_lora_args &a,
-                             hk_lora_low_args &g, uint32_t cus,
-                             uint32_t tile_rows) {
+                             hk_lora_low_args &g, uint32_t cus) {
     const uint32_t k_steps = a.k / HK_BK;
+    float us;
+    const uint32_t tile_rows = hk_gemm_tile_rows(gpu, a.m, a.n, a.k, &us);
     const uint32_t rb = a.rank <= 16 ? 1 : a.rank <= 32 ? 2 : 4;
     const uint32_t turns = std::min(a.count, 3u);
     g.chunks = (a.rank + 16u * rb - 1) / (16u * rb);
@@ -997,10 +998,11 @@ static int hk_lora_run_skinny(struct h3_gpu *gpu, const hk_lora_args &a,
     s.x_bytes = g.x_bytes;
     s.w_bytes = (uint32_t)((uint64_t)a.n * a.k * 2);
     s.split_steps = cut.steps;
-    s.partial = (float *)hk_splitk_space(
+    s.partial = (float *)hk_splitk_try(
         gpu, (size_t)cut.groups * cut.pieces * cut.columns * 4 * cut.mbs *
                  4096);
-    if (!s.partial) return 0;
+    /* the tiles need no sums of the whole output */
+    if (!s.partial) return hk_lora_run_tiles(gpu, a, g, cus);
     const size_t lds = cut.mbs * 4096 * 4 + 16384;
     const hk_lora_skinny_kernel kernel = hk_lora_skinny_pick(a.m, cut);
     if (cut.mbs >= 4) {
@@ -1074,7 +1076,7 @@ static int hk_lora_run(struct h3_gpu *gpu, const hk_lora_args &a) {
         }
     }
     float tiles;
-    const uint32_t tile_rows = hk_gemm_tile_rows(gpu, a.m, a.n, a.k, &tiles);
+    (void)hk_gemm_tile_rows(gpu, a.m, a.n, a.k, &tiles);
     /* over tiles W streams at 3 TB/s at most, the first product and the halves
      * come before the GEMM, and several adapters to a tile are more steps; in
      * the skinny workgroups' launch several adapters are more units (551 rows
@@ -1083,7 +1085,7 @@ static int hk_lora_run(struct h3_gpu *gpu, const hk_lora_args &a) {
             (a.count > 1 ? 18.0f : 14.0f);
     return skinny < (a.count > 1 ? 0.9f : 1.0f) * tiles
                ? hk_lora_run_skinny(gpu, a, g, cus, cut)
-                          : hk_lora_run_tiles(gpu, a, g, cus, tile_rows);
+               : hk_lora_run_tiles(gpu, a, g, cus);
 }
 
 /* elements of an adapter's fragments, a multiple of 512 */

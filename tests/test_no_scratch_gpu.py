@@ -64,3 +64,24 @@ for size in (0, -1):  # without and with scratch
     ro.check(got[covered], want[covered], bound[covered], f"limit {{size}}")
     assert (got[~covered] == 0x4141).all()
 """)
+
+
+@pytest.mark.skipif(not shutil.which("g++"), reason="needs g++")
+@pytest.mark.parametrize("rows,k,n", [(128, 64, 36000), (5, 128, 140000),
+                                      (300, 320, 20480), (1000, 320, 5120)])
+def test_adapters(rows, k, n):
+    """Tiles where the skinny GEMM's sums of the whole output find no room."""
+    run(f"""
+import test_lora_gpu as t
+a = t.make(32, t.spread({rows}, 3, 1), [16, 40, 3], {k}, {n})
+x, w, b, ids = gpu.bf16(a["x"]), gpu.bf16(a["w"]), gpu.bf16(a["b"]), gpu.u32(
+    a["ids"])
+table, y = t.table_of(gpu, a), gpu.new_bf16({rows * n})
+for act, name in ((False, ""), (True, "gelu_")):
+    want, bound = ro.lora(act=act, **a)
+    for size in (8 << 20, -1):  # room for the halves alone, and for all
+        limit(size)
+        gpu.run("h3_hip_linear_lora_" + name + "bf16", y, x, w, b, table, ids,
+                {rows}, {k}, {n})
+        ro.check(gpu.read_bf16(y), want, bound, f"limit {{size}}")
+""")

@@ -68,3 +68,27 @@ for size in (0, -1):
     flash = f"hk_packed_flash<{dim}>"
     joined = f"hk_packed_joined<{64 if dim <= 64 else 128}>"
     assert made == [[flash], [flash, joined]]
+
+
+@pytest.mark.parametrize("gelu", [False, True])
+@pytest.mark.parametrize("rows,k,n", [(39, 2688, 96768), (128, 64, 36000),
+                                      (5, 128, 140000), (300, 320, 20480),
+                                      (1000, 320, 5120)])
+def test_adapters_without_scratch(rows, k, n, gelu):
+    """They go over tiles, which need no sums of the whole output."""
+    made = on_fake("""
+d, u = gpu.new_bf16(16 * k), gpu.new_bf16(16 * n)
+t = gpu.lora_table([d], [u], [16], [1.0], k, n)
+x, w, y = gpu.new_bf16(rows * k), gpu.new_bf16(n * k), gpu.new_bf16(rows * n)
+ids = gpu.u32([0] * rows)
+call = (gpu.L.h3_hip_linear_lora_gelu_bf16 if gelu else
+        gpu.L.h3_hip_linear_lora_bf16)
+gpu.begin()
+out = []
+for size in (8 << 20, -1):
+    fake.fake_largest_block(C.c_size_t(size)); fake.fake_clear()
+    assert call(gpu.h, y, x, w, None, t, ids, rows, k, n), gpu.error()
+    out.append([l[0].split("<")[0] for l in launches()])
+""", rows=rows, k=k, n=n, gelu=gelu)
+    assert made == [["hk_lora_low", "hk_lora_halves", "hk_gemm_lora"],
+                    ["hk_lora_skinny", "hk_lora_join"]]
