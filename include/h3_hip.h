@@ -320,9 +320,11 @@ int h3_hip_linear_lora_gelu_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
  * h head_dim of `query` (likewise key and value, with kv_stride), so Q, K and
  * V may lie in the fused rows of one projection.  The output is
  * [row][heads][head_dim], a tensor of its own.  Numerics as in
- * h3_gpu_sdpa_bf16: F32 online softmax, P rounded to bf16 before P.V.  The
- * scale has to be finite and not negative.  No reference counterpart: the
- * reference serves one request at a time. */
+ * h3_gpu_sdpa_bf16: F32 online softmax, P rounded to bf16 before P.V.  A mask
+ * registered with h3_gpu_sdpa_set_sparse is not applied: its blocks are rows
+ * of one sequence, whatever requests the call packs.  The scale has to be
+ * finite and not negative.  No reference counterpart: the reference serves one
+ * request at a time. */
 h3_gpu_tensor *h3_hip_sdpa_packed_plan(h3_gpu *gpu, const uint32_t *q_first,
                                        const uint32_t *q_rows,
                                        const uint32_t *kv_first,
