@@ -18,13 +18,26 @@
  * round the adapters' part to 8 bits before it is added, two keep 16, below
  * what F32 sums of that length keep.  The activation takes the F32 sum.
  *
- * Measured, in brackets the projection alone in the same run (us): 8 rows x
- * 5120 -> 5120, eight adapters of rank 16, 16.8 (13.7); 39 x 2688 -> 96768
- * 101 (87), 5.3 TB/s; 197 x 5120 -> 5376 32 (36); 778 x 7168 -> 5376 88 (85);
- * 4756 x 5376 -> 21504, ranks 64 and 4, 828 (805), 1.34 PFLOP/s; 6144 x 5120
- * -> 13824 with GELU, ranks up to 128, 690 (667).  W's bytes bound the first
- * two, launches and the chains of dependent loads in them beside that, the
- * matrix cores at the package's power limit the last two.
+ * Measured, in brackets the projection alone in the same run (us; cards differ
+ * by up to 5%): 8 rows x 5120 -> 5120, eight adapters of rank 16, 16.8 (13.7);
+ * 39 x 2688 -> 96768 101 (87), 5.3 TB/s; 197 x 5120 -> 5376 32 (36); 778 x 7168
+ * -> 5376 89 (85); 4756 x 5376 -> 21504, ranks 64 and 4, 828 to 855 (805), 1.3
+ * PFLOP/s; 6144 x 5120 -> 13824 with GELU, ranks up to 128, 684 to 724 (667).
+ * W's bytes bound the first two, launches and the chains of dependent loads in
+ * them beside that; the third its steps of K, in which one wave a SIMD waits
+ * for X and W, turns them through LDS and multiplies in sequence; the fourth
+ * the cut GEMM and, 13.5 us, the two launches before it; the last two the
+ * matrix cores at the package's power limit.
+ *
+ * What a launch is made of follows the table, not the rows' map, which is only
+ * read on the device: workgroups for every rank chunk of the largest adapter
+ * and, up to their rows' number, for every adapter.  Those that find nothing
+ * leave, but are rounds of launches where there are many: 5120 -> 5120, rows of
+ * one adapter of rank 16 out of a table of one, of 64, and of 63 and one of
+ * rank 512: 8 rows 15.2, 15.2 and 17.8 us, 128 rows 26.1, 26.2 and 64.6.  And rows
+ * of many adapters in any order take each tile through all of them: 400 x 5120
+ * -> 13824 at rank 128 106 us with one, 114 with two, 263 with 16 and 546 with
+ * 64; 4756 x 5376 -> 21504, 16 of rank 64, in order 865, mixed 1341.
  *
  * The simple kernels here (one wave per element of x . A^T, one thread per
  * output, sums in sequence) serve H3_HIP_REFERENCE=1 and the shapes that the
@@ -1032,13 +1045,15 @@ static int hk_lora_run_skinny(struct h3_gpu *gpu, const hk_lora_args &a,
  * workgroup of up to 128 rows on a CU and 1.1 with two, more with more rows,
  * the pieces' sums go both ways at 4.5 TB/s; with more rows the first
  * product's units find no room on the CUs that have a workgroup, which a short
- * piece does not hide (133 to 4000 rows of eight K x N: within 20%).  Groups of 128 rows and tiles, measured
- * with one adapter of rank 16 (us): 160 x 320 -> 5120 12.5 and 24.6, 1200 rows
- * 28.3 and 26.2; 512 x 512 -> 1536 14.2 and 31.1, 4000 rows 32.4 and 43.5; 160
- * x 5120 -> 5120 25.6 and 39.1, 384 38.4 and 46.0, 512 58.8 and 54.2; 384 x
- * 5120 -> 13824 109 and 84.  Those and one group: 133 x 5120 -> 13824 69 and
- * 45, 197 rows 63 and 56; 133 x 5376 -> 21504 95 (tiles) and 72; 197 x 5120 ->
- * 5120 30.4 and 31.5. */
+ * piece does not hide.  The constants were fitted by hand to 133 to 4000 rows
+ * of eight K x N with one or two adapters of up to 128 ranks, within 20%; they
+ * know neither the ranks nor, past the first, the number of adapters.
+ * Groups of 128 rows and tiles, measured with one adapter of rank 16 (us): 160
+ * x 320 -> 5120 12.5 and 24.6, 1200 rows 28.3 and 26.2; 512 x 512 -> 1536 14.2
+ * and 31.1, 4000 rows 32.4 and 43.5; 160 x 5120 -> 5120 25.6 and 39.1, 384 38.4
+ * and 46.0, 512 58.8 and 54.2; 384 x 5120 -> 13824 109 and 84.  Those and one
+ * group: 133 x 5120 -> 13824 69 and 45, 197 rows 63 and 56; 133 x 5376 -> 21504
+ * 95 (tiles) and 72; 197 x 5120 -> 5120 30.4 and 31.5. */
 static float hk_lora_skinny_us(const hk_lora_cut &c, uint32_t m, uint32_t n,
                                uint32_t cus) {
     static const float step_us[8] = {0.65f, 0.65f, 0.65f, 0.65f,

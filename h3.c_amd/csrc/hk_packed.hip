@@ -162,25 +162,34 @@ __global__ void __launch_bounds__(256) hk_packed_simple(hk_packed_args a) {
  *     request's keys, so what lies behind them (other requests' rows) reads
  *     as zeros and P = 0 meets no infinity or NaN there;
  *   - DIMS = 64, 96 or 128 dims in LDS rows of 64 or 128 (4000 rows, 24 heads
- *     of 96 over 4: 193 us, computed as 128 dims 222), smaller heads padded: a
+ *     of 96 over 4: 160 us, computed as 128 dims 184), smaller heads padded: a
  *     lane whose piece lies past the head's dims loads from beyond the
  *     resource, zeros;
  *   - tile addresses are 64-bit, so a context may pass 4 GiB;
  *   - NaN scores stay NaN (this file is compiled without the flag that lets
  *     hk_attn.hip assume none).
  *
- * What bounds it, measured: self-attention the matrix cores at the package's
- * power limit (778, 1536 and 2378 rows x 56 heads 257 us, 960 TFLOP/s; rows of
- * 64 with four query heads a key head, 52 us, 860); cross-attention to a text
- * an item's start and end around eight tiles (four clips of 6144 rows 180 us,
- * 620 TFLOP/s and 2.9 TB/s); single rows the bytes of K and V (eight rows over
- * contexts of 4096 to 9720 49 us, 4.7 TB/s) or, with short contexts, the chain
- * item, tiles, joining, store (sixteen rows 13 us, 3.8 TB/s).
+ * What bounds it, measured (cards differ by up to 5%): self-attention products
+ * and exponentials (778, 1536 and 2378 rows x 56 heads 252 to 264 us, 950
+ * TFLOP/s; 6144 rows x 40 heads 705, 1.1 PFLOP/s), near the package's power
+ * limit though not by that alone, as the figures beside hk_flash_fwd below
+ * show; with heads of 64 also a step's barrier and its wait for all loads, as
+ * long for half the products (four query heads a key head, 52 to 55 us, 840
+ * TFLOP/s); cross-attention to a text an item's start and end around eight
+ * tiles, and that items bound by products and items bound by bytes do not
+ * overlap (four clips of 6144 rows 176 to 187 us, the sum of its bytes' 106 and
+ * its products' 73); single rows the bytes of K and V (eight rows over contexts
+ * of 4096 to 9720 49 us, 5 of them the join's: 5.2 TB/s, where a stream of
+ * weights reads 6.4) or, with short contexts, the chain item, tiles, joining,
+ * store (sixteen rows 13 us, 3.8 TB/s).
  *
- * Four waves of 32 rows and two workgroups a CU: with eight waves 6144 rows of
- * self-attention took 720 us for 754, but 4096 rows 344 for 335, 2378 rows x
- * 56 heads 201 for 190 and 6144 rows x 512 keys 96 for 89.  64 rows a wave,
- * which would halve the LDS reads, spill 300 registers at head size 128. */
+ * Four waves of 32 rows and two workgroups a CU.  Beside hk_flash_fwd, whose
+ * eight waves share a tile (one request, us here and there): 2378 rows x 56
+ * heads 172 and 194, 4096 x 40 324 and 334, 6144 x 40 707 and 686.  Eight waves
+ * here, before items were cut: 6144 rows 720 for 754, but 4096 rows 344 for
+ * 335, 2378 rows x 56 heads 201 for 190 and 6144 rows x 512 keys 96 for 89.  64
+ * rows a wave, which would halve the LDS reads, spill 300 registers at head
+ * size 128. */
 
 /* The swizzles of LDS tiles with rows of DP bf16: 16-byte chunk c of row r
  * lies at chunk c ^ key(r).  K's fragment reads take one chunk of 16
@@ -265,10 +274,11 @@ __device__ __forceinline__ void hk_packed_dma16(__amdgpu_buffer_rsrc_t r,
  * is computed, V once P . V is.  Bound by the chain of a step (scores, maximum,
  * exponentials, product: about 1 us, whatever the loads do), of which there
  * are a quarter as many as with the waves on rows: three rows, the longest
- * context 473 keys, 64 heads over 8, 7.0 us instead of 12.6 (13.9 with four
- * stages of tiles instead of two); sixteen rows x 40 heads 12.8 and 14.3; one
- * row, 2566 keys, 24 heads of 96 over 4, 9.0 and 10.9.  Long contexts, bound
- * by K's and V's bytes, are level. */
+ * context 473 keys, 64 heads over 8, 7.4 us instead of 12.9; sixteen rows x 40
+ * heads 13.1 and 14.5; one row, 2566 keys, 24 heads of 96 over 4, 9.8 and 11.8.
+ * Long contexts, bound by K's and V's bytes, are level.  A request's last few
+ * rows beside many full items lose by it: 2185 rows x 40 heads, the last 9 of
+ * each 119 us and 109. */
 template <int DIMS>
 __device__ __forceinline__ void hk_packed_few(const hk_packed_args &a,
                                               const hk_packed_item &it,
@@ -948,16 +958,16 @@ static bool hk_packed_takes(const struct h3_gpu *gpu,
  * - those behind the last full round of one item a CU, where that promises 5%
  *   (two workgroups of matrix products share what one alone would get, so a
  *   CU is one place; self-attention in us, uncut and cut: 1200 rows x 56
- *   heads, 2.2 rounds, 62.8 and 54.8; 2378 x 56, 4.2, 189 and 173; 2560 x 40,
- *   3.1, 158 and 148; counted as two places a CU, 2185 x 40, 2.8 rounds, was
- *   cut and took 129 for 113).
+ *   heads, 2.2 rounds, 62.4 and 54.7; 2378 x 56, 4.2, 187 and 167; 2560 x 40,
+ *   3.1, 150 and 137; 6144 x 40, 7.5, 733 and 705; counted as two places a CU,
+ *   2185 x 40, 2.8 rounds, was cut and took 129 for 113 then).
  *
  * Where 128 rows make few items, items of 32 rows fill the CUs and have a
  * quarter of the steps (hk_packed_few), at the price of K and V four times
  * from L2: up to one a CU, and up to two if they are mostly full (measured with
  * 128 and 32 rows, us: 700 rows of self-attention x 8 heads, 176 small items,
- * 17.2 and 11.2; 537 x 16 over 2, 272, 15.5 and 13.4; 1200 x 12 of 64, 456,
- * 22.3 and 13.1; 300 rows x 24 heads of 96, 512 keys, 240, 12.1 and 8.6; but
+ * 17.7 and 10.3; 537 x 16 over 2, 272, 15.7 and 12.4; 1200 x 12 of 64, 456,
+ * 18.0 and 12.1; 300 rows x 24 heads of 96, 512 keys, 240, 12.0 and 7.9; but
  * 300 rows x 40, 400 and 5 tiles, 11.3 and 12.4; four times 50 rows x 40, 320
  * half empty ones, 13.7 and 15.2). */
 struct hk_packed_work {

@@ -264,10 +264,16 @@ int h3_gpu_linear_gelu_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
  *
  * h3_hip_lora_table copies the adapters, laid out for the kernels, so the
  * given tensors may be freed or changed once it returns (change an adapter by
- * building another table); free the table with h3_gpu_tensor_free.  Adapters
- * and scales have to be finite: rows of several requests share a matrix
- * product, where one adapter's infinity would reach the others' rows.  NULL
- * entries of down and up are allowed at rank 0.
+ * building another table); free the table with h3_gpu_tensor_free.  It holds
+ * each down_a once and each up_a three times, twice with the rank padded to a
+ * multiple of 32, once to 16: at rank 16 five, at rank 4 twenty times its
+ * bytes, at multiples of 32 three.  Building copies every adapter and waits for
+ * the stream, also where one of them is to change.  A call's launches grow with
+ * the table's adapters and largest rank, whichever of them its rows use.
+ *
+ * Adapters and scales have to be finite: rows of several requests share a
+ * matrix product, where one adapter's infinity would reach the others' rows.
+ * NULL entries of down and up are allowed at rank 0.
  *
  * h3_hip_linear_lora_bf16 runs the projection; input_dim and output_dim have
  * to be the table's.  Sums are F32 and the result is rounded once: x . down^T
