@@ -34,10 +34,10 @@
  * and, up to their rows' number, for every adapter.  Those that find nothing
  * leave, but are rounds of launches where there are many: 5120 -> 5120, rows of
  * one adapter of rank 16 out of a table of one, of 64, and of 63 and one of
- * rank 512: 8 rows 15.2, 15.2 and 17.8 us, 128 rows 26.1, 26.2 and 64.6.  And rows
- * of many adapters in any order take each tile through all of them: 400 x 5120
- * -> 13824 at rank 128 106 us with one, 114 with two, 263 with 16 and 546 with
- * 64; 4756 x 5376 -> 21504, 16 of rank 64, in order 865, mixed 1341.
+ * rank 512: 8 rows 15.2, 15.2 and 17.8 us, 128 rows 26.1, 26.2 and 64.6.  And
+ * rows of many adapters in any order meet all of them in each tile or 32 rows:
+ * 400 x 5120 -> 13824 at rank 128 106 us with one, 114 with two, 218 with 16 and
+ * 336 with 64; 4756 x 5376 -> 21504, 16 of rank 64, in order 865, mixed 1341.
  *
  * The simple kernels here (one wave per element of x . A^T, one thread per
  * output, sums in sequence) serve H3_HIP_REFERENCE=1 and the shapes that the
@@ -1045,10 +1045,7 @@ static int hk_lora_run_skinny(struct h3_gpu *gpu, const hk_lora_args &a,
  * workgroup of up to 128 rows on a CU and 1.1 with two, more with more rows,
  * the pieces' sums go both ways at 4.5 TB/s; with more rows the first
  * product's units find no room on the CUs that have a workgroup, which a short
- * piece does not hide.  The constants were fitted by hand to 133 to 4000 rows
- * of eight K x N with one or two adapters of up to 128 ranks, within 20%; they
- * know neither the ranks nor, past the first, the number of adapters.
- * Groups of 128 rows and tiles, measured with one adapter of rank 16 (us): 160
+ * piece does not hide.  Groups of 128 rows and tiles, measured with one adapter of rank 16 (us): 160
  * x 320 -> 5120 12.5 and 24.6, 1200 rows 28.3 and 26.2; 512 x 512 -> 1536 14.2
  * and 31.1, 4000 rows 32.4 and 43.5; 160 x 5120 -> 5120 25.6 and 39.1, 384 38.4
  * and 46.0, 512 58.8 and 54.2; 384 x 5120 -> 13824 109 and 84.  Those and one
@@ -1064,6 +1061,35 @@ static float hk_lora_skinny_us(const hk_lora_cut &c, uint32_t m, uint32_t n,
     const float start = c.mbs <= 4 ? 6.0f : c.pieces > 1 ? 14.0f : 8.0f;
     return (float)rounds * (float)c.steps * step + start +
            (float)m * (float)n * (float)(8 * c.pieces + 2) / 4.5e6f;
+}
+
+/* The adapters that `rows` rows next to each other have, where the table's
+ * follow each other over the call's rows, as those of packed requests do: the
+ * map itself is on the device. */
+static float hk_lora_adapters(const hk_lora_args &a, uint32_t rows) {
+    return std::min((float)a.count,
+                    1.0f + (float)(a.count - 1u) * (float)rows / (float)a.m);
+}
+
+/* What the two estimates, made for one adapter of rank 16, leave out.  An
+ * adapter of a tile is a change of operands and, at padded / 32, steps of 64:
+ * 1 and 1.7 us a round of tiles. */
+static float hk_lora_tiles_more_us(const hk_lora_args &a, uint32_t tile_rows,
+                                   uint32_t cus) {
+    const float rounds =
+        std::max(1.0f, (float)((a.m + tile_rows - 1u) / tile_rows) *
+                           (float)((a.n + HK_BN - 1u) / HK_BN) / (float)cus);
+    return rounds * (hk_lora_adapters(a, tile_rows) *
+                         (1.0f + 1.7f * (float)a.pitch / 32.0f) -
+                     2.7f);
+}
+
+/* An adapter of the join's 32 rows is a B to wait for at every 16 ranks, with
+ * 20 waves on a CU. */
+static float hk_lora_join_more_us(const hk_lora_args &a, uint32_t cus) {
+    const float waves = (float)((a.m + 31u) / 32u) * (float)((a.n + 31u) / 32u);
+    return (hk_lora_adapters(a, 32u) * (float)((a.rank + 15u) / 16u) - 1.0f) *
+           (0.5f + 1.3f * waves / (20.0f * (float)cus));
 }
 
 static int hk_lora_run(struct h3_gpu *gpu, const hk_lora_args &a) {
@@ -1091,14 +1117,17 @@ static int hk_lora_run(struct h3_gpu *gpu, const hk_lora_args &a) {
         }
     }
     float tiles;
-    (void)hk_gemm_tile_rows(gpu, a.m, a.n, a.k, &tiles);
-    /* over tiles W streams at 3 TB/s at most, the first product and the halves
-     * come before the GEMM, and several adapters to a tile are more steps; in
-     * the skinny workgroups' launch several adapters are more units (551 rows
-     * x 5120 -> 5120 of eight, 64 us by the estimate, took 76) */
-    tiles = std::max(tiles, (float)a.n * (float)a.k * 2.0f / 3e6f) +
-            (a.count > 1 ? 18.0f : 14.0f);
-    return skinny < (a.count > 1 ? 0.9f : 1.0f) * tiles
+    const uint32_t tile_rows = hk_gemm_tile_rows(gpu, a.m, a.n, a.k, &tiles);
+    /* Over tiles W streams at 3 TB/s at most, the first product and the halves
+     * come before the GEMM.  The tiles are the safer side of the border.  Timed
+     * both ways, the rule takes the faster one or one within 5% in 87 of 92
+     * calls with one or two adapters (133 to 4000 rows of eight K x N; 12% at
+     * worst) and in 62 of 63 with 4 to 64 whose rows follow each other (6%).
+     * Rows in any order are not known here: 51 of 59, and up to 1.8 times (1536
+     * x 7168 -> 5376, 64 of rank 16: 387 us over tiles, 219). */
+    tiles = std::max(tiles, (float)a.n * (float)a.k * 2.0f / 3e6f) + 14.0f +
+            hk_lora_tiles_more_us(a, tile_rows, cus);
+    return skinny + hk_lora_join_more_us(a, cus) < 0.95f * tiles
                ? hk_lora_run_skinny(gpu, a, g, cus, cut)
                : hk_lora_run_tiles(gpu, a, g, cus);
 }

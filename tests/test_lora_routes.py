@@ -3,7 +3,7 @@
 import pytest
 
 from requests_oracle import on_fake
-from test_lora_tiles_gpu import HEIGHTS, SHAPES, SMALL
+from test_lora_tiles_gpu import CUT, MANY, SEVERAL, SHAPES, SMALL
 
 RUN = """
 out = []
@@ -53,15 +53,40 @@ def test_every_first_product_and_tile_height_is_among_them():
         *(f"gemm<3, {b}>" for b in (5, 6, 8))}
 
 
-@pytest.mark.parametrize("ranks", [
-    (1, 8), (1024, 8), (4, 16, 0, 33, 64, 8, 128), (2,) * 281])
-def test_shapes_stay_with_tiles_whatever_the_adapters(ranks):
-    """Their tests use other tables than SHAPES names."""
-    made = kernels([(*s, ranks, False) for s in [SMALL, *HEIGHTS]
-                    if len(ranks) < 200 or s[0] < 3000])
-    for found in made:
-        assert found[1] == "hk_lora_halves" and \
-            found[2].startswith("hk_gemm_lora<"), found
+def test_shapes_of_other_tables():
+    """The other tests' of test_lora_tiles_gpu.py."""
+    cut = (284, 5120, 6428)
+    cases = [*SEVERAL.items(), *((s, (2,) * 281) for s in MANY),
+             *((SMALL, (r, 8)) for r in (1, 64, 320)),
+             *((CUT, (r, 8)) for r in (4, 33, 64, 1024)),
+             *((s, (16, 33, 8)) for s in (SMALL, (386, 512, 21528), cut)),
+             *((s, r) for s in (SMALL, cut) for r in ((16,), (16, 8, 33, 64)))]
+    for (shape, ranks), found in zip(cases, kernels(
+            [(*s, r, False) for s, r in cases])):
+        assert found[1] == "hk_lora_halves", (shape, ranks[:4], found)
+        assert found[2].startswith("hk_gemm_lora<")
+        assert found[2].startswith("hk_gemm_lora<3") == (
+            shape in (cut, CUT, (562, 2560, 9664), (2725, 2560, 1432)))
+
+
+# us over groups of rows and over tiles, adapters in the order of the rows
+@pytest.mark.parametrize("rows,k,n,ranks,groups", [
+    (400, 5120, 13824, (16,), False),         # 107, 95
+    (400, 5120, 13824, (64, 16), False),      # 114, 101
+    (400, 5120, 13824, (128,) * 16, True),    # 134, 172
+    (400, 5120, 13824, (512,) * 16, True),    # 251, 366
+    (400, 5120, 13824, (16,) * 64, True),     # 112, 196
+    (400, 5120, 13824, (128,) * 64, True),    # 182, 356
+    (1000, 5120, 5120, (16,), False),         # 88, 72
+    (1000, 5120, 5120, (128,) * 64, True),    # 131, 200
+    (1000, 5120, 5120, (16,) * 64, True),     # 96, 118
+    (1000, 5120, 13824, (128,) * 64, False),  # 298, 258
+    (1000, 5120, 13824, (16,) * 64, False),   # 217, 168
+    (2000, 2688, 10752, (128,) * 64, False),  # 267, 207
+    (597, 5120, 5120, (128,) * 64, True)])    # 104, 254
+def test_many_adapters_go_the_faster_way(rows, k, n, ranks, groups):
+    made, = kernels([(rows, k, n, ranks, False)])
+    assert (made[-1] == "hk_lora_join") == groups
 
 
 @pytest.mark.parametrize("rows,k,n,kernel", [

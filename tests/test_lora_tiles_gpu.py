@@ -31,10 +31,18 @@ SHAPES = {
     (374, 5120, 6972, (32, 8)): ("low<2, 2>", "gemm<3, 6>"),
     (2725, 2560, 1432, (64, 16)): ("low<4, 4>", "gemm<3, 8>"),
 }
-# one of each tile height, whole and cut
-HEIGHTS = [(2601, 64, 2872), (2669, 768, 2944), (1177, 768, 6600),
-           (534, 320, 16808), (386, 512, 21528), (284, 5120, 6428),
-           (374, 5120, 6972), (2725, 2560, 1432)]
+# several adapters over each tile height, whole and cut
+SEVEN = (4, 16, 0, 33, 64, 8, 128)
+SEVERAL = {
+    (2601, 64, 2872): SEVEN, (2669, 768, 2944): SEVEN,
+    (1177, 768, 6600): SEVEN, (534, 320, 16808): SEVEN,
+    (386, 512, 21528): SEVEN, (284, 5120, 6428): (16, 8, 33, 64),
+    (374, 5120, 6972): (16, 8, 33, 64), (562, 2560, 9664): SEVEN,
+    (2725, 2560, 1432): SEVEN,
+}
+# two adapters for every three rows of a tile, and more
+MANY = [(8553, 1024, 992), (6773, 512, 1604), (5586, 128, 5488)]
+CUT = (374, 5120, 6972)
 SMALL = (2601, 64, 2872)
 
 
@@ -56,13 +64,13 @@ def test_every_kernel(gpu, shape, act):
 
 
 @pytest.mark.parametrize("act", [False, True])
-@pytest.mark.parametrize("shape", HEIGHTS)
+@pytest.mark.parametrize("shape", SEVERAL)
 def test_adapters_in_any_order(gpu, shape, act):
-    """Seven in every tile, and rows of none."""
+    """All in every tile, and rows of none."""
     rows, k, n = shape
-    check(gpu, make(rows + 1, spread(rows, 7, rows),
-                    [4, 16, 0, 33, 64, 8, 128], k, n, bias=not act,
-                    scale=0.02), act)
+    ranks = SEVERAL[shape]
+    check(gpu, make(rows + 1, spread(rows, len(ranks), rows), ranks, k, n,
+                    bias=not act, scale=0.02), act)
 
 
 @pytest.mark.parametrize("rank", [1, 2, 7, 8, 9, 15, 16, 17, 24, 31, 32, 33, 40,
@@ -74,14 +82,13 @@ def test_ranks(gpu, rank):
 
 @pytest.mark.parametrize("rank", [4, 33, 64, 1024])
 def test_ranks_of_a_cut_launch(gpu, rank):
-    check(gpu, make(rank, parts(284, 2), [rank, 8], 5120, 6428, scale=0.02))
+    rows, k, n = CUT
+    check(gpu, make(rank, parts(rows, 2), [rank, 8], k, n, scale=0.02))
 
 
-@pytest.mark.parametrize("shape", [SMALL, (2669, 768, 2944),
-                                   (534, 320, 16808), (386, 512, 21528),
-                                   (284, 5120, 6428)])
-def test_an_adapter_for_every_row(gpu, shape):
-    """More of them than a tile's list holds lanes of a wave; K in pieces."""
+@pytest.mark.parametrize("shape", MANY)
+def test_an_adapter_for_almost_every_row(gpu, shape):
+    """More of them than a wave has lanes, in each tile's list."""
     rows, k, n = shape
     check(gpu, make(rows + 2, np.arange(rows) * 7 % 281, [2] * 281, k, n,
                     scale=0.02))
