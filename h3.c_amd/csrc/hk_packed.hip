@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(256) hk_packed_simple(hk_packed_args a) {
  * tiles, and that items bound by products and items bound by bytes do not
  * overlap (four clips of 6144 rows 176 to 187 us, the sum of its bytes' 106 and
  * its products' 73); single rows the bytes of K and V (eight rows over contexts
- * of 4096 to 9720 49 us, 5 of them the join's: 5.2 TB/s, where a stream of
+ * of 4096 to 9720 49 us, 5 of them the join's: 5.1 TB/s, where a stream of
  * weights reads 6.4) or, with short contexts, the chain item, tiles, joining,
  * store (sixteen rows 13 us, 3.8 TB/s).
  *
