@@ -15,8 +15,18 @@ void fail_once(size_t bytes) { once = bytes; }
 
 int hipMalloc(void **p, size_t bytes) {
     typedef int (*alloc)(void **, size_t);
-    static const alloc real =
-        (alloc)dlsym(dlopen("libamdhip64.so", RTLD_LAZY), "hipMalloc");
+    static alloc real;
+    if (!real) {
+        /* the one that the backend has loaded */
+        const char *const names[] = {"libamdhip64.so.7", "libamdhip64.so.6",
+                                     "libamdhip64.so"};
+        for (const char *name : names) {
+            void *runtime = real ? NULL
+                                 : dlopen(name, RTLD_LAZY | RTLD_NOLOAD);
+            if (runtime) real = (alloc)dlsym(runtime, "hipMalloc");
+        }
+        if (!real) return 1; /* hipErrorInvalidValue */
+    }
     if (bytes > largest || bytes > once) {
         if (bytes > once) once = ~(size_t)0;
         *p = NULL;
