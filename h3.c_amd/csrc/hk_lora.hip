@@ -98,34 +98,43 @@ struct hk_lora_row {
     uint32_t adapter, unused[3];
 };
 
+/* Workgroups of the kernels below, each thread an element at a time: a launch
+ * has fewer than 2^32 threads. */
+static dim3 hk_lora_pack_grid(uint64_t count) {
+    return dim3((unsigned)std::min<uint64_t>((count + 255) / 256, 1u << 22));
+}
+
 /* Copies a [rows][cols] matrix, `count` elements with zeros behind each row up
  * to `pitch`, with each row `times` over. */
 __global__ void __launch_bounds__(256)
 hk_lora_pack(const uint16_t *src, uint16_t *dst, uint32_t cols, uint32_t pitch,
              uint32_t times, uint64_t count, hk_lora_entry *entry) {
-    const uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x;
-    if (i >= count) return;
-    const uint64_t r = i / pitch;
-    const uint32_t c = (uint32_t)(i - r * pitch);
-    const uint16_t v = c < cols ? src[r * cols + c] : (uint16_t)0;
-    for (uint32_t t = 0; t < times; t++)
-        dst[(r * times + t) * pitch + c] = v;
-    if ((v & 0x7f80u) == 0x7f80u) entry->bad = 1; /* every writer writes 1 */
+    for (uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x; i < count;
+         i += (uint64_t)gridDim.x * 256u) {
+        const uint64_t r = i / pitch;
+        const uint32_t c = (uint32_t)(i - r * pitch);
+        const uint16_t v = c < cols ? src[r * cols + c] : (uint16_t)0;
+        for (uint32_t t = 0; t < times; t++)
+            dst[(r * times + t) * pitch + c] = v;
+        /* every writer writes 1 */
+        if ((v & 0x7f80u) == 0x7f80u) entry->bad = 1;
+    }
 }
 
 /* B ([N][rank]) as hk_lora_entry's fragments. */
 __global__ void __launch_bounds__(256)
 hk_lora_pack_fragments(const uint16_t *src, uint16_t *dst, uint32_t n,
                        uint32_t rank, uint64_t count) {
-    const uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x;
-    if (i >= count) return;
-    const uint32_t at = (uint32_t)(i % 512u), lane = at >> 3;
-    const uint64_t block = i / 512u;
     const uint32_t chunks = (rank + 15u) / 16u;
-    const uint64_t col = block / chunks * 32u + (lane & 31u);
-    const uint32_t k =
-        (uint32_t)(block % chunks) * 16u + (lane >> 5) * 8u + (at & 7u);
-    dst[i] = col < n && k < rank ? src[col * rank + k] : (uint16_t)0;
+    for (uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x; i < count;
+         i += (uint64_t)gridDim.x * 256u) {
+        const uint32_t at = (uint32_t)(i % 512u), lane = at >> 3;
+        const uint64_t block = i / 512u;
+        const uint64_t col = block / chunks * 32u + (lane & 31u);
+        const uint32_t k =
+            (uint32_t)(block % chunks) * 16u + (lane >> 5) * 8u + (at & 7u);
+        dst[i] = col < n && k < rank ? src[col * rank + k] : (uint16_t)0;
+    }
 }
 
 /* low[r][j] = s_a x[r] . A_a[j]: one wave an element at a time. */
@@ -1214,17 +1223,17 @@ h3_gpu_tensor *h3_hip_lora_table(h3_gpu *gpu,
         if (!e.rank) continue;
         const uint64_t d = (uint64_t)e.rank * input_dim;
         const uint64_t u = (uint64_t)e.padded * output_dim;
-        hipLaunchKernelGGL(hk_lora_pack, dim3((unsigned)((d + 255) / 256)),
-                           dim3(256), 0, gpu->stream, HK_CBF16(down[a]),
+        hipLaunchKernelGGL(hk_lora_pack, hk_lora_pack_grid(d), dim3(256), 0,
+                           gpu->stream, HK_CBF16(down[a]),
                            (uint16_t *)e.down, input_dim, input_dim, 1u, d,
                            device + a);
-        hipLaunchKernelGGL(hk_lora_pack, dim3((unsigned)((u + 255) / 256)),
-                           dim3(256), 0, gpu->stream, HK_CBF16(up[a]),
+        hipLaunchKernelGGL(hk_lora_pack, hk_lora_pack_grid(u), dim3(256), 0,
+                           gpu->stream, HK_CBF16(up[a]),
                            (uint16_t *)e.up, e.rank, e.padded, 2u, u,
                            device + a);
         const uint64_t f = hk_lora_fragment_count(output_dim, e.rank);
-        hipLaunchKernelGGL(hk_lora_pack_fragments,
-                           dim3((unsigned)((f + 255) / 256)), dim3(256), 0,
+        hipLaunchKernelGGL(hk_lora_pack_fragments, hk_lora_pack_grid(f),
+                           dim3(256), 0,
                            gpu->stream, HK_CBF16(up[a]),
                            (uint16_t *)e.fragments, output_dim, e.rank, f);
         status = hipGetLastError();

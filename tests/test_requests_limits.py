@@ -92,3 +92,18 @@ for size in (8 << 20, -1):
 """, rows=rows, k=k, n=n, gelu=gelu)
     assert made == [["hk_lora_low", "hk_lora_halves", "hk_gemm_lora"],
                     ["hk_lora_skinny", "hk_lora_join"]]
+
+
+@pytest.mark.parametrize("rank,k,n", [(1024, 64, 4_300_000),
+                                      (1024, 4_300_000, 64), (4, 64, 32)])
+def test_launches_of_large_adapters_stay_within_a_grid(rank, k, n):
+    """B padded and A may have over 2^32 elements."""
+    made = on_fake("""
+d, u = gpu.new_bf16(rank * k), gpu.new_bf16(rank * n)
+fake.fake_clear()
+gpu.lora_table([d], [u], [rank], [1.0], k, n)
+out = launches()
+""", rank=rank, k=k, n=n)
+    assert [kernel for kernel, *_ in made] == [
+        "hk_lora_pack", "hk_lora_pack", "hk_lora_pack_fragments"]
+    assert all(x * threads < 1 << 32 for _, x, _, _, threads, _ in made)
