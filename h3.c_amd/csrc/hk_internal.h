@@ -29,8 +29,9 @@ struct h3_gpu_tensor {
      * output_dim, problems) it was built and validated for; all zero for
      * every other tensor */
     uint32_t group_shape[4];
-    /* host-side record of an adapter table or an attention plan: what kind
-     * it is (0 for every other tensor) and what it was made for */
+    /* host-side record of an adapter table, an attention plan, an 8-bit matrix
+     * or a cache in 8 bits: what kind it is (0 for every other tensor) and
+     * what it was made for */
     struct hk_record {
         uint32_t kind;
         uint32_t n[15];
@@ -38,7 +39,8 @@ struct h3_gpu_tensor {
 };
 
 /* kinds of records */
-enum { HK_RECORD_LORA = 1, HK_RECORD_PACKED = 2 };
+enum { HK_RECORD_LORA = 1, HK_RECORD_PACKED = 2, HK_RECORD_INT8 = 3,
+       HK_RECORD_KV8 = 4 };
 
 struct hk_cache_block;
 struct hk_timing;

@@ -1,0 +1,466 @@
+/* Keys and values cached in 8 bits (h3_hip_kv_int8_new, _store, _read in
+ * h3_hip.h), and attention over them (h3_hip_sdpa_packed_int8_bf16): blocks of
+ * 64 rows, each with one scale for its keys and one for its values a head.
+ *
+ * The codes lie in the order in which the matrix cores take them: a lane's 16
+ * bytes are 16 dims of one key (the A operand of S^T = K . Q^T), or 16 keys of
+ * one dim (of O^T = V^T . P^T), the keys in the order in which a lane of S^T
+ * holds its scores.  So a wave reads 1 KiB at a time, whole lines, and V needs
+ * no transposing reads.  A code is held as code + 128: one byte permutation
+ * makes the f16 number 1024 + byte of it, one packed subtraction the code
+ * (f16 holds whole numbers up to 2048).
+ */
+#include "hk_attn.h"
+#include "hk_int8.h"
+#include "hk_packed.h"
+
+#include <math.h>
+
+#include <algorithm>
+#include <vector>
+
+#define HK_KV8_BLOCK 64u
+#define HK_KV8_RANGES 64u /* of a launch of the store */
+
+/* hk_record.n of a cache */
+enum { HK_KV8_BLOCKS, HK_KV8_HEADS, HK_KV8_DIM };
+
+/* Dims of a block's rows, in whole groups of 32. */
+__host__ __device__ __forceinline__ uint32_t hk_kv8_padded(uint32_t dim) {
+    return (dim + 31u) & ~31u;
+}
+
+/* Where the code of a block's row and dim lies among the block's keys ... */
+__device__ __forceinline__ uint32_t hk_kv8_key_at(uint32_t row, uint32_t dim,
+                                                  uint32_t padded) {
+    return (row >> 5) * padded * 32u + (dim >> 5) * 1024u +
+           ((row & 31u) + ((dim >> 4) & 1u) * 32u) * 16u + (dim & 15u);
+}
+
+/* ... and its values, which follow them: byte b of lane l of 32 rows and 32
+ * dims is dim l % 32 of row 16 (b / 8) + 8 (b / 4 % 2) + 4 (l / 32) + b % 4,
+ * the order of a lane's scores in S^T. */
+__device__ __forceinline__ uint32_t hk_kv8_value_at(uint32_t row, uint32_t dim,
+                                                    uint32_t padded) {
+    const uint32_t byte =
+        ((row >> 4) & 1u) * 8u + ((row >> 3) & 1u) * 4u + (row & 3u);
+    return (row >> 5) * padded * 32u + (dim >> 5) * 1024u +
+           ((dim & 31u) + ((row >> 2) & 1u) * 32u) * 16u + byte;
+}
+
+struct hk_kv8_cache {
+    uint8_t *codes; /* [block][head][keys, values][64 padded] */
+    float2 *scales; /* [block][head]: of the keys, of the values */
+    uint32_t blocks, heads, dim, padded;
+};
+
+static hk_kv8_cache hk_kv8_of(const h3_gpu_tensor *t) {
+    hk_kv8_cache c = {(uint8_t *)t->data, NULL, t->record.n[HK_KV8_BLOCKS],
+                      t->record.n[HK_KV8_HEADS], t->record.n[HK_KV8_DIM], 0};
+    c.padded = hk_kv8_padded(c.dim);
+    c.scales = (float2 *)(c.codes + (size_t)c.blocks * c.heads * 2u *
+                                        HK_KV8_BLOCK * c.padded);
+    return c;
+}
+
+/* ------------------------------------------------------------ the store */
+
+/* Rows [source, + rows) of the keys and values go to rows [cache, + rows) of
+ * the cache, whose blocks are `before` and on of the launch. */
+struct hk_kv8_range {
+    uint32_t cache, source, rows, before;
+};
+
+struct hk_kv8_store_args {
+    hk_kv8_cache cache;
+    const uint16_t *key, *value;
+    uint64_t stride;
+    uint32_t count;
+    hk_kv8_range ranges[HK_KV8_RANGES];
+};
+
+/* One workgroup per block and head: the largest magnitudes of the block's new
+ * rows, then the codes, 16 at a time.  Rows that the block has before the new
+ * ones keep their codes unless the scale grows, rows behind become zeros. */
+__global__ void __launch_bounds__(256) hk_kv8_store(hk_kv8_store_args a) {
+    __shared__ uint32_t tops[16];
+    const hk_kv8_cache &c = a.cache;
+    uint32_t i = 0;
+    while (i + 1 < a.count && a.ranges[i + 1].before <= blockIdx.x) i++;
+    const hk_kv8_range r = a.ranges[i];
+    const uint32_t head = blockIdx.y;
+    const uint32_t block = r.cache / HK_KV8_BLOCK + (blockIdx.x - r.before);
+    /* rows [r0, r1) of the block are new, from row `from` on */
+    const uint64_t row0 = (uint64_t)block * HK_KV8_BLOCK;
+    const uint32_t r0 = r.cache > row0 ? (uint32_t)(r.cache - row0) : 0u;
+    const uint64_t end = (uint64_t)r.cache + r.rows - row0;
+    const uint32_t r1 = end < HK_KV8_BLOCK ? (uint32_t)end : HK_KV8_BLOCK;
+    const uint64_t from = (uint64_t)r.source + (row0 + r0 - r.cache);
+    const uint32_t part = HK_KV8_BLOCK * c.padded;
+    const size_t at = (size_t)block * c.heads + head;
+    for (int which = 0; which < 2; which++) {
+        const uint16_t *x = (which ? a.value : a.key) + from * a.stride +
+                            (uint64_t)head * c.dim;
+        uint32_t most = 0;
+        for (uint32_t e = threadIdx.x; e < (r1 - r0) * c.dim; e += 256u) {
+            const uint32_t row = e / c.dim;
+            most = max(most, hk_magnitude(hk_bf2f(
+                                 x[row * a.stride + (e - row * c.dim)])));
+        }
+        most = hk_block_umax(most, tops);
+        float *scale = (float *)(c.scales + at) + which;
+        const float old = r0 ? *scale : 0.0f;
+        __syncthreads(); /* everyone has it */
+        hk_int8_quantizer code(most);
+        float keep = 1.0f;
+        if (r0 && !(old < code.scale)) {
+            /* the block's scale holds (also where it is NaN) */
+            if (!isnan(code.scale))
+                code = hk_int8_quantizer(hk_magnitude(127.0f * old));
+            if (isnan(old)) code = hk_int8_quantizer(HK_NOT_FINITE);
+            if (!isnan(code.scale)) code.scale = old;
+        } else if (r0) {
+            keep = old / code.scale;
+        }
+        uint8_t *out = c.codes + (at * 2u + which) * part;
+        for (uint32_t u = threadIdx.x; u < part / 16u; u += 256u) {
+            uint4 had = make_uint4(0, 0, 0, 0);
+            if (r0) had = *(const uint4 *)(out + u * 16u);
+            const uint32_t words[4] = {had.x, had.y, had.z, had.w};
+            const uint32_t lane = u & 63u;
+            const uint32_t dim32 = (u >> 6) % (c.padded >> 5) * 32u;
+            const uint32_t row32 = (u >> 6) / (c.padded >> 5) * 32u;
+            uint32_t made[4];
+            for (uint32_t b = 0; b < 16u; b++) {
+                const uint32_t row =
+                    row32 + (which ? 16u * (b >> 3) + 8u * ((b >> 2) & 1u) +
+                                         4u * (lane >> 5) + (b & 3u)
+                                   : lane & 31u);
+                const uint32_t dim =
+                    dim32 + (which ? lane & 31u : 16u * (lane >> 5) + b);
+                int v = 0;
+                if (row >= r0 && row < r1 && dim < c.dim) {
+                    v = (int)code(hk_bf2f(x[(row - r0) * a.stride + dim]));
+                } else if (row < r0) {
+                    v = (int)((words[b >> 2] >> (8u * (b & 3u))) & 255u) - 128;
+                    if (keep < 1.0f) v = (int)rintf((float)v * keep);
+                }
+                const uint32_t byte = (uint32_t)(v + 128) << (8u * (b & 3u));
+                made[b >> 2] = b & 3u ? made[b >> 2] | byte : byte;
+            }
+            *(uint4 *)(out + u * 16u) =
+                make_uint4(made[0], made[1], made[2], made[3]);
+        }
+        if (threadIdx.x == 0) *scale = code.scale;
+    }
+}
+
+__device__ __forceinline__ float hk_kv8_key(const hk_kv8_cache &c,
+                                            const uint8_t *codes, uint32_t row,
+                                            uint32_t dim) {
+    return (float)((int)codes[hk_kv8_key_at(row, dim, c.padded)] - 128);
+}
+
+__device__ __forceinline__ float hk_kv8_value(const hk_kv8_cache &c,
+                                              const uint8_t *codes,
+                                              uint32_t row, uint32_t dim) {
+    return (float)((int)codes[HK_KV8_BLOCK * c.padded +
+                              hk_kv8_value_at(row, dim, c.padded)] -
+                   128);
+}
+
+/* The values of rows [first, + rows), one workgroup per block and head. */
+__global__ void __launch_bounds__(256)
+hk_kv8_read(hk_kv8_cache c, uint16_t *key, uint16_t *value, uint32_t first,
+            uint32_t rows) {
+    const uint32_t block = first / HK_KV8_BLOCK + blockIdx.x;
+    const uint32_t head = blockIdx.y;
+    const size_t at = (size_t)block * c.heads + head;
+    const uint8_t *codes = c.codes + at * 2u * HK_KV8_BLOCK * c.padded;
+    const float2 scale = c.scales[at];
+    const uint64_t row0 = (uint64_t)block * HK_KV8_BLOCK;
+    for (uint32_t e = threadIdx.x; e < HK_KV8_BLOCK * c.dim; e += 256u) {
+        const uint32_t row = e / c.dim, dim = e - row * c.dim;
+        if (row0 + row < first || row0 + row >= (uint64_t)first + rows)
+            continue;
+        const size_t to = ((row0 + row - first) * c.heads + head) * c.dim + dim;
+        key[to] = hk_f2bf(hk_kv8_key(c, codes, row, dim) * scale.x);
+        value[to] = hk_f2bf(hk_kv8_value(c, codes, row, dim) * scale.y);
+    }
+}
+
+/* ---------------------------------------------------------- the attention */
+
+struct hk_kv8_args {
+    hk_packed_args p;
+    hk_kv8_cache cache;
+};
+
+/* One wave per query row and head, 64 keys (a block) a turn, as
+ * hk_packed_simple: H3_HIP_REFERENCE=1 and heads over 128. */
+__device__ void hk_kv8_simple_row(const hk_kv8_args &g, uint32_t nth,
+                                  uint32_t head) {
+    const hk_packed_args &a = g.p;
+    const hk_kv8_cache &c = g.cache;
+    const uint32_t lane = threadIdx.x & 63u;
+    const hk_packed_request r =
+        a.requests[hk_packed_request_of(a.requests, a.request_count, nth)];
+    const uint32_t row = r.q_first + (nth - r.before);
+    const uint32_t kv_head = head / a.group;
+    const uint16_t *q = a.q + row * a.q_stride + (uint64_t)head * a.dim;
+    float top = -INFINITY, sum = 0.0f;
+    float o[HK_PACKED_MAX_DIM / 64];
+    for (uint32_t d = 0; d < HK_PACKED_MAX_DIM / 64; d++) o[d] = 0.0f;
+    for (uint32_t j0 = 0; j0 < r.kv_rows; j0 += HK_KV8_BLOCK) {
+        const uint32_t left = min(HK_KV8_BLOCK, r.kv_rows - j0);
+        const size_t at =
+            (size_t)((r.kv_first + j0) / HK_KV8_BLOCK) * c.heads + kv_head;
+        const uint8_t *codes = c.codes + at * 2u * HK_KV8_BLOCK * c.padded;
+        const float2 scale = c.scales[at];
+        float s = -INFINITY;
+        if (lane < left) {
+            s = 0.0f;
+            for (uint32_t d = 0; d < a.dim; d++)
+                s = fmaf(hk_bf2f(q[d]), hk_kv8_key(c, codes, lane, d), s);
+            s *= scale.x;
+        }
+        const float most = fmaxf(top, hk_wave_max(s));
+        /* every score so far -inf: no weights yet */
+        const float ref = most == -INFINITY ? 0.0f : most;
+        const float keep =
+            top == -INFINITY ? 0.0f : expf((top - ref) * a.scale);
+        const float p = lane < left ? expf((s - ref) * a.scale) : 0.0f;
+        top = most;
+        sum = sum * keep + hk_wave_sum(p);
+        for (uint32_t d = 0; d < HK_PACKED_MAX_DIM / 64; d++) o[d] *= keep;
+        for (uint32_t j = 0; j < left; j++) {
+            const float pj = __shfl(p, j, 64) * scale.y;
+            for (uint32_t d = 0; d < HK_PACKED_MAX_DIM / 64; d++)
+                if (d * 64u + lane < a.dim)
+                    o[d] = fmaf(
+                        pj, hk_kv8_value(c, codes, j, d * 64u + lane), o[d]);
+        }
+    }
+    uint16_t *out = a.o + ((uint64_t)row * a.heads + head) * a.dim;
+    for (uint32_t d = 0; d < HK_PACKED_MAX_DIM / 64; d++)
+        if (d * 64u + lane < a.dim)
+            out[d * 64u + lane] = hk_f2bf(sum == 0.0f ? 0.0f : o[d] / sum);
+}
+
+__global__ void __launch_bounds__(256) hk_kv8_simple(hk_kv8_args g) {
+    for (uint64_t i = (uint64_t)blockIdx.x * 4u + (threadIdx.x >> 6);
+         i < (uint64_t)g.p.rows * g.p.heads; i += (uint64_t)gridDim.x * 4u) {
+        const uint32_t nth = (uint32_t)(i / g.p.heads);
+        hk_kv8_simple_row(g, nth,
+                          (uint32_t)(i - (uint64_t)nth * g.p.heads));
+    }
+}
+
+/* ================================================================ ops */
+
+static int hk_kv8_require(struct h3_gpu *gpu, const h3_gpu_tensor *t) {
+    if (!t || t->record.kind != HK_RECORD_KV8)
+        return hk_fail(gpu, "the cache was not made by h3_hip_kv_int8_new");
+    return 1;
+}
+
+extern "C" {
+
+h3_gpu_tensor *h3_hip_kv_int8_new(h3_gpu *gpu, uint32_t rows,
+                                  uint32_t kv_heads, uint32_t head_dim) {
+    if (!gpu) return NULL;
+    if (!rows || rows > UINT32_MAX - HK_KV8_BLOCK || !kv_heads ||
+        kv_heads > 65535u || !head_dim || head_dim > HK_PACKED_MAX_DIM) {
+        hk_fail(gpu, "8-bit cache of %u rows, %u heads of %u (1 to 2^32 - 65 "
+                     "rows, 1 to 65535 heads of 1 to %u)", rows, kv_heads,
+                head_dim, HK_PACKED_MAX_DIM);
+        return NULL;
+    }
+    const uint32_t blocks = (rows + HK_KV8_BLOCK - 1u) / HK_KV8_BLOCK;
+    /* at most 2^26 blocks x 2^16 heads x 2^15 bytes */
+    const size_t pairs = (size_t)blocks * kv_heads;
+    h3_gpu_tensor *t = h3_gpu_tensor_new_i8(
+        gpu, pairs * (2u * HK_KV8_BLOCK * hk_kv8_padded(head_dim) +
+                      sizeof(float2)));
+    if (!t) return NULL;
+    t->record.kind = HK_RECORD_KV8;
+    t->record.n[HK_KV8_BLOCKS] = blocks;
+    t->record.n[HK_KV8_HEADS] = kv_heads;
+    t->record.n[HK_KV8_DIM] = head_dim;
+    return t;
+}
+
+int h3_hip_kv_int8_store(h3_gpu *gpu, h3_gpu_tensor *cache,
+                         const uint32_t *cache_first,
+                         const uint32_t *source_first, const uint32_t *rows,
+                         uint32_t count, const h3_gpu_tensor *key,
+                         size_t key_offset, const h3_gpu_tensor *value,
+                         size_t value_offset, uint32_t kv_stride) {
+    if (!hk_kv8_require(gpu, cache)) return 0;
+    if (count && (!cache_first || !source_first || !rows))
+        return hk_fail(gpu, "cache store: no ranges");
+    const hk_kv8_cache c = hk_kv8_of(cache);
+    const uint64_t width = (uint64_t)c.heads * c.dim;
+    if (kv_stride < width)
+        return hk_fail(gpu, "cache store: a row stride of %u is under the "
+                            "rows' %llu elements", kv_stride,
+                       (unsigned long long)width);
+    std::vector<hk_kv8_range> ranges;
+    uint64_t source_end = 0;
+    try {
+        std::vector<std::pair<uint32_t, uint32_t>> blocks;
+        for (uint32_t i = 0; i < count; i++) {
+            if (!rows[i]) continue;
+            const uint64_t end = (uint64_t)cache_first[i] + rows[i];
+            if (end > (uint64_t)c.blocks * HK_KV8_BLOCK)
+                return hk_fail(gpu, "cache store: range %u ends behind the "
+                                    "cache's %u blocks of 64 rows", i,
+                               c.blocks);
+            source_end = std::max(source_end,
+                                  (uint64_t)source_first[i] + rows[i]);
+            ranges.push_back({cache_first[i], source_first[i], rows[i], 0});
+            blocks.push_back({cache_first[i] / HK_KV8_BLOCK,
+                              (uint32_t)((end - 1) / HK_KV8_BLOCK)});
+        }
+        std::sort(blocks.begin(), blocks.end());
+        for (size_t i = 1; i < blocks.size(); i++)
+            if (blocks[i].first <= blocks[i - 1].second)
+                return hk_fail(gpu, "cache store: two ranges write rows of "
+                                    "block %u", blocks[i].first);
+    } catch (const std::bad_alloc &) {
+        return hk_fail(gpu, "out of host memory");
+    }
+    if (!hk_require(gpu, key, hk_packed_extent(key_offset, kv_stride,
+                                               source_end, width),
+                    H3_GPU_BF16, "cache store key") ||
+        !hk_require(gpu, value, hk_packed_extent(value_offset, kv_stride,
+                                                 source_end, width),
+                    H3_GPU_BF16, "cache store value") ||
+        !hk_require_active(gpu))
+        return 0;
+    if (ranges.empty()) return 1;
+    hk_op_begin(gpu, "kv_int8_store");
+    hk_kv8_store_args a = {};
+    a.cache = c;
+    a.key = HK_CBF16(key) + key_offset;
+    a.value = HK_CBF16(value) + value_offset;
+    a.stride = kv_stride;
+    /* launches of up to 64 ranges and 2^23 / heads blocks */
+    const uint32_t most = std::max(1u, (1u << 23) / c.heads);
+    uint32_t total = 0;
+    auto launch = [&]() {
+        if (a.count)
+            hipLaunchKernelGGL(hk_kv8_store, dim3(total, c.heads), dim3(256),
+                               0, gpu->stream, a);
+        a.count = total = 0;
+    };
+    for (hk_kv8_range r : ranges) {
+        while (r.rows) {
+            if (a.count == HK_KV8_RANGES || total == most) launch();
+            /* as many of its rows as end with the launch's last block */
+            const uint32_t begun = r.cache % HK_KV8_BLOCK;
+            const uint64_t room =
+                (uint64_t)(most - total) * HK_KV8_BLOCK - begun;
+            const uint32_t n = (uint32_t)std::min<uint64_t>(r.rows, room);
+            a.ranges[a.count++] = {r.cache, r.source, n, total};
+            total += (begun + n + HK_KV8_BLOCK - 1u) / HK_KV8_BLOCK;
+            r.cache += n;
+            r.source += n;
+            r.rows -= n;
+        }
+    }
+    launch();
+    return hk_op_end(gpu, "kv_int8_store", HK_KIND_DIRECT);
+}
+
+int h3_hip_kv_int8_read(h3_gpu *gpu, h3_gpu_tensor *key, h3_gpu_tensor *value,
+                        const h3_gpu_tensor *cache, uint32_t first_row,
+                        uint32_t rows) {
+    if (!hk_kv8_require(gpu, cache)) return 0;
+    const hk_kv8_cache c = hk_kv8_of(cache);
+    if ((uint64_t)first_row + rows > (uint64_t)c.blocks * HK_KV8_BLOCK)
+        return hk_fail(gpu, "cache read: the rows end behind the cache's %u "
+                            "blocks of 64", c.blocks);
+    const size_t width = (size_t)c.heads * c.dim;
+    if (!hk_require(gpu, key, rows * width, H3_GPU_BF16, "cache read key") ||
+        !hk_require(gpu, value, rows * width, H3_GPU_BF16,
+                    "cache read value") ||
+        !hk_require_active(gpu))
+        return 0;
+    if (key == value)
+        return hk_fail(gpu, "cache read: keys and values need a tensor each");
+    if (!rows) return 1;
+    hk_op_begin(gpu, "kv_int8_read");
+    const size_t most = std::max(1u, (1u << 23) / c.heads) * HK_KV8_BLOCK;
+    for (uint64_t done = 0; done < rows;) {
+        const uint32_t at = (uint32_t)(first_row + done);
+        const uint32_t n = (uint32_t)std::min<uint64_t>(
+            rows - done, most - at % HK_KV8_BLOCK);
+        hipLaunchKernelGGL(
+            hk_kv8_read,
+            dim3((at % HK_KV8_BLOCK + n + HK_KV8_BLOCK - 1u) / HK_KV8_BLOCK,
+                 c.heads),
+            dim3(256), 0, gpu->stream, c, HK_BF16(key) + done * width,
+            HK_BF16(value) + done * width, at, n);
+        done += n;
+    }
+    return hk_op_end(gpu, "kv_int8_read", HK_KIND_DIRECT);
+}
+
+int h3_hip_sdpa_packed_int8_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
+                                 const h3_gpu_tensor *query,
+                                 size_t query_offset, uint32_t query_stride,
+                                 const h3_gpu_tensor *cache,
+                                 const h3_gpu_tensor *plan, float scale) {
+    if (!hk_kv8_require(gpu, cache)) return 0;
+    if (!plan || plan->record.kind != HK_RECORD_PACKED)
+        return hk_fail(gpu, "packed attention: the plan was not built by "
+                            "h3_hip_sdpa_packed_plan");
+    const uint32_t *n = plan->record.n;
+    hk_kv8_args a = {};
+    a.cache = hk_kv8_of(cache);
+    hk_packed_of_plan(a.p, plan, scale);
+    if (a.p.kv_heads != a.cache.heads || a.p.dim != a.cache.dim)
+        return hk_fail(gpu, "packed attention: %u key heads of %u in the plan, "
+                            "%u of %u in the cache", a.p.kv_heads, a.p.dim,
+                       a.cache.heads, a.cache.dim);
+    if (n[HK_PACKED_OFF_BLOCKS])
+        return hk_fail(gpu, "packed attention: a request's rows of the cache "
+                            "do not begin at a multiple of 64");
+    if (n[HK_PACKED_KV_END] > (uint64_t)a.cache.blocks * HK_KV8_BLOCK)
+        return hk_fail(gpu, "packed attention: the plan's %u key rows end "
+                            "behind the cache's %u blocks of 64",
+                       n[HK_PACKED_KV_END], a.cache.blocks);
+    const uint64_t q_width = (uint64_t)a.p.heads * a.p.dim;
+    if (query_stride < q_width)
+        return hk_fail(gpu, "packed attention: a row stride of %u is under "
+                            "the rows' %llu elements", query_stride,
+                       (unsigned long long)q_width);
+    if (!isfinite(scale) || scale < 0.0f)
+        return hk_fail(gpu, "packed attention: the scale must be finite and "
+                            "not negative");
+    if (!hk_require(gpu, query,
+                    hk_packed_extent(query_offset, query_stride,
+                                     n[HK_PACKED_Q_END], q_width),
+                    H3_GPU_BF16, "packed query") ||
+        !hk_require(gpu, output, n[HK_PACKED_Q_END] * q_width, H3_GPU_BF16,
+                    "packed output") ||
+        !hk_require_active(gpu))
+        return 0;
+    if (output == query)
+        return hk_fail(gpu, "packed attention: the output must be a tensor "
+                            "of its own");
+    if (!n[HK_PACKED_ROWS]) return 1;
+    a.p.q = HK_CBF16(query) + query_offset;
+    a.p.o = HK_BF16(output);
+    a.p.q_stride = query_stride;
+    hk_op_begin(gpu, "attention_packed_int8");
+    const uint64_t blocks = ((uint64_t)a.p.rows * a.p.heads + 3) / 4;
+    hipLaunchKernelGGL(
+        hk_kv8_simple,
+        dim3((unsigned)(blocks < 1u << 20 ? blocks : 1u << 20)), dim3(256), 0,
+        gpu->stream, a);
+    return hk_op_end(gpu, "attention_packed_int8", HK_KIND_SDPA);
+}
+
+} /* extern "C" */

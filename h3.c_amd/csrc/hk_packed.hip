@@ -19,6 +19,7 @@
 #include "hk_attn.h"
 #include "hk_common.h"
 #include "hk_internal.h"
+#include "hk_packed.h"
 
 #include <math.h>
 #include <stdlib.h>
@@ -30,61 +31,6 @@
 #include <type_traits>
 #include <vector>
 
-#define HK_PACKED_MAX_DIM 256u
-#define HK_PACKED_MAX_KEYS 0xffffff00u /* of a request */
-#define HK_PACKED_WAVES 4u
-#define HK_PACKED_QB (HK_PACKED_WAVES * 32u) /* virtual rows of an item */
-
-/* a request with query rows, in device memory */
-struct hk_packed_request {
-    uint32_t q_first, q_rows, kv_first, kv_rows;
-    uint32_t before; /* query rows of the requests before it in the plan */
-};
-
-/* A work item: virtual rows [row, rows) of a request, at most HK_PACKED_QB, of
- * one key head, over key tiles [tile, tile_end) of the request's keys.  Whole
- * items store their rows; a piece leaves its sums in part `part`.  An item of
- * no rows fills a place in the launch. */
-struct hk_packed_item {
-    uint32_t q_first, rows, row, kv_head;
-    uint32_t kv_first, kv_rows, tile, tile_end;
-    uint32_t part;
-};
-#define HK_PACKED_WHOLE 0xffffffffu
-
-/* The pieces [part, + pieces) of one item's rows. */
-struct hk_packed_join {
-    uint32_t q_first, rows, row, kv_head;
-    uint32_t part, pieces;
-};
-
-/* hk_record.n of a plan */
-enum { HK_PACKED_HEADS, HK_PACKED_KV_HEADS, HK_PACKED_DIM,
-       HK_PACKED_REQUESTS, /* those with query rows */
-       HK_PACKED_ROWS,     /* query rows of all requests */
-       HK_PACKED_Q_END,    /* rows that the query and output tensors hold */
-       HK_PACKED_KV_END,
-       HK_PACKED_ITEMS,    /* entries of each list, which follow each other: */
-       HK_PACKED_JOINS,    /* requests, items, joins */
-       HK_PACKED_JOIN_ROWS, /* the most virtual rows of a join */
-       HK_PACKED_PARTS };
-
-struct hk_packed_args {
-    const uint16_t *q, *k, *v;
-    uint16_t *o;
-    uint64_t q_stride, kv_stride; /* elements from a row to the next */
-    uint32_t heads, kv_heads, dim, group;
-    float scale, scale_log2;
-    const hk_packed_request *requests;
-    uint32_t request_count, rows;
-    const hk_packed_item *items;
-    const hk_packed_join *joins;
-    /* pieces' sums: F32 O [part][HK_PACKED_QB][padded dim], not divided, and
-     * (reference, sum) [part][HK_PACKED_QB] */
-    float *part_o;
-    float2 *part_ml;
-};
-
 /* One wave per (query row, head) at a time, 64 keys a turn: lane j scores key
  * j of the turn, then lane l adds up dims l, l + 64, ... of the turn's values.
  * Running maximum and sum in F32; P stays F32.  The scale multiplies the
@@ -93,14 +39,8 @@ struct hk_packed_args {
 __device__ void hk_packed_simple_row(const hk_packed_args &a, uint32_t nth,
                                      uint32_t head) {
     const uint32_t lane = threadIdx.x & 63u;
-    /* the last request that begins at or before the nth query row */
-    uint32_t low = 0, high = a.request_count;
-    while (high - low > 1) {
-        const uint32_t mid = (low + high) / 2;
-        if (a.requests[mid].before <= nth) low = mid;
-        else high = mid;
-    }
-    const hk_packed_request r = a.requests[low];
+    const hk_packed_request r =
+        a.requests[hk_packed_request_of(a.requests, a.request_count, nth)];
     const uint32_t row = r.q_first + (nth - r.before);
     const uint32_t kv_head = head / (a.heads / a.kv_heads);
     const uint16_t *q = a.q + row * a.q_stride + (uint64_t)head * a.dim;
@@ -904,6 +844,15 @@ __global__ void __launch_bounds__(256) hk_packed_joined(hk_packed_args a) {
         if (lane * PER + e < a.dim) out[lane * PER + e] = hk_f2bf(sum[e] * inv);
 }
 
+void hk_packed_join_pieces(struct h3_gpu *gpu, const hk_packed_args &a,
+                           const uint32_t *n, uint32_t padded) {
+    hipLaunchKernelGGL(padded == 64 ? hk_packed_joined<64>
+                                    : hk_packed_joined<128>,
+                       dim3(n[HK_PACKED_JOINS],
+                            (n[HK_PACKED_JOIN_ROWS] + 3u) / 4u),
+                       dim3(256), 0, gpu->stream, a);
+}
+
 template <int DIMS>
 static void hk_packed_launch(struct h3_gpu *gpu, const hk_packed_args &a,
                              const uint32_t *n) {
@@ -919,11 +868,7 @@ static void hk_packed_launch(struct h3_gpu *gpu, const hk_packed_args &a,
                            dim3(HK_PACKED_WAVES * 64u), lds, gpu->stream,
                            part);
     }
-    if (a.part_o)
-        hipLaunchKernelGGL(hk_packed_joined<DP>,
-                           dim3(n[HK_PACKED_JOINS],
-                                (n[HK_PACKED_JOIN_ROWS] + 3u) / 4u),
-                           dim3(256), 0, gpu->stream, a);
+    if (a.part_o) hk_packed_join_pieces(gpu, a, n, DP);
 }
 
 /* Whether the matrix-core kernel takes these rows: whole 16-byte pieces, 64
@@ -1193,6 +1138,7 @@ h3_gpu_tensor *h3_hip_sdpa_packed_plan(h3_gpu *gpu, const uint32_t *q_first,
     try {
         std::vector<hk_packed_request> list;
         uint64_t rows = 0, q_end = 0, kv_end = 0;
+        bool off_blocks = false;
         for (uint32_t i = 0; i < requests; i++) {
             const uint64_t qe = (uint64_t)q_first[i] + q_rows[i];
             const uint64_t ke = (uint64_t)kv_first[i] + kv_rows[i];
@@ -1213,7 +1159,9 @@ h3_gpu_tensor *h3_hip_sdpa_packed_plan(h3_gpu *gpu, const uint32_t *q_first,
                             (uint32_t)rows});
             rows += q_rows[i];
             q_end = std::max(q_end, qe);
-            if (kv_rows[i]) kv_end = std::max(kv_end, ke);
+            if (!kv_rows[i]) continue;
+            kv_end = std::max(kv_end, ke);
+            off_blocks |= kv_first[i] % HK_KT != 0;
         }
         std::vector<std::pair<uint32_t, uint32_t>> ranges;
         for (const auto &r : list) ranges.push_back({r.q_first, r.q_rows});
@@ -1258,6 +1206,7 @@ h3_gpu_tensor *h3_hip_sdpa_packed_plan(h3_gpu *gpu, const uint32_t *q_first,
         plan->record.n[HK_PACKED_JOINS] = (uint32_t)work.joins.size();
         plan->record.n[HK_PACKED_JOIN_ROWS] = work.join_rows;
         plan->record.n[HK_PACKED_PARTS] = work.parts;
+        plan->record.n[HK_PACKED_OFF_BLOCKS] = off_blocks;
         return plan;
     } catch (const std::bad_alloc &) {
         hk_fail(gpu, "out of host memory");
@@ -1279,13 +1228,6 @@ int h3_hip_sdpa_packed_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
     const uint32_t kv_heads = n[HK_PACKED_KV_HEADS];
     const uint64_t q_width = (uint64_t)heads * dim;
     const uint64_t kv_width = (uint64_t)kv_heads * dim;
-    /* elements that a tensor needs for `rows` rows from `offset` on; sizes
-     * past what an address can hold come out as the largest */
-    auto extent = [](size_t offset, uint64_t stride, uint64_t rows,
-                     uint64_t width) -> size_t {
-        const uint64_t need = rows ? (rows - 1) * stride + width : 0;
-        return offset > SIZE_MAX - need ? SIZE_MAX : offset + need;
-    };
     if (query_stride < q_width || kv_stride < kv_width)
         return hk_fail(gpu, "packed attention: row strides %u and %u are "
                             "under the rows' %llu and %llu elements",
@@ -1295,13 +1237,13 @@ int h3_hip_sdpa_packed_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
         return hk_fail(gpu, "packed attention: the scale must be finite and "
                             "not negative");
     if (!hk_require(gpu, query,
-                    extent(query_offset, query_stride, n[HK_PACKED_Q_END],
+                    hk_packed_extent(query_offset, query_stride, n[HK_PACKED_Q_END],
                            q_width), H3_GPU_BF16, "packed query") ||
         !hk_require(gpu, key,
-                    extent(key_offset, kv_stride, n[HK_PACKED_KV_END],
+                    hk_packed_extent(key_offset, kv_stride, n[HK_PACKED_KV_END],
                            kv_width), H3_GPU_BF16, "packed key") ||
         !hk_require(gpu, value,
-                    extent(value_offset, kv_stride, n[HK_PACKED_KV_END],
+                    hk_packed_extent(value_offset, kv_stride, n[HK_PACKED_KV_END],
                            kv_width), H3_GPU_BF16, "packed value") ||
         !hk_require(gpu, output, n[HK_PACKED_Q_END] * q_width, H3_GPU_BF16,
                     "packed output") ||
@@ -1318,17 +1260,7 @@ int h3_hip_sdpa_packed_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
     a.o = HK_BF16(output);
     a.q_stride = query_stride;
     a.kv_stride = kv_stride;
-    a.heads = heads;
-    a.kv_heads = kv_heads;
-    a.dim = dim;
-    a.scale = scale;
-    a.group = heads / kv_heads;
-    a.scale_log2 = scale * 1.4426950408889634f;
-    a.requests = (const hk_packed_request *)plan->data;
-    a.request_count = n[HK_PACKED_REQUESTS];
-    a.rows = n[HK_PACKED_ROWS];
-    a.items = (const hk_packed_item *)(a.requests + a.request_count);
-    a.joins = (const hk_packed_join *)(a.items + n[HK_PACKED_ITEMS]);
+    hk_packed_of_plan(a, plan, scale);
     hk_op_begin(gpu, "attention_packed");
     if (hk_packed_takes(gpu, a)) {
         const size_t padded = dim <= 64 ? 64 : 128;

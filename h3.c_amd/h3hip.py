@@ -96,6 +96,7 @@ def lib():
         "h3_gpu_has_int8_mlp": (_I, [_P]),
         "h3_gpu_tensor_new_f32": (_P, [_P, _SZ]),
         "h3_gpu_tensor_new_bf16": (_P, [_P, _SZ]),
+        "h3_gpu_tensor_new_i8": (_P, [_P, _SZ]),
         "h3_gpu_tensor_from_f32": (_P, [_P, _P, _SZ]),
         "h3_gpu_tensor_from_bf16": (_P, [_P, _P, _SZ]),
         "h3_gpu_tensor_from_u32": (_P, [_P, _P, _SZ]),
@@ -155,6 +156,25 @@ def lib():
                                          _U32, _U32]),
         "h3_hip_sdpa_packed_bf16": (_I, [_P, _P, _P, _SZ, _U32, _P, _SZ, _P,
                                          _SZ, _U32, _P, _F]),
+        "h3_hip_int8_new": (_P, [_P, _U32, _U32]),
+        "h3_hip_quantize_int8": (_I, [_P, _P, _P, _U32, _U32]),
+        "h3_hip_adaln_int8": (_I, [_P, _P, _P, _P, _P, _P, _U32, _U32, _U32,
+                                   _U32, _U32, _F]),
+        "h3_hip_layer_adaln_int8": (_I, [_P, _P, _P, _P, _P, _P, _P, _U32,
+                                         _U32, _U32, _U32, _U32, _F]),
+        "h3_hip_dequantize_int8": (_I, [_P, _P, _P, _U32, _U32]),
+        "h3_hip_linear_int8_bf16": (_I, [_P, _P, _P, _P, _P, _U32, _U32,
+                                         _U32]),
+        "h3_hip_linear_gelu_int8_bf16": (_I, [_P, _P, _P, _P, _P, _U32, _U32,
+                                              _U32]),
+        "h3_hip_mlp_int8_bf16": (_I, [_P, _P, _P, _P, _P, _U32, _U32, _U32,
+                                      _U32]),
+        "h3_hip_kv_int8_new": (_P, [_P, _U32, _U32, _U32]),
+        "h3_hip_kv_int8_store": (_I, [_P, _P, _P, _P, _P, _U32, _P, _SZ, _P,
+                                      _SZ, _U32]),
+        "h3_hip_kv_int8_read": (_I, [_P, _P, _P, _P, _U32, _U32]),
+        "h3_hip_sdpa_packed_int8_bf16": (_I, [_P, _P, _P, _SZ, _U32, _P, _P,
+                                              _F]),
         "h3_gpu_layer_adaln_bf16": (_I, [_P, _P, _P, _P, _P, _P, _P, _U32,
                                          _U32, _U32, _U32, _U32, _F]),
         "h3_gpu_gate_layer_adaln_bf16": (_I, [_P, _P, _P, _P, _P, _P, _P,
@@ -445,6 +465,30 @@ class Gpu:
         self.check(t, "attention plan")
         self._owned.append(t)
         return t
+
+    def int8(self, rows, columns):
+        """h3_hip_int8_new: room for rows in 8 bits."""
+        t = self.L.h3_hip_int8_new(self.h, rows, columns)
+        self.check(t, "8-bit matrix")
+        self._owned.append(t)
+        return t
+
+    def kv_int8(self, rows, kv_heads, head_dim):
+        """h3_hip_kv_int8_new: a cache of keys and values in 8 bits."""
+        t = self.L.h3_hip_kv_int8_new(self.h, rows, kv_heads, head_dim)
+        self.check(t, "8-bit cache")
+        self._owned.append(t)
+        return t
+
+    def kv_int8_store(self, cache, cache_first, source_first, rows, key,
+                      key_offset, value, value_offset, kv_stride):
+        """h3_hip_kv_int8_store of lists of row numbers, in an open batch."""
+        n = len(rows)
+        self.check(self.L.h3_hip_kv_int8_store(
+            self.h, cache, *((_U32 * n)(*v) for v in (
+                cache_first, source_first, rows)),
+            n, key, key_offset, value, value_offset, kv_stride),
+            "8-bit cache store")
 
     def load(self, path, offset, n, dtype="bf16"):
         """h3_gpu_tensor_load_{bf16,f32}: file bytes -> a new tensor."""

@@ -344,6 +344,117 @@ int h3_hip_sdpa_packed_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
                             size_t value_offset, uint32_t kv_stride,
                             const h3_gpu_tensor *plan, float scale);
 
+/* ---- 8 bits ----
+ *
+ * An 8-bit matrix (h3_hip_int8_new; free it with h3_gpu_tensor_free) holds rows
+ * of 8-bit integers with an F32 scale each: value = code * scale, scale =
+ * max|x| / 127 over the row, code = 127 x / max|x| rounded to nearest, ties to
+ * even.  A row of zeros has scale 0; a row with an infinity or a NaN gets a NaN
+ * scale, and so NaN results, and no other row does.  It is one tensor of type
+ * H3_GPU_I8 whose layout is the backend's own, as its rows have room for
+ * `rows`; calls may use fewer.  columns goes from 1 to 131072.  Weights are
+ * quantised once, [output][input] as for h3_gpu_linear_bf16, so that each
+ * output channel has its scale; activations token by token in the forward.
+ * The reference has 8-bit paths on one of its backends only, behind entries of
+ * other shapes (h3_gpu.h: h3_gpu_linear_int8_bf16 and its kin); those keep
+ * reporting that they are not available here. */
+h3_gpu_tensor *h3_hip_int8_new(h3_gpu *gpu, uint32_t rows, uint32_t columns);
+
+/* Rows of `input` (bf16) in 8 bits; of their adaLN, h3_gpu_adaln_bf16 and
+ * h3_gpu_layer_adaln_bf16 but for the rounding to bf16, which is not made
+ * between the norm and the 8 bits; and the values that rows stand for, rounded
+ * to bf16.  Rows of `output` behind the call's are left as they were. */
+int h3_hip_quantize_int8(h3_gpu *gpu, h3_gpu_tensor *output,
+                         const h3_gpu_tensor *input, uint32_t rows,
+                         uint32_t columns);
+int h3_hip_adaln_int8(h3_gpu *gpu, h3_gpu_tensor *output,
+                      const h3_gpu_tensor *input,
+                      const h3_gpu_tensor *norm_weight,
+                      const h3_gpu_tensor *modulation,
+                      const h3_gpu_tensor *row_map, uint32_t rows,
+                      uint32_t width, uint32_t slots, uint32_t shift_slot,
+                      uint32_t scale_slot, float epsilon);
+int h3_hip_layer_adaln_int8(h3_gpu *gpu, h3_gpu_tensor *output,
+                            const h3_gpu_tensor *input,
+                            const h3_gpu_tensor *norm_weight,
+                            const h3_gpu_tensor *norm_bias,
+                            const h3_gpu_tensor *modulation,
+                            const h3_gpu_tensor *row_map, uint32_t rows,
+                            uint32_t width, uint32_t slots,
+                            uint32_t shift_slot, uint32_t scale_slot,
+                            float epsilon);
+int h3_hip_dequantize_int8(h3_gpu *gpu, h3_gpu_tensor *output,
+                           const h3_gpu_tensor *input, uint32_t rows,
+                           uint32_t columns);
+
+/* y = bf16(act(sum * (input scale * weight scale) + bias)) of 8-bit matrices,
+ * [rows][input_dim] and [output_dim][input_dim]; the sums of products are
+ * exact.  act is nothing or, of the F32 value, the tanh GELU.  bias (bf16) may
+ * be NULL; output must be a tensor of its own. */
+int h3_hip_linear_int8_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
+                            const h3_gpu_tensor *input,
+                            const h3_gpu_tensor *weight,
+                            const h3_gpu_tensor *bias, uint32_t rows,
+                            uint32_t input_dim, uint32_t output_dim);
+int h3_hip_linear_gelu_int8_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
+                                 const h3_gpu_tensor *input,
+                                 const h3_gpu_tensor *weight,
+                                 const h3_gpu_tensor *bias, uint32_t rows,
+                                 uint32_t input_dim, uint32_t output_dim);
+
+/* The gated block of h3_gpu_mlp_bf16 in 8 bits: fc1 ([2 hidden][input], gate
+ * rows first), h = silu(gate) up in F32, rows of h in 8 bits, fc2.  Uses the
+ * context's scratch, which grows on demand: 5 bytes for each of rows x hidden,
+ * up to 9 for at most 128 rows. */
+int h3_hip_mlp_int8_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
+                         const h3_gpu_tensor *input,
+                         const h3_gpu_tensor *fc1_weight,
+                         const h3_gpu_tensor *fc2_weight, uint32_t rows,
+                         uint32_t input_dim, uint32_t hidden_dim,
+                         uint32_t output_dim);
+
+/* A cache of keys and values in 8 bits (free it with h3_gpu_tensor_free): rows
+ * of kv_heads heads of head_dim (1 to 256) in blocks of 64 rows, the last one
+ * whole; each block has one scale for its keys and one for its values a head.
+ *
+ * h3_hip_kv_int8_store writes rows [source_first[i], + rows[i]) of the given
+ * keys and values to rows [cache_first[i], + rows[i]) of the cache, for `count`
+ * ranges (host arrays, read before the call returns).  In their tensors, head
+ * h of row r starts at element offset + r kv_stride + h head_dim, as for
+ * h3_hip_sdpa_packed_bf16.  Ranges must not write into one block.
+ * In a block that a range fills from its first row on, the scales are those of
+ * the new rows alone, whatever the block held.  A range that begins inside a
+ * block goes on behind the rows before it: they stay, and where the new rows
+ * are larger the scale grows to max|new| / 127 and the earlier codes become
+ * round(code * scale / new scale).  Rows of a range's last block behind its
+ * end are cleared.  An infinity or a NaN makes its block's scale a NaN, and the
+ * results of the queries that read the block: rows that no query is to read
+ * are not to be stored.
+ *
+ * h3_hip_kv_int8_read gives the values of rows, rounded to bf16, as
+ * [row][head][head_dim]. */
+h3_gpu_tensor *h3_hip_kv_int8_new(h3_gpu *gpu, uint32_t rows,
+                                  uint32_t kv_heads, uint32_t head_dim);
+int h3_hip_kv_int8_store(h3_gpu *gpu, h3_gpu_tensor *cache,
+                         const uint32_t *cache_first,
+                         const uint32_t *source_first, const uint32_t *rows,
+                         uint32_t count, const h3_gpu_tensor *key,
+                         size_t key_offset, const h3_gpu_tensor *value,
+                         size_t value_offset, uint32_t kv_stride);
+int h3_hip_kv_int8_read(h3_gpu *gpu, h3_gpu_tensor *key, h3_gpu_tensor *value,
+                        const h3_gpu_tensor *cache, uint32_t first_row,
+                        uint32_t rows);
+
+/* h3_hip_sdpa_packed_bf16 over such a cache: the plan's key rows are rows of
+ * the cache, and every request's have to begin at a multiple of 64 (requests
+ * may share them).  Scores, softmax and sums are F32; a weight P is rounded to
+ * 11 bits (f16) before P . V. */
+int h3_hip_sdpa_packed_int8_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
+                                 const h3_gpu_tensor *query,
+                                 size_t query_offset, uint32_t query_stride,
+                                 const h3_gpu_tensor *cache,
+                                 const h3_gpu_tensor *plan, float scale);
+
 /* h3_gpu_patch_linear_bf16_offset / _map (h3_gpu.h:116-135) without the
  * reference's fixed checkpoint shape (5376 outputs from 32 or 96 inputs):
  * any output width and up to 4096 inputs, for reduced-width test models.
