@@ -154,6 +154,24 @@ static inline uint32_t hk_gemm_lds(uint32_t jb) {
     return HK_STAGES * (32u * jb * HK_BK * 2u + HK_TILE_BYTES) + 256u;
 }
 
+/* ------------------------------------------------ the plan of a launch */
+
+/* How the tiles of a launch run: `full` tiles in rounds of one per CU, then
+ * `tail` tiles, cut along K into `splits` pieces of `steps` 64-deep steps when
+ * they would leave over half the CUs idle (splits is 1 otherwise, and the
+ * tail is one more round). */
+struct hk_gemm_rounds {
+    uint32_t full, tail, splits, steps;
+};
+
+hk_gemm_rounds hk_gemm_rounds_of(uint32_t tiles, uint32_t k_steps,
+                                 uint32_t cus, bool may_split);
+/* The tile height, in 32-row units. */
+uint32_t hk_gemm_row_blocks(uint32_t m, uint32_t columns, uint32_t k_steps,
+                            uint32_t cus, bool may_split);
+/* Workgroups for a launch of `tiles` tiles. */
+uint32_t hk_gemm_grid(uint32_t tiles, uint32_t cus);
+
 /* ------------------------------------------------ low-rank adapters */
 
 /* one adapter of a table (hk_lora.hip), in device memory; the kernels read

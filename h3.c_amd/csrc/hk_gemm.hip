@@ -308,7 +308,7 @@ hk_splitk_reduce(hk_gemm_args g, uint32_t splits) {
 /* Workgroups for a launch of `tiles` tiles, one workgroup per CU: the
  * fewest that still finish in the same number of rounds, rounded up to a
  * multiple of the 8 XCDs (480 or 1440 tiles on 256 CUs: 240 workgroups). */
-static uint32_t hk_gemm_grid(uint32_t tiles, uint32_t cus) {
+uint32_t hk_gemm_grid(uint32_t tiles, uint32_t cus) {
     static int persist = -1;
     if (persist < 0) {
         const char *e = getenv("H3_HIP_GEMM_PERSIST");
@@ -398,15 +398,7 @@ static void hk_gemm_launch(struct h3_gpu *gpu, int epilogue, uint32_t jb,
                            gpu->stream, g);
 }
 
-/* How the tiles of a launch run: `full` tiles in rounds of one per CU, then
- * `tail` tiles, cut along K into `splits` pieces of `steps` 64-deep steps when
- * they would leave over half the CUs idle (splits is 1 otherwise, and the
- * tail is one more round). */
-struct hk_gemm_rounds {
-    uint32_t full, tail, splits, steps;
-};
-
-static hk_gemm_rounds hk_gemm_rounds_of(uint32_t tiles, uint32_t k_steps,
+hk_gemm_rounds hk_gemm_rounds_of(uint32_t tiles, uint32_t k_steps,
                                         uint32_t cus, bool may_split) {
     hk_gemm_rounds r = {tiles - tiles % cus, tiles % cus, 1, k_steps};
     if (may_split && r.tail && r.tail * 2 <= cus && k_steps >= 8) {
@@ -471,7 +463,7 @@ static float hk_gemm_estimate(uint32_t jb, uint32_t tiles, uint32_t k_steps,
  * nothing in one row tile (140 x 13824 -> 5120: 52 and 53 us), nor if the
  * pieces cannot be dealt to the XCDs in eights (300 x 14336 -> 5376, 252
  * pieces: 79 and 82 us; 350 x 13824 -> 5120, 240 pieces: 70 and 64). */
-static uint32_t hk_gemm_row_blocks(uint32_t m, uint32_t columns,
+uint32_t hk_gemm_row_blocks(uint32_t m, uint32_t columns,
                                    uint32_t k_steps, uint32_t cus,
                                    bool may_split) {
     const uint32_t high = (m + HK_BM - 1) / HK_BM;

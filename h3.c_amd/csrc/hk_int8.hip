@@ -6,6 +6,8 @@
  */
 #include "hk_int8.h"
 #include "hk_gemm.h"
+#include "hk_skinny.h"
+#include "hk_skinny_tile.h"
 
 #include <math.h>
 
@@ -96,6 +98,123 @@ hk_int8_rows_any(hk_int8_rows_args a, uint32_t first) {
     if (threadIdx.x == 0) a.scales[row] = code.scale;
 }
 
+/* The same with the row in registers, 8 columns a thread and chunk: whole
+ * 16-byte pieces, at most CHUNKS * 2048 columns.  One pass over the row. */
+template <int SOURCE, int CHUNKS>
+__global__ void __launch_bounds__(HK_INT8_THREADS)
+hk_int8_rows_vec(hk_int8_rows_args a, uint32_t first) {
+    __shared__ float sums[16];
+    __shared__ uint32_t tops[16];
+    const uint32_t row = first + blockIdx.x;
+    constexpr bool norm = SOURCE == HK_ROWS_RMS || SOURCE == HK_ROWS_LAYER;
+    constexpr bool layer = SOURCE == HK_ROWS_LAYER;
+    auto column = [](int c) {
+        return (threadIdx.x + (uint32_t)c * HK_INT8_THREADS) * 8u;
+    };
+    auto load8 = [](const uint16_t *from, float *to) {
+        hk_unpack8(*(const uint4 *)from, to);
+    };
+    auto wide8 = [](const float *from, float *to) {
+        *(float4 *)to = *(const float4 *)from;
+        *(float4 *)(to + 4) = *(const float4 *)(from + 4);
+    };
+    float v[CHUNKS][8];
+    float sum = 0.0f;
+#pragma unroll
+    for (int c = 0; c < CHUNKS; c++) {
+        const uint32_t col = column(c);
+        if (col >= a.width) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[c][i] = 0.0f;
+        } else if (SOURCE == HK_ROWS_F32) {
+            wide8(a.wide + (size_t)row * a.wide_pitch + col, v[c]);
+        } else if (SOURCE == HK_ROWS_SWIGLU) {
+            const float *from = a.wide + (size_t)row * a.wide_pitch + col;
+            float u[8];
+            wide8(from, v[c]);
+            wide8(from + a.width, u);
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[c][i] = hk_swiglu_f(v[c][i], u[i]);
+        } else {
+            load8(a.input + (size_t)row * a.width + col, v[c]);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) sum += layer ? v[c][i] : v[c][i] * v[c][i];
+    }
+    if (norm) {
+        const float mean =
+            layer ? hk_block_sum(sum, sums) / (float)a.width : 0.0f;
+        if (layer) {
+            sum = 0.0f;
+#pragma unroll
+            for (int c = 0; c < CHUNKS; c++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    v[c][i] -= mean;
+                    if (column(c) < a.width)
+                        sum = fmaf(v[c][i], v[c][i], sum);
+                }
+        }
+        const float inverse =
+            1.0f / sqrtf(hk_block_sum(sum, sums) / (float)a.width +
+                         a.epsilon);
+        const uint16_t *shift = NULL, *scale = NULL;
+        if (a.modulation) {
+            const size_t base = (size_t)a.row_map[row] * a.slots;
+            shift = a.modulation + (base + a.shift_slot) * a.width;
+            scale = a.modulation + (base + a.scale_slot) * a.width;
+        }
+#pragma unroll
+        for (int c = 0; c < CHUNKS; c++) {
+            const uint32_t col = column(c);
+            if (col >= a.width) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[c][i] = 0.0f;
+                continue;
+            }
+            float w[8], b[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[c][i] *= inverse;
+            if (a.weight) {
+                load8(a.weight + col, w);
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[c][i] *= w[i];
+            }
+            if (layer && a.bias) {
+                load8(a.bias + col, b);
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[c][i] += b[i];
+            }
+            if (shift) {
+                load8(scale + col, w);
+                load8(shift + col, b);
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    v[c][i] = v[c][i] * (1.0f + w[i]) + b[i];
+            }
+        }
+    }
+    uint32_t most = 0;
+#pragma unroll
+    for (int c = 0; c < CHUNKS; c++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) most = max(most, hk_magnitude(v[c][i]));
+    const hk_int8_quantizer code(hk_block_umax(most, tops));
+    int8_t *out = a.codes + (size_t)row * a.pitch;
+#pragma unroll
+    for (int c = 0; c < CHUNKS; c++) {
+        /* zeros from the row's end to that of its last line */
+        const uint32_t col = column(c);
+        if (col < a.pitch)
+            *(uint2 *)(out + col) = make_uint2(
+                hk_int8_pack4(code(v[c][0]), code(v[c][1]), code(v[c][2]),
+                              code(v[c][3])),
+                hk_int8_pack4(code(v[c][4]), code(v[c][5]), code(v[c][6]),
+                              code(v[c][7])));
+    }
+    if (threadIdx.x == 0) a.scales[row] = code.scale;
+}
+
 __global__ void __launch_bounds__(HK_INT8_THREADS)
 hk_int8_values(const int8_t *codes, const float *scales, uint16_t *out,
                uint32_t width, uint32_t pitch, uint32_t first) {
@@ -116,9 +235,19 @@ static void hk_int8_each_rows(uint32_t rows, F launch) {
 
 template <int SOURCE>
 static void hk_int8_rows(struct h3_gpu *gpu, const hk_int8_rows_args &a) {
+    const bool whole =
+        a.width % 8u == 0 && a.wide_pitch % 4u == 0 &&
+        (((uintptr_t)a.input | (uintptr_t)a.weight | (uintptr_t)a.bias |
+          (uintptr_t)a.modulation | (uintptr_t)a.wide) & 15u) == 0;
+    void (*kernel)(hk_int8_rows_args, uint32_t) =
+        !whole || a.pitch > 16384u || gpu->reference_kernels
+            ? hk_int8_rows_any<SOURCE>
+        : a.pitch <= 2048u ? hk_int8_rows_vec<SOURCE, 1>
+        : a.pitch <= 6144u ? hk_int8_rows_vec<SOURCE, 3>
+                           : hk_int8_rows_vec<SOURCE, 8>;
     hk_int8_each_rows(a.rows, [&](uint32_t first, uint32_t rows) {
-        hipLaunchKernelGGL(hk_int8_rows_any<SOURCE>, dim3(rows),
-                           dim3(HK_INT8_THREADS), 0, gpu->stream, a, first);
+        hipLaunchKernelGGL(kernel, dim3(rows), dim3(HK_INT8_THREADS), 0,
+                           gpu->stream, a, first);
     });
 }
 
@@ -181,12 +310,389 @@ static void hk_int8_simple_run(struct h3_gpu *gpu, const hk_int8_matrix &x,
                            x.pitch, gelu, first);
 }
 
+/* ------------------------------------- the products on the matrix cores */
+
+/* Operands of a launch beside hk_gemm_args: the rows' scales, and where the
+ * gated block's activation goes in F32. */
+struct hk_int8_ext {
+    const float *xs, *ws;
+    float *wide;
+    uint32_t wide_pitch;
+};
+
+#define HK_TRACE(p) ((void)0)
+#define HK_TRACE_CLOCK(p) ((void)0)
+#define HK_TRACE_VALUE(p, v) ((void)0)
+#define HK_KERNEL_INT8
+#define HK_KERNEL_NAME hk_int8_gemm
+#define HK_KERNEL_TEMPLATE template <int EPI, bool GROUP, int ROW_BLOCKS>
+#define HK_KERNEL_JB ROW_BLOCKS
+#include "hk_gemm_kernel.inc"
+
+/* Four columns of a row from their sums. */
+struct hk_int8_out {
+    const float *xs, *ws;
+    const uint16_t *bias;
+    uint16_t *out;
+    float *wide; /* in F32 instead, rows of n */
+    uint32_t n;
+    int gelu;
+};
+
+__device__ __forceinline__ void hk_int8_finish(const hk_int8_out &o,
+                                               uint32_t row, uint32_t col,
+                                               hk_v4i sums) {
+    const float sx = o.xs[row];
+    float y[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        y[e] = hk_int8_value(sums[e], sx, o.ws[col + e]);
+        if (o.bias && col + e < o.n) y[e] += hk_bf2f(o.bias[col + e]);
+        if (o.gelu) y[e] = hk_gelu_tanh_f(y[e]);
+    }
+    const size_t at = (size_t)row * o.n + col;
+    const bool whole = o.n % 4u == 0;
+    if (o.wide && whole) {
+        *(float4 *)(o.wide + at) = make_float4(y[0], y[1], y[2], y[3]);
+    } else if (whole) {
+        *(uint2 *)(o.out + at) =
+            make_uint2(hk_pack2(y[0], y[1]), hk_pack2(y[2], y[3]));
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            if (col + e >= o.n) continue;
+            if (o.wide) o.wide[at + e] = y[e];
+            else o.out[at + e] = hk_f2bf(y[e]);
+        }
+    }
+}
+
+/* Up to 128 rows: the skinny GEMM's loop (hk_skinny_tile.h) over bytes. */
+template <int MB, int XA>
+__global__ void __launch_bounds__(256)
+hk_int8_skinny(hk_skinny_args g, hk_int8_out o) {
+    hk_i32x16 acc[MB];
+    hk_skinny_sums<MB, XA, HK_LOAD_ONCE>(g, g.w, blockIdx.x, blockIdx.y, acc);
+    const uint32_t lane = threadIdx.x & 63u, row = lane & 31u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t tile = blockIdx.x * 4u + wave;
+    if (tile * 32u >= g.n) return;
+    if (g.partial) {
+        hk_skinny_partial<MB>((hk_v4i *)g.partial,
+                              (size_t)blockIdx.y * gridDim.x * 4u + tile, g.m,
+                              acc);
+        return;
+    }
+#pragma unroll
+    for (int mb = 0; mb < MB; mb++) {
+        if (mb * 32u + row >= g.m) continue;
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const uint32_t col = tile * 32u + q * 8u + (lane >> 5) * 4u;
+            if (col < g.n)
+                hk_int8_finish(o, mb * 32u + row, col,
+                               hk_v4i{acc[mb][q * 4], acc[mb][q * 4 + 1],
+                                      acc[mb][q * 4 + 2],
+                                      acc[mb][q * 4 + 3]});
+        }
+    }
+}
+
+/* Adds the pieces, as hk_skinny_reduce. */
+__global__ void __launch_bounds__(256)
+hk_int8_skinny_reduce(hk_skinny_args g, hk_int8_out o, uint32_t mbs,
+                      uint32_t tiles, uint32_t splits) {
+    const uint32_t lane = threadIdx.x & 63u, q = threadIdx.x >> 6;
+    const uint32_t tile = blockIdx.x / mbs, mb = blockIdx.x % mbs;
+    const uint32_t row = mb * 32u + (lane & 31u);
+    const uint32_t col = tile * 32u + q * 8u + (lane >> 5) * 4u;
+    if (row >= g.m || col >= g.n) return;
+    const size_t stride = (size_t)tiles * mbs * 256u;
+    const hk_v4i *p =
+        (const hk_v4i *)g.partial + (size_t)blockIdx.x * 256u + threadIdx.x;
+    hk_v4i sum = *p;
+    for (uint32_t s = 1; s < splits; s++) sum += p[s * stride];
+    hk_int8_finish(o, row, col, sum);
+}
+
+/* Adds the pieces of tiles, as hk_splitk_reduce: 4 columns a thread. */
+__global__ void __launch_bounds__(256)
+hk_int8_tile_reduce(hk_gemm_args g, hk_int8_out o, uint32_t splits) {
+    const uint32_t blocks = g.tile_rows / 4u;
+    const uint32_t part = blockIdx.x / blocks;
+    const uint32_t row = (blockIdx.x - part * blocks) * 4u + (threadIdx.x >> 6);
+    const uint32_t tcol = (threadIdx.x & 63u) * 4u;
+    uint32_t tile_m, tile_n;
+    hk_tile_coords(g.tile_base + part, g.tiles_m, g.tiles_n, tile_m, tile_n);
+    const uint32_t m = tile_m * g.tile_rows + row, n = tile_n * HK_BN + tcol;
+    if (m >= g.m || n >= g.n) return;
+    const size_t tile = (size_t)g.tile_rows * HK_BN;
+    const size_t stride = g.part_tiles * tile / 4u;
+    const hk_v4i *p = (const hk_v4i *)((const int *)g.partial + part * tile +
+                                       row * HK_BN + tcol);
+    hk_v4i sum = *p;
+    for (uint32_t s = 1; s < splits; s++) sum += p[s * stride];
+    hk_int8_finish(o, m, n, sum);
+}
+
+/* The same of the gated block: F32 rows of its activation. */
+__global__ void __launch_bounds__(256)
+hk_int8_gated_reduce(hk_gemm_args g, hk_int8_ext scaled, uint32_t splits) {
+    const uint32_t blocks = g.tile_rows / 8u;
+    const uint32_t part = blockIdx.x / blocks;
+    const uint32_t row = (blockIdx.x - part * blocks) * 8u + (threadIdx.x >> 5);
+    const uint32_t c4 = (threadIdx.x & 31u) * 4u;
+    uint32_t tile_m, tile_n;
+    hk_tile_coords(g.tile_base + part, g.tiles_m, g.tiles_n, tile_m, tile_n);
+    const uint32_t m = tile_m * g.tile_rows + row, n = tile_n * 128u + c4;
+    if (m >= g.m || n >= g.n) return;
+    const size_t tile = (size_t)g.tile_rows * HK_BN;
+    const size_t stride = g.part_tiles * tile / 4u;
+    /* 64 gate columns, then their 64 up ones */
+    const hk_v4i *p =
+        (const hk_v4i *)((const int *)g.partial + part * tile + row * HK_BN +
+                         (c4 >> 6) * 128u + (c4 & 63u));
+    hk_v4i gate = p[0], up = p[16];
+    for (uint32_t s = 1; s < splits; s++) {
+        gate += p[s * stride];
+        up += p[s * stride + 16u];
+    }
+    const float sx = scaled.xs[m];
+    float y[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        y[e] = hk_swiglu_f(
+            hk_int8_value(gate[e], sx, scaled.ws[n + e]),
+            hk_int8_value(up[e], sx, scaled.ws[g.n + n + e]));
+    /* (rows are padded to whole pieces) */
+    *(float4 *)(scaled.wide + (size_t)m * scaled.wide_pitch + n) =
+        make_float4(y[0], y[1], y[2], y[3]);
+}
+
+typedef void (*hk_int8_kernel)(hk_gemm_args, hk_int8_ext);
+
+template <int EPI>
+static hk_int8_kernel hk_int8_pick(uint32_t jb) {
+    switch (jb) {
+    case 4: return hk_int8_gemm<EPI, false, 4>;
+    case 5: return hk_int8_gemm<EPI, false, 5>;
+    case 6: return hk_int8_gemm<EPI, false, 6>;
+    case 7: return hk_int8_gemm<EPI, false, 7>;
+    default: return hk_int8_gemm<EPI, false, 8>;
+    }
+}
+
+static hk_int8_kernel hk_int8_pick_epi(int epilogue, uint32_t jb) {
+    switch (epilogue) {
+    case HK_EPI_SWIGLU: return hk_int8_pick<HK_EPI_SWIGLU>(jb);
+    case HK_EPI_GELU_F32: return hk_int8_pick<HK_EPI_GELU_F32>(jb);
+    case HK_EPI_PARTIAL: return hk_int8_pick<HK_EPI_PARTIAL>(jb);
+    case HK_EPI_PARTIAL_SWIGLU: return hk_int8_pick<HK_EPI_PARTIAL_SWIGLU>(jb);
+    default: return hk_int8_pick<HK_EPI_STORE>(jb);
+    }
+}
+
+/* beside the tiles: scales and bias */
+static uint32_t hk_int8_lds(uint32_t jb) {
+    return hk_gemm_lds(jb) + 768u * sizeof(float);
+}
+
+static void hk_int8_launch(struct h3_gpu *gpu, int epilogue, uint32_t jb,
+                           uint32_t workgroups, const hk_gemm_args &g,
+                           const hk_int8_ext &e) {
+    static uint64_t ready = 0; /* devices, as in hk_gemm_lds_setup */
+    const uint64_t bit = 1ull << (gpu->device & 63);
+    if (!(ready & bit)) {
+        for (uint32_t j = 4; j <= 8; j++)
+            for (int epi : {HK_EPI_STORE, HK_EPI_GELU_F32, HK_EPI_SWIGLU,
+                            HK_EPI_PARTIAL, HK_EPI_PARTIAL_SWIGLU})
+                (void)hipFuncSetAttribute(
+                    (const void *)hk_int8_pick_epi(epi, j),
+                    hipFuncAttributeMaxDynamicSharedMemorySize,
+                    (int)hk_int8_lds(j));
+        ready |= bit;
+    }
+    hipLaunchKernelGGL(hk_int8_pick_epi(epilogue, jb), dim3(workgroups),
+                       dim3(HK_GEMM_THREADS), hk_int8_lds(jb), gpu->stream, g,
+                       e);
+}
+
+static uint32_t hk_int8_cus(const struct h3_gpu *gpu) {
+    return gpu->num_cus > 0 ? (uint32_t)gpu->num_cus : 256u;
+}
+
+/* Rows whose bytes, and a K offset behind them, end below 2^32. */
+static uint32_t hk_int8_reach(uint32_t pitch) {
+    return (0xffffffffu - pitch - 4096u) / pitch;
+}
+
+/* x . w^T over tiles, in the plan of the bf16 GEMM: a K step is 128 bytes of
+ * a row on both, and takes as long.  `gated`: the activation of n columns, of
+ * 2 n rows of w, into e.wide; else o's rows. */
+static void hk_int8_tiles(struct h3_gpu *gpu, const hk_int8_matrix &x,
+                          const hk_int8_matrix &w, uint32_t n, bool gated,
+                          const hk_int8_out &o, hk_int8_ext e) {
+    const uint32_t cus = hk_int8_cus(gpu), k_steps = x.pitch / HK_INT8_LINE;
+    hk_gemm_args g = {};
+    g.x = (const uint16_t *)x.codes;
+    g.w = (const uint16_t *)w.codes;
+    g.bias = o.bias;
+    g.c = o.out;
+    g.m = x.rows;
+    g.n = n;
+    g.k = x.pitch / 2u;
+    g.tiles_n = (n + (gated ? 127u : HK_BN - 1u)) / (gated ? 128u : HK_BN);
+    const uint32_t jb =
+        hk_gemm_row_blocks(g.m, g.tiles_n, k_steps, cus, true);
+    g.tile_rows = 32u * jb;
+    g.tiles_m = (g.m + g.tile_rows - 1u) / g.tile_rows;
+    g.x_bytes = x.rows * x.pitch;
+    g.w_bytes = w.rows * w.pitch;
+    g.tile_count = g.tiles_m * g.tiles_n;
+    const int epilogue = gated    ? HK_EPI_SWIGLU
+                         : o.gelu ? HK_EPI_GELU_F32
+                                  : HK_EPI_STORE;
+    const hk_gemm_rounds r =
+        hk_gemm_rounds_of(g.tile_count, k_steps, cus, true);
+    float *partial = NULL;
+    if (r.splits > 1)
+        partial = (float *)hk_splitk_try(
+            gpu, (size_t)r.splits * r.tail * g.tile_rows * HK_BN * 4);
+    if (!partial) { /* or, without scratch, one more round */
+        hk_int8_launch(gpu, epilogue, jb, hk_gemm_grid(g.tile_count, cus), g,
+                       e);
+        return;
+    }
+    if (r.full) {
+        g.tile_count = r.full;
+        hk_int8_launch(gpu, epilogue, jb, hk_gemm_grid(r.full, cus), g, e);
+    }
+    g.partial = partial;
+    g.split_steps = r.steps;
+    g.tile_base = r.full;
+    g.part_tiles = r.tail;
+    hk_int8_launch(gpu, gated ? HK_EPI_PARTIAL_SWIGLU : HK_EPI_PARTIAL, jb,
+                   r.tail * r.splits, g, e);
+    if (gated)
+        hipLaunchKernelGGL(hk_int8_gated_reduce,
+                           dim3(r.tail * (g.tile_rows / 8u)), dim3(256), 0,
+                           gpu->stream, g, e, r.splits);
+    else
+        hipLaunchKernelGGL(hk_int8_tile_reduce,
+                           dim3(r.tail * (g.tile_rows / 4u)), dim3(256), 0,
+                           gpu->stream, g, o, r.splits);
+}
+
+/* Up to 128 rows, as hk_gemm_skinny_run. */
+static void hk_int8_few(struct h3_gpu *gpu, const hk_int8_matrix &x,
+                        const hk_int8_matrix &w, const hk_int8_out &o) {
+    const uint32_t cus = hk_int8_cus(gpu), k_steps = x.pitch / HK_INT8_LINE;
+    const uint32_t mbs = (x.rows + 31u) / 32u, wgs = (o.n + 127u) / 128u;
+    hk_skinny_args g = {};
+    g.x = (const uint16_t *)x.codes;
+    g.w = (const uint16_t *)w.codes;
+    g.m = x.rows;
+    g.n = o.n;
+    g.k = x.pitch / 2u;
+    g.x_bytes = x.rows * x.pitch;
+    g.w_bytes = w.rows * w.pitch;
+    g.split_steps = k_steps;
+    uint32_t splits = std::min(cus / wgs, k_steps / 8u);
+    if (splits > 1) {
+        /* whole turns of the kernel's ring of 4 */
+        g.split_steps = ((k_steps + splits - 1u) / splits + 3u) & ~3u;
+        splits = (k_steps + g.split_steps - 1u) / g.split_steps;
+    }
+    if (splits > 1)
+        g.partial = (float *)hk_splitk_try(
+            gpu, (size_t)splits * wgs * 4 * mbs * 4096);
+    if (!g.partial) splits = 1;
+    static uint64_t ready = 0;
+    const uint64_t bit = 1ull << (gpu->device & 63);
+    if (!(ready & bit)) {
+        (void)hipFuncSetAttribute((const void *)hk_int8_skinny<4, 3>,
+                                  hipFuncAttributeMaxDynamicSharedMemorySize,
+                                  4 * 4096 * 4 + 16384);
+        ready |= bit;
+    }
+    void (*kernel)(hk_skinny_args, hk_int8_out) =
+        mbs == 1   ? hk_int8_skinny<1, 3>
+        : mbs == 2 ? hk_int8_skinny<2, 3>
+        : mbs == 3 ? hk_int8_skinny<3, 3>
+                   : hk_int8_skinny<4, 3>;
+    hipLaunchKernelGGL(kernel, dim3(wgs, splits), dim3(256),
+                       mbs * 4096 * 4 + 16384, gpu->stream, g, o);
+    if (splits > 1)
+        hipLaunchKernelGGL(hk_int8_skinny_reduce, dim3((o.n + 31u) / 32u * mbs),
+                           dim3(256), 0, gpu->stream, g, o, mbs, wgs * 4u,
+                           splits);
+}
+
+/* Whether x . w^T runs on the matrix cores: everything but weights of 4 GiB
+ * and more, whose rows the buffer offsets do not reach. */
+static bool hk_int8_fast(const struct h3_gpu *gpu, const hk_int8_matrix &w) {
+    return !gpu->reference_kernels && w.rows <= hk_int8_reach(w.pitch);
+}
+
+enum { HK_INT8_FEW_ROWS = 128 };
+
 /* bf16 rows of x . w^T. */
-static int hk_int8_linear(struct h3_gpu *gpu, const hk_int8_matrix &x,
-                          const hk_int8_matrix &w, const uint16_t *bias,
-                          uint16_t *out, int gelu) {
-    hk_int8_simple_run(gpu, x, w, bias, out, NULL, gelu);
-    return 1;
+static void hk_int8_linear(struct h3_gpu *gpu, hk_int8_matrix x,
+                           const hk_int8_matrix &w, const uint16_t *bias,
+                           uint16_t *out, int gelu) {
+    if (!hk_int8_fast(gpu, w)) {
+        hk_int8_simple_run(gpu, x, w, bias, out, NULL, gelu);
+        return;
+    }
+    hk_int8_out o = {x.scales, w.scales, bias, out, NULL, w.rows, gelu};
+    const uint32_t most = hk_int8_reach(x.pitch);
+    for (uint32_t left = x.rows; left; left -= x.rows) {
+        x.rows = std::min(left, most);
+        if (x.rows <= HK_INT8_FEW_ROWS)
+            hk_int8_few(gpu, x, w, o);
+        else
+            hk_int8_tiles(gpu, x, w, w.rows, false, o,
+                          {o.xs, o.ws, NULL, 0});
+        x.codes += (size_t)x.rows * x.pitch;
+        o.xs += x.rows;
+        o.out += (size_t)x.rows * o.n;
+    }
+}
+
+/* h = silu(x . gate^T) (x . up^T) in 8 bits, by way of F32 rows in `wide`
+ * ([rows][2 hidden] at most). */
+static void hk_int8_gated(struct h3_gpu *gpu, hk_int8_matrix x,
+                          const hk_int8_matrix &w, uint32_t hidden,
+                          float *wide, const hk_int8_matrix &h) {
+    hk_int8_rows_args a = {};
+    a.wide = wide;
+    a.codes = (int8_t *)h.codes;
+    a.scales = (float *)h.scales;
+    a.rows = x.rows;
+    a.width = hidden;
+    a.pitch = h.pitch;
+    const bool fast = hk_int8_fast(gpu, w);
+    if (!fast || x.rows <= HK_INT8_FEW_ROWS) {
+        a.wide_pitch = 2 * hidden;
+        if (fast)
+            hk_int8_few(gpu, x, w, {x.scales, w.scales, NULL, NULL, wide,
+                                    2 * hidden, 0});
+        else
+            hk_int8_simple_run(gpu, x, w, NULL, NULL, wide, 0);
+        hk_int8_rows<HK_ROWS_SWIGLU>(gpu, a);
+        return;
+    }
+    a.wide_pitch = (hidden + 3u) & ~3u;
+    const uint32_t most = hk_int8_reach(x.pitch);
+    hk_int8_ext e = {x.scales, w.scales, wide, a.wide_pitch};
+    for (uint32_t left = x.rows; left; left -= x.rows) {
+        x.rows = std::min(left, most);
+        hk_int8_tiles(gpu, x, w, hidden, true, {}, e);
+        x.codes += (size_t)x.rows * x.pitch;
+        e.xs += x.rows;
+        e.wide += (size_t)x.rows * e.wide_pitch;
+    }
+    hk_int8_rows<HK_ROWS_F32>(gpu, a);
 }
 
 /* ================================================================ ops */
@@ -348,10 +854,9 @@ static int hk_int8_linear_op(h3_gpu *gpu, h3_gpu_tensor *output,
     if (!rows || !output_dim) return 1;
     const char *name = gelu ? "gemm_int8_gelu" : "gemm_int8";
     hk_op_begin(gpu, name);
-    if (!hk_int8_linear(gpu, hk_int8_of(input, rows),
-                        hk_int8_of(weight, output_dim),
-                        bias ? HK_CBF16(bias) : NULL, HK_BF16(output), gelu))
-        return 0;
+    hk_int8_linear(gpu, hk_int8_of(input, rows),
+                   hk_int8_of(weight, output_dim),
+                   bias ? HK_CBF16(bias) : NULL, HK_BF16(output), gelu);
     return hk_op_end(gpu, name, HK_KIND_LINEAR);
 }
 
@@ -392,35 +897,29 @@ int h3_hip_mlp_int8_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
         !hk_require_active(gpu))
         return 0;
     if (!rows || !output_dim) return 1;
-    /* F32 rows of the first product, then h in 8 bits */
+    /* F32 rows of the activation or, where they are few or go through the
+     * simple kernel, of both projections, then h in 8 bits */
+    const hk_int8_matrix w1 = hk_int8_of(fc1_weight, 2 * hidden_dim);
     const uint32_t pitch = fc2_weight->record.n[HK_INT8_PITCH];
-    const size_t wide_bytes =
-        ((size_t)rows * 2 * hidden_dim * 4 + 255) & ~(size_t)255;
+    const size_t wide =
+        rows > HK_INT8_FEW_ROWS && hk_int8_fast(gpu, w1)
+            ? ((size_t)hidden_dim + 3u) & ~(size_t)3u
+            : 2 * (size_t)hidden_dim;
+    const size_t wide_bytes = (rows * wide * 4 + 255) & ~(size_t)255;
     const size_t code_bytes = (size_t)rows * pitch;
     uint8_t *space = (uint8_t *)hk_workspace(
         gpu, wide_bytes + code_bytes + ((size_t)rows + 255u) / 256u * 1024u);
     if (!space) return 0;
-    hk_int8_matrix h = {(int8_t *)(space + wide_bytes),
-                        (float *)(space + wide_bytes + code_bytes), rows,
-                        pitch};
+    const hk_int8_matrix h = {(int8_t *)(space + wide_bytes),
+                              (float *)(space + wide_bytes + code_bytes), rows,
+                              pitch};
     hk_op_begin(gpu, "gemm_int8_swiglu");
-    hk_int8_rows_args a = {};
-    a.wide = (float *)space;
-    a.codes = (int8_t *)h.codes;
-    a.scales = (float *)h.scales;
-    a.rows = rows;
-    a.width = hidden_dim;
-    a.pitch = pitch;
-    a.wide_pitch = 2 * hidden_dim;
-    hk_int8_simple_run(gpu, hk_int8_of(input, rows),
-                       hk_int8_of(fc1_weight, 2 * hidden_dim), NULL, NULL,
-                       (float *)space, 0);
-    hk_int8_rows<HK_ROWS_SWIGLU>(gpu, a);
+    hk_int8_gated(gpu, hk_int8_of(input, rows), w1, hidden_dim,
+                  (float *)space, h);
     if (!hk_op_end(gpu, "gemm_int8_swiglu", HK_KIND_LINEAR)) return 0;
     hk_op_begin(gpu, "gemm_int8");
-    if (!hk_int8_linear(gpu, h, hk_int8_of(fc2_weight, output_dim), NULL,
-                        HK_BF16(output), 0))
-        return 0;
+    hk_int8_linear(gpu, h, hk_int8_of(fc2_weight, output_dim), NULL,
+                   HK_BF16(output), 0);
     return hk_op_end(gpu, "gemm_int8", HK_KIND_LINEAR);
 }
 

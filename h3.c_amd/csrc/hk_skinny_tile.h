@@ -65,24 +65,29 @@ struct hk_skinny_args {
     uint16_t *c1;
 };
 
-/* Workgroup (x, y, z) of `columns` x `pieces` ones a problem. */
-template <int MB, int XA, int W_POLICY = HK_LOAD_ONCE>
-__device__ __forceinline__ void hk_skinny_tile(const hk_skinny_args &g,
-                                               uint32_t x, uint32_t y,
-                                               uint32_t z, uint32_t columns,
-                                               uint32_t pieces) {
+typedef int hk_i32x16 __attribute__((ext_vector_type(16)));
+
+/* One product of a k step: 16 bf16 a row, or (whole-number sums) 32 bytes. */
+__device__ __forceinline__ void hk_skinny_mfma(hk_f32x16 &acc, hk_v4i w,
+                                               hk_v4i x) {
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+        __builtin_bit_cast(hk_bf16x8, w), __builtin_bit_cast(hk_bf16x8, x),
+        acc, 0, 0, 0);
+}
+
+__device__ __forceinline__ void hk_skinny_mfma(hk_i32x16 &acc, hk_v4i w,
+                                               hk_v4i x) {
+    acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(w, x, acc, 0, 0, 0);
+}
+
+/* The sums of piece y of workgroup x's columns: acc[mb][r] =
+ * C[mb*32 + row][n0 + (r/4)*8 + half*4 + r%4], n0 = (4 x + wave) 32, row and
+ * half of the lane.  Rows of bytes count K in pairs. */
+template <int MB, int XA, int W_POLICY, typename SUMS>
+__device__ __forceinline__ void hk_skinny_sums(const hk_skinny_args &g,
+                                               const uint16_t *w, uint32_t x,
+                                               uint32_t y, SUMS (&acc)[MB]) {
     const uint32_t n = g.n, m = g.m, k = g.k;
-    const uint16_t *w = g.w, *bias = g.bias;
-    uint16_t *c = g.c;
-    if (g.group) {
-        w = (const uint16_t *)hk_group_word(g.group, 3 * z);
-        bias = (const uint16_t *)hk_group_word(g.group, 3 * z + 1);
-        c = (uint16_t *)hk_group_word(g.group, 3 * z + 2);
-    } else if (z) {
-        w = g.w1;
-        bias = g.bias1;
-        c = g.c1;
-    }
     /* k steps of this split; its byte offset goes in the scalar offsets */
     const uint32_t base = g.partial ? y * g.split_steps : 0u;
     const uint32_t steps =
@@ -131,15 +136,14 @@ __device__ __forceinline__ void hk_skinny_tile(const hk_skinny_args &g,
     /* fragment of X rows mb*32 + row, logical chunk 2q + half */
     auto read_x = [&](int buf, int mb, int q) {
         const uint32_t r = mb * 32u + row;
-        return *(const hk_bf16x8 *)(
+        return *(const hk_v4i *)(
             hk_xs + buf * XSTAGE + r * 128u +
             (((2u * q + half) ^ hk_swz_key(r)) << 4));
     };
-    hk_f32x16 acc[MB];
 #pragma unroll
     for (int mb = 0; mb < MB; mb++)
 #pragma unroll
-        for (int r = 0; r < 16; r++) acc[mb][r] = 0.0f;
+        for (int r = 0; r < 16; r++) acc[mb][r] = 0;
     /* The waits below count loads: a step's X loads must leave before its W
      * loads, and steps in order.  Nothing else orders them (they write LDS
      * and registers) up to the next step's barrier, which they do not
@@ -181,9 +185,8 @@ __device__ __forceinline__ void hk_skinny_tile(const hk_skinny_args &g,
         for (int q = 0; q < 4; q++)
 #pragma unroll
             for (int mb = 0; mb < MB; mb++)
-                acc[mb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                    __builtin_bit_cast(hk_bf16x8, wfrag[q]),
-                    read_x(d % (XA + 1), mb, q), acc[mb], 0, 0, 0);
+                hk_skinny_mfma(acc[mb], wfrag[q],
+                               read_x(d % (XA + 1), mb, q));
     };
     uint32_t s0 = 0;
     for (; XA == 1 ? s0 < steps : s0 + D <= steps; s0 += D) {
@@ -217,24 +220,57 @@ __device__ __forceinline__ void hk_skinny_tile(const hk_skinny_args &g,
     }
     /* no load to LDS outlives the workgroup */
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    /* acc[mb][r] = C[mb*32 + row][n0 + (r/4)*8 + half*4 + r%4] */
+}
+
+/* A piece's sums, [32-column tile][MB][4][64 lanes] of four, `tile` counted
+ * over the pieces: whole lines, each (mb, q) is a wave's 64 16-byte ones. */
+template <int MB, typename SUMS, typename FOUR>
+__device__ __forceinline__ void hk_skinny_partial(FOUR *partial, size_t tile,
+                                                  uint32_t m,
+                                                  const SUMS (&acc)[MB]) {
+    const uint32_t lane = threadIdx.x & 63u, row = lane & 31u;
+    FOUR *part = partial + tile * (MB * 256u);
+#pragma unroll
+    for (int mb = 0; mb < MB; mb++) {
+        if (mb * 32u + row >= m) continue;
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+            part[(mb * 4u + q) * 64u + lane] =
+                FOUR{acc[mb][q * 4], acc[mb][q * 4 + 1], acc[mb][q * 4 + 2],
+                     acc[mb][q * 4 + 3]};
+    }
+}
+
+/* Workgroup (x, y, z) of `columns` x `pieces` ones a problem. */
+template <int MB, int XA, int W_POLICY = HK_LOAD_ONCE>
+__device__ __forceinline__ void hk_skinny_tile(const hk_skinny_args &g,
+                                               uint32_t x, uint32_t y,
+                                               uint32_t z, uint32_t columns,
+                                               uint32_t pieces) {
+    const uint32_t n = g.n, m = g.m;
+    const uint16_t *w = g.w, *bias = g.bias;
+    uint16_t *c = g.c;
+    if (g.group) {
+        w = (const uint16_t *)hk_group_word(g.group, 3 * z);
+        bias = (const uint16_t *)hk_group_word(g.group, 3 * z + 1);
+        c = (uint16_t *)hk_group_word(g.group, 3 * z + 2);
+    } else if (z) {
+        w = g.w1;
+        bias = g.bias1;
+        c = g.c1;
+    }
+    hk_f32x16 acc[MB];
+    hk_skinny_sums<MB, XA, W_POLICY>(g, w, x, y, acc);
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t row = lane & 31u, half = lane >> 5;
+    const uint32_t n0 = (x * 4u + wave) * 32u;
     if (g.partial) {
-        /* whole lines: each (mb, q) is a wave's 64 16-byte pieces */
-        hk_f32x4 *part =
-            (hk_f32x4 *)g.partial +
-            (((size_t)z * pieces + y) * columns * 4u +
-             x * 4u + wave) *
-                (MB * 256u);
         if (n0 >= n) return;
-#pragma unroll
-        for (int mb = 0; mb < MB; mb++) {
-            if (mb * 32u + row >= m) continue;
-#pragma unroll
-            for (int q = 0; q < 4; q++)
-                part[(mb * 4u + q) * 64u + lane] =
-                    hk_f32x4{acc[mb][q * 4], acc[mb][q * 4 + 1],
-                             acc[mb][q * 4 + 2], acc[mb][q * 4 + 3]};
-        }
+        hk_skinny_partial<MB>((hk_f32x4 *)g.partial,
+                              ((size_t)z * pieces + y) * columns * 4u +
+                                  x * 4u + wave,
+                              m, acc);
         return;
     }
 #pragma unroll
