@@ -256,6 +256,517 @@ __global__ void __launch_bounds__(256) hk_kv8_simple(hk_kv8_args g) {
     }
 }
 
+/* ------------------------------------------------- the matrix-core kernel
+ *
+ * The plan's items (hk_packed.h), a block of 64 keys a tile: S^T = K . Q^T with
+ * the Q fragments in registers, the softmax in the lanes that hold a query's
+ * scores, O^T = V^T . P^T.  Codes and P are f16, which holds codes exactly and
+ * is made of them in two instructions a pair; scores are multiplied by the
+ * block's key scale, the block's product by its value scale as it is added to
+ * O.  A query row is scaled by a power of two of its own to f16's range, which
+ * loses nothing of a bf16 within 2^27 of the row's largest.
+ *
+ * P = 2^((s - m) L + 7) against a reference m (a score, L = scale log2(e)) that
+ * moves when a lane's sum of P passes 2^15: so f16 holds every P, to 11 bits
+ * those over 2^-21 of the largest; the factor 2^7 is in the sums too. */
+typedef _Float16 hk_f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 hk_f16x8 __attribute__((ext_vector_type(8)));
+
+#define HK_KV8_LIFT 7.0f
+#define HK_KV8_MOST 0x1p15f
+
+/* Four codes (+ 128) as f16: byte b is the low byte of 1024 + b. */
+__device__ __forceinline__ uint2 hk_kv8_f16(uint32_t codes) {
+    const hk_f16x2 less = {(_Float16)-1152.0f, (_Float16)-1152.0f};
+    const hk_f16x2 low =
+        __builtin_bit_cast(hk_f16x2, __builtin_amdgcn_perm(
+                                         0x64646464u, codes, 0x04010400u)) +
+        less;
+    const hk_f16x2 high =
+        __builtin_bit_cast(hk_f16x2, __builtin_amdgcn_perm(
+                                         0x64646464u, codes, 0x04030402u)) +
+        less;
+    return make_uint2(__builtin_bit_cast(uint32_t, low),
+                      __builtin_bit_cast(uint32_t, high));
+}
+
+/* A lane's 16 bytes as two fragments of 8. */
+__device__ __forceinline__ void hk_kv8_fragments(uint4 codes, uint4 (&f)[2]) {
+    const uint2 a = hk_kv8_f16(codes.x), b = hk_kv8_f16(codes.y);
+    const uint2 c = hk_kv8_f16(codes.z), d = hk_kv8_f16(codes.w);
+    f[0] = make_uint4(a.x, a.y, b.x, b.y);
+    f[1] = make_uint4(c.x, c.y, d.x, d.y);
+}
+
+__device__ __forceinline__ hk_f32x16 hk_kv8_mfma(uint4 a, hk_f16x8 b,
+                                                 hk_f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(
+        __builtin_bit_cast(hk_f16x8, a), b, c, 0, 0, 0);
+}
+
+/* Whether -(m L) is far from zero, infinite or NaN (hk_packed.hip). */
+__device__ __forceinline__ bool hk_kv8_far(float neg) {
+    return !(fabsf(neg) < 0x1p10f);
+}
+
+/* A wave's 32 virtual rows, lane % 32, and what it has of their sums. */
+template <int DIMS> struct hk_kv8_wave {
+    static constexpr int NK = DIMS / 16, ND = DIMS / 32;
+    hk_f16x8 q[NK];   /* dims 32 (k / 2) + 16 half + 8 (k % 2) .. + 8 */
+    float q_scale;    /* of the row */
+    hk_f32x16 o[ND];
+    float m, neg;     /* the reference, -(m L); unset: -+ infinity */
+    float l;
+
+    __device__ __forceinline__ void start(const hk_packed_args &a,
+                                          const hk_packed_item &it,
+                                          uint32_t vrow) {
+        const uint32_t half = (threadIdx.x & 63u) >> 5;
+        float x[NK][8];
+        const bool live = vrow < it.rows;
+        const uint32_t r = vrow / a.group, g = vrow - r * a.group;
+        const uint16_t *row =
+            a.q + ((uint64_t)it.q_first + r) * a.q_stride +
+            (uint64_t)(it.kv_head * a.group + g) * a.dim;
+        const bool whole =
+            a.dim % 8u == 0 && a.q_stride % 8u == 0 &&
+            ((uintptr_t)a.q & 15u) == 0;
+        uint32_t most = 0;
+#pragma unroll
+        for (int k = 0; k < NK; k++) {
+            const uint32_t d = (k >> 1) * 32u + half * 16u + (k & 1) * 8u;
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[k][e] = 0.0f;
+            if (live && whole && d < a.dim) {
+                hk_unpack8(*(const uint4 *)(row + d), x[k]);
+            } else if (live && !whole) {
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    if (d + e < a.dim) x[k][e] = hk_bf2f(row[d + e]);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; e++) most = max(most, hk_magnitude(x[k][e]));
+        }
+        most = max(most, (uint32_t)__shfl_xor(most, 32, 64));
+        /* to [2^13, 2^14) */
+        const int by = 13 + 127 - (int)(most >> 23);
+        q_scale = ldexpf(1.0f, -by);
+#pragma unroll
+        for (int k = 0; k < NK; k++)
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                q[k][e] = (_Float16)ldexpf(x[k][e], by);
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
+        m = -INFINITY;
+        neg = INFINITY;
+        l = 0.0f;
+    }
+
+    /* Scores (of products with the codes) to P, with the block's key scale;
+     * `keys` of the block's rows count. */
+    __device__ __forceinline__ void softmax(hk_f32x16 (&s)[2],
+                                            hk_f16x8 (&p)[2][2], float scale,
+                                            uint32_t keys, float L) {
+        const uint32_t half = (threadIdx.x & 63u) >> 5;
+        const float by = q_scale * scale;
+#pragma unroll
+        for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[kt][r] *= by;
+        if (keys < HK_KV8_BLOCK) {
+#pragma unroll
+            for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+                    if (kt * 32u + (r >> 2) * 8u + half * 4u + (r & 3) >= keys)
+                        s[kt][r] = -INFINITY;
+        }
+        auto exps = [&](float less) -> float {
+            float sum = 0.0f;
+            less += HK_KV8_LIFT;
+#pragma unroll
+            for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const float e = __builtin_amdgcn_exp2f(
+                        __builtin_fmaf(s[kt][r], L, less));
+                    sum += e;
+                    p[kt][r >> 3][r & 7] = (_Float16)e;
+                }
+            return sum;
+        };
+        const bool far = hk_kv8_far(neg); /* or unset */
+        float sum = far ? 0.0f : exps(neg);
+        /* (a NaN sum stays) */
+        uint32_t move = far || sum > HK_KV8_MOST;
+        if (__builtin_amdgcn_ballot_w64(move)) {
+            /* a row's other half's too, but no other row's */
+            const auto both =
+                __builtin_amdgcn_permlane32_swap(move, move, false, false);
+            move = both[0] | both[1];
+            float mx = -INFINITY;
+#pragma unroll
+            for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) mx = fmaxf(mx, s[kt][r]);
+            const auto sw = __builtin_amdgcn_permlane32_swap(
+                __float_as_uint(mx), __float_as_uint(mx), false, false);
+            mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+            const float now = move ? fmaxf(m, mx) : m;
+            const float ref = now == -INFINITY ? 0.0f : now;
+            const float c =
+                move ? __builtin_amdgcn_exp2f((m - ref) * L) : 1.0f;
+            m = now; /* unset while every score is -inf */
+            neg = -(now * L);
+            float less = -(ref * L);
+            if (__builtin_amdgcn_ballot_w64(hk_kv8_far(less))) {
+                const float off = hk_kv8_far(less) ? ref : 0.0f;
+#pragma unroll
+                for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) s[kt][r] -= off;
+                if (hk_kv8_far(less)) less = 0.0f;
+            }
+            l *= c;
+#pragma unroll
+            for (int d = 0; d < ND; d++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) o[d][r] *= c;
+            sum = exps(less);
+        }
+        l += sum;
+    }
+
+    /* o[d] += scale * the block's product, two groups of 32 dims at a time */
+    template <typename F>
+    __device__ __forceinline__ void values(const hk_f16x8 (&p)[2][2],
+                                           float scale, F fragments) {
+#pragma unroll
+        for (int d0 = 0; d0 < ND; d0 += 2) {
+            hk_f32x16 t[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) t[i][r] = 0.0f;
+#pragma unroll
+            for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    if (d0 + i >= ND) continue;
+                    uint4 f[2];
+                    fragments(kt, d0 + i, f);
+                    t[i] = hk_kv8_mfma(f[0], p[kt][0], t[i]);
+                    t[i] = hk_kv8_mfma(f[1], p[kt][1], t[i]);
+                }
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+                    if (d0 + i < ND)
+                        o[d0 + i][r] = __builtin_fmaf(t[i][r], scale,
+                                                      o[d0 + i][r]);
+        }
+    }
+
+    template <typename F>
+    __device__ __forceinline__ void scores(hk_f32x16 (&s)[2], F fragments) {
+#pragma unroll
+        for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[kt][r] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < ND; j++)
+#pragma unroll
+            for (int kt = 0; kt < 2; kt++) {
+                uint4 f[2];
+                fragments(kt, j, f);
+                s[kt] = hk_kv8_mfma(f[0], q[2 * j], s[kt]);
+                s[kt] = hk_kv8_mfma(f[1], q[2 * j + 1], s[kt]);
+            }
+    }
+};
+
+/* Eight dims of an output row. */
+__device__ __forceinline__ void hk_kv8_put(const hk_packed_args &a,
+                                           const hk_packed_item &it,
+                                           uint32_t vrow, uint32_t dim,
+                                           const float *v, bool whole) {
+    const uint32_t r = vrow / a.group, g = vrow - r * a.group;
+    uint16_t *to = a.o + (((uint64_t)it.q_first + r) * a.heads +
+                          it.kv_head * a.group + g) * a.dim + dim;
+    if (whole) {
+        if (dim < a.dim) *(uint4 *)to = hk_pack8(v);
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+        if (dim + e < a.dim) to[e] = hk_f2bf(v[e]);
+}
+
+/* An item of at most 32 rows: the waves share its rows and split its blocks,
+ * wave w every fourth from the wth on, each straight from the cache into its
+ * registers; then their sums are joined. */
+template <int DIMS>
+__device__ __forceinline__ void hk_kv8_few(const hk_kv8_args &g,
+                                           const hk_packed_item &it,
+                                           float *lds) {
+    constexpr int ND = DIMS / 32, UNITS = DIMS / 16; /* of K or V */
+    constexpr int DP = DIMS <= 64 ? 64 : 128;
+    const hk_packed_args &a = g.p;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t col = lane & 31u, half = lane >> 5;
+    const uint32_t vrow = it.row + col;
+    hk_kv8_wave<DIMS> w;
+    w.start(a, it, vrow);
+    const uint32_t first = it.kv_first / HK_KV8_BLOCK;
+    auto block_at = [&](uint32_t tile) {
+        return (size_t)(first + tile) * g.cache.heads + it.kv_head;
+    };
+    uint4 k[UNITS], v[UNITS];
+    auto load = [&](uint32_t tile, int which, uint4 (&to)[UNITS]) {
+        const uint4 *from =
+            (const uint4 *)(g.cache.codes +
+                            (block_at(tile) * 2u + which) *
+                                (HK_KV8_BLOCK * DIMS)) +
+            lane;
+#pragma unroll
+        for (int u = 0; u < UNITS; u++) to[u] = from[u * 64];
+    };
+    uint32_t tile = it.tile + wave;
+    if (tile < it.tile_end) {
+        load(tile, 0, k);
+        load(tile, 1, v);
+    }
+    for (; tile < it.tile_end; tile += HK_PACKED_WAVES) {
+        const float2 scale = g.cache.scales[block_at(tile)];
+        /* past the last block, that one again, which no one uses */
+        const uint32_t next =
+            tile + HK_PACKED_WAVES < it.tile_end ? tile + HK_PACKED_WAVES
+                                                 : tile;
+        hk_f32x16 s[2];
+        w.scores(s, [&](int kt, int j, uint4 (&f)[2]) {
+            hk_kv8_fragments(k[kt * ND + j], f);
+        });
+        load(next, 0, k);
+        hk_f16x8 p[2][2];
+        w.softmax(s, p, scale.x, it.kv_rows - tile * HK_KV8_BLOCK,
+                  a.scale_log2);
+        w.values(p, scale.y, [&](int kt, int d, uint4 (&f)[2]) {
+            hk_kv8_fragments(v[kt * ND + d], f);
+        });
+        load(next, 1, v);
+    }
+    /* references and sums of each row, then O scaled to the common reference
+     * (and by 1 / L for a whole item) */
+    float2 *ml = (float2 *)lds;
+    const float own = w.l + __shfl_xor(w.l, 32, 64);
+    if (half == 0) ml[wave * 32u + col] = make_float2(w.m, own);
+    __syncthreads();
+    float top = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (uint32_t i = 0; i < HK_PACKED_WAVES; i++)
+        top = fmaxf(top, ml[i * 32u + col].x);
+    const float ref = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+    for (uint32_t i = 0; i < HK_PACKED_WAVES; i++) {
+        const float2 x = ml[i * 32u + col];
+        l += __builtin_amdgcn_exp2f((x.x - ref) * a.scale_log2) * x.y;
+    }
+    const bool all = it.part == HK_PACKED_WHOLE;
+    float weight = __builtin_amdgcn_exp2f((w.m - ref) * a.scale_log2);
+    if (all) weight *= l == 0.0f ? 0.0f : 1.0f / l;
+    else if (wave == 0 && half == 0 && vrow < it.rows)
+        a.part_ml[(size_t)it.part * HK_PACKED_QB + col] = make_float2(top, l);
+    __syncthreads();
+    /* rows of DIMS F32, 16-byte chunk c of row r at c ^ (r % 8) */
+    float *mine = lds + wave * (32u * DIMS);
+#pragma unroll
+    for (int d = 0; d < ND; d++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t c = d * 8u + i * 2u + half;
+            *(float4 *)(mine + col * DIMS + ((c ^ (col & 7u)) << 2)) =
+                make_float4(w.o[d][i * 4] * weight, w.o[d][i * 4 + 1] * weight,
+                            w.o[d][i * 4 + 2] * weight,
+                            w.o[d][i * 4 + 3] * weight);
+        }
+    __syncthreads();
+    const bool whole = a.dim % 8u == 0;
+    for (uint32_t at = tid; at < 32u * DIMS / 8u; at += 256u) {
+        const uint32_t r = at / (DIMS / 8u), c = at % (DIMS / 8u) * 2u;
+        if (it.row + r >= it.rows) continue;
+        float sum[8] = {};
+#pragma unroll
+        for (uint32_t i = 0; i < HK_PACKED_WAVES; i++)
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                sum[e] += lds[i * (32u * DIMS) + r * DIMS +
+                              (((c + (e >> 2)) ^ (r & 7u)) << 2) + (e & 3)];
+        if (all) {
+            hk_kv8_put(a, it, it.row + r, c * 4u, sum, whole);
+            continue;
+        }
+        float *part = a.part_o +
+                      ((size_t)it.part * HK_PACKED_QB + r) * DP + c * 4u;
+        *(float4 *)part = make_float4(sum[0], sum[1], sum[2], sum[3]);
+        *(float4 *)(part + 4) = make_float4(sum[4], sum[5], sum[6], sum[7]);
+    }
+}
+
+/* Larger items, four waves of 32 rows: the waves make f16 of a block's codes
+ * together, in LDS, in the order of the fragments, one block ahead of the
+ * products and with the next one's codes in their registers. */
+template <int DIMS>
+__global__ void __launch_bounds__(256, 2) hk_kv8_flash(hk_kv8_args g) {
+    constexpr int ND = DIMS / 32;
+    constexpr int DP = DIMS <= 64 ? 64 : 128;
+    constexpr uint32_t STAGE = 256u * DIMS; /* bytes of a block in f16 */
+    constexpr int UNITS = DIMS / 32;        /* 16-byte pieces a thread */
+    extern __shared__ __attribute__((aligned(16))) uint8_t hk_lds[];
+    const hk_packed_args &a = g.p;
+    hk_packed_item it = a.items[blockIdx.x];
+    if (it.row >= it.rows) return;
+    if (!a.part_o && it.part != HK_PACKED_WHOLE) {
+        /* no room for pieces' sums: the first one takes all keys */
+        if (it.tile) return;
+        it.tile_end = (it.kv_rows + HK_KV8_BLOCK - 1u) / HK_KV8_BLOCK;
+        it.part = HK_PACKED_WHOLE;
+    }
+    if (it.rows - it.row <= 32u) {
+        hk_kv8_few<DIMS>(g, it, (float *)hk_lds);
+        return;
+    }
+    const uint32_t tid = threadIdx.x, lane = tid & 63u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t col = lane & 31u, half = lane >> 5;
+    const uint32_t vrow0 = it.row + wave * 32u, vrow = vrow0 + col;
+    const uint32_t first = it.kv_first / HK_KV8_BLOCK;
+    auto block_at = [&](uint32_t tile) {
+        return (size_t)(first + tile) * g.cache.heads + it.kv_head;
+    };
+    /* a block's keys and values lie together: piece u of thread t is its
+     * (256 u + t)th */
+    uint4 ahead[UNITS];
+    auto load = [&](uint32_t tile) {
+        const uint4 *from =
+            (const uint4 *)(g.cache.codes +
+                            block_at(tile) * (2u * HK_KV8_BLOCK * DIMS)) +
+            tid;
+#pragma unroll
+        for (int u = 0; u < UNITS; u++) ahead[u] = from[u * 256];
+    };
+    auto convert = [&](uint32_t stage) {
+#pragma unroll
+        for (int u = 0; u < UNITS; u++) {
+            uint4 f[2];
+            hk_kv8_fragments(ahead[u], f);
+            uint8_t *to =
+                hk_lds + stage * STAGE + (u * 4u + wave) * 2048u + lane * 16u;
+            *(uint4 *)to = f[0];
+            *(uint4 *)(to + 1024) = f[1];
+        }
+    };
+    const uint32_t n = it.tile_end - it.tile;
+    if (n) load(it.tile);
+    hk_kv8_wave<DIMS> w;
+    w.start(a, it, vrow);
+    /* a wave whose rows all lie past the request's converts its share and
+     * meets every barrier, and computes nothing */
+    const bool live = vrow0 < it.rows;
+    if (n) {
+        convert(0);
+        if (n > 1) load(it.tile + 1u);
+    }
+    __syncthreads();
+    for (uint32_t i = 0; i < n; i++) {
+        const uint32_t tile = it.tile + i;
+        const uint8_t *stage = hk_lds + (i & 1u) * STAGE + lane * 16u;
+        if (i + 1 < n) {
+            convert((i & 1u) ^ 1u);
+            load(i + 2 < n ? tile + 2u : tile);
+        }
+        if (live) {
+            const float2 scale = g.cache.scales[block_at(tile)];
+            hk_f32x16 s[2];
+            w.scores(s, [&](int kt, int j, uint4 (&f)[2]) {
+                const uint8_t *at = stage + (kt * ND + j) * 2048u;
+                f[0] = *(const uint4 *)at;
+                f[1] = *(const uint4 *)(at + 1024);
+            });
+            hk_f16x8 p[2][2];
+            w.softmax(s, p, scale.x, it.kv_rows - tile * HK_KV8_BLOCK,
+                      a.scale_log2);
+            w.values(p, scale.y, [&](int kt, int d, uint4 (&f)[2]) {
+                const uint8_t *at = stage + (2 * ND + kt * ND + d) * 2048u;
+                f[0] = *(const uint4 *)at;
+                f[1] = *(const uint4 *)(at + 1024);
+            });
+        }
+        __syncthreads();
+    }
+    const float l = w.l + __shfl_xor(w.l, 32, 64);
+    const bool all = it.part == HK_PACKED_WHOLE;
+    /* no keys, or none with weight: zeros (a NaN sum gives NaN) */
+    const float weight = !all ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+    if (!all && half == 0 && vrow < it.rows)
+        a.part_ml[(size_t)it.part * HK_PACKED_QB + wave * 32u + col] =
+            make_float2(w.m, l);
+    /* The wave's rows go through LDS of its own, 32 dims at a time in rows of
+     * 128 bytes, 16-byte chunk c of row r at c ^ (r % 8). */
+    float *mine = (float *)(hk_lds + wave * 4096u);
+    const bool whole = a.dim % 8u == 0;
+#pragma unroll
+    for (int d = 0; d < ND; d++) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            *(float4 *)(mine + col * 32u +
+                        (((i * 2u + half) ^ (col & 7u)) << 2)) =
+                make_float4(w.o[d][i * 4] * weight, w.o[d][i * 4 + 1] * weight,
+                            w.o[d][i * 4 + 2] * weight,
+                            w.o[d][i * 4 + 3] * weight);
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const uint32_t r = i * 16u + (lane >> 2), c = (lane & 3u) * 2u;
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                v[e] = mine[r * 32u + (((c + (e >> 2)) ^ (r & 7u)) << 2) +
+                            (e & 3)];
+            if (vrow0 + r >= it.rows) continue;
+            if (all) {
+                hk_kv8_put(a, it, vrow0 + r, d * 32u + c * 4u, v, whole);
+                continue;
+            }
+            float *part = a.part_o +
+                          ((size_t)it.part * HK_PACKED_QB + wave * 32u + r) *
+                              DP + d * 32u + c * 4u;
+            *(float4 *)part = make_float4(v[0], v[1], v[2], v[3]);
+            *(float4 *)(part + 4) = make_float4(v[4], v[5], v[6], v[7]);
+        }
+    }
+}
+
+template <int DIMS>
+static void hk_kv8_launch(struct h3_gpu *gpu, const hk_kv8_args &g,
+                          const uint32_t *n) {
+    /* two blocks in f16; the join of few rows' waves takes as much */
+    const uint32_t lds = 2u * 256u * DIMS;
+    const uint32_t most = 1u << 23; /* below 2^32 threads, turns of the XCDs */
+    for (uint32_t first = 0; first < n[HK_PACKED_ITEMS]; first += most) {
+        hk_kv8_args part = g;
+        part.p.items += first;
+        hipLaunchKernelGGL(hk_kv8_flash<DIMS>,
+                           dim3(std::min(n[HK_PACKED_ITEMS] - first, most)),
+                           dim3(256), lds, gpu->stream, part);
+    }
+    if (g.p.part_o)
+        hk_packed_join_pieces(gpu, g.p, n, DIMS <= 64 ? 64u : 128u);
+}
+
 /* ================================================================ ops */
 
 static int hk_kv8_require(struct h3_gpu *gpu, const h3_gpu_tensor *t) {
@@ -455,6 +966,25 @@ int h3_hip_sdpa_packed_int8_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
     a.p.o = HK_BF16(output);
     a.p.q_stride = query_stride;
     hk_op_begin(gpu, "attention_packed_int8");
+    /* (a scale of 0 times -inf, what keys past the end are set to, is no
+     * -inf) */
+    if (!gpu->reference_kernels && a.p.dim <= 128u &&
+        a.p.scale_log2 > 0x1p-100f && isfinite(a.p.scale_log2)) {
+        const size_t padded = a.p.dim <= 64u ? 64u : 128u;
+        const size_t rows = (size_t)n[HK_PACKED_PARTS] * HK_PACKED_QB;
+        if (rows)
+            a.p.part_o = (float *)hk_splitk_try(
+                gpu, rows * (padded * sizeof(float) + sizeof(float2)));
+        /* without scratch, items run whole */
+        if (a.p.part_o) a.p.part_ml = (float2 *)(a.p.part_o + rows * padded);
+        switch (a.cache.padded) {
+        case 32: hk_kv8_launch<32>(gpu, a, n); break;
+        case 64: hk_kv8_launch<64>(gpu, a, n); break;
+        case 96: hk_kv8_launch<96>(gpu, a, n); break;
+        default: hk_kv8_launch<128>(gpu, a, n);
+        }
+        return hk_op_end(gpu, "attention_packed_int8", HK_KIND_SDPA);
+    }
     const uint64_t blocks = ((uint64_t)a.p.rows * a.p.heads + 3) / 4;
     hipLaunchKernelGGL(
         hk_kv8_simple,

@@ -209,17 +209,18 @@ def attention(q, cache, ranges, heads, kv_heads, dim, scale):
             p = np.exp(s - s.max(1, keepdims=True))
             p /= p.sum(1, keepdims=True)
             o[qf:qf + qn, h] = p @ vs
-            # a score: the products' sum (each row of q also loses at most
-            # 2^-25 of its largest magnitude where f16 holds it), the scales,
-            # doubtful codes, the rounding of the exponent's argument
+            # a score: the products' sum (f16 holds a row of q, scaled to
+            # 2^13, but for what is under 2^-25 there), the scales, doubtful
+            # codes, the rounding of the exponent's argument
             top = np.abs(qs).max(1, keepdims=True)
             off = ((dim + 6) * F32 * (np.abs(qs) @ np.abs(ks).T) +
-                   2.0 ** -24 * top * np.abs(ks).sum(1) +
+                   2.0 ** -38 * top * np.abs(ks).sum(1) +
                    np.abs(qs) @ dk.T).max(1, keepdims=True) * scale + \
                 2.0 ** -22
-            # P rounds to f16 or, below 2^-14 of its largest, by 2^-25
+            # P rounds to 11 bits, or by 2^-25 at most, lifted by 2^7 against a
+            # reference that is at most the largest
             bound[qf:qf + qn, h] = (p @ np.abs(vs)) * (
                 2.0 ** -11 + 2 * np.expm1(off) + 2 * (kn + 64) * F32) + \
-                p @ dv + 2.0 ** -25 * p.max(1, keepdims=True) * \
+                p @ dv + 2.0 ** -32 * p.max(1, keepdims=True) * \
                 np.abs(vs).sum(0)
     return o, rounded(o, bound), covered
