@@ -79,16 +79,41 @@ struct hk_kv8_store_args {
     hk_kv8_range ranges[HK_KV8_RANGES];
 };
 
-/* One workgroup per block and head: the largest magnitudes of the block's new
- * rows, then the codes, 16 at a time.  Rows that the block has before the new
- * ones keep their codes unless the scale grows, rows behind become zeros. */
+/* A thread's piece of a block's keys or values: eight dims, from `dim` on, of
+ * four rows, from `row` on.  Its codes are whole words of either order: four
+ * dims of a row, four rows of a dim. */
+struct hk_kv8_piece {
+    uint32_t row, dim;
+    __device__ __forceinline__ hk_kv8_piece(uint32_t at, uint32_t padded) {
+        row = at / (padded >> 3) * 4u;
+        dim = at % (padded >> 3) * 8u;
+    }
+};
+
+/* The image of a block's keys or values in LDS, as the cache has it, but that
+ * 16-byte piece p lies at p ^ (p / 8 % 8): the words that threads write and
+ * read at a time lie 16 bytes apart, over few banks. */
+__device__ __forceinline__ uint32_t hk_kv8_image(uint32_t byte) {
+    return byte ^ ((byte >> 3) & 0x70u);
+}
+
+/* One workgroup per block, head and one of keys and values: the new rows into
+ * registers, their largest magnitude, the codes by way of the block's image in
+ * LDS, whole lines to the cache.  A block whose first row is new takes its
+ * scale from the new rows and zeros in the others; in any other its rows keep
+ * their codes unless the scale grows, and where it does not, the new rows'
+ * bytes alone are written. */
 __global__ void __launch_bounds__(256) hk_kv8_store(hk_kv8_store_args a) {
     __shared__ uint32_t tops[16];
+    extern __shared__ __attribute__((aligned(16))) uint8_t image[];
     const hk_kv8_cache &c = a.cache;
-    uint32_t i = 0;
-    while (i + 1 < a.count && a.ranges[i + 1].before <= blockIdx.x) i++;
-    const hk_kv8_range r = a.ranges[i];
-    const uint32_t head = blockIdx.y;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u;
+    /* the last range that begins at or before the launch's block, a lane for
+     * each (64 of them): scalar loads one after the other took 3 us */
+    const uint64_t begun = __builtin_amdgcn_ballot_w64(
+        lane < a.count && a.ranges[lane].before <= blockIdx.x);
+    const hk_kv8_range r = a.ranges[__popcll(begun) - 1];
+    const uint32_t head = blockIdx.y, which = blockIdx.z;
     const uint32_t block = r.cache / HK_KV8_BLOCK + (blockIdx.x - r.before);
     /* rows [r0, r1) of the block are new, from row `from` on */
     const uint64_t row0 = (uint64_t)block * HK_KV8_BLOCK;
@@ -97,63 +122,200 @@ __global__ void __launch_bounds__(256) hk_kv8_store(hk_kv8_store_args a) {
     const uint32_t r1 = end < HK_KV8_BLOCK ? (uint32_t)end : HK_KV8_BLOCK;
     const uint64_t from = (uint64_t)r.source + (row0 + r0 - r.cache);
     const uint32_t part = HK_KV8_BLOCK * c.padded;
+    const uint32_t pieces = part / 32u;
     const size_t at = (size_t)block * c.heads + head;
-    for (int which = 0; which < 2; which++) {
-        const uint16_t *x = (which ? a.value : a.key) + from * a.stride +
-                            (uint64_t)head * c.dim;
-        uint32_t most = 0;
-        for (uint32_t e = threadIdx.x; e < (r1 - r0) * c.dim; e += 256u) {
-            const uint32_t row = e / c.dim;
-            most = max(most, hk_magnitude(hk_bf2f(
-                                 x[row * a.stride + (e - row * c.dim)])));
-        }
-        most = hk_block_umax(most, tops);
-        float *scale = (float *)(c.scales + at) + which;
-        const float old = r0 ? *scale : 0.0f;
-        __syncthreads(); /* everyone has it */
-        hk_int8_quantizer code(most);
-        float keep = 1.0f;
-        if (r0 && !(old < code.scale)) {
-            /* the block's scale holds (also where it is NaN) */
-            if (!isnan(code.scale))
-                code = hk_int8_quantizer(hk_magnitude(127.0f * old));
-            if (isnan(old)) code = hk_int8_quantizer(HK_NOT_FINITE);
-            if (!isnan(code.scale)) code.scale = old;
-        } else if (r0) {
-            keep = old / code.scale;
-        }
-        uint8_t *out = c.codes + (at * 2u + which) * part;
-        for (uint32_t u = threadIdx.x; u < part / 16u; u += 256u) {
-            uint4 had = make_uint4(0, 0, 0, 0);
-            if (r0) had = *(const uint4 *)(out + u * 16u);
-            const uint32_t words[4] = {had.x, had.y, had.z, had.w};
-            const uint32_t lane = u & 63u;
-            const uint32_t dim32 = (u >> 6) % (c.padded >> 5) * 32u;
-            const uint32_t row32 = (u >> 6) / (c.padded >> 5) * 32u;
-            uint32_t made[4];
-            for (uint32_t b = 0; b < 16u; b++) {
-                const uint32_t row =
-                    row32 + (which ? 16u * (b >> 3) + 8u * ((b >> 2) & 1u) +
-                                         4u * (lane >> 5) + (b & 3u)
-                                   : lane & 31u);
-                const uint32_t dim =
-                    dim32 + (which ? lane & 31u : 16u * (lane >> 5) + b);
-                int v = 0;
-                if (row >= r0 && row < r1 && dim < c.dim) {
-                    v = (int)code(hk_bf2f(x[(row - r0) * a.stride + dim]));
-                } else if (row < r0) {
-                    v = (int)((words[b >> 2] >> (8u * (b & 3u))) & 255u) - 128;
-                    if (keep < 1.0f) v = (int)rintf((float)v * keep);
+    const uint16_t *x = (which ? a.value : a.key) + from * a.stride +
+                        (uint64_t)head * c.dim;
+    const bool whole = c.dim % 8u == 0 && a.stride % 8u == 0 &&
+                       ((uintptr_t)(which ? a.value : a.key) & 15u) == 0;
+    float *scale = (float *)(c.scales + at) + which;
+    const float old = r0 ? *scale : 0.0f;
+    /* up to 512 pieces: two a thread */
+    uint4 rows[2][4];
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const hk_kv8_piece p(tid + k * 256u, c.padded);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            const uint32_t row = p.row + e;
+            if (tid + k * 256u < pieces && row >= r0 && row < r1 &&
+                p.dim < c.dim) {
+                const uint16_t *y = x + (row - r0) * a.stride + p.dim;
+                if (whole) {
+                    v = *(const uint4 *)y;
+                } else {
+                    uint32_t w[4] = {};
+#pragma unroll
+                    for (int d = 0; d < 8; d++)
+                        if (p.dim + d < c.dim)
+                            w[d >> 1] |= (uint32_t)y[d] << (16 * (d & 1));
+                    v = make_uint4(w[0], w[1], w[2], w[3]);
                 }
-                const uint32_t byte = (uint32_t)(v + 128) << (8u * (b & 3u));
-                made[b >> 2] = b & 3u ? made[b >> 2] | byte : byte;
             }
-            *(uint4 *)(out + u * 16u) =
-                make_uint4(made[0], made[1], made[2], made[3]);
+            rows[k][e] = v;
         }
-        if (threadIdx.x == 0) *scale = code.scale;
+    }
+    uint32_t most = 0;
+#pragma unroll
+    for (int k = 0; k < 2; k++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            float f[8];
+            hk_unpack8(rows[k][e], f);
+#pragma unroll
+            for (int d = 0; d < 8; d++) most = max(most, hk_magnitude(f[d]));
+        }
+    most = hk_block_umax(most, tops); /* (everyone has the old scale by then) */
+    hk_int8_quantizer code(most);
+    float keep = 1.0f;
+    if (r0 && !(old < code.scale)) {
+        /* the block's scale holds (also where it is NaN) */
+        if (!isnan(code.scale))
+            code = hk_int8_quantizer(hk_magnitude(127.0f * old));
+        if (isnan(old)) code = hk_int8_quantizer(HK_NOT_FINITE);
+        if (!isnan(code.scale)) code.scale = old;
+    } else if (r0) {
+        keep = old / code.scale;
+    }
+    if (tid == 0) *scale = code.scale;
+    uint8_t *out = c.codes + (at * 2u + which) * part;
+    /* (the same for the whole workgroup) */
+    const bool few = r0 && !(keep < 1.0f);
+    if (r0 && !few) {
+        for (uint32_t u = tid; u < part / 16u; u += 256u) {
+            const uint4 had = *(const uint4 *)(out + u * 16u);
+            uint32_t w[4] = {had.x, had.y, had.z, had.w};
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                float f[4];
+#pragma unroll
+                for (int b = 0; b < 4; b++)
+                    f[b] = rintf((float)((int)((w[j] >> (8 * b)) & 255u) -
+                                         128) * keep) + 128.0f;
+                w[j] = hk_int8_pack4(f[0], f[1], f[2], f[3]);
+            }
+            *(uint4 *)(image + hk_kv8_image(u * 16u)) =
+                make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const hk_kv8_piece p(tid + k * 256u, c.padded);
+        /* none of its rows are new, nor to be cleared */
+        if (tid + k * 256u >= pieces ||
+            (r0 && (p.row + 4u <= r0 || p.row >= r1)))
+            continue;
+        float f[4][8];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            hk_unpack8(rows[k][e], f[e]);
+#pragma unroll
+            for (int d = 0; d < 8; d++) f[e][d] = code(f[e][d]) + 128.0f;
+        }
+        uint8_t *to = few ? out : image;
+        auto place = [&](uint32_t byte) {
+            return few ? byte : hk_kv8_image(byte);
+        };
+        const bool all = !r0 || (p.row >= r0 && p.row + 4u <= r1);
+        if (which == 0) {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (all || (p.row + e >= r0 && p.row + e < r1))
+                    *(uint2 *)(to + place(hk_kv8_key_at(p.row + e, p.dim,
+                                                        c.padded))) =
+                        make_uint2(hk_int8_pack4(f[e][0], f[e][1], f[e][2],
+                                                 f[e][3]),
+                                   hk_int8_pack4(f[e][4], f[e][5], f[e][6],
+                                                 f[e][7]));
+            continue;
+        }
+#pragma unroll
+        for (int d = 0; d < 8; d++) {
+            uint8_t *word =
+                to + place(hk_kv8_value_at(p.row, p.dim + d, c.padded));
+            const uint32_t w =
+                hk_int8_pack4(f[0][d], f[1][d], f[2][d], f[3][d]);
+            if (all) {
+                *(uint32_t *)word = w;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (p.row + e >= r0 && p.row + e < r1)
+                        word[e] = (uint8_t)(w >> (8 * e));
+            }
+        }
+    }
+    if (few) return;
+    __syncthreads();
+    for (uint32_t u = tid; u < part / 16u; u += 256u)
+        *(uint4 *)(out + u * 16u) =
+            *(const uint4 *)(image + hk_kv8_image(u * 16u));
+}
+
+/* The values of rows [first, + rows), one workgroup per block, head and one of
+ * keys and values, by way of the block's image in LDS. */
+__global__ void __launch_bounds__(256)
+hk_kv8_read(hk_kv8_cache c, uint16_t *key, uint16_t *value, uint32_t first,
+            uint32_t rows) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t image[];
+    const uint32_t block = first / HK_KV8_BLOCK + blockIdx.x;
+    const uint32_t head = blockIdx.y, which = blockIdx.z, tid = threadIdx.x;
+    const size_t at = (size_t)block * c.heads + head;
+    const uint32_t part = HK_KV8_BLOCK * c.padded;
+    const uint8_t *codes = c.codes + (at * 2u + which) * part;
+    const float scale = ((const float *)(c.scales + at))[which];
+    const uint64_t row0 = (uint64_t)block * HK_KV8_BLOCK;
+    for (uint32_t u = tid; u < part / 16u; u += 256u)
+        *(uint4 *)(image + hk_kv8_image(u * 16u)) =
+            *(const uint4 *)(codes + u * 16u);
+    __syncthreads();
+    for (uint32_t k = tid; k < part / 32u; k += 256u) {
+        const hk_kv8_piece p(k, c.padded);
+        float f[4][8];
+        auto value_of = [&](uint32_t word, int byte) {
+            return ((float)((word >> (8 * byte)) & 255u) - 128.0f) * scale;
+        };
+        if (which == 0) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const uint2 w = *(const uint2 *)(
+                    image +
+                    hk_kv8_image(hk_kv8_key_at(p.row + e, p.dim, c.padded)));
+#pragma unroll
+                for (int d = 0; d < 8; d++)
+                    f[e][d] = value_of(d < 4 ? w.x : w.y, d & 3);
+            }
+        } else {
+#pragma unroll
+            for (int d = 0; d < 8; d++) {
+                const uint32_t w = *(const uint32_t *)(
+                    image +
+                    hk_kv8_image(hk_kv8_value_at(p.row, p.dim + d, c.padded)));
+#pragma unroll
+                for (int e = 0; e < 4; e++) f[e][d] = value_of(w, e);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const uint64_t row = row0 + p.row + e;
+            if (row < first || row >= (uint64_t)first + rows || p.dim >= c.dim)
+                continue;
+            uint16_t *to = (which ? value : key) +
+                           ((row - first) * c.heads + head) * c.dim + p.dim;
+            if (c.dim % 8u == 0) {
+                *(uint4 *)to = hk_pack8(f[e]);
+            } else {
+#pragma unroll
+                for (int d = 0; d < 8; d++)
+                    if (p.dim + d < c.dim) to[d] = hk_f2bf(f[e][d]);
+            }
+        }
     }
 }
+
+/* ---------------------------------------------------------- the attention */
 
 __device__ __forceinline__ float hk_kv8_key(const hk_kv8_cache &c,
                                             const uint8_t *codes, uint32_t row,
@@ -168,28 +330,6 @@ __device__ __forceinline__ float hk_kv8_value(const hk_kv8_cache &c,
                               hk_kv8_value_at(row, dim, c.padded)] -
                    128);
 }
-
-/* The values of rows [first, + rows), one workgroup per block and head. */
-__global__ void __launch_bounds__(256)
-hk_kv8_read(hk_kv8_cache c, uint16_t *key, uint16_t *value, uint32_t first,
-            uint32_t rows) {
-    const uint32_t block = first / HK_KV8_BLOCK + blockIdx.x;
-    const uint32_t head = blockIdx.y;
-    const size_t at = (size_t)block * c.heads + head;
-    const uint8_t *codes = c.codes + at * 2u * HK_KV8_BLOCK * c.padded;
-    const float2 scale = c.scales[at];
-    const uint64_t row0 = (uint64_t)block * HK_KV8_BLOCK;
-    for (uint32_t e = threadIdx.x; e < HK_KV8_BLOCK * c.dim; e += 256u) {
-        const uint32_t row = e / c.dim, dim = e - row * c.dim;
-        if (row0 + row < first || row0 + row >= (uint64_t)first + rows)
-            continue;
-        const size_t to = ((row0 + row - first) * c.heads + head) * c.dim + dim;
-        key[to] = hk_f2bf(hk_kv8_key(c, codes, row, dim) * scale.x);
-        value[to] = hk_f2bf(hk_kv8_value(c, codes, row, dim) * scale.y);
-    }
-}
-
-/* ---------------------------------------------------------- the attention */
 
 struct hk_kv8_args {
     hk_packed_args p;
@@ -261,14 +401,19 @@ __global__ void __launch_bounds__(256) hk_kv8_simple(hk_kv8_args g) {
  * The plan's items (hk_packed.h), a block of 64 keys a tile: S^T = K . Q^T with
  * the Q fragments in registers, the softmax in the lanes that hold a query's
  * scores, O^T = V^T . P^T.  Codes and P are f16, which holds codes exactly and
- * is made of them in two instructions a pair; scores are multiplied by the
- * block's key scale, the block's product by its value scale as it is added to
- * O.  A query row is scaled by a power of two of its own to f16's range, which
- * loses nothing of a bf16 within 2^27 of the row's largest.
+ * is made of them in two instructions a pair.  A query row is scaled by a power
+ * of two of its own to f16's range, which loses nothing of a bf16 within 2^27
+ * of the row's largest; that and the block's key scale go into the factor of
+ * the exponent.
  *
  * P = 2^((s - m) L + 7) against a reference m (a score, L = scale log2(e)) that
  * moves when a lane's sum of P passes 2^15: so f16 holds every P, to 11 bits
- * those over 2^-21 of the largest; the factor 2^7 is in the sums too. */
+ * those over 2^-21 of the largest; the factor 2^7 is in the sums too.  A
+ * block's product is multiplied by its value scale as it is added to O: 64
+ * multiply-adds a lane.  (Taken into the exponents, with O in the largest scale
+ * of the item's blocks, they went, but the scales had to be looked through
+ * first and blocks far below them have a loop of their own, and four clips of
+ * 6144 rows took 230 us for 224.) */
 typedef _Float16 hk_f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 hk_f16x8 __attribute__((ext_vector_type(8)));
 
@@ -365,18 +510,21 @@ template <int DIMS> struct hk_kv8_wave {
         l = 0.0f;
     }
 
-    /* Scores (of products with the codes) to P, with the block's key scale;
-     * `keys` of the block's rows count. */
+    /* Raw scores (products with the codes) to P; `keys` of the block's rows
+     * count. */
     __device__ __forceinline__ void softmax(hk_f32x16 (&s)[2],
-                                            hk_f16x8 (&p)[2][2], float scale,
-                                            uint32_t keys, float L) {
+                                            hk_f16x8 (&p)[2][2],
+                                            float scale, uint32_t keys,
+                                            float L) {
         const uint32_t half = (threadIdx.x & 63u) >> 5;
-        const float by = q_scale * scale;
-#pragma unroll
-        for (int kt = 0; kt < 2; kt++)
-#pragma unroll
-            for (int r = 0; r < 16; r++) s[kt][r] *= by;
+        /* a row or block of zeros: scores of 0, whatever multiplies them, and
+         * -inf stays -inf */
+        float by = q_scale * scale;
+        if (by == 0.0f) by = 0x1p-100f;
+        float own = by * L;
+        if (own == 0.0f) own = 0x1p-126f;
         if (keys < HK_KV8_BLOCK) {
+            asm volatile(""); /* a branch, not 32 selects in every block */
 #pragma unroll
             for (int kt = 0; kt < 2; kt++)
 #pragma unroll
@@ -392,7 +540,7 @@ template <int DIMS> struct hk_kv8_wave {
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
                     const float e = __builtin_amdgcn_exp2f(
-                        __builtin_fmaf(s[kt][r], L, less));
+                        __builtin_fmaf(s[kt][r], own, less));
                     sum += e;
                     p[kt][r >> 3][r & 7] = (_Float16)e;
                 }
@@ -412,6 +560,7 @@ template <int DIMS> struct hk_kv8_wave {
             for (int kt = 0; kt < 2; kt++)
 #pragma unroll
                 for (int r = 0; r < 16; r++) mx = fmaxf(mx, s[kt][r]);
+            mx *= by;
             const auto sw = __builtin_amdgcn_permlane32_swap(
                 __float_as_uint(mx), __float_as_uint(mx), false, false);
             mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
@@ -423,11 +572,18 @@ template <int DIMS> struct hk_kv8_wave {
             neg = -(now * L);
             float less = -(ref * L);
             if (__builtin_amdgcn_ballot_w64(hk_kv8_far(less))) {
+                /* scores as they are, rounded as the reference was, and the
+                 * reference off them first, which is exact near it */
                 const float off = hk_kv8_far(less) ? ref : 0.0f;
 #pragma unroll
                 for (int kt = 0; kt < 2; kt++)
 #pragma unroll
-                    for (int r = 0; r < 16; r++) s[kt][r] -= off;
+                    for (int r = 0; r < 16; r++) {
+                        float x = s[kt][r] * by;
+                        asm volatile("" : "+v"(x)); /* no fused add */
+                        s[kt][r] = x - off;
+                    }
+                own = L;
                 if (hk_kv8_far(less)) less = 0.0f;
             }
             l *= c;
@@ -440,7 +596,7 @@ template <int DIMS> struct hk_kv8_wave {
         l += sum;
     }
 
-    /* o[d] += scale * the block's product, two groups of 32 dims at a time */
+    /* o += scale * the block's product, two groups of 32 dims at a time */
     template <typename F>
     __device__ __forceinline__ void values(const hk_f16x8 (&p)[2][2],
                                            float scale, F fragments) {
@@ -471,8 +627,9 @@ template <int DIMS> struct hk_kv8_wave {
         }
     }
 
-    template <typename F>
-    __device__ __forceinline__ void scores(hk_f32x16 (&s)[2], F fragments) {
+    template <typename Q, typename F>
+    __device__ __forceinline__ void scores(hk_f32x16 (&s)[2], Q query,
+                                           F fragments) {
 #pragma unroll
         for (int kt = 0; kt < 2; kt++)
 #pragma unroll
@@ -483,8 +640,8 @@ template <int DIMS> struct hk_kv8_wave {
             for (int kt = 0; kt < 2; kt++) {
                 uint4 f[2];
                 fragments(kt, j, f);
-                s[kt] = hk_kv8_mfma(f[0], q[2 * j], s[kt]);
-                s[kt] = hk_kv8_mfma(f[1], q[2 * j + 1], s[kt]);
+                s[kt] = hk_kv8_mfma(f[0], query(2 * j), s[kt]);
+                s[kt] = hk_kv8_mfma(f[1], query(2 * j + 1), s[kt]);
             }
     }
 };
@@ -506,22 +663,36 @@ __device__ __forceinline__ void hk_kv8_put(const hk_packed_args &a,
         if (dim + e < a.dim) to[e] = hk_f2bf(v[e]);
 }
 
-/* An item of at most 32 rows: the waves share its rows and split its blocks,
+/* The item of a workgroup, if its rows are few or many; false: nothing to do. */
+__device__ __forceinline__ bool hk_kv8_item(const hk_packed_args &a, bool few,
+                                            hk_packed_item &it) {
+    it = a.items[blockIdx.x];
+    if (it.row >= it.rows || (it.rows - it.row <= 32u) != few) return false;
+    if (!a.part_o && it.part != HK_PACKED_WHOLE) {
+        /* no room for pieces' sums: the first one takes all keys */
+        if (it.tile) return false;
+        it.tile_end = (it.kv_rows + HK_KV8_BLOCK - 1u) / HK_KV8_BLOCK;
+        it.part = HK_PACKED_WHOLE;
+    }
+    return true;
+}
+
+/* Items of at most 32 rows: the waves share the rows and split the blocks,
  * wave w every fourth from the wth on, each straight from the cache into its
  * registers; then their sums are joined. */
 template <int DIMS>
-__device__ __forceinline__ void hk_kv8_few(const hk_kv8_args &g,
-                                           const hk_packed_item &it,
-                                           float *lds) {
+__global__ void __launch_bounds__(256, 2) hk_kv8_few(hk_kv8_args g) {
     constexpr int ND = DIMS / 32, UNITS = DIMS / 16; /* of K or V */
     constexpr int DP = DIMS <= 64 ? 64 : 128;
+    extern __shared__ __attribute__((aligned(16))) uint8_t hk_lds[];
+    float *lds = (float *)hk_lds;
     const hk_packed_args &a = g.p;
+    hk_packed_item it;
+    if (!hk_kv8_item(a, true, it)) return;
     const uint32_t tid = threadIdx.x, lane = tid & 63u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t col = lane & 31u, half = lane >> 5;
     const uint32_t vrow = it.row + col;
-    hk_kv8_wave<DIMS> w;
-    w.start(a, it, vrow);
     const uint32_t first = it.kv_first / HK_KV8_BLOCK;
     auto block_at = [&](uint32_t tile) {
         return (size_t)(first + tile) * g.cache.heads + it.kv_head;
@@ -537,20 +708,35 @@ __device__ __forceinline__ void hk_kv8_few(const hk_kv8_args &g,
         for (int u = 0; u < UNITS; u++) to[u] = from[u * 64];
     };
     uint32_t tile = it.tile + wave;
+    float2 ahead = make_float2(0.0f, 0.0f);
     if (tile < it.tile_end) {
+        ahead = g.cache.scales[block_at(tile)];
         load(tile, 0, k);
         load(tile, 1, v);
     }
+    hk_kv8_wave<DIMS> w;
+    w.start(a, it, vrow);
+    /* the queries, the same for all waves, wait in LDS: in registers beside a
+     * block's keys and values they spilled */
+    hk_f16x8 *queries = (hk_f16x8 *)lds + lane;
+    if (wave == 0) {
+#pragma unroll
+        for (int i = 0; i < DIMS / 16; i++) queries[i * 64] = w.q[i];
+    }
+    __syncthreads();
     for (; tile < it.tile_end; tile += HK_PACKED_WAVES) {
-        const float2 scale = g.cache.scales[block_at(tile)];
+        const float2 scale = ahead;
         /* past the last block, that one again, which no one uses */
         const uint32_t next =
             tile + HK_PACKED_WAVES < it.tile_end ? tile + HK_PACKED_WAVES
                                                  : tile;
         hk_f32x16 s[2];
-        w.scores(s, [&](int kt, int j, uint4 (&f)[2]) {
-            hk_kv8_fragments(k[kt * ND + j], f);
-        });
+        w.scores(
+            s, [&](int i) { return queries[i * 64]; },
+            [&](int kt, int j, uint4 (&f)[2]) {
+                hk_kv8_fragments(k[kt * ND + j], f);
+            });
+        ahead = g.cache.scales[block_at(next)];
         load(next, 0, k);
         hk_f16x8 p[2][2];
         w.softmax(s, p, scale.x, it.kv_rows - tile * HK_KV8_BLOCK,
@@ -562,6 +748,7 @@ __device__ __forceinline__ void hk_kv8_few(const hk_kv8_args &g,
     }
     /* references and sums of each row, then O scaled to the common reference
      * (and by 1 / L for a whole item) */
+    __syncthreads();
     float2 *ml = (float2 *)lds;
     const float own = w.l + __shfl_xor(w.l, 32, 64);
     if (half == 0) ml[wave * 32u + col] = make_float2(w.m, own);
@@ -628,18 +815,8 @@ __global__ void __launch_bounds__(256, 2) hk_kv8_flash(hk_kv8_args g) {
     constexpr int UNITS = DIMS / 32;        /* 16-byte pieces a thread */
     extern __shared__ __attribute__((aligned(16))) uint8_t hk_lds[];
     const hk_packed_args &a = g.p;
-    hk_packed_item it = a.items[blockIdx.x];
-    if (it.row >= it.rows) return;
-    if (!a.part_o && it.part != HK_PACKED_WHOLE) {
-        /* no room for pieces' sums: the first one takes all keys */
-        if (it.tile) return;
-        it.tile_end = (it.kv_rows + HK_KV8_BLOCK - 1u) / HK_KV8_BLOCK;
-        it.part = HK_PACKED_WHOLE;
-    }
-    if (it.rows - it.row <= 32u) {
-        hk_kv8_few<DIMS>(g, it, (float *)hk_lds);
-        return;
-    }
+    hk_packed_item it;
+    if (!hk_kv8_item(a, false, it)) return;
     const uint32_t tid = threadIdx.x, lane = tid & 63u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t col = lane & 31u, half = lane >> 5;
@@ -671,7 +848,11 @@ __global__ void __launch_bounds__(256, 2) hk_kv8_flash(hk_kv8_args g) {
         }
     };
     const uint32_t n = it.tile_end - it.tile;
-    if (n) load(it.tile);
+    float2 ahead_scale = make_float2(0.0f, 0.0f);
+    if (n) {
+        ahead_scale = g.cache.scales[block_at(it.tile)];
+        load(it.tile);
+    }
     hk_kv8_wave<DIMS> w;
     w.start(a, it, vrow);
     /* a wave whose rows all lie past the request's converts its share and
@@ -685,18 +866,21 @@ __global__ void __launch_bounds__(256, 2) hk_kv8_flash(hk_kv8_args g) {
     for (uint32_t i = 0; i < n; i++) {
         const uint32_t tile = it.tile + i;
         const uint8_t *stage = hk_lds + (i & 1u) * STAGE + lane * 16u;
+        const float2 scale = ahead_scale;
         if (i + 1 < n) {
             convert((i & 1u) ^ 1u);
+            ahead_scale = g.cache.scales[block_at(tile + 1u)];
             load(i + 2 < n ? tile + 2u : tile);
         }
         if (live) {
-            const float2 scale = g.cache.scales[block_at(tile)];
             hk_f32x16 s[2];
-            w.scores(s, [&](int kt, int j, uint4 (&f)[2]) {
-                const uint8_t *at = stage + (kt * ND + j) * 2048u;
-                f[0] = *(const uint4 *)at;
-                f[1] = *(const uint4 *)(at + 1024);
-            });
+            w.scores(
+                s, [&](int k) { return w.q[k]; },
+                [&](int kt, int j, uint4 (&f)[2]) {
+                    const uint8_t *at = stage + (kt * ND + j) * 2048u;
+                    f[0] = *(const uint4 *)at;
+                    f[1] = *(const uint4 *)(at + 1024);
+                });
             hk_f16x8 p[2][2];
             w.softmax(s, p, scale.x, it.kv_rows - tile * HK_KV8_BLOCK,
                       a.scale_log2);
@@ -759,9 +943,14 @@ static void hk_kv8_launch(struct h3_gpu *gpu, const hk_kv8_args &g,
     for (uint32_t first = 0; first < n[HK_PACKED_ITEMS]; first += most) {
         hk_kv8_args part = g;
         part.p.items += first;
-        hipLaunchKernelGGL(hk_kv8_flash<DIMS>,
-                           dim3(std::min(n[HK_PACKED_ITEMS] - first, most)),
-                           dim3(256), lds, gpu->stream, part);
+        const dim3 grid(std::min(n[HK_PACKED_ITEMS] - first, most));
+        /* (a workgroup whose item is the other kernel's ends at once) */
+        if (n[HK_PACKED_MANY])
+            hipLaunchKernelGGL(hk_kv8_flash<DIMS>, grid, dim3(256), lds,
+                               gpu->stream, part);
+        if (n[HK_PACKED_FEW])
+            hipLaunchKernelGGL(hk_kv8_few<DIMS>, grid, dim3(256), lds,
+                               gpu->stream, part);
     }
     if (g.p.part_o)
         hk_packed_join_pieces(gpu, g.p, n, DIMS <= 64 ? 64u : 128u);
@@ -856,13 +1045,13 @@ int h3_hip_kv_int8_store(h3_gpu *gpu, h3_gpu_tensor *cache,
     a.key = HK_CBF16(key) + key_offset;
     a.value = HK_CBF16(value) + value_offset;
     a.stride = kv_stride;
-    /* launches of up to 64 ranges and 2^23 / heads blocks */
-    const uint32_t most = std::max(1u, (1u << 23) / c.heads);
+    /* launches of up to 64 ranges and 2^22 / heads blocks */
+    const uint32_t most = std::max(1u, (1u << 22) / c.heads);
     uint32_t total = 0;
     auto launch = [&]() {
         if (a.count)
-            hipLaunchKernelGGL(hk_kv8_store, dim3(total, c.heads), dim3(256),
-                               0, gpu->stream, a);
+            hipLaunchKernelGGL(hk_kv8_store, dim3(total, c.heads, 2), dim3(256),
+                               HK_KV8_BLOCK * c.padded, gpu->stream, a);
         a.count = total = 0;
     };
     for (hk_kv8_range r : ranges) {
@@ -902,7 +1091,7 @@ int h3_hip_kv_int8_read(h3_gpu *gpu, h3_gpu_tensor *key, h3_gpu_tensor *value,
         return hk_fail(gpu, "cache read: keys and values need a tensor each");
     if (!rows) return 1;
     hk_op_begin(gpu, "kv_int8_read");
-    const size_t most = std::max(1u, (1u << 23) / c.heads) * HK_KV8_BLOCK;
+    const size_t most = std::max(1u, (1u << 22) / c.heads) * HK_KV8_BLOCK;
     for (uint64_t done = 0; done < rows;) {
         const uint32_t at = (uint32_t)(first_row + done);
         const uint32_t n = (uint32_t)std::min<uint64_t>(
@@ -910,8 +1099,9 @@ int h3_hip_kv_int8_read(h3_gpu *gpu, h3_gpu_tensor *key, h3_gpu_tensor *value,
         hipLaunchKernelGGL(
             hk_kv8_read,
             dim3((at % HK_KV8_BLOCK + n + HK_KV8_BLOCK - 1u) / HK_KV8_BLOCK,
-                 c.heads),
-            dim3(256), 0, gpu->stream, c, HK_BF16(key) + done * width,
+                 c.heads, 2),
+            dim3(256), HK_KV8_BLOCK * c.padded, gpu->stream, c,
+            HK_BF16(key) + done * width,
             HK_BF16(value) + done * width, at, n);
         done += n;
     }

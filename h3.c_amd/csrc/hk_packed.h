@@ -45,7 +45,8 @@ enum { HK_PACKED_HEADS, HK_PACKED_KV_HEADS, HK_PACKED_DIM,
        HK_PACKED_JOINS,    /* requests, items, joins */
        HK_PACKED_JOIN_ROWS, /* the most virtual rows of a join */
        HK_PACKED_PARTS,
-       HK_PACKED_OFF_BLOCKS /* a request's keys begin inside 64 rows */ };
+       HK_PACKED_OFF_BLOCKS, /* a request's keys begin inside 64 rows */
+       HK_PACKED_FEW, HK_PACKED_MANY /* items of up to 32 rows, and over */ };
 
 struct hk_packed_args {
     const uint16_t *q, *k, *v;

@@ -1207,6 +1207,10 @@ h3_gpu_tensor *h3_hip_sdpa_packed_plan(h3_gpu *gpu, const uint32_t *q_first,
         plan->record.n[HK_PACKED_JOIN_ROWS] = work.join_rows;
         plan->record.n[HK_PACKED_PARTS] = work.parts;
         plan->record.n[HK_PACKED_OFF_BLOCKS] = off_blocks;
+        for (const hk_packed_item &item : work.items)
+            if (item.row < item.rows)
+                plan->record.n[item.rows - item.row <= 32u ? HK_PACKED_FEW
+                                                           : HK_PACKED_MANY]++;
         return plan;
     } catch (const std::bad_alloc &) {
         hk_fail(gpu, "out of host memory");

@@ -422,14 +422,13 @@ int h3_hip_mlp_int8_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
  * ranges (host arrays, read before the call returns).  In their tensors, head
  * h of row r starts at element offset + r kv_stride + h head_dim, as for
  * h3_hip_sdpa_packed_bf16.  Ranges must not write into one block.
- * In a block that a range fills from its first row on, the scales are those of
- * the new rows alone, whatever the block held.  A range that begins inside a
- * block goes on behind the rows before it: they stay, and where the new rows
- * are larger the scale grows to max|new| / 127 and the earlier codes become
- * round(code * scale / new scale).  Rows of a range's last block behind its
- * end are cleared.  An infinity or a NaN makes its block's scale a NaN, and the
- * results of the queries that read the block: rows that no query is to read
- * are not to be stored.
+ * In a block whose first row is among a range's, the scales are those of the
+ * new rows alone, whatever the block held, and rows behind the range's end
+ * become zeros.  A range that begins inside a block leaves the block's other
+ * rows: where the new rows are larger, the scale grows to max|new| / 127 and
+ * the codes there were become round(code * scale / new scale).  An infinity or
+ * a NaN makes its block's scale a NaN, and the results of the queries that
+ * read the block: rows that no query is to read are not to be stored.
  *
  * h3_hip_kv_int8_read gives the values of rows, rounded to bf16, as
  * [row][head][head_dim]. */

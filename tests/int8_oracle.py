@@ -152,34 +152,32 @@ class Cache:
             # not finite: a NaN scale, codes of 0
             bad = ~np.isfinite(most)
             s = np.where(bad, np.float32(np.nan), s)
+            rest = slice(at, at + 64)
             if r0 > at:
                 old = self.s[block]
                 grows = old < s
                 keep = np.where(grows, old.astype(np.float64) /
                                 np.where(grows, s, 1), 1.0)
-                was = self.c[at:r0] * keep[None, :, :, None]
-                self.c[at:r0] = np.rint(was)
+                was = self.c[rest] * keep[None, :, :, None]
+                self.c[rest] = np.rint(was)
                 # the factor and the product round in F32
-                self.doubtful[at:r0] |= np.abs(
+                self.doubtful[rest] |= np.abs(
                     was - np.floor(was) - 0.5) <= 4 * HALF * np.abs(was)
                 top = np.where(grows, most, 127 * old.astype(np.float64))
                 s = np.where(bad | np.isnan(old), np.float32(np.nan),
                              np.where(grows, s, old))
+                # 127 * scale rounds where the scale stays
+                off = 127 * 4 * HALF
             else:
-                top = most
+                self.c[rest] = 0
+                self.doubtful[rest] = False
+                top, off = most, -1.0
             top = np.where(np.isnan(s) | (top == 0), 1.0, top)
             q = np.where(np.isnan(s)[None, :, :, None], 0,
                          127 * np.nan_to_num(new, posinf=0, neginf=0) /
                          top[None, :, :, None])
             self.c[r0:r1] = np.rint(q)
-            if r0 > at:
-                # 127 * scale rounds where the scale stays
-                self.doubtful[r0:r1] |= np.abs(
-                    q - np.floor(q) - 0.5) <= 127 * 4 * HALF
-            else:
-                self.doubtful[r0:r1] = False
-            self.c[r1:at + 64] = 0
-            self.doubtful[r1:at + 64] = False
+            self.doubtful[r0:r1] = np.abs(q - np.floor(q) - 0.5) <= off
             self.s[block] = s
 
     def steps(self):

@@ -106,6 +106,17 @@ def test_store_begins_anew(gpu):
     kv.check(0, 128)
 
 
+@pytest.mark.parametrize("std", [0.5, 3.0])
+def test_store_inside(gpu, std):
+    """Rows in a block's middle: the ones before and behind stay."""
+    for first, n in ((64 + 1, 1), (64 + 5, 3), (64 + 30, 34), (64 + 62, 2),
+                     (64 + 7, 60)):
+        kv = Kv(gpu, 192, 2, 80)
+        kv.store([0], [192])
+        kv.store([first], [n], std=std)
+        kv.check(0, 192)
+
+
 def test_store_many_ranges(gpu):
     """More ranges than a launch takes, out of order."""
     order = np.random.default_rng(3).permutation(150)
@@ -241,6 +252,37 @@ def test_many_rows(gpu):
 def test_scores_large_and_small(gpu, std):
     """One key has all the weight, or all have the same."""
     Case(gpu, [70, 1], [300, 700], 2, 2, 128, std=std).check()
+
+
+@pytest.mark.parametrize("powers", [
+    [0, 3, 5, -3, -7, 4, 0, -5], [-90, 0, 30, -90, 60, 60, 90, 0],
+    [60, -60, -61, -59, 60, -60, 0, -99], [0, -8, -9, -10, -7, -7, -6, -5]])
+def test_blocks_of_unlike_scales(gpu, powers):
+    """Values whose blocks' scales lie near and far from each other, the keys'
+    the other way round, so that some rows attend to small values alone."""
+    def change(rows):
+        v = ro.wide(rows, *rows.shape)
+        for block, power in enumerate(powers):
+            at = slice(64 * block, 64 * block + 64)
+            v[at, 2 * 128:] *= 2.0 ** power
+            v[at, :2 * 128] *= 1 + 0.2 * (block % 3)
+        rows[:] = io.bits(v.astype(np.float32)).reshape(rows.shape)
+    c = Case(gpu, [70, 1, 1], [512, 512, 300], 2, 2, 128, share=True)
+    c.kv.store([0], [512], change=change)
+    c.check()
+    # one block has all the weight of each row, by turns
+    q = np.zeros((c.rows, 2, 128))
+    q[np.arange(c.rows), :, np.arange(c.rows) % 8] = 1000
+    c.q = io.bits(q.astype(np.float32)).ravel()
+
+    def mark(rows):
+        change(rows)
+        k = rows[:, :2 * 128].reshape(-1, 2, 128)
+        for block in range(8):
+            k[64 * block:64 * block + 64, :, :8] = 0
+            k[64 * block:64 * block + 64, :, block] = 0x3f80
+    c.kv.store([0], [512], change=mark)
+    c.check()
 
 
 def test_queries_out_of_f16(gpu):
