@@ -98,10 +98,34 @@ hk_int8_rows_any(hk_int8_rows_args a, uint32_t first) {
     if (threadIdx.x == 0) a.scales[row] = code.scale;
 }
 
-/* The same with the row in registers, 8 columns a thread and chunk: whole
- * 16-byte pieces, at most CHUNKS * 2048 columns.  One pass over the row. */
-template <int SOURCE, int CHUNKS>
-__global__ void __launch_bounds__(HK_INT8_THREADS)
+/* Eight values from any element on, zeros from the `left`th. */
+__device__ __forceinline__ void hk_int8_load8(const uint16_t *from,
+                                              uint32_t left, float *to) {
+    if (left >= 8u) {
+        uint4 v;
+        __builtin_memcpy(&v, from, 16); /* rows of odd widths: not aligned */
+        hk_unpack8(v, to);
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 8u; i++)
+            to[i] = i < left ? hk_bf2f(from[i]) : 0.0f;
+    }
+}
+
+__device__ __forceinline__ void hk_int8_load8(const float *from, uint32_t left,
+                                              float *to) {
+    if (left >= 8u) {
+        __builtin_memcpy(to, from, 32);
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 8u; i++) to[i] = i < left ? from[i] : 0.0f;
+    }
+}
+
+/* The same with the row in registers, 8 columns a thread and chunk: at most
+ * CHUNKS * THREADS * 8 columns.  One pass over the row. */
+template <int SOURCE, int CHUNKS, int THREADS>
+__global__ void __launch_bounds__(THREADS)
 hk_int8_rows_vec(hk_int8_rows_args a, uint32_t first) {
     __shared__ float sums[16];
     __shared__ uint32_t tops[16];
@@ -109,34 +133,28 @@ hk_int8_rows_vec(hk_int8_rows_args a, uint32_t first) {
     constexpr bool norm = SOURCE == HK_ROWS_RMS || SOURCE == HK_ROWS_LAYER;
     constexpr bool layer = SOURCE == HK_ROWS_LAYER;
     auto column = [](int c) {
-        return (threadIdx.x + (uint32_t)c * HK_INT8_THREADS) * 8u;
-    };
-    auto load8 = [](const uint16_t *from, float *to) {
-        hk_unpack8(*(const uint4 *)from, to);
-    };
-    auto wide8 = [](const float *from, float *to) {
-        *(float4 *)to = *(const float4 *)from;
-        *(float4 *)(to + 4) = *(const float4 *)(from + 4);
+        return (threadIdx.x + (uint32_t)c * THREADS) * 8u;
     };
     float v[CHUNKS][8];
     float sum = 0.0f;
 #pragma unroll
     for (int c = 0; c < CHUNKS; c++) {
-        const uint32_t col = column(c);
+        const uint32_t col = column(c), left = a.width - col;
         if (col >= a.width) {
 #pragma unroll
             for (int i = 0; i < 8; i++) v[c][i] = 0.0f;
         } else if (SOURCE == HK_ROWS_F32) {
-            wide8(a.wide + (size_t)row * a.wide_pitch + col, v[c]);
+            hk_int8_load8(a.wide + (size_t)row * a.wide_pitch + col, left,
+                          v[c]);
         } else if (SOURCE == HK_ROWS_SWIGLU) {
             const float *from = a.wide + (size_t)row * a.wide_pitch + col;
             float u[8];
-            wide8(from, v[c]);
-            wide8(from + a.width, u);
+            hk_int8_load8(from, left, v[c]);
+            hk_int8_load8(from + a.width, left, u);
 #pragma unroll
             for (int i = 0; i < 8; i++) v[c][i] = hk_swiglu_f(v[c][i], u[i]);
         } else {
-            load8(a.input + (size_t)row * a.width + col, v[c]);
+            hk_int8_load8(a.input + (size_t)row * a.width + col, left, v[c]);
         }
 #pragma unroll
         for (int i = 0; i < 8; i++) sum += layer ? v[c][i] : v[c][i] * v[c][i];
@@ -151,7 +169,7 @@ hk_int8_rows_vec(hk_int8_rows_args a, uint32_t first) {
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
                     v[c][i] -= mean;
-                    if (column(c) < a.width)
+                    if (column(c) + i < a.width)
                         sum = fmaf(v[c][i], v[c][i], sum);
                 }
         }
@@ -166,7 +184,7 @@ hk_int8_rows_vec(hk_int8_rows_args a, uint32_t first) {
         }
 #pragma unroll
         for (int c = 0; c < CHUNKS; c++) {
-            const uint32_t col = column(c);
+            const uint32_t col = column(c), left = a.width - col;
             if (col >= a.width) {
 #pragma unroll
                 for (int i = 0; i < 8; i++) v[c][i] = 0.0f;
@@ -176,21 +194,26 @@ hk_int8_rows_vec(hk_int8_rows_args a, uint32_t first) {
 #pragma unroll
             for (int i = 0; i < 8; i++) v[c][i] *= inverse;
             if (a.weight) {
-                load8(a.weight + col, w);
+                hk_int8_load8(a.weight + col, left, w);
 #pragma unroll
                 for (int i = 0; i < 8; i++) v[c][i] *= w[i];
             }
             if (layer && a.bias) {
-                load8(a.bias + col, b);
+                hk_int8_load8(a.bias + col, left, b);
 #pragma unroll
                 for (int i = 0; i < 8; i++) v[c][i] += b[i];
             }
             if (shift) {
-                load8(scale + col, w);
-                load8(shift + col, b);
+                hk_int8_load8(scale + col, left, w);
+                hk_int8_load8(shift + col, left, b);
 #pragma unroll
                 for (int i = 0; i < 8; i++)
                     v[c][i] = v[c][i] * (1.0f + w[i]) + b[i];
+            }
+            if (left < 8u) { /* past the row's end, whatever came of it */
+#pragma unroll
+                for (uint32_t i = 0; i < 8u; i++)
+                    if (i >= left) v[c][i] = 0.0f;
             }
         }
     }
@@ -233,31 +256,35 @@ static void hk_int8_each_rows(uint32_t rows, F launch) {
         launch(first, std::min(rows - first, most));
 }
 
+/* A row's threads: where there are few rows, more of them, as there is nothing
+ * else to hide a row's latency (one row of 14336: 6.4 us with 256). */
 template <int SOURCE>
 static void hk_int8_rows(struct h3_gpu *gpu, const hk_int8_rows_args &a) {
-    const bool whole =
-        a.width % 8u == 0 && a.wide_pitch % 4u == 0 &&
-        (((uintptr_t)a.input | (uintptr_t)a.weight | (uintptr_t)a.bias |
-          (uintptr_t)a.modulation | (uintptr_t)a.wide) & 15u) == 0;
+    const bool few = a.rows <= 512u && a.pitch > 2048u;
     void (*kernel)(hk_int8_rows_args, uint32_t) =
-        !whole || a.pitch > 16384u || gpu->reference_kernels
-            ? hk_int8_rows_any<SOURCE>
-        : a.pitch <= 2048u ? hk_int8_rows_vec<SOURCE, 1>
-        : a.pitch <= 6144u ? hk_int8_rows_vec<SOURCE, 3>
-                           : hk_int8_rows_vec<SOURCE, 8>;
+        a.pitch > 16384u || gpu->reference_kernels ? hk_int8_rows_any<SOURCE>
+        : few && a.pitch <= 8192u ? hk_int8_rows_vec<SOURCE, 1, 1024>
+        : few                     ? hk_int8_rows_vec<SOURCE, 2, 1024>
+        : a.pitch <= 2048u        ? hk_int8_rows_vec<SOURCE, 1, 256>
+        : a.pitch <= 6144u        ? hk_int8_rows_vec<SOURCE, 3, 256>
+                                  : hk_int8_rows_vec<SOURCE, 8, 256>;
+    const uint32_t threads =
+        few && a.pitch <= 16384u && !gpu->reference_kernels ? 1024u : 256u;
     hk_int8_each_rows(a.rows, [&](uint32_t first, uint32_t rows) {
-        hipLaunchKernelGGL(kernel, dim3(rows), dim3(HK_INT8_THREADS), 0,
-                           gpu->stream, a, first);
+        hipLaunchKernelGGL(kernel, dim3(rows), dim3(threads), 0, gpu->stream,
+                           a, first);
     });
 }
 
 /* ------------------------------------------------------------ the products */
 
-/* What is made of the sums: act(acc sx sw + bias).  The scales are multiplied
- * first: their product with the sum passes F32's range only where the result
- * does. */
-__device__ __forceinline__ float hk_int8_value(int acc, float sx, float sw) {
-    return (float)acc * (sx * sw);
+/* What is made of the sums: acc sx sw + bias, in every kernel with the same
+ * roundings.  The scales are multiplied first: their product with the sum
+ * passes F32's range only where the result does.  -0 is no bias: x + -0 is
+ * x. */
+__device__ __forceinline__ float hk_int8_value(int acc, float sx, float sw,
+                                               float bias = -0.0f) {
+    return __builtin_fmaf((float)acc, sx * sw, bias);
 }
 
 /* One thread per output: H3_HIP_REFERENCE=1.  `wide` or `out`. */
@@ -279,8 +306,8 @@ hk_int8_simple(const int8_t *x, const float *xs, const int8_t *w,
         sum = __builtin_amdgcn_sdot4(a.z, b.z, sum, false);
         sum = __builtin_amdgcn_sdot4(a.w, b.w, sum, false);
     }
-    float y = hk_int8_value(sum, xs[row], ws[col]);
-    if (bias) y += hk_bf2f(bias[col]);
+    float y = hk_int8_value(sum, xs[row], ws[col],
+                            bias ? hk_bf2f(bias[col]) : -0.0f);
     if (gelu) y = hk_gelu_tanh_f(y);
     if (wide) wide[row * n + col] = y;
     else out[row * n + col] = hk_f2bf(y);
@@ -339,17 +366,34 @@ struct hk_int8_out {
     int gelu;
 };
 
+/* The scales and bias of columns [col, + 4). */
+struct hk_int8_columns {
+    float scale[4], bias[4];
+    __device__ __forceinline__ void load(const hk_int8_out &o, uint32_t col) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            scale[e] = o.ws[col + e];
+            bias[e] = o.bias && col + e < o.n ? hk_bf2f(o.bias[col + e])
+                                              : -0.0f;
+        }
+    }
+};
+
+__device__ __forceinline__ float hk_int8_made(const hk_int8_out &o, float sx,
+                                             float sw, float bias, int sum) {
+    const float y = hk_int8_value(sum, sx, sw, bias);
+    return o.gelu ? hk_gelu_tanh_f(y) : y;
+}
+
 __device__ __forceinline__ void hk_int8_finish(const hk_int8_out &o,
                                                uint32_t row, uint32_t col,
+                                               float sx,
+                                               const hk_int8_columns &c,
                                                hk_v4i sums) {
-    const float sx = o.xs[row];
     float y[4];
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-        y[e] = hk_int8_value(sums[e], sx, o.ws[col + e]);
-        if (o.bias && col + e < o.n) y[e] += hk_bf2f(o.bias[col + e]);
-        if (o.gelu) y[e] = hk_gelu_tanh_f(y[e]);
-    }
+    for (int e = 0; e < 4; e++)
+        y[e] = hk_int8_made(o, sx, c.scale[e], c.bias[e], sums[e]);
     const size_t at = (size_t)row * o.n + col;
     const bool whole = o.n % 4u == 0;
     if (o.wide && whole) {
@@ -357,6 +401,9 @@ __device__ __forceinline__ void hk_int8_finish(const hk_int8_out &o,
     } else if (whole) {
         *(uint2 *)(o.out + at) =
             make_uint2(hk_pack2(y[0], y[1]), hk_pack2(y[2], y[3]));
+    } else if (!o.wide && o.n % 2u == 0) {
+        *(uint32_t *)(o.out + at) = hk_pack2(y[0], y[1]);
+        if (col + 2u < o.n) *(uint32_t *)(o.out + at + 2) = hk_pack2(y[2], y[3]);
     } else {
 #pragma unroll
         for (int e = 0; e < 4; e++) {
@@ -367,10 +414,83 @@ __device__ __forceinline__ void hk_int8_finish(const hk_int8_out &o,
     }
 }
 
-/* Up to 128 rows: the skinny GEMM's loop (hk_skinny_tile.h) over bytes. */
+/* One row, on the vector units: a wave takes COLUMNS rows of W, each lane 16
+ * bytes of every 1024, against X's row in LDS, and adds up its lanes.  W
+ * streams from HBM once, in loads of whole KiB, with no pieces of K to join in
+ * a second launch: 5120 -> 5120 7.3 us, 14336 -> 5376 14.8, 1024 -> 2048 3.5,
+ * as MFMA tiles 9.7, 16.9 and 6.4; 5376 -> 28672 is level (25.4, 6.1 TB/s).  Of
+ * more rows the reads of X from LDS are too many (two rows 5120 -> 5120 9.2 and
+ * 9.7, 14336 -> 5376 21 and 17). */
+template <int COLUMNS>
+__global__ void __launch_bounds__(256)
+hk_int8_dot(hk_skinny_args g, hk_int8_out o, uint32_t pitch) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t xs[];
+    const uint32_t tid = threadIdx.x, lane = tid & 63u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t chunks = pitch / 16u;
+    const uint32_t col0 = (blockIdx.x * 4u + wave) * COLUMNS;
+    constexpr int AHEAD = 4; /* loads of a row of W on their way */
+    const hk_v4i *w[COLUMNS];
+#pragma unroll
+    for (int c = 0; c < COLUMNS; c++)
+        w[c] = (const hk_v4i *)((const uint8_t *)g.w +
+                                (size_t)min(col0 + c, g.n - 1u) * pitch);
+    hk_v4i next[AHEAD][COLUMNS];
+    auto load = [&](uint32_t at, hk_v4i (&to)[COLUMNS]) {
+#pragma unroll
+        for (int c = 0; c < COLUMNS; c++)
+            to[c] = at < chunks ? __builtin_nontemporal_load(w[c] + at)
+                                : hk_v4i{0, 0, 0, 0};
+    };
+#pragma unroll
+    for (int i = 0; i < AHEAD; i++) load(i * 64u + lane, next[i]);
+    for (uint32_t i = tid; i < chunks; i += 256u)
+        *(hk_v4i *)(xs + i * 16u) = ((const hk_v4i *)g.x)[i];
+    __syncthreads();
+    int sum[COLUMNS] = {};
+    for (uint32_t first = 0; first < chunks; first += AHEAD * 64u) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) {
+            const uint32_t at = first + i * 64u + lane;
+            hk_v4i now[COLUMNS];
+#pragma unroll
+            for (int c = 0; c < COLUMNS; c++) now[c] = next[i][c];
+            load(at + AHEAD * 64u, next[i]);
+            /* past the end W is zeros, and X any bytes of it */
+            const hk_v4i x =
+                *(const hk_v4i *)(xs + min(at, chunks - 1u) * 16u);
+#pragma unroll
+            for (int c = 0; c < COLUMNS; c++)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    sum[c] = __builtin_amdgcn_sdot4(now[c][e], x[e], sum[c],
+                                                    false);
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < COLUMNS; c++) {
+        int v = sum[c];
+#pragma unroll
+        for (int off = 32; off; off >>= 1) v += __shfl_xor(v, off, 64);
+        const uint32_t col = col0 + c;
+        if (lane != (uint32_t)c || col >= g.n) continue;
+        const float y =
+            hk_int8_made(o, o.xs[0], o.ws[col],
+                         o.bias ? hk_bf2f(o.bias[col]) : -0.0f, v);
+        if (o.wide) o.wide[col] = y;
+        else o.out[col] = hk_f2bf(y);
+    }
+}
+
+/* Few rows: the skinny GEMM's loop (hk_skinny_tile.h) over bytes, `rows` of them
+ * a workgroup, groups of rows in the grid's third dimension. */
 template <int MB, int XA>
 __global__ void __launch_bounds__(256)
-hk_int8_skinny(hk_skinny_args g, hk_int8_out o) {
+hk_int8_skinny(hk_skinny_args g, hk_int8_out o, uint32_t rows) {
+    const uint32_t row0 = blockIdx.z * rows;
+    g.x += (size_t)row0 * g.k;
+    g.m = min(g.m - row0, rows);
+    g.x_bytes = g.m * g.k * 2u;
     hk_i32x16 acc[MB];
     hk_skinny_sums<MB, XA, HK_LOAD_ONCE>(g, g.w, blockIdx.x, blockIdx.y, acc);
     const uint32_t lane = threadIdx.x & 63u, row = lane & 31u;
@@ -379,10 +499,21 @@ hk_int8_skinny(hk_skinny_args g, hk_int8_out o) {
     if (tile * 32u >= g.n) return;
     if (g.partial) {
         hk_skinny_partial<MB>((hk_v4i *)g.partial,
-                              (size_t)blockIdx.y * gridDim.x * 4u + tile, g.m,
-                              acc);
+                              ((size_t)blockIdx.z * gridDim.y + blockIdx.y) *
+                                      gridDim.x * 4u + tile,
+                              g.m, acc);
         return;
     }
+    /* all loads before the first store, which the compiler takes to change
+     * what they read: one after the other they took 8 of 13 us of a call */
+    hk_int8_columns columns[4];
+    float sx[MB];
+#pragma unroll
+    for (int q = 0; q < 4; q++)
+        columns[q].load(o, tile * 32u + q * 8u + (lane >> 5) * 4u);
+#pragma unroll
+    for (int mb = 0; mb < MB; mb++)
+        sx[mb] = o.xs[row0 + min(mb * 32u + row, g.m - 1u)];
 #pragma unroll
     for (int mb = 0; mb < MB; mb++) {
         if (mb * 32u + row >= g.m) continue;
@@ -390,7 +521,8 @@ hk_int8_skinny(hk_skinny_args g, hk_int8_out o) {
         for (int q = 0; q < 4; q++) {
             const uint32_t col = tile * 32u + q * 8u + (lane >> 5) * 4u;
             if (col < g.n)
-                hk_int8_finish(o, mb * 32u + row, col,
+                hk_int8_finish(o, row0 + mb * 32u + row, col, sx[mb],
+                               columns[q],
                                hk_v4i{acc[mb][q * 4], acc[mb][q * 4 + 1],
                                       acc[mb][q * 4 + 2],
                                       acc[mb][q * 4 + 3]});
@@ -401,18 +533,23 @@ hk_int8_skinny(hk_skinny_args g, hk_int8_out o) {
 /* Adds the pieces, as hk_skinny_reduce. */
 __global__ void __launch_bounds__(256)
 hk_int8_skinny_reduce(hk_skinny_args g, hk_int8_out o, uint32_t mbs,
-                      uint32_t tiles, uint32_t splits) {
+                      uint32_t tiles, uint32_t splits, uint32_t rows) {
     const uint32_t lane = threadIdx.x & 63u, q = threadIdx.x >> 6;
     const uint32_t tile = blockIdx.x / mbs, mb = blockIdx.x % mbs;
     const uint32_t row = mb * 32u + (lane & 31u);
     const uint32_t col = tile * 32u + q * 8u + (lane >> 5) * 4u;
-    if (row >= g.m || col >= g.n) return;
+    const uint32_t row0 = blockIdx.y * rows;
+    if (row >= min(g.m - row0, rows) || col >= g.n) return;
     const size_t stride = (size_t)tiles * mbs * 256u;
-    const hk_v4i *p =
-        (const hk_v4i *)g.partial + (size_t)blockIdx.x * 256u + threadIdx.x;
+    const hk_v4i *p = (const hk_v4i *)g.partial +
+                      blockIdx.y * splits * stride +
+                      (size_t)blockIdx.x * 256u + threadIdx.x;
+    hk_int8_columns columns;
+    columns.load(o, col);
+    const float sx = o.xs[row0 + row];
     hk_v4i sum = *p;
     for (uint32_t s = 1; s < splits; s++) sum += p[s * stride];
-    hk_int8_finish(o, row, col, sum);
+    hk_int8_finish(o, row0 + row, col, sx, columns, sum);
 }
 
 /* Adds the pieces of tiles, as hk_splitk_reduce: 4 columns a thread. */
@@ -430,9 +567,12 @@ hk_int8_tile_reduce(hk_gemm_args g, hk_int8_out o, uint32_t splits) {
     const size_t stride = g.part_tiles * tile / 4u;
     const hk_v4i *p = (const hk_v4i *)((const int *)g.partial + part * tile +
                                        row * HK_BN + tcol);
+    hk_int8_columns columns;
+    columns.load(o, n);
+    const float sx = o.xs[m];
     hk_v4i sum = *p;
     for (uint32_t s = 1; s < splits; s++) sum += p[s * stride];
-    hk_int8_finish(o, m, n, sum);
+    hk_int8_finish(o, m, n, sx, columns, sum);
 }
 
 /* The same of the gated block: F32 rows of its activation. */
@@ -583,49 +723,105 @@ static void hk_int8_tiles(struct h3_gpu *gpu, const hk_int8_matrix &x,
                            gpu->stream, g, o, r.splits);
 }
 
-/* Up to 128 rows, as hk_gemm_skinny_run. */
+/* How few rows run: groups of up to 128, and K in pieces where one workgroup
+ * per 128 columns and group leaves CUs idle (hk_gemm_skinny_run). */
+struct hk_int8_few_plan {
+    uint32_t groups, mbs, columns, splits, steps;
+};
+
+static hk_int8_few_plan hk_int8_few_planned(uint32_t cus, uint32_t m,
+                                            uint32_t n, uint32_t k_steps) {
+    hk_int8_few_plan p;
+    p.groups = (m + 127u) / 128u;
+    p.mbs = ((m + p.groups - 1u) / p.groups + 31u) / 32u;
+    p.columns = (n + 127u) / 128u;
+    p.splits = std::max(
+        1u, std::min(cus / (p.columns * p.groups), k_steps / 8u));
+    p.steps = k_steps;
+    if (p.splits > 1) {
+        /* whole turns of the kernel's ring of 4 */
+        p.steps = ((k_steps + p.splits - 1u) / p.splits + 3u) & ~3u;
+        p.splits = (k_steps + p.steps - 1u) / p.steps;
+    }
+    return p;
+}
+
 static void hk_int8_few(struct h3_gpu *gpu, const hk_int8_matrix &x,
                         const hk_int8_matrix &w, const hk_int8_out &o) {
-    const uint32_t cus = hk_int8_cus(gpu), k_steps = x.pitch / HK_INT8_LINE;
-    const uint32_t mbs = (x.rows + 31u) / 32u, wgs = (o.n + 127u) / 128u;
     hk_skinny_args g = {};
     g.x = (const uint16_t *)x.codes;
     g.w = (const uint16_t *)w.codes;
     g.m = x.rows;
     g.n = o.n;
     g.k = x.pitch / 2u;
-    g.x_bytes = x.rows * x.pitch;
     g.w_bytes = w.rows * w.pitch;
-    g.split_steps = k_steps;
-    uint32_t splits = std::min(cus / wgs, k_steps / 8u);
-    if (splits > 1) {
-        /* whole turns of the kernel's ring of 4 */
-        g.split_steps = ((k_steps + splits - 1u) / splits + 3u) & ~3u;
-        splits = (k_steps + g.split_steps - 1u) / g.split_steps;
-    }
-    if (splits > 1)
-        g.partial = (float *)hk_splitk_try(
-            gpu, (size_t)splits * wgs * 4 * mbs * 4096);
-    if (!g.partial) splits = 1;
     static uint64_t ready = 0;
     const uint64_t bit = 1ull << (gpu->device & 63);
     if (!(ready & bit)) {
         (void)hipFuncSetAttribute((const void *)hk_int8_skinny<4, 3>,
                                   hipFuncAttributeMaxDynamicSharedMemorySize,
                                   4 * 4096 * 4 + 16384);
+        for (auto dot : {hk_int8_dot<1>, hk_int8_dot<2>})
+            (void)hipFuncSetAttribute(
+                (const void *)dot, hipFuncAttributeMaxDynamicSharedMemorySize,
+                HK_INT8_MOST_COLUMNS);
         ready |= bit;
     }
-    void (*kernel)(hk_skinny_args, hk_int8_out) =
-        mbs == 1   ? hk_int8_skinny<1, 3>
-        : mbs == 2 ? hk_int8_skinny<2, 3>
-        : mbs == 3 ? hk_int8_skinny<3, 3>
-                   : hk_int8_skinny<4, 3>;
-    hipLaunchKernelGGL(kernel, dim3(wgs, splits), dim3(256),
-                       mbs * 4096 * 4 + 16384, gpu->stream, g, o);
-    if (splits > 1)
-        hipLaunchKernelGGL(hk_int8_skinny_reduce, dim3((o.n + 31u) / 32u * mbs),
-                           dim3(256), 0, gpu->stream, g, o, mbs, wgs * 4u,
-                           splits);
+    if (x.rows == 1) {
+        /* two columns a wave where that leaves it eight turns of the CUs */
+        const uint32_t per = o.n > 16384u ? 2u : 1u;
+        hipLaunchKernelGGL(per == 2u ? hk_int8_dot<2> : hk_int8_dot<1>,
+                           dim3((o.n + 4u * per - 1u) / (4u * per)), dim3(256),
+                           x.pitch, gpu->stream, g, o, x.pitch);
+        return;
+    }
+    hk_int8_few_plan p = hk_int8_few_planned(hk_int8_cus(gpu), x.rows, o.n,
+                                             x.pitch / HK_INT8_LINE);
+    g.split_steps = p.steps;
+    if (p.splits > 1)
+        g.partial = (float *)hk_splitk_try(
+            gpu, (size_t)p.groups * p.splits * p.columns * 4 * p.mbs * 4096);
+    if (!g.partial) p.splits = 1; /* no scratch: in one piece */
+    void (*kernel)(hk_skinny_args, hk_int8_out, uint32_t) =
+        p.mbs == 1   ? hk_int8_skinny<1, 3>
+        : p.mbs == 2 ? hk_int8_skinny<2, 3>
+        : p.mbs == 3 ? hk_int8_skinny<3, 3>
+                     : hk_int8_skinny<4, 3>;
+    hipLaunchKernelGGL(kernel, dim3(p.columns, p.splits, p.groups), dim3(256),
+                       p.mbs * 4096 * 4 + 16384, gpu->stream, g, o,
+                       32u * p.mbs);
+    if (p.splits > 1)
+        hipLaunchKernelGGL(hk_int8_skinny_reduce,
+                           dim3((o.n + 31u) / 32u * p.mbs, p.groups),
+                           dim3(256), 0, gpu->stream, g, o, p.mbs,
+                           p.columns * 4u, p.splits, 32u * p.mbs);
+}
+
+/* Whether m rows run there rather than over tiles: up to 128 always, more of
+ * them where the estimates say so, which were held against both ways at 117
+ * sizes of 140 to 1024 rows (320 to 14336 -> 640 to 21504 columns).  The pick
+ * is within 6% of the faster one at all but a K of 320 beside 13824 columns
+ * (10.7 us and 13.9).  Us, here and over tiles: 197 x 1283 -> 2051 16 and 23,
+ * 300 x 2675 -> 1001 14.5 and 20, 512 x 5120 -> 5120 32 and 39, 1024 x 5120 ->
+ * 1024 19 and 31; 777 x 5120 -> 5120 54 and 43, 1024 x 5376 -> 21504 205 and
+ * 111.  Few tiles are cut along K, and their pieces' sums cost as much as the
+ * products; here a workgroup has an eighth of a tile. */
+static bool hk_int8_takes_few(const struct h3_gpu *gpu, uint32_t m, uint32_t n,
+                              uint32_t pitch) {
+    if (m <= 128u) return true;
+    if (m > 1024u) return false;
+    const uint32_t cus = hk_int8_cus(gpu);
+    const hk_int8_few_plan p =
+        hk_int8_few_planned(cus, m, n, pitch / HK_INT8_LINE);
+    const uint32_t workgroups = p.columns * p.groups * p.splits;
+    const float rounds =
+        workgroups <= cus ? 1.0f
+                          : 0.8f * (float)((workgroups + cus - 1u) / cus);
+    const float us = (5.6f + 0.7f * (float)p.steps) * rounds +
+                     (p.splits > 1 ? 4.5f : 0.0f);
+    float tiles;
+    (void)hk_gemm_tile_rows(gpu, m, n, pitch / 2u, &tiles);
+    return us < tiles;
 }
 
 /* Whether x . w^T runs on the matrix cores: everything but weights of 4 GiB
@@ -633,8 +829,6 @@ static void hk_int8_few(struct h3_gpu *gpu, const hk_int8_matrix &x,
 static bool hk_int8_fast(const struct h3_gpu *gpu, const hk_int8_matrix &w) {
     return !gpu->reference_kernels && w.rows <= hk_int8_reach(w.pitch);
 }
-
-enum { HK_INT8_FEW_ROWS = 128 };
 
 /* bf16 rows of x . w^T. */
 static void hk_int8_linear(struct h3_gpu *gpu, hk_int8_matrix x,
@@ -648,7 +842,7 @@ static void hk_int8_linear(struct h3_gpu *gpu, hk_int8_matrix x,
     const uint32_t most = hk_int8_reach(x.pitch);
     for (uint32_t left = x.rows; left; left -= x.rows) {
         x.rows = std::min(left, most);
-        if (x.rows <= HK_INT8_FEW_ROWS)
+        if (hk_int8_takes_few(gpu, x.rows, w.rows, x.pitch))
             hk_int8_few(gpu, x, w, o);
         else
             hk_int8_tiles(gpu, x, w, w.rows, false, o,
@@ -659,8 +853,17 @@ static void hk_int8_linear(struct h3_gpu *gpu, hk_int8_matrix x,
     }
 }
 
-/* h = silu(x . gate^T) (x . up^T) in 8 bits, by way of F32 rows in `wide`
- * ([rows][2 hidden] at most). */
+/* Whether the gated block's first product goes over tiles, whose epilogue
+ * leaves the activation; else both projections are left. */
+static bool hk_int8_gated_tiles(const struct h3_gpu *gpu,
+                                const hk_int8_matrix &x,
+                                const hk_int8_matrix &w) {
+    return hk_int8_fast(gpu, w) &&
+           !hk_int8_takes_few(gpu, x.rows, w.rows, x.pitch);
+}
+
+/* h = silu(x . gate^T) (x . up^T) in 8 bits, by way of F32 rows in `wide`, of
+ * (hidden + 3) / 4 * 4 elements over tiles and 2 hidden else. */
 static void hk_int8_gated(struct h3_gpu *gpu, hk_int8_matrix x,
                           const hk_int8_matrix &w, uint32_t hidden,
                           float *wide, const hk_int8_matrix &h) {
@@ -671,10 +874,9 @@ static void hk_int8_gated(struct h3_gpu *gpu, hk_int8_matrix x,
     a.rows = x.rows;
     a.width = hidden;
     a.pitch = h.pitch;
-    const bool fast = hk_int8_fast(gpu, w);
-    if (!fast || x.rows <= HK_INT8_FEW_ROWS) {
+    if (!hk_int8_gated_tiles(gpu, x, w)) {
         a.wide_pitch = 2 * hidden;
-        if (fast)
+        if (hk_int8_fast(gpu, w))
             hk_int8_few(gpu, x, w, {x.scales, w.scales, NULL, NULL, wide,
                                     2 * hidden, 0});
         else
@@ -899,10 +1101,11 @@ int h3_hip_mlp_int8_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
     if (!rows || !output_dim) return 1;
     /* F32 rows of the activation or, where they are few or go through the
      * simple kernel, of both projections, then h in 8 bits */
+    const hk_int8_matrix x = hk_int8_of(input, rows);
     const hk_int8_matrix w1 = hk_int8_of(fc1_weight, 2 * hidden_dim);
     const uint32_t pitch = fc2_weight->record.n[HK_INT8_PITCH];
     const size_t wide =
-        rows > HK_INT8_FEW_ROWS && hk_int8_fast(gpu, w1)
+        hk_int8_gated_tiles(gpu, x, w1)
             ? ((size_t)hidden_dim + 3u) & ~(size_t)3u
             : 2 * (size_t)hidden_dim;
     const size_t wide_bytes = (rows * wide * 4 + 255) & ~(size_t)255;
@@ -914,8 +1117,7 @@ int h3_hip_mlp_int8_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
                               (float *)(space + wide_bytes + code_bytes), rows,
                               pitch};
     hk_op_begin(gpu, "gemm_int8_swiglu");
-    hk_int8_gated(gpu, hk_int8_of(input, rows), w1, hidden_dim,
-                  (float *)space, h);
+    hk_int8_gated(gpu, x, w1, hidden_dim, (float *)space, h);
     if (!hk_op_end(gpu, "gemm_int8_swiglu", HK_KIND_LINEAR)) return 0;
     hk_op_begin(gpu, "gemm_int8");
     hk_int8_linear(gpu, h, hk_int8_of(fc2_weight, output_dim), NULL,
