@@ -34,7 +34,7 @@ struct h3_gpu_tensor {
      * what it was made for */
     struct hk_record {
         uint32_t kind;
-        uint32_t n[15];
+        uint32_t n[20];
     } record;
 };
 

@@ -254,19 +254,16 @@ __global__ void __launch_bounds__(256) hk_kv8_store(hk_kv8_store_args a) {
             *(const uint4 *)(image + hk_kv8_image(u * 16u));
 }
 
-/* The values of rows [first, + rows), one workgroup per block, head and one of
- * keys and values, by way of the block's image in LDS. */
-__global__ void __launch_bounds__(256)
-hk_kv8_read(hk_kv8_cache c, uint16_t *key, uint16_t *value, uint32_t first,
-            uint32_t rows) {
-    extern __shared__ __attribute__((aligned(16))) uint8_t image[];
-    const uint32_t block = first / HK_KV8_BLOCK + blockIdx.x;
-    const uint32_t head = blockIdx.y, which = blockIdx.z, tid = threadIdx.x;
-    const size_t at = (size_t)block * c.heads + head;
+/* Values of a block's keys or values (blockIdx.z) of a head, by way of the
+ * block's image in LDS: the codes times `scale`, element d of row r at row(r) +
+ * d, where row() is not NULL. */
+template <typename ROW>
+__device__ __forceinline__ void hk_kv8_rows(const hk_kv8_cache &c, size_t at,
+                                            uint32_t which, float scale,
+                                            uint8_t *image, ROW row_of) {
+    const uint32_t tid = threadIdx.x;
     const uint32_t part = HK_KV8_BLOCK * c.padded;
     const uint8_t *codes = c.codes + (at * 2u + which) * part;
-    const float scale = ((const float *)(c.scales + at))[which];
-    const uint64_t row0 = (uint64_t)block * HK_KV8_BLOCK;
     for (uint32_t u = tid; u < part / 16u; u += 256u)
         *(uint4 *)(image + hk_kv8_image(u * 16u)) =
             *(const uint4 *)(codes + u * 16u);
@@ -299,11 +296,9 @@ hk_kv8_read(hk_kv8_cache c, uint16_t *key, uint16_t *value, uint32_t first,
         }
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            const uint64_t row = row0 + p.row + e;
-            if (row < first || row >= (uint64_t)first + rows || p.dim >= c.dim)
-                continue;
-            uint16_t *to = (which ? value : key) +
-                           ((row - first) * c.heads + head) * c.dim + p.dim;
+            uint16_t *to = p.dim < c.dim ? row_of(p.row + e) : NULL;
+            if (!to) continue;
+            to += p.dim;
             if (c.dim % 8u == 0) {
                 *(uint4 *)to = hk_pack8(f[e]);
             } else {
@@ -313,6 +308,49 @@ hk_kv8_read(hk_kv8_cache c, uint16_t *key, uint16_t *value, uint32_t first,
             }
         }
     }
+}
+
+/* The values of rows [first, + rows). */
+__global__ void __launch_bounds__(256)
+hk_kv8_read(hk_kv8_cache c, uint16_t *key, uint16_t *value, uint32_t first,
+            uint32_t rows) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t image[];
+    const uint32_t block = first / HK_KV8_BLOCK + blockIdx.x;
+    const uint32_t head = blockIdx.y, which = blockIdx.z;
+    const size_t at = (size_t)block * c.heads + head;
+    const uint64_t row0 = (uint64_t)block * HK_KV8_BLOCK;
+    hk_kv8_rows(c, at, which, ((const float *)(c.scales + at))[which], image,
+                [&](uint32_t r) -> uint16_t * {
+                    const uint64_t row = row0 + r;
+                    if (row < first || row >= (uint64_t)first + rows)
+                        return NULL;
+                    return (which ? value : key) +
+                           ((row - first) * c.heads + head) * c.dim;
+                });
+}
+
+/* A plan's spans of blocks as bf16 rows, [block][64][keys, values][head][dim]:
+ * the keys' codes, which bf16 holds, and the values, rounded. */
+__global__ void __launch_bounds__(256)
+hk_kv8_unpack(hk_kv8_cache c, const hk_packed_span *spans, uint32_t count,
+              uint16_t *out, uint32_t first) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t image[];
+    const uint32_t to = first + blockIdx.x;
+    uint32_t low = 0, high = count; /* the last span that begins by then */
+    while (high - low > 1u) {
+        const uint32_t mid = (low + high) / 2u;
+        if (spans[mid].at <= to) low = mid;
+        else high = mid;
+    }
+    const uint32_t block = spans[low].block + (to - spans[low].at);
+    const uint32_t head = blockIdx.y, which = blockIdx.z;
+    const uint64_t row0 = (uint64_t)to * HK_KV8_BLOCK;
+    const size_t at = (size_t)block * c.heads + head;
+    hk_kv8_rows(c, at, which, which ? c.scales[at].y : 1.0f, image,
+                [&](uint32_t r) -> uint16_t * {
+                    return out + (((row0 + r) * 2u + which) * c.heads + head) *
+                                     c.dim;
+                });
 }
 
 /* ---------------------------------------------------------- the attention */
@@ -663,20 +701,6 @@ __device__ __forceinline__ void hk_kv8_put(const hk_packed_args &a,
         if (dim + e < a.dim) to[e] = hk_f2bf(v[e]);
 }
 
-/* The item of a workgroup, if its rows are few or many; false: nothing to do. */
-__device__ __forceinline__ bool hk_kv8_item(const hk_packed_args &a, bool few,
-                                            hk_packed_item &it) {
-    it = a.items[blockIdx.x];
-    if (it.row >= it.rows || (it.rows - it.row <= 32u) != few) return false;
-    if (!a.part_o && it.part != HK_PACKED_WHOLE) {
-        /* no room for pieces' sums: the first one takes all keys */
-        if (it.tile) return false;
-        it.tile_end = (it.kv_rows + HK_KV8_BLOCK - 1u) / HK_KV8_BLOCK;
-        it.part = HK_PACKED_WHOLE;
-    }
-    return true;
-}
-
 /* Items of at most 32 rows: the waves share the rows and split the blocks,
  * wave w every fourth from the wth on, each straight from the cache into its
  * registers; then their sums are joined. */
@@ -687,8 +711,14 @@ __global__ void __launch_bounds__(256, 2) hk_kv8_few(hk_kv8_args g) {
     extern __shared__ __attribute__((aligned(16))) uint8_t hk_lds[];
     float *lds = (float *)hk_lds;
     const hk_packed_args &a = g.p;
-    hk_packed_item it;
-    if (!hk_kv8_item(a, true, it)) return;
+    hk_packed_item it = a.items[blockIdx.x];
+    if (it.row >= it.rows || it.rows - it.row > 32u) return;
+    if (!a.part_o && it.part != HK_PACKED_WHOLE) {
+        /* no room for pieces' sums: the first one takes all keys */
+        if (it.tile) return;
+        it.tile_end = (it.kv_rows + HK_KV8_BLOCK - 1u) / HK_KV8_BLOCK;
+        it.part = HK_PACKED_WHOLE;
+    }
     const uint32_t tid = threadIdx.x, lane = tid & 63u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t col = lane & 31u, half = lane >> 5;
@@ -804,156 +834,50 @@ __global__ void __launch_bounds__(256, 2) hk_kv8_few(hk_kv8_args g) {
     }
 }
 
-/* Larger items, four waves of 32 rows: the waves make f16 of a block's codes
- * together, in LDS, in the order of the fragments, one block ahead of the
- * products and with the next one's codes in their registers. */
 template <int DIMS>
-__global__ void __launch_bounds__(256, 2) hk_kv8_flash(hk_kv8_args g) {
-    constexpr int ND = DIMS / 32;
-    constexpr int DP = DIMS <= 64 ? 64 : 128;
-    constexpr uint32_t STAGE = 256u * DIMS; /* bytes of a block in f16 */
-    constexpr int UNITS = DIMS / 32;        /* 16-byte pieces a thread */
-    extern __shared__ __attribute__((aligned(16))) uint8_t hk_lds[];
-    const hk_packed_args &a = g.p;
-    hk_packed_item it;
-    if (!hk_kv8_item(a, false, it)) return;
-    const uint32_t tid = threadIdx.x, lane = tid & 63u;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const uint32_t col = lane & 31u, half = lane >> 5;
-    const uint32_t vrow0 = it.row + wave * 32u, vrow = vrow0 + col;
-    const uint32_t first = it.kv_first / HK_KV8_BLOCK;
-    auto block_at = [&](uint32_t tile) {
-        return (size_t)(first + tile) * g.cache.heads + it.kv_head;
-    };
-    /* a block's keys and values lie together: piece u of thread t is its
-     * (256 u + t)th */
-    uint4 ahead[UNITS];
-    auto load = [&](uint32_t tile) {
-        const uint4 *from =
-            (const uint4 *)(g.cache.codes +
-                            block_at(tile) * (2u * HK_KV8_BLOCK * DIMS)) +
-            tid;
-#pragma unroll
-        for (int u = 0; u < UNITS; u++) ahead[u] = from[u * 256];
-    };
-    auto convert = [&](uint32_t stage) {
-#pragma unroll
-        for (int u = 0; u < UNITS; u++) {
-            uint4 f[2];
-            hk_kv8_fragments(ahead[u], f);
-            uint8_t *to =
-                hk_lds + stage * STAGE + (u * 4u + wave) * 2048u + lane * 16u;
-            *(uint4 *)to = f[0];
-            *(uint4 *)(to + 1024) = f[1];
-        }
-    };
-    const uint32_t n = it.tile_end - it.tile;
-    float2 ahead_scale = make_float2(0.0f, 0.0f);
-    if (n) {
-        ahead_scale = g.cache.scales[block_at(it.tile)];
-        load(it.tile);
-    }
-    hk_kv8_wave<DIMS> w;
-    w.start(a, it, vrow);
-    /* a wave whose rows all lie past the request's converts its share and
-     * meets every barrier, and computes nothing */
-    const bool live = vrow0 < it.rows;
-    if (n) {
-        convert(0);
-        if (n > 1) load(it.tile + 1u);
-    }
-    __syncthreads();
-    for (uint32_t i = 0; i < n; i++) {
-        const uint32_t tile = it.tile + i;
-        const uint8_t *stage = hk_lds + (i & 1u) * STAGE + lane * 16u;
-        const float2 scale = ahead_scale;
-        if (i + 1 < n) {
-            convert((i & 1u) ^ 1u);
-            ahead_scale = g.cache.scales[block_at(tile + 1u)];
-            load(i + 2 < n ? tile + 2u : tile);
-        }
-        if (live) {
-            hk_f32x16 s[2];
-            w.scores(
-                s, [&](int k) { return w.q[k]; },
-                [&](int kt, int j, uint4 (&f)[2]) {
-                    const uint8_t *at = stage + (kt * ND + j) * 2048u;
-                    f[0] = *(const uint4 *)at;
-                    f[1] = *(const uint4 *)(at + 1024);
-                });
-            hk_f16x8 p[2][2];
-            w.softmax(s, p, scale.x, it.kv_rows - tile * HK_KV8_BLOCK,
-                      a.scale_log2);
-            w.values(p, scale.y, [&](int kt, int d, uint4 (&f)[2]) {
-                const uint8_t *at = stage + (2 * ND + kt * ND + d) * 2048u;
-                f[0] = *(const uint4 *)at;
-                f[1] = *(const uint4 *)(at + 1024);
-            });
-        }
-        __syncthreads();
-    }
-    const float l = w.l + __shfl_xor(w.l, 32, 64);
-    const bool all = it.part == HK_PACKED_WHOLE;
-    /* no keys, or none with weight: zeros (a NaN sum gives NaN) */
-    const float weight = !all ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
-    if (!all && half == 0 && vrow < it.rows)
-        a.part_ml[(size_t)it.part * HK_PACKED_QB + wave * 32u + col] =
-            make_float2(w.m, l);
-    /* The wave's rows go through LDS of its own, 32 dims at a time in rows of
-     * 128 bytes, 16-byte chunk c of row r at c ^ (r % 8). */
-    float *mine = (float *)(hk_lds + wave * 4096u);
-    const bool whole = a.dim % 8u == 0;
-#pragma unroll
-    for (int d = 0; d < ND; d++) {
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            *(float4 *)(mine + col * 32u +
-                        (((i * 2u + half) ^ (col & 7u)) << 2)) =
-                make_float4(w.o[d][i * 4] * weight, w.o[d][i * 4 + 1] * weight,
-                            w.o[d][i * 4 + 2] * weight,
-                            w.o[d][i * 4 + 3] * weight);
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const uint32_t r = i * 16u + (lane >> 2), c = (lane & 3u) * 2u;
-            float v[8];
-#pragma unroll
-            for (int e = 0; e < 8; e++)
-                v[e] = mine[r * 32u + (((c + (e >> 2)) ^ (r & 7u)) << 2) +
-                            (e & 3)];
-            if (vrow0 + r >= it.rows) continue;
-            if (all) {
-                hk_kv8_put(a, it, vrow0 + r, d * 32u + c * 4u, v, whole);
-                continue;
-            }
-            float *part = a.part_o +
-                          ((size_t)it.part * HK_PACKED_QB + wave * 32u + r) *
-                              DP + d * 32u + c * 4u;
-            *(float4 *)part = make_float4(v[0], v[1], v[2], v[3]);
-            *(float4 *)(part + 4) = make_float4(v[4], v[5], v[6], v[7]);
-        }
-    }
-}
-
-template <int DIMS>
-static void hk_kv8_launch(struct h3_gpu *gpu, const hk_kv8_args &g,
-                          const uint32_t *n) {
-    /* two blocks in f16; the join of few rows' waves takes as much */
-    const uint32_t lds = 2u * 256u * DIMS;
+static void hk_kv8_launch_few(struct h3_gpu *gpu, const hk_kv8_args &g,
+                              const uint32_t *n) {
+    const uint32_t lds = 4u * 32u * DIMS * 4u; /* the waves' O */
     const uint32_t most = 1u << 23; /* below 2^32 threads, turns of the XCDs */
     for (uint32_t first = 0; first < n[HK_PACKED_ITEMS]; first += most) {
         hk_kv8_args part = g;
         part.p.items += first;
-        const dim3 grid(std::min(n[HK_PACKED_ITEMS] - first, most));
-        /* (a workgroup whose item is the other kernel's ends at once) */
-        if (n[HK_PACKED_MANY])
-            hipLaunchKernelGGL(hk_kv8_flash<DIMS>, grid, dim3(256), lds,
-                               gpu->stream, part);
-        if (n[HK_PACKED_FEW])
-            hipLaunchKernelGGL(hk_kv8_few<DIMS>, grid, dim3(256), lds,
-                               gpu->stream, part);
+        hipLaunchKernelGGL(hk_kv8_few<DIMS>,
+                           dim3(std::min(n[HK_PACKED_ITEMS] - first, most)),
+                           dim3(256), lds, gpu->stream, part);
     }
-    if (g.p.part_o)
-        hk_packed_join_pieces(gpu, g.p, n, DIMS <= 64 ? 64u : 128u);
+}
+
+/* Unpacks the blocks that items of many rows read, for the kernel over rows
+ * (hk_packed_codes): once a call, where each item would do it again.  The
+ * kernel over rows is bound by the sum of its products and its vector
+ * instructions, and making f16 of codes and scaling each block's product added
+ * an eighth to those.  The values are rounded to bf16 on the way: their scale
+ * on P would round alike for all keys of a block, and on the sums cost the
+ * multiplications.  0 without memory for the rows. */
+static int hk_kv8_many(struct h3_gpu *gpu, const hk_kv8_args &g,
+                       const uint32_t *n) {
+    const hk_kv8_cache &c = g.cache;
+    const size_t width = (size_t)c.heads * c.dim;
+    const uint32_t blocks = n[HK_PACKED_SPAN_BLOCKS];
+    hk_packed_args a = g.p;
+    if (blocks) {
+        uint16_t *rows = (uint16_t *)hk_workspace(
+            gpu, (size_t)blocks * HK_KV8_BLOCK * 2u * width * 2u);
+        if (!rows) return 0;
+        const uint32_t most = std::max(1u, (1u << 22) / c.heads);
+        for (uint32_t first = 0; first < blocks; first += most)
+            hipLaunchKernelGGL(
+                hk_kv8_unpack, dim3(std::min(blocks - first, most), c.heads, 2),
+                dim3(256), HK_KV8_BLOCK * c.padded, gpu->stream, c, a.spans,
+                n[HK_PACKED_SPANS], rows, first);
+        a.k = rows;
+        a.v = rows + width;
+    }
+    a.kv_stride = 2u * width;
+    a.key_scales = (const float *)c.scales;
+    hk_packed_many_scaled(gpu, a, n);
+    return 1;
 }
 
 /* ================================================================ ops */
@@ -1156,23 +1080,28 @@ int h3_hip_sdpa_packed_int8_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
     a.p.o = HK_BF16(output);
     a.p.q_stride = query_stride;
     hk_op_begin(gpu, "attention_packed_int8");
-    /* (a scale of 0 times -inf, what keys past the end are set to, is no
-     * -inf) */
+    /* few rows: any head of up to 128; many: what the kernel over rows takes.
+     * (A scale of 0 times -inf, what keys past the end are set to, is no
+     * -inf.) */
+    a.p.kv_stride = 2u * (uint64_t)a.cache.heads * a.cache.dim;
     if (!gpu->reference_kernels && a.p.dim <= 128u &&
-        a.p.scale_log2 > 0x1p-100f && isfinite(a.p.scale_log2)) {
-        const size_t padded = a.p.dim <= 64u ? 64u : 128u;
+        a.p.scale_log2 > 0x1p-100f && isfinite(a.p.scale_log2) &&
+        (!n[HK_PACKED_MANY] || hk_packed_takes(gpu, a.p))) {
+        const uint32_t padded = a.p.dim <= 64u ? 64u : 128u;
         const size_t rows = (size_t)n[HK_PACKED_PARTS] * HK_PACKED_QB;
         if (rows)
             a.p.part_o = (float *)hk_splitk_try(
                 gpu, rows * (padded * sizeof(float) + sizeof(float2)));
         /* without scratch, items run whole */
         if (a.p.part_o) a.p.part_ml = (float2 *)(a.p.part_o + rows * padded);
-        switch (a.cache.padded) {
-        case 32: hk_kv8_launch<32>(gpu, a, n); break;
-        case 64: hk_kv8_launch<64>(gpu, a, n); break;
-        case 96: hk_kv8_launch<96>(gpu, a, n); break;
-        default: hk_kv8_launch<128>(gpu, a, n);
-        }
+        if (n[HK_PACKED_MANY] && !hk_kv8_many(gpu, a, n)) return 0;
+        if (n[HK_PACKED_FEW]) switch (a.cache.padded) {
+            case 32: hk_kv8_launch_few<32>(gpu, a, n); break;
+            case 64: hk_kv8_launch_few<64>(gpu, a, n); break;
+            case 96: hk_kv8_launch_few<96>(gpu, a, n); break;
+            default: hk_kv8_launch_few<128>(gpu, a, n);
+            }
+        if (a.p.part_o) hk_packed_join_pieces(gpu, a.p, n, padded);
         return hk_op_end(gpu, "attention_packed_int8", HK_KIND_SDPA);
     }
     const uint64_t blocks = ((uint64_t)a.p.rows * a.p.heads + 3) / 4;

@@ -46,7 +46,17 @@ enum { HK_PACKED_HEADS, HK_PACKED_KV_HEADS, HK_PACKED_DIM,
        HK_PACKED_JOIN_ROWS, /* the most virtual rows of a join */
        HK_PACKED_PARTS,
        HK_PACKED_OFF_BLOCKS, /* a request's keys begin inside 64 rows */
-       HK_PACKED_FEW, HK_PACKED_MANY /* items of up to 32 rows, and over */ };
+       HK_PACKED_FEW, HK_PACKED_MANY, /* items of up to 32 rows, and over */
+       HK_PACKED_SPANS, HK_PACKED_SPAN_BLOCKS };
+
+/* For a cache in blocks of 64 rows that is unpacked into rows for the items of
+ * many rows: blocks [block, + blocks) of it, which those items read, go to
+ * blocks [at, + blocks) of the rows.  Behind a plan's lists follow, if any
+ * request has such items and all begin at whole blocks, a word for each item,
+ * the first of its keys among those rows, and the spans. */
+struct hk_packed_span {
+    uint32_t block, at, blocks;
+};
 
 struct hk_packed_args {
     const uint16_t *q, *k, *v;
@@ -62,6 +72,11 @@ struct hk_packed_args {
      * (reference, sum) [part][HK_PACKED_QB] */
     float *part_o;
     float2 *part_ml;
+    /* keys that are codes (hk_packed_codes): the items' first rows, and the
+     * keys' scales, [block][key head][2] */
+    const uint32_t *kv_at;
+    const hk_packed_span *spans;
+    const float *key_scales;
 };
 
 /* The last request that begins at or before the plan's nth query row. */
@@ -91,6 +106,8 @@ static inline void hk_packed_of_plan(hk_packed_args &a,
     a.rows = n[HK_PACKED_ROWS];
     a.items = (const hk_packed_item *)(a.requests + a.request_count);
     a.joins = (const hk_packed_join *)(a.items + n[HK_PACKED_ITEMS]);
+    a.kv_at = (const uint32_t *)(a.joins + n[HK_PACKED_JOINS]);
+    a.spans = (const hk_packed_span *)(a.kv_at + n[HK_PACKED_ITEMS]);
 }
 
 /* Elements that a tensor needs for `rows` rows from `offset` on; sizes past
@@ -101,6 +118,11 @@ static inline size_t hk_packed_extent(size_t offset, uint64_t stride,
     return offset > SIZE_MAX - need ? SIZE_MAX : offset + need;
 }
 
+/* Whether the matrix-core kernel takes these rows. */
+bool hk_packed_takes(const struct h3_gpu *gpu, const hk_packed_args &a);
+/* Launches it on the items of many rows, over codes. */
+void hk_packed_many_scaled(struct h3_gpu *gpu, const hk_packed_args &a,
+                           const uint32_t *n);
 /* Launches the join of pieces' sums in rows of `padded` (64 or 128) dims. */
 void hk_packed_join_pieces(struct h3_gpu *gpu, const hk_packed_args &a,
                            const uint32_t *n, uint32_t padded);

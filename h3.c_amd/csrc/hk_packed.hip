@@ -26,6 +26,7 @@
 
 #include <algorithm>
 #include <functional>
+#include <map>
 #include <new>
 #include <queue>
 #include <type_traits>
@@ -447,9 +448,11 @@ __device__ __forceinline__ void hk_packed_few(const hk_packed_args &a,
     }
 }
 
-template <int DIMS>
-__global__ void __launch_bounds__(HK_PACKED_WAVES * 64, 2)
-hk_packed_flash(hk_packed_args a) {
+/* SCALED: keys are codes, whole numbers to 127 as bf16, of blocks of 64 rows
+ * with a scale each (hk_kv8.hip), which goes into L; references are scores as
+ * they are. */
+template <int DIMS, bool SCALED>
+__device__ __forceinline__ void hk_packed_item_of(const hk_packed_args &a) {
     constexpr int DP = DIMS <= 64 ? 64 : 128;
     constexpr int NK = DIMS / 16, ND = DIMS / 32, CHUNKS = DP / 8;
     constexpr uint32_t ROW = DP * 2u, TILE = HK_KT * ROW, STAGE = 2u * TILE;
@@ -469,7 +472,7 @@ hk_packed_flash(hk_packed_args a) {
         it.part = HK_PACKED_WHOLE;
     }
     if (it.rows - it.row <= 32u) {
-        hk_packed_few<DIMS>(a, it, hk_lds);
+        if (!SCALED) hk_packed_few<DIMS>(a, it, hk_lds);
         return;
     }
     const uint32_t dim_chunks = a.dim >> 3;
@@ -489,7 +492,15 @@ hk_packed_flash(hk_packed_args a) {
         v_off[i] = vc < dim_chunks ? row * stride + vc * 16u : 0x80000000u;
     }
     const uint64_t kv_base =
-        (uint64_t)it.kv_first * a.kv_stride + (uint64_t)it.kv_head * a.dim;
+        (uint64_t)(SCALED ? a.kv_at[blockIdx.x] : it.kv_first) * a.kv_stride +
+        (uint64_t)it.kv_head * a.dim;
+    /* the scale of the tile's block, loaded a tile ahead */
+    const float *block_scales =
+        SCALED ? a.key_scales +
+                     2u * ((size_t)(it.kv_first / HK_KT) * a.kv_heads +
+                           it.kv_head)
+               : NULL;
+    float ahead = 0.0f;
     auto issue_tile = [&](uint32_t tile, uint32_t stage) {
         const uint32_t kv0 = tile * HK_KT;
         const uint64_t base = kv_base + kv0 * a.kv_stride;
@@ -509,6 +520,7 @@ hk_packed_flash(hk_packed_args a) {
             hk_packed_dma16(kr, st + (wave * DMA + i) * 1024u, k_off[i]);
     };
     const uint32_t n = it.tile_end - it.tile;
+    if (SCALED && n) ahead = block_scales[2u * (size_t)it.tile * a.kv_heads];
     if (n) issue_tile(it.tile, 0);
 
     /* Q fragments, the B operand of S^T = K . Q^T: k-step ks of this lane's
@@ -576,8 +588,18 @@ hk_packed_flash(hk_packed_args a) {
                          auto tail_tag) {
         constexpr uint32_t stage = decltype(stage_tag)::value;
         constexpr bool tail = decltype(tail_tag)::value;
+        const float scale = ahead;
+        if (SCALED && more)
+            ahead = block_scales[2u * (size_t)(tile + 1u) * a.kv_heads];
         if (more) issue_tile(tile + 1u, stage ^ 1u);
         if (live) {
+        /* what multiplies a raw score: of a block of zeros they are 0, and -inf
+         * has to stay it */
+        float L = a.scale_log2;
+        if (SCALED) {
+            L = fmaxf(L * scale, 0x1p-120f);
+            if (isnan(scale)) L = scale; /* which fmaxf leaves out */
+        }
         hk_f32x16 s[2];
 #pragma unroll
         for (int kt = 0; kt < 2; kt++)
@@ -621,7 +643,7 @@ hk_packed_flash(hk_packed_args a) {
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
                     p[r] = __builtin_amdgcn_exp2f(
-                        __builtin_fmaf(s[kt][r], a.scale_log2, less));
+                        __builtin_fmaf(s[kt][r], L, less));
                     sum += p[r];
                 }
 #pragma unroll
@@ -648,6 +670,7 @@ hk_packed_flash(hk_packed_args a) {
             for (int kt = 0; kt < 2; kt++)
 #pragma unroll
                 for (int r = 0; r < 16; r++) mx = fmaxf(mx, s[kt][r]);
+            if (SCALED) mx *= scale;
             const auto sw = __builtin_amdgcn_permlane32_swap(
                 __float_as_uint(mx), __float_as_uint(mx), false, false);
             mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
@@ -665,7 +688,15 @@ hk_packed_flash(hk_packed_args a) {
 #pragma unroll
                 for (int kt = 0; kt < 2; kt++)
 #pragma unroll
-                    for (int r = 0; r < 16; r++) s[kt][r] -= by;
+                    for (int r = 0; r < 16; r++) {
+                        if (SCALED) {
+                            /* as the reference was rounded: no fused add */
+                            s[kt][r] *= scale;
+                            asm volatile("" : "+v"(s[kt][r]));
+                        }
+                        s[kt][r] -= by;
+                    }
+                if (SCALED) L = a.scale_log2;
                 if (hk_packed_far(less)) less = 0.0f;
             }
             l_part *= c;
@@ -791,6 +822,18 @@ hk_packed_flash(hk_packed_args a) {
     }
 }
 
+template <int DIMS>
+__global__ void __launch_bounds__(HK_PACKED_WAVES * 64, 2)
+hk_packed_flash(hk_packed_args a) {
+    hk_packed_item_of<DIMS, false>(a);
+}
+
+template <int DIMS>
+__global__ void __launch_bounds__(HK_PACKED_WAVES * 64, 2)
+hk_packed_codes(hk_packed_args a) {
+    hk_packed_item_of<DIMS, true>(a);
+}
+
 /* Joins the pieces of an item's rows: with the pieces' references m_p, sums
  * l_p and undivided O_p, O = sum_p w_p O_p / sum_p w_p l_p with w_p =
  * 2^((m_p - M) L), M = max_p m_p, in piece order.  A wave per row; a lane
@@ -853,7 +896,7 @@ void hk_packed_join_pieces(struct h3_gpu *gpu, const hk_packed_args &a,
                        dim3(256), 0, gpu->stream, a);
 }
 
-template <int DIMS>
+template <int DIMS, bool SCALED>
 static void hk_packed_launch(struct h3_gpu *gpu, const hk_packed_args &a,
                              const uint32_t *n) {
     constexpr int DP = DIMS <= 64 ? 64 : 128;
@@ -863,20 +906,28 @@ static void hk_packed_launch(struct h3_gpu *gpu, const hk_packed_args &a,
     for (uint32_t first = 0; first < n[HK_PACKED_ITEMS]; first += most) {
         hk_packed_args part = a;
         part.items = a.items + first;
-        hipLaunchKernelGGL(hk_packed_flash<DIMS>,
+        part.kv_at = a.kv_at + first;
+        hipLaunchKernelGGL(SCALED ? hk_packed_codes<DIMS>
+                                  : hk_packed_flash<DIMS>,
                            dim3(std::min(n[HK_PACKED_ITEMS] - first, most)),
                            dim3(HK_PACKED_WAVES * 64u), lds, gpu->stream,
                            part);
     }
-    if (a.part_o) hk_packed_join_pieces(gpu, a, n, DP);
+    if (!SCALED && a.part_o) hk_packed_join_pieces(gpu, a, n, DP);
+}
+
+void hk_packed_many_scaled(struct h3_gpu *gpu, const hk_packed_args &a,
+                           const uint32_t *n) {
+    if (a.dim <= 64) hk_packed_launch<64, true>(gpu, a, n);
+    else if (a.dim <= 96) hk_packed_launch<96, true>(gpu, a, n);
+    else hk_packed_launch<128, true>(gpu, a, n);
 }
 
 /* Whether the matrix-core kernel takes these rows: whole 16-byte pieces, 64
  * key rows and 128 query and output rows below 2^31 bytes (the reach of lane
  * offsets), and a scale that -inf times it is -inf, what keys past the end are
  * set to, and 0 times it 0. */
-static bool hk_packed_takes(const struct h3_gpu *gpu,
-                            const hk_packed_args &a) {
+bool hk_packed_takes(const struct h3_gpu *gpu, const hk_packed_args &a) {
     return !gpu->reference_kernels && a.dim % 8u == 0 && a.dim <= 128u &&
            a.q_stride % 8u == 0 && a.kv_stride % 8u == 0 &&
            a.kv_stride < (1u << 24) && a.q_stride < (1u << 23) &&
@@ -1191,9 +1242,37 @@ h3_gpu_tensor *h3_hip_sdpa_packed_plan(h3_gpu *gpu, const uint32_t *q_first,
         add(work.items.data(), work.items.size() * sizeof(work.items[0]));
         add(work.joins.data(), work.joins.size() * sizeof(work.joins[0]));
         if (words.empty()) words.push_back(0);
+        const size_t lists = words.size();
+        uint32_t few = 0, many = 0, span_blocks = 0;
+        std::map<uint32_t, hk_packed_span> spans; /* by their first block */
+        for (const hk_packed_item &item : work.items) {
+            if (item.row >= item.rows) continue;
+            (item.rows - item.row <= 32u ? few : many)++;
+            if (off_blocks || item.rows - item.row <= 32u || !item.kv_rows)
+                continue;
+            hk_packed_span &s = spans[item.kv_first / HK_KT];
+            s.block = item.kv_first / HK_KT;
+            s.blocks = std::max(
+                s.blocks, (uint32_t)(((uint64_t)item.kv_rows + HK_KT - 1) /
+                                     HK_KT));
+        }
+        for (auto &s : spans) {
+            s.second.at = span_blocks;
+            span_blocks += s.second.blocks;
+        }
+        if (!spans.empty()) {
+            for (const hk_packed_item &item : work.items) {
+                const auto s = item.row < item.rows
+                                   ? spans.find(item.kv_first / HK_KT)
+                                   : spans.end();
+                words.push_back(s == spans.end() ? 0u : s->second.at * HK_KT);
+            }
+            for (const auto &s : spans) add(&s.second, sizeof(s.second));
+        }
         h3_gpu_tensor *plan =
             h3_gpu_tensor_from_u32(gpu, words.data(), words.size());
         if (!plan) return NULL;
+        plan->elements = lists;
         plan->record.kind = HK_RECORD_PACKED;
         plan->record.n[HK_PACKED_HEADS] = heads;
         plan->record.n[HK_PACKED_KV_HEADS] = kv_heads;
@@ -1207,10 +1286,10 @@ h3_gpu_tensor *h3_hip_sdpa_packed_plan(h3_gpu *gpu, const uint32_t *q_first,
         plan->record.n[HK_PACKED_JOIN_ROWS] = work.join_rows;
         plan->record.n[HK_PACKED_PARTS] = work.parts;
         plan->record.n[HK_PACKED_OFF_BLOCKS] = off_blocks;
-        for (const hk_packed_item &item : work.items)
-            if (item.row < item.rows)
-                plan->record.n[item.rows - item.row <= 32u ? HK_PACKED_FEW
-                                                           : HK_PACKED_MANY]++;
+        plan->record.n[HK_PACKED_FEW] = few;
+        plan->record.n[HK_PACKED_MANY] = many;
+        plan->record.n[HK_PACKED_SPANS] = (uint32_t)spans.size();
+        plan->record.n[HK_PACKED_SPAN_BLOCKS] = span_blocks;
         return plan;
     } catch (const std::bad_alloc &) {
         hk_fail(gpu, "out of host memory");
@@ -1275,11 +1354,11 @@ int h3_hip_sdpa_packed_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
         /* without scratch, items run whole */
         if (a.part_o) a.part_ml = (float2 *)(a.part_o + rows * padded);
         if (dim <= 64)
-            hk_packed_launch<64>(gpu, a, n);
+            hk_packed_launch<64, false>(gpu, a, n);
         else if (dim <= 96)
-            hk_packed_launch<96>(gpu, a, n);
+            hk_packed_launch<96, false>(gpu, a, n);
         else
-            hk_packed_launch<128>(gpu, a, n);
+            hk_packed_launch<128, false>(gpu, a, n);
         return hk_op_end(gpu, "attention_packed", HK_KIND_SDPA);
     }
     const uint64_t blocks = ((uint64_t)a.rows * heads + 3) / 4;

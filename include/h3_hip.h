@@ -446,8 +446,11 @@ int h3_hip_kv_int8_read(h3_gpu *gpu, h3_gpu_tensor *key, h3_gpu_tensor *value,
 
 /* h3_hip_sdpa_packed_bf16 over such a cache: the plan's key rows are rows of
  * the cache, and every request's have to begin at a multiple of 64 (requests
- * may share them).  Scores, softmax and sums are F32; a weight P is rounded to
- * 11 bits (f16) before P . V. */
+ * may share them).  Scores, softmax and sums are F32, of keys as the codes and
+ * scales say.  P is rounded before P . V: to 11 bits (f16) where at most 32 query
+ * rows share a key head, to bf16 else, and there the values are too.  Blocks of
+ * such requests are unpacked into the context's scratch, 4 bytes for each row,
+ * key head and dim of them, which grows on demand. */
 int h3_hip_sdpa_packed_int8_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
                                  const h3_gpu_tensor *query,
                                  size_t query_offset, uint32_t query_stride,

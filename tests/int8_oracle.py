@@ -215,10 +215,12 @@ def attention(q, cache, ranges, heads, kv_heads, dim, scale):
                    2.0 ** -38 * top * np.abs(ks).sum(1) +
                    np.abs(qs) @ dk.T).max(1, keepdims=True) * scale + \
                 2.0 ** -22
-            # P rounds to 11 bits, or by 2^-25 at most, lifted by 2^7 against a
-            # reference that is at most the largest
+            # few rows of a key head: P rounds to 11 bits, or by 2^-25 at most,
+            # lifted by 2^7 against a reference that is at most the largest;
+            # else P and the values round to bf16
             bound[qf:qf + qn, h] = (p @ np.abs(vs)) * (
-                2.0 ** -11 + 2 * np.expm1(off) + 2 * (kn + 64) * F32) + \
+                (2.0 ** -11 if qn * group <= 32 else 2.01 * BF16) +
+                2 * np.expm1(off) + 2 * (kn + 64) * F32) + \
                 p @ dv + 2.0 ** -32 * p.max(1, keepdims=True) * \
                 np.abs(vs).sum(0)
     return o, rounded(o, bound), covered
