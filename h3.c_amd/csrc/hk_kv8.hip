@@ -434,24 +434,19 @@ __global__ void __launch_bounds__(256) hk_kv8_simple(hk_kv8_args g) {
     }
 }
 
-/* ------------------------------------------------- the matrix-core kernel
+/* -------------------------------------------- few rows on the matrix cores
  *
- * The plan's items (hk_packed.h), a block of 64 keys a tile: S^T = K . Q^T with
- * the Q fragments in registers, the softmax in the lanes that hold a query's
- * scores, O^T = V^T . P^T.  Codes and P are f16, which holds codes exactly and
- * is made of them in two instructions a pair.  A query row is scaled by a power
- * of two of its own to f16's range, which loses nothing of a bf16 within 2^27
- * of the row's largest; that and the block's key scale go into the factor of
- * the exponent.
+ * The plan's items of at most 32 rows (hk_packed.h), 32 keys a step: S^T = K .
+ * Q^T, the softmax in the lanes that hold a query's scores, O^T = V^T . P^T.
+ * Codes and P are f16, which holds codes exactly and is made of them in two
+ * instructions a pair.  A query row is scaled by a power of two of its own to
+ * f16's range, which loses nothing of a bf16 within 2^27 of the row's largest;
+ * that and the block's key scale go into the factor of the exponent.  The
+ * product with the values is multiplied by their scale as it is added to O.
  *
  * P = 2^((s - m) L + 7) against a reference m (a score, L = scale log2(e)) that
  * moves when a lane's sum of P passes 2^15: so f16 holds every P, to 11 bits
- * those over 2^-21 of the largest; the factor 2^7 is in the sums too.  A
- * block's product is multiplied by its value scale as it is added to O: 64
- * multiply-adds a lane.  (Taken into the exponents, with O in the largest scale
- * of the item's blocks, they went, but the scales had to be looked through
- * first and blocks far below them have a loop of their own, and four clips of
- * 6144 rows took 230 us for 224.) */
+ * those over 2^-21 of the largest; the factor 2^7 is in the sums too. */
 typedef _Float16 hk_f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 hk_f16x8 __attribute__((ext_vector_type(8)));
 
@@ -548,10 +543,8 @@ template <int DIMS> struct hk_kv8_wave {
         l = 0.0f;
     }
 
-    /* Raw scores (products with the codes) to P; `keys` of the block's rows
-     * count. */
-    __device__ __forceinline__ void softmax(hk_f32x16 (&s)[2],
-                                            hk_f16x8 (&p)[2][2],
+    /* Raw scores (products with the codes) to P; `keys` of the step's count. */
+    __device__ __forceinline__ void softmax(hk_f32x16 &s, hk_f16x8 (&p)[2],
                                             float scale, uint32_t keys,
                                             float L) {
         const uint32_t half = (threadIdx.x & 63u) >> 5;
@@ -561,27 +554,23 @@ template <int DIMS> struct hk_kv8_wave {
         if (by == 0.0f) by = 0x1p-100f;
         float own = by * L;
         if (own == 0.0f) own = 0x1p-126f;
-        if (keys < HK_KV8_BLOCK) {
-            asm volatile(""); /* a branch, not 32 selects in every block */
+        if (keys < 32u) {
+            asm volatile(""); /* a branch, not 16 selects in every step */
 #pragma unroll
-            for (int kt = 0; kt < 2; kt++)
-#pragma unroll
-                for (int r = 0; r < 16; r++)
-                    if (kt * 32u + (r >> 2) * 8u + half * 4u + (r & 3) >= keys)
-                        s[kt][r] = -INFINITY;
+            for (int r = 0; r < 16; r++)
+                if ((r >> 2) * 8u + half * 4u + (r & 3) >= keys)
+                    s[r] = -INFINITY;
         }
         auto exps = [&](float less) -> float {
             float sum = 0.0f;
             less += HK_KV8_LIFT;
 #pragma unroll
-            for (int kt = 0; kt < 2; kt++)
-#pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    const float e = __builtin_amdgcn_exp2f(
-                        __builtin_fmaf(s[kt][r], own, less));
-                    sum += e;
-                    p[kt][r >> 3][r & 7] = (_Float16)e;
-                }
+            for (int r = 0; r < 16; r++) {
+                const float e = __builtin_amdgcn_exp2f(
+                    __builtin_fmaf(s[r], own, less));
+                sum += e;
+                p[r >> 3][r & 7] = (_Float16)e;
+            }
             return sum;
         };
         const bool far = hk_kv8_far(neg); /* or unset */
@@ -595,9 +584,7 @@ template <int DIMS> struct hk_kv8_wave {
             move = both[0] | both[1];
             float mx = -INFINITY;
 #pragma unroll
-            for (int kt = 0; kt < 2; kt++)
-#pragma unroll
-                for (int r = 0; r < 16; r++) mx = fmaxf(mx, s[kt][r]);
+            for (int r = 0; r < 16; r++) mx = fmaxf(mx, s[r]);
             mx *= by;
             const auto sw = __builtin_amdgcn_permlane32_swap(
                 __float_as_uint(mx), __float_as_uint(mx), false, false);
@@ -614,13 +601,11 @@ template <int DIMS> struct hk_kv8_wave {
                  * reference off them first, which is exact near it */
                 const float off = hk_kv8_far(less) ? ref : 0.0f;
 #pragma unroll
-                for (int kt = 0; kt < 2; kt++)
-#pragma unroll
-                    for (int r = 0; r < 16; r++) {
-                        float x = s[kt][r] * by;
-                        asm volatile("" : "+v"(x)); /* no fused add */
-                        s[kt][r] = x - off;
-                    }
+                for (int r = 0; r < 16; r++) {
+                    float x = s[r] * by;
+                    asm volatile("" : "+v"(x)); /* no fused add */
+                    s[r] = x - off;
+                }
                 own = L;
                 if (hk_kv8_far(less)) less = 0.0f;
             }
@@ -634,27 +619,22 @@ template <int DIMS> struct hk_kv8_wave {
         l += sum;
     }
 
-    /* o += scale * the block's product, two groups of 32 dims at a time */
-    template <typename F>
-    __device__ __forceinline__ void values(const hk_f16x8 (&p)[2][2],
-                                           float scale, F fragments) {
+    /* o += scale * the step's product, two groups of 32 dims at a time */
+    __device__ __forceinline__ void values(const hk_f16x8 (&p)[2], float scale,
+                                           const uint4 (&codes)[ND]) {
 #pragma unroll
         for (int d0 = 0; d0 < ND; d0 += 2) {
             hk_f32x16 t[2];
 #pragma unroll
-            for (int i = 0; i < 2; i++)
+            for (int i = 0; i < 2; i++) {
+                if (d0 + i >= ND) continue;
 #pragma unroll
                 for (int r = 0; r < 16; r++) t[i][r] = 0.0f;
-#pragma unroll
-            for (int kt = 0; kt < 2; kt++)
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    if (d0 + i >= ND) continue;
-                    uint4 f[2];
-                    fragments(kt, d0 + i, f);
-                    t[i] = hk_kv8_mfma(f[0], p[kt][0], t[i]);
-                    t[i] = hk_kv8_mfma(f[1], p[kt][1], t[i]);
-                }
+                uint4 f[2];
+                hk_kv8_fragments(codes[d0 + i], f);
+                t[i] = hk_kv8_mfma(f[0], p[0], t[i]);
+                t[i] = hk_kv8_mfma(f[1], p[1], t[i]);
+            }
 #pragma unroll
             for (int i = 0; i < 2; i++)
 #pragma unroll
@@ -663,24 +643,6 @@ template <int DIMS> struct hk_kv8_wave {
                         o[d0 + i][r] = __builtin_fmaf(t[i][r], scale,
                                                       o[d0 + i][r]);
         }
-    }
-
-    template <typename Q, typename F>
-    __device__ __forceinline__ void scores(hk_f32x16 (&s)[2], Q query,
-                                           F fragments) {
-#pragma unroll
-        for (int kt = 0; kt < 2; kt++)
-#pragma unroll
-            for (int r = 0; r < 16; r++) s[kt][r] = 0.0f;
-#pragma unroll
-        for (int j = 0; j < ND; j++)
-#pragma unroll
-            for (int kt = 0; kt < 2; kt++) {
-                uint4 f[2];
-                fragments(kt, j, f);
-                s[kt] = hk_kv8_mfma(f[0], query(2 * j), s[kt]);
-                s[kt] = hk_kv8_mfma(f[1], query(2 * j + 1), s[kt]);
-            }
     }
 };
 
@@ -701,12 +663,12 @@ __device__ __forceinline__ void hk_kv8_put(const hk_packed_args &a,
         if (dim + e < a.dim) to[e] = hk_f2bf(v[e]);
 }
 
-/* Items of at most 32 rows: the waves share the rows and split the blocks,
- * wave w every fourth from the wth on, each straight from the cache into its
- * registers; then their sums are joined. */
+/* The waves share the item's rows and split its keys, wave w every fourth 32 of
+ * them from the wth on, straight from the cache into its registers; then their
+ * sums are joined, 64 dims at a time. */
 template <int DIMS>
-__global__ void __launch_bounds__(256, 2) hk_kv8_few(hk_kv8_args g) {
-    constexpr int ND = DIMS / 32, UNITS = DIMS / 16; /* of K or V */
+__global__ void __launch_bounds__(256, 3) hk_kv8_few(hk_kv8_args g) {
+    constexpr int ND = DIMS / 32;
     constexpr int DP = DIMS <= 64 ? 64 : 128;
     extern __shared__ __attribute__((aligned(16))) uint8_t hk_lds[];
     float *lds = (float *)hk_lds;
@@ -724,56 +686,58 @@ __global__ void __launch_bounds__(256, 2) hk_kv8_few(hk_kv8_args g) {
     const uint32_t col = lane & 31u, half = lane >> 5;
     const uint32_t vrow = it.row + col;
     const uint32_t first = it.kv_first / HK_KV8_BLOCK;
-    auto block_at = [&](uint32_t tile) {
-        return (size_t)(first + tile) * g.cache.heads + it.kv_head;
+    /* steps of 32 keys, two a block */
+    auto block_at = [&](uint32_t step) {
+        return (size_t)(first + (step >> 1)) * g.cache.heads + it.kv_head;
     };
-    uint4 k[UNITS], v[UNITS];
-    auto load = [&](uint32_t tile, int which, uint4 (&to)[UNITS]) {
+    uint4 k[ND], v[ND];
+    auto load = [&](uint32_t step, int which, uint4 (&to)[ND]) {
         const uint4 *from =
             (const uint4 *)(g.cache.codes +
-                            (block_at(tile) * 2u + which) *
-                                (HK_KV8_BLOCK * DIMS)) +
+                            ((block_at(step) * 2u + which) * 2u + (step & 1u)) *
+                                (32u * DIMS)) +
             lane;
 #pragma unroll
-        for (int u = 0; u < UNITS; u++) to[u] = from[u * 64];
+        for (int u = 0; u < ND; u++) to[u] = from[u * 64];
     };
-    uint32_t tile = it.tile + wave;
+    const uint32_t last =
+        min(it.tile_end * 2u, (it.kv_rows + 31u) / 32u); /* (below 2^28) */
+    uint32_t step = it.tile * 2u + wave;
     float2 ahead = make_float2(0.0f, 0.0f);
-    if (tile < it.tile_end) {
-        ahead = g.cache.scales[block_at(tile)];
-        load(tile, 0, k);
-        load(tile, 1, v);
+    if (step < last) {
+        ahead = g.cache.scales[block_at(step)];
+        load(step, 0, k);
+        load(step, 1, v);
     }
     hk_kv8_wave<DIMS> w;
     w.start(a, it, vrow);
-    /* the queries, the same for all waves, wait in LDS: in registers beside a
-     * block's keys and values they spilled */
+    /* the queries, the same for all waves, wait in LDS */
     hk_f16x8 *queries = (hk_f16x8 *)lds + lane;
     if (wave == 0) {
 #pragma unroll
         for (int i = 0; i < DIMS / 16; i++) queries[i * 64] = w.q[i];
     }
     __syncthreads();
-    for (; tile < it.tile_end; tile += HK_PACKED_WAVES) {
+    for (; step < last; step += HK_PACKED_WAVES) {
         const float2 scale = ahead;
-        /* past the last block, that one again, which no one uses */
+        /* past the last step, that one again, which no one uses */
         const uint32_t next =
-            tile + HK_PACKED_WAVES < it.tile_end ? tile + HK_PACKED_WAVES
-                                                 : tile;
-        hk_f32x16 s[2];
-        w.scores(
-            s, [&](int i) { return queries[i * 64]; },
-            [&](int kt, int j, uint4 (&f)[2]) {
-                hk_kv8_fragments(k[kt * ND + j], f);
-            });
+            step + HK_PACKED_WAVES < last ? step + HK_PACKED_WAVES : step;
+        hk_f32x16 s;
+#pragma unroll
+        for (int r = 0; r < 16; r++) s[r] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < ND; j++) {
+            uint4 f[2];
+            hk_kv8_fragments(k[j], f);
+            s = hk_kv8_mfma(f[0], queries[2 * j * 64], s);
+            s = hk_kv8_mfma(f[1], queries[(2 * j + 1) * 64], s);
+        }
         ahead = g.cache.scales[block_at(next)];
         load(next, 0, k);
-        hk_f16x8 p[2][2];
-        w.softmax(s, p, scale.x, it.kv_rows - tile * HK_KV8_BLOCK,
-                  a.scale_log2);
-        w.values(p, scale.y, [&](int kt, int d, uint4 (&f)[2]) {
-            hk_kv8_fragments(v[kt * ND + d], f);
-        });
+        hk_f16x8 p[2];
+        w.softmax(s, p, scale.x, it.kv_rows - step * 32u, a.scale_log2);
+        w.values(p, scale.y, v);
         load(next, 1, v);
     }
     /* references and sums of each row, then O scaled to the common reference
@@ -798,46 +762,51 @@ __global__ void __launch_bounds__(256, 2) hk_kv8_few(hk_kv8_args g) {
     if (all) weight *= l == 0.0f ? 0.0f : 1.0f / l;
     else if (wave == 0 && half == 0 && vrow < it.rows)
         a.part_ml[(size_t)it.part * HK_PACKED_QB + col] = make_float2(top, l);
-    __syncthreads();
-    /* rows of DIMS F32, 16-byte chunk c of row r at c ^ (r % 8) */
-    float *mine = lds + wave * (32u * DIMS);
-#pragma unroll
-    for (int d = 0; d < ND; d++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const uint32_t c = d * 8u + i * 2u + half;
-            *(float4 *)(mine + col * DIMS + ((c ^ (col & 7u)) << 2)) =
-                make_float4(w.o[d][i * 4] * weight, w.o[d][i * 4 + 1] * weight,
-                            w.o[d][i * 4 + 2] * weight,
-                            w.o[d][i * 4 + 3] * weight);
-        }
-    __syncthreads();
     const bool whole = a.dim % 8u == 0;
-    for (uint32_t at = tid; at < 32u * DIMS / 8u; at += 256u) {
-        const uint32_t r = at / (DIMS / 8u), c = at % (DIMS / 8u) * 2u;
-        if (it.row + r >= it.rows) continue;
-        float sum[8] = {};
+#pragma unroll
+    for (int d0 = 0; d0 < ND; d0 += 2) {
+        /* rows of 64 F32 a wave, 16-byte chunk c of row r at c ^ (r % 16) */
+        __syncthreads();
+#pragma unroll
+        for (int d = 0; d < 2; d++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if (d0 + d >= ND) continue;
+                const uint32_t c = d * 8u + i * 2u + half;
+                const hk_f32x16 &o = w.o[d0 + d];
+                *(float4 *)(lds + wave * 2048u + col * 64u +
+                            ((c ^ (col & 15u)) << 2)) =
+                    make_float4(o[i * 4] * weight, o[i * 4 + 1] * weight,
+                                o[i * 4 + 2] * weight, o[i * 4 + 3] * weight);
+            }
+        __syncthreads();
+        const uint32_t r = tid >> 3, c = (tid & 7u) * 2u;
+        const uint32_t dim = d0 * 32u + c * 4u;
+        if (it.row + r >= it.rows || dim >= DIMS) continue;
+        hk_f32x4 sum[2] = {};
 #pragma unroll
         for (uint32_t i = 0; i < HK_PACKED_WAVES; i++)
 #pragma unroll
-            for (int e = 0; e < 8; e++)
-                sum[e] += lds[i * (32u * DIMS) + r * DIMS +
-                              (((c + (e >> 2)) ^ (r & 7u)) << 2) + (e & 3)];
+            for (int e = 0; e < 2; e++)
+                sum[e] += *(const hk_f32x4 *)(lds + i * 2048u + r * 64u +
+                                              (((c + e) ^ (r & 15u)) << 2));
         if (all) {
-            hk_kv8_put(a, it, it.row + r, c * 4u, sum, whole);
+            const float y[8] = {sum[0][0], sum[0][1], sum[0][2], sum[0][3],
+                                sum[1][0], sum[1][1], sum[1][2], sum[1][3]};
+            hk_kv8_put(a, it, it.row + r, dim, y, whole);
             continue;
         }
-        float *part = a.part_o +
-                      ((size_t)it.part * HK_PACKED_QB + r) * DP + c * 4u;
-        *(float4 *)part = make_float4(sum[0], sum[1], sum[2], sum[3]);
-        *(float4 *)(part + 4) = make_float4(sum[4], sum[5], sum[6], sum[7]);
+        float *part =
+            a.part_o + ((size_t)it.part * HK_PACKED_QB + r) * DP + dim;
+        *(hk_f32x4 *)part = sum[0];
+        *(hk_f32x4 *)(part + 4) = sum[1];
     }
 }
 
 template <int DIMS>
 static void hk_kv8_launch_few(struct h3_gpu *gpu, const hk_kv8_args &g,
                               const uint32_t *n) {
-    const uint32_t lds = 4u * 32u * DIMS * 4u; /* the waves' O */
+    const uint32_t lds = 4u * 32u * 64u * 4u; /* 64 dims of the waves' O */
     const uint32_t most = 1u << 23; /* below 2^32 threads, turns of the XCDs */
     for (uint32_t first = 0; first < n[HK_PACKED_ITEMS]; first += most) {
         hk_kv8_args part = g;
