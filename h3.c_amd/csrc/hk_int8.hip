@@ -491,43 +491,43 @@ hk_int8_skinny(hk_skinny_args g, hk_int8_out o, uint32_t rows) {
     g.x += (size_t)row0 * g.k;
     g.m = min(g.m - row0, rows);
     g.x_bytes = g.m * g.k * 2u;
-    hk_i32x16 acc[MB];
-    hk_skinny_sums<MB, XA, HK_LOAD_ONCE>(g, g.w, blockIdx.x, blockIdx.y, acc);
-    const uint32_t lane = threadIdx.x & 63u, row = lane & 31u;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t tile = blockIdx.x * 4u + wave;
-    if (tile * 32u >= g.n) return;
-    if (g.partial) {
-        hk_skinny_partial<MB>((hk_v4i *)g.partial,
-                              ((size_t)blockIdx.z * gridDim.y + blockIdx.y) *
-                                      gridDim.x * 4u + tile,
-                              g.m, acc);
-        return;
-    }
-    /* all loads before the first store, which the compiler takes to change
-     * what they read: one after the other they took 8 of 13 us of a call */
-    hk_int8_columns columns[4];
-    float sx[MB];
-#pragma unroll
-    for (int q = 0; q < 4; q++)
-        columns[q].load(o, tile * 32u + q * 8u + (lane >> 5) * 4u);
-#pragma unroll
-    for (int mb = 0; mb < MB; mb++)
-        sx[mb] = o.xs[row0 + min(mb * 32u + row, g.m - 1u)];
-#pragma unroll
-    for (int mb = 0; mb < MB; mb++) {
-        if (mb * 32u + row >= g.m) continue;
-#pragma unroll
-        for (int q = 0; q < 4; q++) {
-            const uint32_t col = tile * 32u + q * 8u + (lane >> 5) * 4u;
-            if (col < g.n)
-                hk_int8_finish(o, row0 + mb * 32u + row, col, sx[mb],
-                               columns[q],
-                               hk_v4i{acc[mb][q * 4], acc[mb][q * 4 + 1],
-                                      acc[mb][q * 4 + 2],
-                                      acc[mb][q * 4 + 3]});
+    const auto use = [&](const hk_i32x16(&acc)[MB], uint32_t n0, uint32_t row,
+                         uint32_t half) {
+        if (n0 >= g.n) return;
+        if (g.partial) {
+            hk_skinny_partial<MB>((hk_v4i *)g.partial,
+                                  ((size_t)blockIdx.z * gridDim.y + blockIdx.y) *
+                                          gridDim.x * 4u + n0 / 32u,
+                                  g.m, acc);
+            return;
         }
-    }
+        /* all loads before the first store, which the compiler takes to change
+         * what they read: one after the other they took 8 of 13 us of a call */
+        hk_int8_columns columns[4];
+        float sx[MB];
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+            columns[q].load(o, n0 + q * 8u + half * 4u);
+#pragma unroll
+        for (int mb = 0; mb < MB; mb++)
+            sx[mb] = o.xs[row0 + min(mb * 32u + row, g.m - 1u)];
+#pragma unroll
+        for (int mb = 0; mb < MB; mb++) {
+            if (mb * 32u + row >= g.m) continue;
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const uint32_t col = n0 + q * 8u + half * 4u;
+                if (col < g.n)
+                    hk_int8_finish(o, row0 + mb * 32u + row, col, sx[mb],
+                                   columns[q],
+                                   hk_v4i{acc[mb][q * 4], acc[mb][q * 4 + 1],
+                                          acc[mb][q * 4 + 2],
+                                          acc[mb][q * 4 + 3]});
+            }
+        }
+    };
+    hk_skinny_sums<MB, XA, HK_LOAD_ONCE, hk_i32x16>(g, g.w, blockIdx.x,
+                                                    blockIdx.y, use);
 }
 
 /* Adds the pieces, as hk_skinny_reduce. */
