@@ -482,52 +482,84 @@ hk_int8_dot(hk_skinny_args g, hk_int8_out o, uint32_t pitch) {
     }
 }
 
-/* Few rows: the skinny GEMM's loop (hk_skinny_tile.h) over bytes, `rows` of them
- * a workgroup, groups of rows in the grid's third dimension. */
-template <int MB, int XA>
+/* How few rows run: groups of 32 mbs rows, and K in pieces where one workgroup
+ * per 128 columns and group leaves CUs idle (hk_gemm_skinny_run). */
+struct hk_int8_few_plan {
+    uint32_t groups, mbs, columns, splits, steps;
+};
+
+/* Few rows: the skinny GEMM's loop (hk_skinny_tile.h) over bytes, a workgroup
+ * per 128 columns, piece of K and group of rows.  The groups of the same columns
+ * follow each other on the same XCD, which has W's lines in its L2 after the
+ * first (workgroup i runs on XCD i % 8): with the groups last in the grid 300 x
+ * 1001 -> 5350 took 9.8 us, now 8.8, 256 x 5120 -> 13824 39.3 and 35.4.  A lone
+ * group keeps the grid's order (128 x 5376 -> 28672: 37 us, dealt so 40). */
+template <int MB>
 __global__ void __launch_bounds__(256)
-hk_int8_skinny(hk_skinny_args g, hk_int8_out o, uint32_t rows) {
-    const uint32_t row0 = blockIdx.z * rows;
+hk_int8_skinny(hk_skinny_args g, hk_int8_out o, hk_int8_few_plan plan) {
+    uint32_t at = blockIdx.x;
+    if (plan.groups > 1u)
+        at = at % 8u * (gridDim.x / 8u) + at / 8u;
+    const uint32_t unit = at / plan.groups, z = at - unit * plan.groups;
+    const uint32_t y = unit / plan.columns, x = unit - y * plan.columns;
+    if (y >= plan.splits) return;
+    const uint32_t rows = plan.mbs * 32u, row0 = z * rows;
     g.x += (size_t)row0 * g.k;
     g.m = min(g.m - row0, rows);
     g.x_bytes = g.m * g.k * 2u;
+    /* a lane's four columns of each eighth row, and the scales of rows lane and
+     * lane + 64: on their way during the loop */
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    hk_int8_columns columns;
+    float sx[(MB + 1) / 2];
+    if (!g.partial) {
+        columns.load(o, (x * 4u + wave) * 32u + (lane & 7u) * 4u);
+#pragma unroll
+        for (uint32_t i = 0; i < (MB + 1) / 2; i++)
+            sx[i] = o.xs[row0 + min(i * 64u + lane, g.m - 1u)];
+    }
     const auto use = [&](const hk_i32x16(&acc)[MB], uint32_t n0, uint32_t row,
-                         uint32_t half) {
+                         uint32_t half, uint8_t *wbuf) {
         if (n0 >= g.n) return;
         if (g.partial) {
             hk_skinny_partial<MB>((hk_v4i *)g.partial,
-                                  ((size_t)blockIdx.z * gridDim.y + blockIdx.y) *
-                                          gridDim.x * 4u + n0 / 32u,
+                                  ((size_t)z * plan.splits + y) *
+                                          plan.columns * 4u + n0 / 32u,
                                   g.m, acc);
             return;
         }
-        /* all loads before the first store, which the compiler takes to change
-         * what they read: one after the other they took 8 of 13 us of a call */
-        hk_int8_columns columns[4];
-        float sx[MB];
+        /* all loads are in before the first store: behind one, a wait for them
+         * would be one for the stores as well */
 #pragma unroll
-        for (int q = 0; q < 4; q++)
-            columns[q].load(o, n0 + q * 8u + half * 4u);
+        for (int e = 0; e < 4; e++)
+            asm volatile("" : "+v"(columns.scale[e]), "+v"(columns.bias[e]));
 #pragma unroll
-        for (int mb = 0; mb < MB; mb++)
-            sx[mb] = o.xs[row0 + min(mb * 32u + row, g.m - 1u)];
+        for (int i = 0; i < (MB + 1) / 2; i++) asm volatile("" : "+v"(sx[i]));
+        const uint32_t col = n0 + (lane & 7u) * 4u;
 #pragma unroll
         for (int mb = 0; mb < MB; mb++) {
-            if (mb * 32u + row >= g.m) continue;
+            /* through the wave's LDS, so that eight lanes write a row's 32
+             * columns: rows of 128 bytes, 16-byte chunk c of row r at c ^ r % 8 */
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                const uint32_t col = n0 + q * 8u + half * 4u;
-                if (col < g.n)
-                    hk_int8_finish(o, row0 + mb * 32u + row, col, sx[mb],
-                                   columns[q],
-                                   hk_v4i{acc[mb][q * 4], acc[mb][q * 4 + 1],
-                                          acc[mb][q * 4 + 2],
-                                          acc[mb][q * 4 + 3]});
+            for (uint32_t q = 0; q < 4; q++)
+                *(hk_v4i *)(wbuf + row * 128u +
+                            (((q * 2u + half) ^ (row & 7u)) << 4)) =
+                    hk_v4i{acc[mb][q * 4], acc[mb][q * 4 + 1],
+                           acc[mb][q * 4 + 2], acc[mb][q * 4 + 3]};
+#pragma unroll 1
+            for (uint32_t i = 0; i < 4; i++) {
+                const uint32_t r = i * 8u + (lane >> 3);
+                const hk_v4i sums = *(const hk_v4i *)(
+                    wbuf + r * 128u + (((lane & 7u) ^ (r & 7u)) << 4));
+                const float s = __shfl(sx[mb / 2], (mb & 1) * 32 + r, 64);
+                if (mb * 32u + r < g.m && col < g.n)
+                    hk_int8_finish(o, row0 + mb * 32u + r, col, s, columns,
+                                   sums);
             }
         }
     };
-    hk_skinny_sums<MB, XA, HK_LOAD_ONCE, hk_i32x16>(g, g.w, blockIdx.x,
-                                                    blockIdx.y, use);
+    hk_skinny_sums<MB, 3, HK_LOAD_ONCE, hk_i32x16>(g, g.w, x, y, use);
 }
 
 /* Adds the pieces, as hk_skinny_reduce. */
@@ -723,27 +755,48 @@ static void hk_int8_tiles(struct h3_gpu *gpu, const hk_int8_matrix &x,
                            gpu->stream, g, o, r.splits);
 }
 
-/* How few rows run: groups of up to 128, and K in pieces where one workgroup
- * per 128 columns and group leaves CUs idle (hk_gemm_skinny_run). */
-struct hk_int8_few_plan {
-    uint32_t groups, mbs, columns, splits, steps;
-};
-
+/* The plan of the least estimated time, which it returns: a step of K takes
+ * 0.18 us and 0.11 per 32 rows, what comes before and after the steps 2.4 and
+ * 0.95, joining pieces 4.5; more workgroups than CUs share them, four at once,
+ * and the groups' reads of W end at 6.5 TB/s.  (us by rows of a group, 32 / 64 /
+ * 96 / 128: 512 x 1024 -> 1024 5.9 / 7.6 / 9.3 / 11.3, 300 x 2675 -> 1001 10.3 /
+ * 11.3 / 12.6 / 14.4, 197 x 5120 -> 5120 33 / 24.1 / 20.5 / 22.5, 256 x 5120 ->
+ * 13824 70 / 46 / 53 / 35.) */
 static hk_int8_few_plan hk_int8_few_planned(uint32_t cus, uint32_t m,
-                                            uint32_t n, uint32_t k_steps) {
-    hk_int8_few_plan p;
-    p.groups = (m + 127u) / 128u;
-    p.mbs = ((m + p.groups - 1u) / p.groups + 31u) / 32u;
-    p.columns = (n + 127u) / 128u;
-    p.splits = std::max(
-        1u, std::min(cus / (p.columns * p.groups), k_steps / 8u));
-    p.steps = k_steps;
-    if (p.splits > 1) {
-        /* whole turns of the kernel's ring of 4 */
-        p.steps = ((k_steps + p.splits - 1u) / p.splits + 3u) & ~3u;
-        p.splits = (k_steps + p.steps - 1u) / p.steps;
+                                            uint32_t n, uint32_t k_steps,
+                                            float *us) {
+    hk_int8_few_plan best = {};
+    for (uint32_t most = 1; most <= 4; most++) {
+        hk_int8_few_plan p;
+        p.groups = (m + 32u * most - 1u) / (32u * most);
+        p.mbs = ((m + p.groups - 1u) / p.groups + 31u) / 32u;
+        if (p.mbs < most) continue; /* (that many groups have been tried) */
+        p.columns = (n + 127u) / 128u;
+        p.splits = std::max(
+            1u, std::min(cus / (p.columns * p.groups), k_steps / 8u));
+        p.steps = k_steps;
+        if (p.splits > 1) {
+            /* whole turns of the kernel's ring of 4 */
+            p.steps = ((k_steps + p.splits - 1u) / p.splits + 3u) & ~3u;
+            p.splits = (k_steps + p.steps - 1u) / p.steps;
+        }
+        const uint32_t workgroups = p.columns * p.groups * p.splits;
+        const float rounds =
+            workgroups <= cus
+                ? 1.0f
+                : 0.9f * (float)((workgroups + cus - 1u) / cus);
+        const float step = 0.18f + 0.11f * (float)p.mbs;
+        float t = (2.4f + 0.95f * (float)p.mbs + step * (float)p.steps) *
+                      rounds +
+                  (p.splits > 1 ? 4.5f : 0.0f);
+        t = std::max(t, (float)p.groups * (float)n * (float)k_steps *
+                            ((float)HK_INT8_LINE / 6.5e6f));
+        if (!best.groups || t < *us) {
+            best = p;
+            *us = t;
+        }
     }
-    return p;
+    return best;
 }
 
 static void hk_int8_few(struct h3_gpu *gpu, const hk_int8_matrix &x,
@@ -758,7 +811,7 @@ static void hk_int8_few(struct h3_gpu *gpu, const hk_int8_matrix &x,
     static uint64_t ready = 0;
     const uint64_t bit = 1ull << (gpu->device & 63);
     if (!(ready & bit)) {
-        (void)hipFuncSetAttribute((const void *)hk_int8_skinny<4, 3>,
+        (void)hipFuncSetAttribute((const void *)hk_int8_skinny<4>,
                                   hipFuncAttributeMaxDynamicSharedMemorySize,
                                   4 * 4096 * 4 + 16384);
         for (auto dot : {hk_int8_dot<1>, hk_int8_dot<2>})
@@ -775,21 +828,24 @@ static void hk_int8_few(struct h3_gpu *gpu, const hk_int8_matrix &x,
                            x.pitch, gpu->stream, g, o, x.pitch);
         return;
     }
+    float us;
     hk_int8_few_plan p = hk_int8_few_planned(hk_int8_cus(gpu), x.rows, o.n,
-                                             x.pitch / HK_INT8_LINE);
+                                             x.pitch / HK_INT8_LINE, &us);
     g.split_steps = p.steps;
     if (p.splits > 1)
         g.partial = (float *)hk_splitk_try(
             gpu, (size_t)p.groups * p.splits * p.columns * 4 * p.mbs * 4096);
     if (!g.partial) p.splits = 1; /* no scratch: in one piece */
-    void (*kernel)(hk_skinny_args, hk_int8_out, uint32_t) =
-        p.mbs == 1   ? hk_int8_skinny<1, 3>
-        : p.mbs == 2 ? hk_int8_skinny<2, 3>
-        : p.mbs == 3 ? hk_int8_skinny<3, 3>
-                     : hk_int8_skinny<4, 3>;
-    hipLaunchKernelGGL(kernel, dim3(p.columns, p.splits, p.groups), dim3(256),
-                       p.mbs * 4096 * 4 + 16384, gpu->stream, g, o,
-                       32u * p.mbs);
+    void (*kernel)(hk_skinny_args, hk_int8_out, hk_int8_few_plan) =
+        p.mbs == 1   ? hk_int8_skinny<1>
+        : p.mbs == 2 ? hk_int8_skinny<2>
+        : p.mbs == 3 ? hk_int8_skinny<3>
+                     : hk_int8_skinny<4>;
+    const uint32_t workgroups = p.columns * p.splits * p.groups;
+    hipLaunchKernelGGL(kernel,
+                       dim3(p.groups > 1u ? (workgroups + 7u) & ~7u : workgroups),
+                       dim3(256), p.mbs * 4096 * 4 + 16384, gpu->stream, g, o,
+                       p);
     if (p.splits > 1)
         hipLaunchKernelGGL(hk_int8_skinny_reduce,
                            dim3((o.n + 31u) / 32u * p.mbs, p.groups),
@@ -798,30 +854,23 @@ static void hk_int8_few(struct h3_gpu *gpu, const hk_int8_matrix &x,
 }
 
 /* Whether m rows run there rather than over tiles: up to 128 always, more of
- * them where the estimates say so, which were held against both ways at 117
- * sizes of 140 to 1024 rows (320 to 14336 -> 640 to 21504 columns).  The pick
- * is within 6% of the faster one at all but a K of 320 beside 13824 columns
- * (10.7 us and 13.9).  Us, here and over tiles: 197 x 1283 -> 2051 16 and 23,
- * 300 x 2675 -> 1001 14.5 and 20, 512 x 5120 -> 5120 32 and 39, 1024 x 5120 ->
- * 1024 19 and 31; 777 x 5120 -> 5120 54 and 43, 1024 x 5376 -> 21504 205 and
- * 111.  Few tiles are cut along K, and their pieces' sums cost as much as the
- * products; here a workgroup has an eighth of a tile. */
+ * them where the estimates say so (the tiles' is the bf16 GEMM's, a little above
+ * what these take), held against both ways at 110 sizes of 160 to 6144 rows (320
+ * to 13824 -> 320 to 28672 columns) and 36 of the gated block: the pick is
+ * within 12% of the faster one.  Us, here and over tiles: 300 x 5120 -> 2560 17.6
+ * and 23.5, 512 x 512 -> 1024 4.8 and 15, 1024 x 1024 -> 4096 12.8 and 33, 2378 x
+ * 5120 -> 640 21.5 and 32; 1024 x 5120 -> 13824 112 and 63, 2378 x 1024 -> 4096
+ * 26.7 and 17.4.  Few tiles are cut along K, and their pieces' sums cost as much
+ * as the products. */
 static bool hk_int8_takes_few(const struct h3_gpu *gpu, uint32_t m, uint32_t n,
                               uint32_t pitch) {
     if (m <= 128u) return true;
-    if (m > 1024u) return false;
-    const uint32_t cus = hk_int8_cus(gpu);
-    const hk_int8_few_plan p =
-        hk_int8_few_planned(cus, m, n, pitch / HK_INT8_LINE);
-    const uint32_t workgroups = p.columns * p.groups * p.splits;
-    const float rounds =
-        workgroups <= cus ? 1.0f
-                          : 0.8f * (float)((workgroups + cus - 1u) / cus);
-    const float us = (5.6f + 0.7f * (float)p.steps) * rounds +
-                     (p.splits > 1 ? 4.5f : 0.0f);
+    float us;
+    (void)hk_int8_few_planned(hk_int8_cus(gpu), m, n, pitch / HK_INT8_LINE,
+                              &us);
     float tiles;
     (void)hk_gemm_tile_rows(gpu, m, n, pitch / 2u, &tiles);
-    return us < tiles;
+    return us < 0.95f * tiles;
 }
 
 /* Whether x . w^T runs on the matrix cores: everything but weights of 4 GiB

@@ -80,11 +80,11 @@ __device__ __forceinline__ void hk_skinny_mfma(hk_i32x16 &acc, hk_v4i w,
     acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(w, x, acc, 0, 0, 0);
 }
 
-/* use(acc, n0, row, half) with the sums of piece y of workgroup x's columns:
- * acc[mb][r] = C[mb*32 + row][n0 + (r/4)*8 + half*4 + r%4], n0 = (4 x + wave)
- * 32, row and half of the lane.  Rows of bytes count K in pairs.  (With sums
- * that a caller holds, the compiler moves them about: 39 x 256 -> 10240, 5.0 us
- * for 4.8.) */
+/* use(acc, n0, row, half, wbuf) with the sums of piece y of workgroup x's
+ * columns: acc[mb][r] = C[mb*32 + row][n0 + (r/4)*8 + half*4 + r%4], n0 = (4 x +
+ * wave) 32, row and half of the lane, wbuf 4 KiB of LDS that are the wave's own.
+ * Rows of bytes count K in pairs.  (With sums that a caller holds, the compiler
+ * moves them about: 39 x 256 -> 10240, 5.0 us for 4.8.) */
 template <int MB, int XA, int W_POLICY, typename SUMS, typename USE>
 __device__ __forceinline__ void hk_skinny_sums(const hk_skinny_args &g,
                                                const uint16_t *w, uint32_t x,
@@ -223,7 +223,7 @@ __device__ __forceinline__ void hk_skinny_sums(const hk_skinny_args &g,
     }
     /* no load to LDS outlives the workgroup */
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    use(acc, n0, row, half);
+    use(acc, n0, row, half, wbuf);
 }
 
 /* A piece's sums, [32-column tile][MB][4][64 lanes] of four, `tile` counted
@@ -270,7 +270,7 @@ __device__ __forceinline__ void hk_skinny_tile(const hk_skinny_args &g,
         c = g.c1;
     }
     const auto use = [&](const hk_f32x16(&acc)[MB], uint32_t n0, uint32_t row,
-                         uint32_t half) {
+                         uint32_t half, uint8_t *) {
         if (g.partial) {
             if (n0 >= n) return;
             hk_skinny_partial<MB>(
