@@ -33,21 +33,27 @@ __device__ __forceinline__ uint32_t hk_magnitude(float v) {
     return __float_as_uint(v) & 0x7fffffffu;
 }
 
+/* (in registers; six turns through LDS took 0.3 us of a row's 2.6) */
 __device__ __forceinline__ uint32_t hk_wave_umax(uint32_t v) {
-#pragma unroll
-    for (int offset = 32; offset; offset >>= 1)
-        v = max(v, (uint32_t)__shfl_xor(v, offset, 64));
-    return v;
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xb1, 15, 15, true));
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4e, 15, 15, true));
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x124, 15, 15, true));
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x128, 15, 15, true));
+    const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max(a[0], a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return max(b[0], b[1]);
 }
 
 /* Over the workgroup; scratch as in hk_block_sum. */
 __device__ __forceinline__ uint32_t hk_block_umax(uint32_t v,
-                                                  uint32_t *scratch) {
+                                                  uint32_t *scratch,
+                                                  uint32_t waves) {
     v = hk_wave_umax(v);
-    const uint32_t waves = blockDim.x >> 6;
     __syncthreads();
     if ((threadIdx.x & 63u) == 0) scratch[threadIdx.x >> 6] = v;
     __syncthreads();
+#pragma unroll
     for (uint32_t w = 0; w < waves; w++) v = max(v, scratch[w]);
     return v;
 }

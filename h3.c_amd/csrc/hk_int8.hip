@@ -91,7 +91,7 @@ hk_int8_rows_any(hk_int8_rows_args a, uint32_t first) {
     uint32_t most = 0;
     for (uint32_t c = threadIdx.x; c < a.width; c += HK_INT8_THREADS)
         most = max(most, hk_magnitude(value(c)));
-    const hk_int8_quantizer code(hk_block_umax(most, tops));
+    const hk_int8_quantizer code(hk_block_umax(most, tops, HK_INT8_THREADS / 64u));
     int8_t *out = a.codes + (size_t)row * a.pitch;
     for (uint32_t c = threadIdx.x; c < a.pitch; c += HK_INT8_THREADS)
         out[c] = c < a.width ? (int8_t)(int)code(value(c)) : (int8_t)0;
@@ -222,7 +222,7 @@ hk_int8_rows_vec(hk_int8_rows_args a, uint32_t first) {
     for (int c = 0; c < CHUNKS; c++)
 #pragma unroll
         for (int i = 0; i < 8; i++) most = max(most, hk_magnitude(v[c][i]));
-    const hk_int8_quantizer code(hk_block_umax(most, tops));
+    const hk_int8_quantizer code(hk_block_umax(most, tops, THREADS / 64u));
     int8_t *out = a.codes + (size_t)row * a.pitch;
 #pragma unroll
     for (int c = 0; c < CHUNKS; c++) {

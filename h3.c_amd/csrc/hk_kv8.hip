@@ -102,7 +102,9 @@ __device__ __forceinline__ uint32_t hk_kv8_image(uint32_t byte) {
  * LDS, whole lines to the cache.  A block whose first row is new takes its
  * scale from the new rows and zeros in the others; in any other its rows keep
  * their codes unless the scale grows, and where it does not, the new rows'
- * bytes alone are written. */
+ * bytes alone are written.  PIECES of the block are a thread's, and ALIGNED rows
+ * are read 16 bytes at a time. */
+template <int PIECES, bool ALIGNED>
 __global__ void __launch_bounds__(256) hk_kv8_store(hk_kv8_store_args a) {
     __shared__ uint32_t tops[16];
     extern __shared__ __attribute__((aligned(16))) uint8_t image[];
@@ -110,9 +112,15 @@ __global__ void __launch_bounds__(256) hk_kv8_store(hk_kv8_store_args a) {
     const uint32_t tid = threadIdx.x, lane = tid & 63u;
     /* the last range that begins at or before the launch's block, a lane for
      * each (64 of them): scalar loads one after the other took 3 us */
+    const hk_kv8_range mine = a.ranges[lane];
     const uint64_t begun = __builtin_amdgcn_ballot_w64(
-        lane < a.count && a.ranges[lane].before <= blockIdx.x);
-    const hk_kv8_range r = a.ranges[__popcll(begun) - 1];
+        lane < a.count && mine.before <= blockIdx.x);
+    const int last = __popcll(begun) - 1;
+    const hk_kv8_range r = {
+        (uint32_t)__builtin_amdgcn_readlane((int)mine.cache, last),
+        (uint32_t)__builtin_amdgcn_readlane((int)mine.source, last),
+        (uint32_t)__builtin_amdgcn_readlane((int)mine.rows, last),
+        (uint32_t)__builtin_amdgcn_readlane((int)mine.before, last)};
     const uint32_t head = blockIdx.y, which = blockIdx.z;
     const uint32_t block = r.cache / HK_KV8_BLOCK + (blockIdx.x - r.before);
     /* rows [r0, r1) of the block are new, from row `from` on */
@@ -126,39 +134,40 @@ __global__ void __launch_bounds__(256) hk_kv8_store(hk_kv8_store_args a) {
     const size_t at = (size_t)block * c.heads + head;
     const uint16_t *x = (which ? a.value : a.key) + from * a.stride +
                         (uint64_t)head * c.dim;
-    const bool whole = c.dim % 8u == 0 && a.stride % 8u == 0 &&
-                       ((uintptr_t)(which ? a.value : a.key) & 15u) == 0;
     float *scale = (float *)(c.scales + at) + which;
     const float old = r0 ? *scale : 0.0f;
-    /* up to 512 pieces: two a thread */
-    uint4 rows[2][4];
+    uint4 rows[PIECES][4];
 #pragma unroll
-    for (int k = 0; k < 2; k++) {
+    for (int k = 0; k < PIECES; k++) {
         const hk_kv8_piece p(tid + k * 256u, c.padded);
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            uint4 v = make_uint4(0, 0, 0, 0);
             const uint32_t row = p.row + e;
-            if (tid + k * 256u < pieces && row >= r0 && row < r1 &&
-                p.dim < c.dim) {
+            const bool has = row >= r0 && row < r1 && p.dim < c.dim;
+            uint32_t w[4] = {};
+            if (ALIGNED) {
+                /* some new row's where it has none: no branch, behind which
+                 * the loads would wait for each other */
+                const uint4 v = *(const uint4 *)(
+                    x + (min(max(row, r0), r1 - 1u) - r0) * a.stride +
+                    min(p.dim, c.dim - 8u));
+                w[0] = has ? v.x : 0u;
+                w[1] = has ? v.y : 0u;
+                w[2] = has ? v.z : 0u;
+                w[3] = has ? v.w : 0u;
+            } else if (has) {
                 const uint16_t *y = x + (row - r0) * a.stride + p.dim;
-                if (whole) {
-                    v = *(const uint4 *)y;
-                } else {
-                    uint32_t w[4] = {};
 #pragma unroll
-                    for (int d = 0; d < 8; d++)
-                        if (p.dim + d < c.dim)
-                            w[d >> 1] |= (uint32_t)y[d] << (16 * (d & 1));
-                    v = make_uint4(w[0], w[1], w[2], w[3]);
-                }
+                for (int d = 0; d < 8; d++)
+                    if (p.dim + d < c.dim)
+                        w[d >> 1] |= (uint32_t)y[d] << (16 * (d & 1));
             }
-            rows[k][e] = v;
+            rows[k][e] = make_uint4(w[0], w[1], w[2], w[3]);
         }
     }
     uint32_t most = 0;
 #pragma unroll
-    for (int k = 0; k < 2; k++)
+    for (int k = 0; k < PIECES; k++)
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             float f[8];
@@ -166,7 +175,7 @@ __global__ void __launch_bounds__(256) hk_kv8_store(hk_kv8_store_args a) {
 #pragma unroll
             for (int d = 0; d < 8; d++) most = max(most, hk_magnitude(f[d]));
         }
-    most = hk_block_umax(most, tops); /* (everyone has the old scale by then) */
+    most = hk_block_umax(most, tops, 4u); /* (all have the old scale) */
     hk_int8_quantizer code(most);
     float keep = 1.0f;
     if (r0 && !(old < code.scale)) {
@@ -200,54 +209,56 @@ __global__ void __launch_bounds__(256) hk_kv8_store(hk_kv8_store_args a) {
         }
         __syncthreads();
     }
+    auto put = [&](auto place) {
 #pragma unroll
-    for (int k = 0; k < 2; k++) {
-        const hk_kv8_piece p(tid + k * 256u, c.padded);
-        /* none of its rows are new, nor to be cleared */
-        if (tid + k * 256u >= pieces ||
-            (r0 && (p.row + 4u <= r0 || p.row >= r1)))
-            continue;
-        float f[4][8];
+        for (int k = 0; k < PIECES; k++) {
+            const hk_kv8_piece p(tid + k * 256u, c.padded);
+            /* none of its rows are new, nor to be cleared */
+            if (tid + k * 256u >= pieces ||
+                (r0 && (p.row + 4u <= r0 || p.row >= r1)))
+                continue;
+            float f[4][8];
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            hk_unpack8(rows[k][e], f[e]);
+            for (int e = 0; e < 4; e++) {
+                hk_unpack8(rows[k][e], f[e]);
 #pragma unroll
-            for (int d = 0; d < 8; d++) f[e][d] = code(f[e][d]) + 128.0f;
-        }
-        uint8_t *to = few ? out : image;
-        auto place = [&](uint32_t byte) {
-            return few ? byte : hk_kv8_image(byte);
-        };
-        const bool all = !r0 || (p.row >= r0 && p.row + 4u <= r1);
-        if (which == 0) {
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                if (all || (p.row + e >= r0 && p.row + e < r1))
-                    *(uint2 *)(to + place(hk_kv8_key_at(p.row + e, p.dim,
-                                                        c.padded))) =
-                        make_uint2(hk_int8_pack4(f[e][0], f[e][1], f[e][2],
-                                                 f[e][3]),
-                                   hk_int8_pack4(f[e][4], f[e][5], f[e][6],
-                                                 f[e][7]));
-            continue;
-        }
-#pragma unroll
-        for (int d = 0; d < 8; d++) {
-            uint8_t *word =
-                to + place(hk_kv8_value_at(p.row, p.dim + d, c.padded));
-            const uint32_t w =
-                hk_int8_pack4(f[0][d], f[1][d], f[2][d], f[3][d]);
-            if (all) {
-                *(uint32_t *)word = w;
-            } else {
+                for (int d = 0; d < 8; d++) f[e][d] = code(f[e][d]) + 128.0f;
+            }
+            const bool all = !r0 || (p.row >= r0 && p.row + 4u <= r1);
+            if (which == 0) {
 #pragma unroll
                 for (int e = 0; e < 4; e++)
-                    if (p.row + e >= r0 && p.row + e < r1)
-                        word[e] = (uint8_t)(w >> (8 * e));
+                    if (all || (p.row + e >= r0 && p.row + e < r1))
+                        *(uint2 *)place(
+                            hk_kv8_key_at(p.row + e, p.dim, c.padded)) =
+                            make_uint2(hk_int8_pack4(f[e][0], f[e][1], f[e][2],
+                                                     f[e][3]),
+                                       hk_int8_pack4(f[e][4], f[e][5], f[e][6],
+                                                     f[e][7]));
+                continue;
+            }
+#pragma unroll
+            for (int d = 0; d < 8; d++) {
+                uint8_t *word =
+                    place(hk_kv8_value_at(p.row, p.dim + d, c.padded));
+                const uint32_t w =
+                    hk_int8_pack4(f[0][d], f[1][d], f[2][d], f[3][d]);
+                if (all) {
+                    *(uint32_t *)word = w;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (p.row + e >= r0 && p.row + e < r1)
+                            word[e] = (uint8_t)(w >> (8 * e));
+                }
             }
         }
+    };
+    if (few) {
+        put([&](uint32_t byte) { return out + byte; });
+        return;
     }
-    if (few) return;
+    put([&](uint32_t byte) { return image + hk_kv8_image(byte); });
     __syncthreads();
     for (uint32_t u = tid; u < part / 16u; u += 256u)
         *(uint4 *)(out + u * 16u) =
@@ -941,9 +952,15 @@ int h3_hip_kv_int8_store(h3_gpu *gpu, h3_gpu_tensor *cache,
     /* launches of up to 64 ranges and 2^22 / heads blocks */
     const uint32_t most = std::max(1u, (1u << 22) / c.heads);
     uint32_t total = 0;
+    const bool aligned = c.dim % 8u == 0 && kv_stride % 8u == 0 &&
+                         (((uintptr_t)a.key | (uintptr_t)a.value) & 15u) == 0;
+    auto kernel = c.padded > 128u
+                      ? aligned ? hk_kv8_store<2, true> : hk_kv8_store<2, false>
+                  : aligned ? hk_kv8_store<1, true>
+                            : hk_kv8_store<1, false>;
     auto launch = [&]() {
         if (a.count)
-            hipLaunchKernelGGL(hk_kv8_store, dim3(total, c.heads, 2), dim3(256),
+            hipLaunchKernelGGL(kernel, dim3(total, c.heads, 2), dim3(256),
                                HK_KV8_BLOCK * c.padded, gpu->stream, a);
         a.count = total = 0;
     };
