@@ -834,17 +834,14 @@ static void hk_kv8_launch_few(struct h3_gpu *gpu, const hk_kv8_args &g,
  * instructions, and making f16 of codes and scaling each block's product added
  * an eighth to those.  The values are rounded to bf16 on the way: their scale
  * on P would round alike for all keys of a block, and on the sums cost the
- * multiplications.  0 without memory for the rows. */
-static int hk_kv8_many(struct h3_gpu *gpu, const hk_kv8_args &g,
-                       const uint32_t *n) {
+ * multiplications. */
+static void hk_kv8_many(struct h3_gpu *gpu, const hk_kv8_args &g,
+                        const uint32_t *n, uint16_t *rows) {
     const hk_kv8_cache &c = g.cache;
     const size_t width = (size_t)c.heads * c.dim;
     const uint32_t blocks = n[HK_PACKED_SPAN_BLOCKS];
     hk_packed_args a = g.p;
     if (blocks) {
-        uint16_t *rows = (uint16_t *)hk_workspace(
-            gpu, (size_t)blocks * HK_KV8_BLOCK * 2u * width * 2u);
-        if (!rows) return 0;
         const uint32_t most = std::max(1u, (1u << 22) / c.heads);
         for (uint32_t first = 0; first < blocks; first += most)
             hipLaunchKernelGGL(
@@ -857,7 +854,6 @@ static int hk_kv8_many(struct h3_gpu *gpu, const hk_kv8_args &g,
     a.kv_stride = 2u * width;
     a.key_scales = (const float *)c.scales;
     hk_packed_many_scaled(gpu, a, n);
-    return 1;
 }
 
 /* ================================================================ ops */
@@ -1065,14 +1061,22 @@ int h3_hip_sdpa_packed_int8_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
     a.p.q = HK_CBF16(query) + query_offset;
     a.p.o = HK_BF16(output);
     a.p.q_stride = query_stride;
-    hk_op_begin(gpu, "attention_packed_int8");
     /* few rows: any head of up to 128; many: what the kernel over rows takes.
      * (A scale of 0 times -inf, what keys past the end are set to, is no
      * -inf.) */
     a.p.kv_stride = 2u * (uint64_t)a.cache.heads * a.cache.dim;
-    if (!gpu->reference_kernels && a.p.dim <= 128u &&
-        a.p.scale_log2 > 0x1p-100f && isfinite(a.p.scale_log2) &&
-        (!n[HK_PACKED_MANY] || hk_packed_takes(gpu, a.p))) {
+    const bool fast = !gpu->reference_kernels && a.p.dim <= 128u &&
+                      a.p.scale_log2 > 0x1p-100f && isfinite(a.p.scale_log2) &&
+                      (!n[HK_PACKED_MANY] || hk_packed_takes(gpu, a.p));
+    uint16_t *unpacked = NULL;
+    if (fast && n[HK_PACKED_SPAN_BLOCKS]) {
+        unpacked = (uint16_t *)hk_workspace(
+            gpu, (size_t)n[HK_PACKED_SPAN_BLOCKS] * HK_KV8_BLOCK * 2u *
+                     a.cache.heads * a.cache.dim * sizeof(uint16_t));
+        if (!unpacked) return 0;
+    }
+    hk_op_begin(gpu, "attention_packed_int8");
+    if (fast) {
         const uint32_t padded = a.p.dim <= 64u ? 64u : 128u;
         const size_t rows = (size_t)n[HK_PACKED_PARTS] * HK_PACKED_QB;
         if (rows)
@@ -1080,7 +1084,7 @@ int h3_hip_sdpa_packed_int8_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
                 gpu, rows * (padded * sizeof(float) + sizeof(float2)));
         /* without scratch, items run whole */
         if (a.p.part_o) a.p.part_ml = (float2 *)(a.p.part_o + rows * padded);
-        if (n[HK_PACKED_MANY] && !hk_kv8_many(gpu, a, n)) return 0;
+        if (n[HK_PACKED_MANY]) hk_kv8_many(gpu, a, n, unpacked);
         if (n[HK_PACKED_FEW]) switch (a.cache.padded) {
             case 32: hk_kv8_launch_few<32>(gpu, a, n); break;
             case 64: hk_kv8_launch_few<64>(gpu, a, n); break;

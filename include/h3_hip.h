@@ -405,7 +405,7 @@ int h3_hip_linear_gelu_int8_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
 /* The gated block of h3_gpu_mlp_bf16 in 8 bits: fc1 ([2 hidden][input], gate
  * rows first), h = silu(gate) up in F32, rows of h in 8 bits, fc2.  Uses the
  * context's scratch, which grows on demand: 5 bytes for each of rows x hidden,
- * up to 9 for at most 128 rows. */
+ * 9 where the rows are few enough to run without tiles. */
 int h3_hip_mlp_int8_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
                          const h3_gpu_tensor *input,
                          const h3_gpu_tensor *fc1_weight,
@@ -447,10 +447,11 @@ int h3_hip_kv_int8_read(h3_gpu *gpu, h3_gpu_tensor *key, h3_gpu_tensor *value,
 /* h3_hip_sdpa_packed_bf16 over such a cache: the plan's key rows are rows of
  * the cache, and every request's have to begin at a multiple of 64 (requests
  * may share them).  Scores, softmax and sums are F32, of keys as the codes and
- * scales say.  P is rounded before P . V: to 11 bits (f16) where at most 32 query
- * rows share a key head, to bf16 else, and there the values are too.  Blocks of
- * such requests are unpacked into the context's scratch, 4 bytes for each row,
- * key head and dim of them, which grows on demand. */
+ * scales say.  P is rounded before P . V: to 11 bits (f16) where the plan has items
+ * of up to 32 query rows of a key head, as where a request has no more, to bf16
+ * else, and there the values are too.  Blocks that such items read are unpacked
+ * into the context's scratch, 4 bytes for each row, key head and dim of them,
+ * which grows on demand. */
 int h3_hip_sdpa_packed_int8_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
                                  const h3_gpu_tensor *query,
                                  size_t query_offset, uint32_t query_stride,

@@ -146,7 +146,9 @@ SHAPES = [(1, 1, 1), (1, 128, 4), (2, 130, 31), (5, 64, 33), (32, 256, 128),
           (33, 300, 129), (64, 1024, 96), (65, 129, 257), (97, 640, 500),
           (128, 2000, 260), (129, 128, 128), (130, 500, 1000), (200, 1283, 513),
           (256, 512, 256), (257, 384, 255), (300, 2049, 771), (513, 257, 300),
-          (700, 896, 130), (1025, 128, 2), (1100, 640, 1111)]
+          (700, 896, 130), (1025, 128, 2), (1100, 640, 1111),
+          (40, 256, 1030), (70, 3000, 640), (100, 2000, 2100),
+          (150, 1283, 1411), (180, 2176, 129), (1500, 300, 100)]
 
 
 class Product:
