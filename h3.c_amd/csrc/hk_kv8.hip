@@ -19,6 +19,8 @@
 #include <algorithm>
 #include <vector>
 
+typedef _Float16 hk_f16x8 __attribute__((ext_vector_type(8)));
+
 #define HK_KV8_BLOCK 64u
 #define HK_KV8_RANGES 64u /* of a launch of the store */
 
@@ -268,7 +270,7 @@ __global__ void __launch_bounds__(256) hk_kv8_store(hk_kv8_store_args a) {
 /* Values of a block's keys or values (blockIdx.z) of a head, by way of the
  * block's image in LDS: the codes times `scale`, element d of row r at row(r) +
  * d, where row() is not NULL. */
-template <typename ROW>
+template <bool F16, typename ROW>
 __device__ __forceinline__ void hk_kv8_rows(const hk_kv8_cache &c, size_t at,
                                             uint32_t which, float scale,
                                             uint8_t *image, ROW row_of) {
@@ -310,7 +312,12 @@ __device__ __forceinline__ void hk_kv8_rows(const hk_kv8_cache &c, size_t at,
             uint16_t *to = p.dim < c.dim ? row_of(p.row + e) : NULL;
             if (!to) continue;
             to += p.dim;
-            if (c.dim % 8u == 0) {
+            if (F16 && which) { /* (dims in whole eights) */
+                hk_f16x8 v;
+#pragma unroll
+                for (int d = 0; d < 8; d++) v[d] = (_Float16)f[e][d];
+                *(hk_f16x8 *)to = v;
+            } else if (c.dim % 8u == 0) {
                 *(uint4 *)to = hk_pack8(f[e]);
             } else {
 #pragma unroll
@@ -330,8 +337,8 @@ hk_kv8_read(hk_kv8_cache c, uint16_t *key, uint16_t *value, uint32_t first,
     const uint32_t head = blockIdx.y, which = blockIdx.z;
     const size_t at = (size_t)block * c.heads + head;
     const uint64_t row0 = (uint64_t)block * HK_KV8_BLOCK;
-    hk_kv8_rows(c, at, which, ((const float *)(c.scales + at))[which], image,
-                [&](uint32_t r) -> uint16_t * {
+    hk_kv8_rows<false>(c, at, which, ((const float *)(c.scales + at))[which],
+                image, [&](uint32_t r) -> uint16_t * {
                     const uint64_t row = row0 + r;
                     if (row < first || row >= (uint64_t)first + rows)
                         return NULL;
@@ -340,11 +347,14 @@ hk_kv8_read(hk_kv8_cache c, uint16_t *key, uint16_t *value, uint32_t first,
                 });
 }
 
-/* A plan's spans of blocks as bf16 rows, [block][64][keys, values][head][dim]:
- * the keys' codes, which bf16 holds, and the values, rounded. */
+/* A plan's spans of blocks as rows, [block][64][keys, values][head][dim]: the
+ * keys' codes as bf16, which holds them, and the values as f16, divided by a
+ * power of two that leaves the span's largest in f16's range, 2^15 at most, and
+ * rounded to 11 bits (those under 2^-29 of it to fewer). */
 __global__ void __launch_bounds__(256)
 hk_kv8_unpack(hk_kv8_cache c, const hk_packed_span *spans, uint32_t count,
-              uint16_t *out, uint32_t first) {
+              uint16_t *out, float *units, uint32_t first) {
+    __shared__ uint32_t tops[16];
     extern __shared__ __attribute__((aligned(16))) uint8_t image[];
     const uint32_t to = first + blockIdx.x;
     uint32_t low = 0, high = count; /* the last span that begins by then */
@@ -353,15 +363,32 @@ hk_kv8_unpack(hk_kv8_cache c, const hk_packed_span *spans, uint32_t count,
         if (spans[mid].at <= to) low = mid;
         else high = mid;
     }
-    const uint32_t block = spans[low].block + (to - spans[low].at);
+    const hk_packed_span span = spans[low];
+    const uint32_t block = span.block + (to - span.at);
     const uint32_t head = blockIdx.y, which = blockIdx.z;
     const uint64_t row0 = (uint64_t)to * HK_KV8_BLOCK;
     const size_t at = (size_t)block * c.heads + head;
-    hk_kv8_rows(c, at, which, which ? c.scales[at].y : 1.0f, image,
-                [&](uint32_t r) -> uint16_t * {
-                    return out + (((row0 + r) * 2u + which) * c.heads + head) *
-                                     c.dim;
-                });
+    float scale = 1.0f;
+    if (which) {
+        uint32_t most = 0;
+        for (uint32_t i = threadIdx.x; i < span.blocks; i += 256u) {
+            const uint32_t s = hk_magnitude(
+                c.scales[((size_t)span.block + i) * c.heads + head].y);
+            if (s < HK_NOT_FINITE) most = max(most, s);
+        }
+        most = hk_block_umax(most, tops, 4u);
+        /* 127 scales over the unit are below 2^15 */
+        const uint32_t exponent = max(most >> 23, 8u) - 7u;
+        if (to == span.at && threadIdx.x == 0)
+            units[(size_t)to * c.heads + head] =
+                __uint_as_float(exponent << 23);
+        scale = c.scales[at].y * __uint_as_float((254u - exponent) << 23);
+    }
+    hk_kv8_rows<true>(c, at, which, scale, image,
+                      [&](uint32_t r) -> uint16_t * {
+                          return out + (((row0 + r) * 2u + which) * c.heads +
+                                        head) * c.dim;
+                      });
 }
 
 /* ---------------------------------------------------------- the attention */
@@ -459,7 +486,6 @@ __global__ void __launch_bounds__(256) hk_kv8_simple(hk_kv8_args g) {
  * moves when a lane's sum of P passes 2^15: so f16 holds every P, to 11 bits
  * those over 2^-21 of the largest; the factor 2^7 is in the sums too. */
 typedef _Float16 hk_f16x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 hk_f16x8 __attribute__((ext_vector_type(8)));
 
 #define HK_KV8_LIFT 7.0f
 #define HK_KV8_MOST 0x1p15f
@@ -832,11 +858,10 @@ static void hk_kv8_launch_few(struct h3_gpu *gpu, const hk_kv8_args &g,
  * (hk_packed_codes): once a call, where each item would do it again.  The
  * kernel over rows is bound by the sum of its products and its vector
  * instructions, and making f16 of codes and scaling each block's product added
- * an eighth to those.  The values are rounded to bf16 on the way: their scale
- * on P would round alike for all keys of a block, and on the sums cost the
- * multiplications. */
+ * an eighth to those.  The values' scales are in the rows: on P they would round
+ * alike for all keys of a block, on the sums cost the multiplications. */
 static void hk_kv8_many(struct h3_gpu *gpu, const hk_kv8_args &g,
-                        const uint32_t *n, uint16_t *rows) {
+                        const uint32_t *n, uint16_t *rows, float *units) {
     const hk_kv8_cache &c = g.cache;
     const size_t width = (size_t)c.heads * c.dim;
     const uint32_t blocks = n[HK_PACKED_SPAN_BLOCKS];
@@ -847,12 +872,13 @@ static void hk_kv8_many(struct h3_gpu *gpu, const hk_kv8_args &g,
             hipLaunchKernelGGL(
                 hk_kv8_unpack, dim3(std::min(blocks - first, most), c.heads, 2),
                 dim3(256), HK_KV8_BLOCK * c.padded, gpu->stream, c, a.spans,
-                n[HK_PACKED_SPANS], rows, first);
+                n[HK_PACKED_SPANS], rows, units, first);
         a.k = rows;
         a.v = rows + width;
     }
     a.kv_stride = 2u * width;
     a.key_scales = (const float *)c.scales;
+    a.value_units = units;
     hk_packed_many_scaled(gpu, a, n);
 }
 
@@ -1069,11 +1095,14 @@ int h3_hip_sdpa_packed_int8_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
                       a.p.scale_log2 > 0x1p-100f && isfinite(a.p.scale_log2) &&
                       (!n[HK_PACKED_MANY] || hk_packed_takes(gpu, a.p));
     uint16_t *unpacked = NULL;
+    float *units = NULL;
     if (fast && n[HK_PACKED_SPAN_BLOCKS]) {
+        const size_t heads = (size_t)n[HK_PACKED_SPAN_BLOCKS] * a.cache.heads;
+        const size_t elements = heads * HK_KV8_BLOCK * 2u * a.cache.dim;
         unpacked = (uint16_t *)hk_workspace(
-            gpu, (size_t)n[HK_PACKED_SPAN_BLOCKS] * HK_KV8_BLOCK * 2u *
-                     a.cache.heads * a.cache.dim * sizeof(uint16_t));
+            gpu, elements * sizeof(uint16_t) + heads * sizeof(float));
         if (!unpacked) return 0;
+        units = (float *)(unpacked + elements);
     }
     hk_op_begin(gpu, "attention_packed_int8");
     if (fast) {
@@ -1084,7 +1113,7 @@ int h3_hip_sdpa_packed_int8_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
                 gpu, rows * (padded * sizeof(float) + sizeof(float2)));
         /* without scratch, items run whole */
         if (a.p.part_o) a.p.part_ml = (float2 *)(a.p.part_o + rows * padded);
-        if (n[HK_PACKED_MANY]) hk_kv8_many(gpu, a, n, unpacked);
+        if (n[HK_PACKED_MANY]) hk_kv8_many(gpu, a, n, unpacked, units);
         if (n[HK_PACKED_FEW]) switch (a.cache.padded) {
             case 32: hk_kv8_launch_few<32>(gpu, a, n); break;
             case 64: hk_kv8_launch_few<64>(gpu, a, n); break;

@@ -72,11 +72,12 @@ struct hk_packed_args {
      * (reference, sum) [part][HK_PACKED_QB] */
     float *part_o;
     float2 *part_ml;
-    /* keys that are codes (hk_packed_codes): the items' first rows, and the
-     * keys' scales, [block][key head][2] */
+    /* keys that are codes (hk_packed_codes): the items' first rows, the keys'
+     * scales, [block][key head][2], and what the values are divided by, of a
+     * span's first block [block among the spans'][key head] */
     const uint32_t *kv_at;
     const hk_packed_span *spans;
-    const float *key_scales;
+    const float *key_scales, *value_units;
 };
 
 /* The last request that begins at or before the plan's nth query row. */

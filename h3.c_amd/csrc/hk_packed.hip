@@ -448,9 +448,13 @@ __device__ __forceinline__ void hk_packed_few(const hk_packed_args &a,
     }
 }
 
+typedef _Float16 hk_packed_f16x8 __attribute__((ext_vector_type(8)));
+
 /* SCALED: keys are codes, whole numbers to 127 as bf16, of blocks of 64 rows
- * with a scale each (hk_kv8.hip), which goes into L; references are scores as
- * they are. */
+ * with a scale each, which goes into L; references are scores as they are.
+ * Values are f16, divided by a power of two of the request's and the head's
+ * (hk_kv8.hip), and so are P, times 2^7, which move at 2^15: P rounds to 11
+ * bits over 2^-21 of the largest. */
 template <int DIMS, bool SCALED>
 __device__ __forceinline__ void hk_packed_item_of(const hk_packed_args &a) {
     constexpr int DP = DIMS <= 64 ? 64 : 128;
@@ -501,6 +505,11 @@ __device__ __forceinline__ void hk_packed_item_of(const hk_packed_args &a) {
                            it.kv_head)
                : NULL;
     float ahead = 0.0f;
+    const float unit =
+        SCALED && it.tile_end != it.tile
+            ? a.value_units[(size_t)(a.kv_at[blockIdx.x] / HK_KT) * a.kv_heads +
+                            it.kv_head]
+            : 1.0f;
     auto issue_tile = [&](uint32_t tile, uint32_t stage) {
         const uint32_t kv0 = tile * HK_KT;
         const uint64_t base = kv_base + kv0 * a.kv_stride;
@@ -634,9 +643,12 @@ __device__ __forceinline__ void hk_packed_item_of(const hk_packed_args &a) {
          * unrounded P: the result is off by 2^-8 of a weight at most where F32
          * weights would leave it at the rounding of the output, 0.0023 and
          * 0.0017 of its norm for 1500 keys. */
-        hk_bf16x8 pf[2][2];
+        typedef std::conditional_t<SCALED, hk_packed_f16x8, hk_bf16x8> frag;
+        typedef std::conditional_t<SCALED, _Float16, __bf16> rounded;
+        frag pf[2][2];
         auto exps = [&](float less) -> float {
             float sum = 0.0f;
+            if (SCALED) less += 7.0f;
 #pragma unroll
             for (int kt = 0; kt < 2; kt++) {
                 float p[16];
@@ -648,9 +660,9 @@ __device__ __forceinline__ void hk_packed_item_of(const hk_packed_args &a) {
                 }
 #pragma unroll
                 for (int st = 0; st < 2; st++) {
-                    hk_bf16x8 v;
+                    frag v;
 #pragma unroll
-                    for (int e = 0; e < 8; e++) v[e] = (__bf16)p[st * 8 + e];
+                    for (int e = 0; e < 8; e++) v[e] = (rounded)p[st * 8 + e];
                     pf[kt][st] = v;
                 }
             }
@@ -658,7 +670,7 @@ __device__ __forceinline__ void hk_packed_item_of(const hk_packed_args &a) {
         };
         const bool far = hk_packed_far(neg); /* or unset */
         float sum = far ? 0.0f : exps(neg);
-        uint32_t move = far || sum > 0x1p32f;
+        uint32_t move = far || sum > (SCALED ? 0x1p15f : 0x1p32f);
         if (__builtin_amdgcn_ballot_w64(move)) {
             /* a row's other half's too, but no other row's: what a row comes
              * to does not depend on the rows beside it */
@@ -725,9 +737,14 @@ __device__ __forceinline__ void hk_packed_item_of(const hk_packed_args &a) {
             for (int d = 0; d < ND; d++) {
                 const hk_v4i both = {vt[i & 1][d][0][0], vt[i & 1][d][0][1],
                                      vt[i & 1][d][1][0], vt[i & 1][d][1][1]};
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                    __builtin_bit_cast(hk_bf16x8, both), pf[kt][st], o[d], 0,
-                    0, 0);
+                if constexpr (SCALED)
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+                        __builtin_bit_cast(frag, both), pf[kt][st], o[d], 0, 0,
+                        0);
+                else
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                        __builtin_bit_cast(frag, both), pf[kt][st], o[d], 0, 0,
+                        0);
             }
         }
         } /* live */
@@ -765,6 +782,10 @@ __device__ __forceinline__ void hk_packed_item_of(const hk_packed_args &a) {
         float *part = a.part_o + (size_t)it.part * HK_PACKED_QB * DP;
 #pragma unroll
         for (int d = 0; d < ND; d++) {
+            if (SCALED) {
+#pragma unroll
+                for (int r = 0; r < 16; r++) o[d][r] *= unit;
+            }
 #pragma unroll
             for (int blk = 0; blk < 4; blk++) {
                 const uint32_t c = blk * 2u + half;
@@ -788,7 +809,8 @@ __device__ __forceinline__ void hk_packed_item_of(const hk_packed_args &a) {
         return;
     }
     /* no keys, or none with weight: zeros (a NaN sum gives NaN) */
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    if (SCALED) inv *= unit;
     uint8_t *ow = hk_lds + wave * (32u * ROW);
 #pragma unroll
     for (int d = 0; d < ND; d++)
@@ -1244,17 +1266,21 @@ h3_gpu_tensor *h3_hip_sdpa_packed_plan(h3_gpu *gpu, const uint32_t *q_first,
         if (words.empty()) words.push_back(0);
         const size_t lists = words.size();
         uint32_t few = 0, many = 0, span_blocks = 0;
-        std::map<uint32_t, hk_packed_span> spans; /* by their first block */
+        /* by their first block and their number: what a request comes to does
+         * not depend on keys that only others read */
+        std::map<std::pair<uint32_t, uint32_t>, hk_packed_span> spans;
+        auto span_of = [](const hk_packed_item &item) {
+            return std::make_pair(
+                item.kv_first / HK_KT,
+                (uint32_t)(((uint64_t)item.kv_rows + HK_KT - 1) / HK_KT));
+        };
         for (const hk_packed_item &item : work.items) {
             if (item.row >= item.rows) continue;
             (item.rows - item.row <= 32u ? few : many)++;
             if (off_blocks || item.rows - item.row <= 32u || !item.kv_rows)
                 continue;
-            hk_packed_span &s = spans[item.kv_first / HK_KT];
-            s.block = item.kv_first / HK_KT;
-            s.blocks = std::max(
-                s.blocks, (uint32_t)(((uint64_t)item.kv_rows + HK_KT - 1) /
-                                     HK_KT));
+            const auto span = span_of(item);
+            spans[span] = {span.first, 0, span.second};
         }
         for (auto &s : spans) {
             s.second.at = span_blocks;
@@ -1263,7 +1289,7 @@ h3_gpu_tensor *h3_hip_sdpa_packed_plan(h3_gpu *gpu, const uint32_t *q_first,
         if (!spans.empty()) {
             for (const hk_packed_item &item : work.items) {
                 const auto s = item.row < item.rows
-                                   ? spans.find(item.kv_first / HK_KT)
+                                   ? spans.find(span_of(item))
                                    : spans.end();
                 words.push_back(s == spans.end() ? 0u : s->second.at * HK_KT);
             }

@@ -447,11 +447,11 @@ int h3_hip_kv_int8_read(h3_gpu *gpu, h3_gpu_tensor *key, h3_gpu_tensor *value,
 /* h3_hip_sdpa_packed_bf16 over such a cache: the plan's key rows are rows of
  * the cache, and every request's have to begin at a multiple of 64 (requests
  * may share them).  Scores, softmax and sums are F32, of keys as the codes and
- * scales say.  P is rounded before P . V: to 11 bits (f16) where the plan has items
- * of up to 32 query rows of a key head, as where a request has no more, to bf16
- * else, and there the values are too.  Blocks that such items read are unpacked
- * into the context's scratch, 4 bytes for each row, key head and dim of them,
- * which grows on demand. */
+ * scales say.  P is rounded to 11 bits (f16) before P . V.  Blocks that the plan's
+ * items of more than 32 query rows read are unpacked into the context's scratch,
+ * which grows on demand, 4 bytes for each row, key head and dim of them; there
+ * the values are rounded to 11 bits as well, those under 2^-29 of the largest of
+ * the request and key head to fewer. */
 int h3_hip_sdpa_packed_int8_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
                                  const h3_gpu_tensor *query,
                                  size_t query_offset, uint32_t query_stride,

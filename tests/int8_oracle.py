@@ -215,12 +215,16 @@ def attention(q, cache, ranges, heads, kv_heads, dim, scale):
                    2.0 ** -38 * top * np.abs(ks).sum(1) +
                    np.abs(qs) @ dk.T).max(1, keepdims=True) * scale + \
                 2.0 ** -22
-            # few rows of a key head: P rounds to 11 bits, or by 2^-25 at most,
-            # lifted by 2^7 against a reference that is at most the largest;
-            # else P and the values round to bf16
+            # P rounds to 11 bits, or by 2^-25 at most, lifted by 2^7 against a
+            # reference that is at most the largest; of many rows of a key head
+            # the values round to 11 bits too, or by 2^-25 of a unit that is at
+            # most 2^-14 of the largest value its blocks have codes for
             bound[qf:qf + qn, h] = (p @ np.abs(vs)) * (
-                (2.0 ** -11 if qn * group <= 32 else 2.01 * BF16) +
+                (2.0 ** -11 if qn * group <= 32 else 2.01 * 2.0 ** -11) +
                 2 * np.expm1(off) + 2 * (kn + 64) * F32) + \
                 p @ dv + 2.0 ** -32 * p.max(1, keepdims=True) * \
                 np.abs(vs).sum(0)
+            if qn * group > 32:
+                top = cache.s[kf // 64:(kf + kn + 63) // 64, 1, h // group]
+                bound[qf:qf + qn, h] += 2.0 ** -39 * 127 * top.max()
     return o, rounded(o, bound), covered

@@ -335,3 +335,32 @@ def test_next_tokens(gpu):
         c.kv.store([f + n for f, n in zip(c.kf, c.kn)], [1, 1], std=1.5)
         c.kn = [n + 1 for n in c.kn]
         c.check()
+
+
+@pytest.mark.parametrize("powers", [[0, 9, -9, 4], [-60, -70, -50, -55],
+                                    [60, 70, 50, 66], [0, 40, -40, 3]])
+def test_many_rows_of_unlike_scales(gpu, powers):
+    """Items of 128 rows, whose values share a unit."""
+    def change(rows):
+        v = ro.wide(rows, *rows.shape)
+        for block, power in enumerate(powers):
+            v[64 * block:64 * block + 64, 8 * 64:] *= 2.0 ** power
+        rows[:] = io.bits(v.astype(np.float32)).reshape(rows.shape)
+    c = Case(gpu, [4096], [256], 8, 8, 64)
+    c.kv.store([0], [256], change=change)
+    c.check()
+    assert np.isfinite(ro.wide(c.run(), 4096, 512)).all()
+
+
+def test_keys_of_others_have_no_part(gpu):
+    """Two requests share their first blocks; the longer one's last blocks are
+    larger by 2^90 or not finite."""
+    c = Case(gpu, [4096, 4096], [128, 256], 8, 8, 64, share=True)
+    first = c.check()[:4096]
+
+    def change(rows):
+        v = ro.wide(rows, *rows.shape) * 2.0 ** 90
+        rows[:] = io.bits(v.astype(np.float32)).reshape(rows.shape)
+        rows[70] = 0x7f80
+    c.kv.store([128], [128], change=change)
+    assert np.array_equal(first, c.run()[:4096])
