@@ -65,6 +65,12 @@ static hk_kv8_cache hk_kv8_of(const h3_gpu_tensor *t) {
     return c;
 }
 
+/* A new cache's scales: 0, whatever its codes. */
+__global__ void __launch_bounds__(256) hk_kv8_clear(float2 *scales, size_t n) {
+    const size_t i = (size_t)blockIdx.x * 256u + threadIdx.x;
+    if (i < n) scales[i] = make_float2(0.0f, 0.0f);
+}
+
 /* ------------------------------------------------------------ the store */
 
 /* Rows [source, + rows) of the keys and values go to rows [cache, + rows) of
@@ -913,6 +919,19 @@ h3_gpu_tensor *h3_hip_kv_int8_new(h3_gpu *gpu, uint32_t rows,
     t->record.n[HK_KV8_BLOCKS] = blocks;
     t->record.n[HK_KV8_HEADS] = kv_heads;
     t->record.n[HK_KV8_DIM] = head_dim;
+    /* launches of up to 2^31 threads */
+    float2 *scales = hk_kv8_of(t).scales;
+    for (size_t first = 0; first < pairs; first += (size_t)1 << 31) {
+        const size_t n = std::min(pairs - first, (size_t)1 << 31);
+        hipLaunchKernelGGL(hk_kv8_clear, dim3((unsigned)((n + 255u) / 256u)),
+                           dim3(256), 0, gpu->stream, scales + first, n);
+    }
+    const hipError_t status = hipGetLastError();
+    if (status != hipSuccess) {
+        hk_fail_hip(gpu, "8-bit cache", status);
+        h3_gpu_tensor_free(t);
+        return NULL;
+    }
     return t;
 }
 

@@ -416,6 +416,7 @@ int h3_hip_mlp_int8_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
 /* A cache of keys and values in 8 bits (free it with h3_gpu_tensor_free): rows
  * of kv_heads heads of head_dim (1 to 256) in blocks of 64 rows, the last one
  * whole; each block has one scale for its keys and one for its values a head.
+ * Rows that have never been stored are zeros.
  *
  * h3_hip_kv_int8_store writes rows [source_first[i], + rows[i]) of the given
  * keys and values to rows [cache_first[i], + rows[i]) of the cache, for `count`

@@ -117,6 +117,17 @@ def test_store_inside(gpu, std):
         kv.check(0, 192)
 
 
+def test_new_cache_is_zeros(gpu):
+    """Also in memory that held something else."""
+    for _ in range(2):
+        kv = Kv(gpu, 5000, 3, 64)
+        kv.check(0, 5000)
+        kv.store([3, 200], [2, 5], std=1e-3)
+        kv.check(0, 5000)
+        kv.store([0], [5000], std=30.0)
+        gpu.free(kv.t)
+
+
 def test_store_many_ranges(gpu):
     """More ranges than a launch takes, out of order."""
     order = np.random.default_rng(3).permutation(150)
