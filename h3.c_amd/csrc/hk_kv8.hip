@@ -1079,6 +1079,9 @@ int h3_hip_sdpa_packed_int8_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
     if (n[HK_PACKED_OFF_BLOCKS])
         return hk_fail(gpu, "packed attention: a request's rows of the cache "
                             "do not begin at a multiple of 64");
+    if (n[HK_PACKED_SPAN_BLOCKS] == HK_PACKED_TOO_MANY)
+        return hk_fail(gpu, "packed attention: over 2^32 rows of the cache to "
+                            "unpack");
     if (n[HK_PACKED_KV_END] > (uint64_t)a.cache.blocks * HK_KV8_BLOCK)
         return hk_fail(gpu, "packed attention: the plan's %u key rows end "
                             "behind the cache's %u blocks of 64",

@@ -48,6 +48,7 @@ enum { HK_PACKED_HEADS, HK_PACKED_KV_HEADS, HK_PACKED_DIM,
        HK_PACKED_OFF_BLOCKS, /* a request's keys begin inside 64 rows */
        HK_PACKED_FEW, HK_PACKED_MANY, /* items of up to 32 rows, and over */
        HK_PACKED_SPANS, HK_PACKED_SPAN_BLOCKS };
+#define HK_PACKED_TOO_MANY UINT32_MAX /* blocks of spans: they have no list */
 
 /* For a cache in blocks of 64 rows that is unpacked into rows for the items of
  * many rows: blocks [block, + blocks) of it, which those items read, go to

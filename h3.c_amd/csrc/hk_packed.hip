@@ -1284,6 +1284,12 @@ h3_gpu_tensor *h3_hip_sdpa_packed_plan(h3_gpu *gpu, const uint32_t *q_first,
         }
         for (auto &s : spans) {
             s.second.at = span_blocks;
+            /* their rows are numbered in 32 bits */
+            if (s.second.blocks > UINT32_MAX / HK_KT - span_blocks) {
+                span_blocks = HK_PACKED_TOO_MANY;
+                spans.clear();
+                break;
+            }
             span_blocks += s.second.blocks;
         }
         if (!spans.empty()) {

@@ -196,6 +196,10 @@ KV = "not made by h3_hip_kv_int8_new"
     ("attend(plan=plan(dim=32))", "2 key heads of 32 in the plan"),
     ("attend(plan=plan(kf=[0, 65]))", "begin at a multiple of 64"),
     ("attend(plan=plan(kf=[0, 192]))", "the plan's 292 key rows end behind"),
+    ("attend(plan=plan(qn=[20000, 20000], qf=[0, 20000], kf=[0, 64], "
+     "kn=[2**31, 2**31 + 640]))", "over 2^32 rows of the cache to unpack"),
+    ("attend(plan=plan(qn=[20000, 20000], qf=[0, 20000], kf=[0, 64], "
+     "kn=[2**31, 2**31 - 640]))", "2147483648 key rows end behind"),
     ("attend(qs=255)", "under the rows'"), ("attend(scale=-1.0)", "finite"),
     ("attend(scale=float('nan'))", "finite"),
     ("attend(scale=float('inf'))", "finite"),
