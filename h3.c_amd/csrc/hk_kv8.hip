@@ -543,34 +543,56 @@ template <int DIMS> struct hk_kv8_wave {
     float m, neg;     /* the reference, -(m L); unset: -+ infinity */
     float l;
 
-    __device__ __forceinline__ void start(const hk_packed_args &a,
-                                          const hk_packed_item &it,
-                                          uint32_t vrow) {
+    /* Its query row, zeros where there is none.  Whole pieces are loaded
+     * without a branch, behind which each would wait for the one before. */
+    __device__ __forceinline__ void load(const hk_packed_args &a,
+                                         const hk_packed_item &it,
+                                         uint32_t vrow, uint4 (&raw)[NK]) {
         const uint32_t half = (threadIdx.x & 63u) >> 5;
-        float x[NK][8];
-        const bool live = vrow < it.rows;
-        const uint32_t r = vrow / a.group, g = vrow - r * a.group;
+        const uint32_t of = min(vrow, it.rows - 1u);
+        const uint32_t r = of / a.group, g = of - r * a.group;
         const uint16_t *row =
             a.q + ((uint64_t)it.q_first + r) * a.q_stride +
             (uint64_t)(it.kv_head * a.group + g) * a.dim;
-        const bool whole =
-            a.dim % 8u == 0 && a.q_stride % 8u == 0 &&
-            ((uintptr_t)a.q & 15u) == 0;
+        if (a.dim % 8u == 0 && a.q_stride % 8u == 0 &&
+            ((uintptr_t)a.q & 15u) == 0) {
+#pragma unroll
+            for (int k = 0; k < NK; k++)
+                raw[k] = *(const uint4 *)(
+                    row + min((k >> 1) * 32u + half * 16u + (k & 1) * 8u,
+                              a.dim - 8u));
+        } else {
+#pragma unroll
+            for (int k = 0; k < NK; k++) {
+                uint32_t w[4] = {};
+#pragma unroll
+                for (uint32_t e = 0; e < 8u; e++) {
+                    const uint32_t d =
+                        (k >> 1) * 32u + half * 16u + (k & 1) * 8u + e;
+                    if (d < a.dim) w[e >> 1] |= (uint32_t)row[d] << (16 * (e & 1));
+                }
+                raw[k] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        }
+    }
+
+    __device__ __forceinline__ void start(const hk_packed_args &a,
+                                          const hk_packed_item &it,
+                                          uint32_t vrow,
+                                          const uint4 (&raw)[NK]) {
+        const uint32_t half = (threadIdx.x & 63u) >> 5;
+        float x[NK][8];
         uint32_t most = 0;
 #pragma unroll
         for (int k = 0; k < NK; k++) {
             const uint32_t d = (k >> 1) * 32u + half * 16u + (k & 1) * 8u;
+            const bool has = vrow < it.rows && d < a.dim;
+            hk_unpack8(raw[k], x[k]);
 #pragma unroll
-            for (int e = 0; e < 8; e++) x[k][e] = 0.0f;
-            if (live && whole && d < a.dim) {
-                hk_unpack8(*(const uint4 *)(row + d), x[k]);
-            } else if (live && !whole) {
-#pragma unroll
-                for (int e = 0; e < 8; e++)
-                    if (d + e < a.dim) x[k][e] = hk_bf2f(row[d + e]);
+            for (int e = 0; e < 8; e++) {
+                x[k][e] = has ? x[k][e] : 0.0f;
+                most = max(most, hk_magnitude(x[k][e]));
             }
-#pragma unroll
-            for (int e = 0; e < 8; e++) most = max(most, hk_magnitude(x[k][e]));
         }
         most = max(most, (uint32_t)__shfl_xor(most, 32, 64));
         /* to [2^13, 2^14) */
@@ -713,11 +735,10 @@ __device__ __forceinline__ void hk_kv8_put(const hk_packed_args &a,
 /* The waves share the item's rows and split its keys, wave w every fourth 32 of
  * them from the wth on, straight from the cache into its registers; then their
  * sums are joined, 64 dims at a time.  Long contexts are bound by the cache's
- * bytes (8 rows of 64 heads over 8, 4096 to 9720 keys: 22.7 us, 5.1 TB/s), short
+ * bytes (8 rows of 64 heads over 8, 4096 to 9720 keys: 21 us, 5.5 TB/s), short
  * ones by the chain of item, keys, scores and join (16 rows of 40 heads, 20 to
- * 512 keys: 12 us).  32 keys a step and 32 KB of LDS let three workgroups share a
- * CU: 640 items of 300 keys 15.4 us, 21.3 with 64 a step, which leaves room for
- * two. */
+ * 512 keys: 11 us).  32 keys a step and 32 KB of LDS let three workgroups share a
+ * CU: 640 items of 300 keys 14.0 us; 64 a step leave room for two, 21. */
 template <int DIMS>
 __global__ void __launch_bounds__(256, 3) hk_kv8_few(hk_kv8_args g) {
     constexpr int ND = DIMS / 32;
@@ -756,13 +777,15 @@ __global__ void __launch_bounds__(256, 3) hk_kv8_few(hk_kv8_args g) {
         min(it.tile_end * 2u, (it.kv_rows + 31u) / 32u); /* (below 2^28) */
     uint32_t step = it.tile * 2u + wave;
     float2 ahead = make_float2(0.0f, 0.0f);
+    hk_kv8_wave<DIMS> w;
+    uint4 raw[DIMS / 16];
+    w.load(a, it, vrow, raw);
     if (step < last) {
         ahead = g.cache.scales[block_at(step)];
         load(step, 0, k);
         load(step, 1, v);
     }
-    hk_kv8_wave<DIMS> w;
-    w.start(a, it, vrow);
+    w.start(a, it, vrow, raw);
     /* the queries, the same for all waves, wait in LDS */
     hk_f16x8 *queries = (hk_f16x8 *)lds + lane;
     if (wave == 0) {
