@@ -99,35 +99,45 @@ hk_int8_rows_any(hk_int8_rows_args a, uint32_t first) {
     if (threadIdx.x == 0) a.scales[row] = code.scale;
 }
 
-/* Eight values from any element on, zeros from the `left`th. */
-__device__ __forceinline__ void hk_int8_load8(const uint16_t *from,
-                                              uint32_t left, float *to) {
-    if (left >= 8u) {
-        uint4 v;
-        __builtin_memcpy(&v, from, 16); /* rows of odd widths: not aligned */
-        hk_unpack8(v, to);
+/* Elements [col, + 8) of a row, zeros behind its end.  EIGHTS: the width is a
+ * multiple of 8, and behind the end stands whatever else the row has.  There is
+ * no branch then, behind which a load would wait for those before (4756 x 14336
+ * in bf16 31 us for 35, behind an RMS norm 45 for 64). */
+template <bool EIGHTS>
+__device__ __forceinline__ uint4 hk_int8_piece(const uint16_t *row,
+                                               uint32_t col, uint32_t width) {
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (EIGHTS || col + 8u <= width) {
+        __builtin_memcpy(&v, row + (EIGHTS ? min(col, width - 8u) : col),
+                         16); /* rows of odd widths: not aligned */
+    } else if (col < width) {
+        uint32_t w[4] = {};
+#pragma unroll
+        for (uint32_t i = 0; i < 8u; i++)
+            if (col + i < width)
+                w[i >> 1] |= (uint32_t)row[col + i] << (16u * (i & 1u));
+        v = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    return v;
+}
+
+template <bool EIGHTS>
+__device__ __forceinline__ void hk_int8_piece(const float *row, uint32_t col,
+                                              uint32_t width, float *to) {
+    if (EIGHTS || col + 8u <= width) {
+        __builtin_memcpy(to, row + (EIGHTS ? min(col, width - 8u) : col), 32);
     } else {
 #pragma unroll
         for (uint32_t i = 0; i < 8u; i++)
-            to[i] = i < left ? hk_bf2f(from[i]) : 0.0f;
-    }
-}
-
-__device__ __forceinline__ void hk_int8_load8(const float *from, uint32_t left,
-                                              float *to) {
-    if (left >= 8u) {
-        __builtin_memcpy(to, from, 32);
-    } else {
-#pragma unroll
-        for (uint32_t i = 0; i < 8u; i++) to[i] = i < left ? from[i] : 0.0f;
+            to[i] = col + i < width ? row[col + i] : 0.0f;
     }
 }
 
 /* The same with the row in registers, 8 columns a thread and chunk: at most
  * CHUNKS * THREADS * 8 columns.  One pass over the row, bound by HBM: 4756 rows
- * of 14336 in F32 67 us (5.1 TB/s), 6144 x 5120 in bf16 19 us (5.0 TB/s); a row
+ * of 14336 in F32 67 us (5.1 TB/s), 6144 x 5120 in bf16 16 us (5.9 TB/s); a row
  * alone by its chain of loads, maximum and codes, 2.1 us. */
-template <int SOURCE, int CHUNKS, int THREADS>
+template <int SOURCE, int CHUNKS, int THREADS, bool EIGHTS>
 __global__ void __launch_bounds__(THREADS)
 hk_int8_rows_vec(hk_int8_rows_args a, uint32_t first) {
     __shared__ float sums[16];
@@ -139,84 +149,110 @@ hk_int8_rows_vec(hk_int8_rows_args a, uint32_t first) {
         return (threadIdx.x + (uint32_t)c * THREADS) * 8u;
     };
     float v[CHUNKS][8];
-    float sum = 0.0f;
+    if (SOURCE == HK_ROWS_F32 || SOURCE == HK_ROWS_SWIGLU) {
+        const float *from = a.wide + (size_t)row * a.wide_pitch;
+        float u[CHUNKS][8];
 #pragma unroll
-    for (int c = 0; c < CHUNKS; c++) {
-        const uint32_t col = column(c), left = a.width - col;
-        if (col >= a.width) {
-#pragma unroll
-            for (int i = 0; i < 8; i++) v[c][i] = 0.0f;
-        } else if (SOURCE == HK_ROWS_F32) {
-            hk_int8_load8(a.wide + (size_t)row * a.wide_pitch + col, left,
-                          v[c]);
-        } else if (SOURCE == HK_ROWS_SWIGLU) {
-            const float *from = a.wide + (size_t)row * a.wide_pitch + col;
-            float u[8];
-            hk_int8_load8(from, left, v[c]);
-            hk_int8_load8(from + a.width, left, u);
-#pragma unroll
-            for (int i = 0; i < 8; i++) v[c][i] = hk_swiglu_f(v[c][i], u[i]);
-        } else {
-            hk_int8_load8(a.input + (size_t)row * a.width + col, left, v[c]);
+        for (int c = 0; c < CHUNKS; c++) {
+            hk_int8_piece<EIGHTS>(from, column(c), a.width, v[c]);
+            if (SOURCE == HK_ROWS_SWIGLU)
+                hk_int8_piece<EIGHTS>(from + a.width, column(c), a.width, u[c]);
         }
-#pragma unroll
-        for (int i = 0; i < 8; i++) sum += layer ? v[c][i] : v[c][i] * v[c][i];
-    }
-    if (norm) {
-        const float mean =
-            layer ? hk_block_sum(sum, sums) / (float)a.width : 0.0f;
-        if (layer) {
-            sum = 0.0f;
+        if (SOURCE == HK_ROWS_SWIGLU) {
 #pragma unroll
             for (int c = 0; c < CHUNKS; c++)
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    v[c][i] -= mean;
-                    if (column(c) + i < a.width)
-                        sum = fmaf(v[c][i], v[c][i], sum);
+                for (int i = 0; i < 8; i++)
+                    v[c][i] = hk_swiglu_f(v[c][i], u[c][i]);
+        }
+        if (EIGHTS) {
+#pragma unroll
+            for (int c = 0; c < CHUNKS; c++)
+                if (column(c) >= a.width) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) v[c][i] = 0.0f;
                 }
         }
-        const float inverse =
-            1.0f / sqrtf(hk_block_sum(sum, sums) / (float)a.width +
-                         a.epsilon);
+    } else {
+        const uint16_t *from = a.input + (size_t)row * a.width;
+        uint4 raw[CHUNKS];
+#pragma unroll
+        for (int c = 0; c < CHUNKS; c++)
+            raw[c] = hk_int8_piece<EIGHTS>(from, column(c), a.width);
         const uint16_t *shift = NULL, *scale = NULL;
-        if (a.modulation) {
+        if (norm && a.modulation) {
             const size_t base = (size_t)a.row_map[row] * a.slots;
             shift = a.modulation + (base + a.shift_slot) * a.width;
             scale = a.modulation + (base + a.scale_slot) * a.width;
         }
+        float sum = 0.0f;
 #pragma unroll
         for (int c = 0; c < CHUNKS; c++) {
-            const uint32_t col = column(c), left = a.width - col;
-            if (col >= a.width) {
+            hk_unpack8(raw[c], v[c]);
+            if (EIGHTS && column(c) >= a.width) {
 #pragma unroll
                 for (int i = 0; i < 8; i++) v[c][i] = 0.0f;
-                continue;
             }
-            float w[8], b[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[c][i] *= inverse;
-            if (a.weight) {
-                hk_int8_load8(a.weight + col, left, w);
+            for (int i = 0; i < 8; i++)
+                sum += layer ? v[c][i] : v[c][i] * v[c][i];
+        }
+        if (norm) {
+            const float mean =
+                layer ? hk_block_sum(sum, sums) / (float)a.width : 0.0f;
+            if (layer) {
+                sum = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 8; i++) v[c][i] *= w[i];
+                for (int c = 0; c < CHUNKS; c++)
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        v[c][i] -= mean;
+                        if (column(c) + (EIGHTS ? 0 : i) < a.width)
+                            sum = fmaf(v[c][i], v[c][i], sum);
+                    }
             }
-            if (layer && a.bias) {
-                hk_int8_load8(a.bias + col, left, b);
+            const float inverse =
+                1.0f / sqrtf(hk_block_sum(sum, sums) / (float)a.width +
+                             a.epsilon);
 #pragma unroll
-                for (int i = 0; i < 8; i++) v[c][i] += b[i];
-            }
-            if (shift) {
-                hk_int8_load8(scale + col, left, w);
-                hk_int8_load8(shift + col, left, b);
+            for (int c = 0; c < CHUNKS; c++) {
+                float w[8], b[8];
+                uint4 weight, bias, scales, shifts; /* on their way at once */
+                auto load = [&](uint4 &to, const uint16_t *from) {
+                    to = hk_int8_piece<EIGHTS>(from, column(c), a.width);
+                };
+                if (a.weight) load(weight, a.weight);
+                if (layer && a.bias) load(bias, a.bias);
+                if (shift) {
+                    load(scales, scale);
+                    load(shifts, shift);
+                }
 #pragma unroll
-                for (int i = 0; i < 8; i++)
-                    v[c][i] = v[c][i] * (1.0f + w[i]) + b[i];
-            }
-            if (left < 8u) { /* past the row's end, whatever came of it */
+                for (int i = 0; i < 8; i++) v[c][i] *= inverse;
+                if (a.weight) {
+                    hk_unpack8(weight, w);
 #pragma unroll
-                for (uint32_t i = 0; i < 8u; i++)
-                    if (i >= left) v[c][i] = 0.0f;
+                    for (int i = 0; i < 8; i++) v[c][i] *= w[i];
+                }
+                if (layer && a.bias) {
+                    hk_unpack8(bias, b);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) v[c][i] += b[i];
+                }
+                if (shift) {
+                    hk_unpack8(scales, w);
+                    hk_unpack8(shifts, b);
+#pragma unroll
+                    for (int i = 0; i < 8; i++)
+                        v[c][i] = v[c][i] * (1.0f + w[i]) + b[i];
+                }
+                /* past the row's end, whatever came of it */
+                if (column(c) + 8u > a.width) {
+#pragma unroll
+                    for (uint32_t i = 0; i < 8u; i++)
+                        if (EIGHTS || column(c) + i >= a.width)
+                            v[c][i] = 0.0f;
+                }
             }
         }
     }
@@ -259,20 +295,29 @@ static void hk_int8_each_rows(uint32_t rows, F launch) {
         launch(first, std::min(rows - first, most));
 }
 
+typedef void (*hk_int8_rows_kernel)(hk_int8_rows_args, uint32_t);
+
+template <int SOURCE, bool EIGHTS>
+static hk_int8_rows_kernel hk_int8_rows_pick(bool few, uint32_t pitch) {
+    if (few)
+        return pitch <= 8192u ? hk_int8_rows_vec<SOURCE, 1, 1024, EIGHTS>
+                              : hk_int8_rows_vec<SOURCE, 2, 1024, EIGHTS>;
+    return pitch <= 2048u   ? hk_int8_rows_vec<SOURCE, 1, 256, EIGHTS>
+           : pitch <= 6144u ? hk_int8_rows_vec<SOURCE, 3, 256, EIGHTS>
+                            : hk_int8_rows_vec<SOURCE, 8, 256, EIGHTS>;
+}
+
 /* A row's threads: where there are few rows, more of them, as there is nothing
  * else to hide a row's latency (one row of 14336: 6.4 us with 256). */
 template <int SOURCE>
 static void hk_int8_rows(struct h3_gpu *gpu, const hk_int8_rows_args &a) {
     const bool few = a.rows <= 512u && a.pitch > 2048u;
-    void (*kernel)(hk_int8_rows_args, uint32_t) =
-        a.pitch > 16384u || gpu->reference_kernels ? hk_int8_rows_any<SOURCE>
-        : few && a.pitch <= 8192u ? hk_int8_rows_vec<SOURCE, 1, 1024>
-        : few                     ? hk_int8_rows_vec<SOURCE, 2, 1024>
-        : a.pitch <= 2048u        ? hk_int8_rows_vec<SOURCE, 1, 256>
-        : a.pitch <= 6144u        ? hk_int8_rows_vec<SOURCE, 3, 256>
-                                  : hk_int8_rows_vec<SOURCE, 8, 256>;
-    const uint32_t threads =
-        few && a.pitch <= 16384u && !gpu->reference_kernels ? 1024u : 256u;
+    const bool any = a.pitch > 16384u || gpu->reference_kernels;
+    const hk_int8_rows_kernel kernel =
+        any                  ? hk_int8_rows_any<SOURCE>
+        : a.width % 8u == 0u ? hk_int8_rows_pick<SOURCE, true>(few, a.pitch)
+                             : hk_int8_rows_pick<SOURCE, false>(few, a.pitch);
+    const uint32_t threads = few && !any ? 1024u : 256u;
     hk_int8_each_rows(a.rows, [&](uint32_t first, uint32_t rows) {
         hipLaunchKernelGGL(kernel, dim3(rows), dim3(threads), 0, gpu->stream,
                            a, first);
