@@ -335,6 +335,11 @@ __device__ __forceinline__ float hk_int8_value(int acc, float sx, float sw,
     return __builtin_fmaf((float)acc, sx * sw, bias);
 }
 
+/* The elements of an F32 row of n, padded to whole 16-byte pieces. */
+__host__ __device__ __forceinline__ uint32_t hk_int8_fours(uint32_t n) {
+    return (n + 3u) & ~3u;
+}
+
 /* One thread per output: H3_HIP_REFERENCE=1.  `wide` or `out`. */
 __global__ void __launch_bounds__(256)
 hk_int8_simple(const int8_t *x, const float *xs, const int8_t *w,
@@ -357,7 +362,7 @@ hk_int8_simple(const int8_t *x, const float *xs, const int8_t *w,
     float y = hk_int8_value(sum, xs[row], ws[col],
                             bias ? hk_bf2f(bias[col]) : -0.0f);
     if (gelu) y = hk_gelu_tanh_f(y);
-    if (wide) wide[row * n + col] = y;
+    if (wide) wide[row * hk_int8_fours(n) + col] = y;
     else out[row * n + col] = hk_f2bf(y);
 }
 
@@ -413,7 +418,7 @@ struct hk_int8_out {
     const float *xs, *ws;
     const uint16_t *bias;
     uint16_t *out;
-    float *wide; /* in F32 instead, rows of n */
+    float *wide; /* in F32 instead, padded rows */
     uint32_t n;
     int gelu;
 };
@@ -446,23 +451,21 @@ __device__ __forceinline__ void hk_int8_finish(const hk_int8_out &o,
 #pragma unroll
     for (int e = 0; e < 4; e++)
         y[e] = hk_int8_made(o, sx, c.scale[e], c.bias[e], sums[e]);
-    const size_t at = (size_t)row * o.n + col;
-    const bool whole = o.n % 4u == 0;
-    if (o.wide && whole) {
-        *(float4 *)(o.wide + at) = make_float4(y[0], y[1], y[2], y[3]);
-    } else if (whole) {
-        *(uint2 *)(o.out + at) =
-            make_uint2(hk_pack2(y[0], y[1]), hk_pack2(y[2], y[3]));
-    } else if (!o.wide && o.n % 2u == 0) {
-        *(uint32_t *)(o.out + at) = hk_pack2(y[0], y[1]);
-        if (col + 2u < o.n) *(uint32_t *)(o.out + at + 2) = hk_pack2(y[2], y[3]);
+    if (o.wide) {
+        *(float4 *)(o.wide + (size_t)row * hk_int8_fours(o.n) + col) =
+            make_float4(y[0], y[1], y[2], y[3]);
+        return;
+    }
+    uint16_t *to = o.out + (size_t)row * o.n + col;
+    if (o.n % 4u == 0) {
+        *(uint2 *)to = make_uint2(hk_pack2(y[0], y[1]), hk_pack2(y[2], y[3]));
+    } else if (o.n % 2u == 0) {
+        *(uint32_t *)to = hk_pack2(y[0], y[1]);
+        if (col + 2u < o.n) *(uint32_t *)(to + 2) = hk_pack2(y[2], y[3]);
     } else {
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            if (col + e >= o.n) continue;
-            if (o.wide) o.wide[at + e] = y[e];
-            else o.out[at + e] = hk_f2bf(y[e]);
-        }
+        for (int e = 0; e < 4; e++)
+            if (col + e < o.n) to[e] = hk_f2bf(y[e]);
     }
 }
 
@@ -964,7 +967,7 @@ static bool hk_int8_gated_tiles(const struct h3_gpu *gpu,
 }
 
 /* h = silu(x . gate^T) (x . up^T) in 8 bits, by way of F32 rows in `wide`, of
- * (hidden + 3) / 4 * 4 elements over tiles and 2 hidden else. */
+ * `hidden` elements over tiles and 2 hidden else, padded. */
 static void hk_int8_gated(struct h3_gpu *gpu, hk_int8_matrix x,
                           const hk_int8_matrix &w, uint32_t hidden,
                           float *wide, const hk_int8_matrix &h) {
@@ -976,7 +979,7 @@ static void hk_int8_gated(struct h3_gpu *gpu, hk_int8_matrix x,
     a.width = hidden;
     a.pitch = h.pitch;
     if (!hk_int8_gated_tiles(gpu, x, w)) {
-        a.wide_pitch = 2 * hidden;
+        a.wide_pitch = hk_int8_fours(2 * hidden);
         if (hk_int8_fast(gpu, w))
             hk_int8_few(gpu, x, w, {x.scales, w.scales, NULL, NULL, wide,
                                     2 * hidden, 0});
@@ -985,7 +988,7 @@ static void hk_int8_gated(struct h3_gpu *gpu, hk_int8_matrix x,
         hk_int8_rows<HK_ROWS_SWIGLU>(gpu, a);
         return;
     }
-    a.wide_pitch = (hidden + 3u) & ~3u;
+    a.wide_pitch = hk_int8_fours(hidden);
     const uint32_t most = hk_int8_reach(x.pitch);
     hk_int8_ext e = {x.scales, w.scales, wide, a.wide_pitch};
     for (uint32_t left = x.rows; left; left -= x.rows) {
@@ -1205,10 +1208,8 @@ int h3_hip_mlp_int8_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
     const hk_int8_matrix x = hk_int8_of(input, rows);
     const hk_int8_matrix w1 = hk_int8_of(fc1_weight, 2 * hidden_dim);
     const uint32_t pitch = fc2_weight->record.n[HK_INT8_PITCH];
-    const size_t wide =
-        hk_int8_gated_tiles(gpu, x, w1)
-            ? ((size_t)hidden_dim + 3u) & ~(size_t)3u
-            : 2 * (size_t)hidden_dim;
+    const size_t wide = hk_int8_fours(
+        hk_int8_gated_tiles(gpu, x, w1) ? hidden_dim : 2 * hidden_dim);
     const size_t wide_bytes = (rows * wide * 4 + 255) & ~(size_t)255;
     const size_t code_bytes = (size_t)rows * pitch;
     uint8_t *space = (uint8_t *)hk_workspace(
