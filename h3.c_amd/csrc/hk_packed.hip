@@ -495,9 +495,12 @@ __device__ __forceinline__ void hk_packed_item_of(const hk_packed_args &a) {
         k_off[i] = kc < dim_chunks ? row * stride + kc * 16u : 0x80000000u;
         v_off[i] = vc < dim_chunks ? row * stride + vc * 16u : 0x80000000u;
     }
-    const uint64_t kv_base =
-        (uint64_t)(SCALED ? a.kv_at[blockIdx.x] : it.kv_first) * a.kv_stride +
-        (uint64_t)it.kv_head * a.dim;
+    /* (a plan of requests without keys has no list of their places) */
+    const uint32_t kv_first = !SCALED                   ? it.kv_first
+                              : it.tile_end != it.tile ? a.kv_at[blockIdx.x]
+                                                       : 0u;
+    const uint64_t kv_base = (uint64_t)kv_first * a.kv_stride +
+                             (uint64_t)it.kv_head * a.dim;
     /* the scale of the tile's block, loaded a tile ahead */
     const float *block_scales =
         SCALED ? a.key_scales +
@@ -507,7 +510,7 @@ __device__ __forceinline__ void hk_packed_item_of(const hk_packed_args &a) {
     float ahead = 0.0f;
     const float unit =
         SCALED && it.tile_end != it.tile
-            ? a.value_units[(size_t)(a.kv_at[blockIdx.x] / HK_KT) * a.kv_heads +
+            ? a.value_units[(size_t)(kv_first / HK_KT) * a.kv_heads +
                             it.kv_head]
             : 1.0f;
     auto issue_tile = [&](uint32_t tile, uint32_t stage) {

@@ -363,6 +363,13 @@ def test_many_rows_of_unlike_scales(gpu, powers):
     assert np.isfinite(ro.wide(c.run(), 4096, 512)).all()
 
 
+@pytest.mark.parametrize("qn", [[6144], [1, 6144, 3], [2]])
+def test_requests_without_keys(gpu, qn):
+    """A plan that has nothing to unpack."""
+    c = Case(gpu, qn, [0] * len(qn), 8, 8, 64)
+    assert not c.check().any()
+
+
 def test_keys_of_others_have_no_part(gpu):
     """Two requests share their first blocks; the longer one's last blocks are
     larger by 2^90 or not finite."""
