@@ -541,6 +541,7 @@ hk_int8_dot(hk_skinny_args g, hk_int8_out o, uint32_t pitch) {
  * per 128 columns and group leaves CUs idle (hk_gemm_skinny_run). */
 struct hk_int8_few_plan {
     uint32_t groups, mbs, columns, splits, steps;
+    uint32_t narrow; /* waves of hk_int8_narrow, else 0 */
 };
 
 /* Few rows: the skinny GEMM's loop (hk_skinny_tile.h) over bytes, a workgroup
@@ -615,6 +616,105 @@ hk_int8_skinny(hk_skinny_args g, hk_int8_out o, hk_int8_few_plan plan) {
         }
     };
     hk_skinny_sums<MB, 3, HK_LOAD_ONCE, hk_i32x16>(g, g.w, x, y, use);
+}
+
+/* Narrow products: a workgroup per 32 columns and 32 rows, whose waves take a
+ * part of K each and join their sums in LDS, so that there are workgroups enough
+ * and no second launch.  W takes its turn through LDS as there, X comes as
+ * fragments, which costs more the more rows there are: bound by the steps'
+ * latency, or by W's and X's bytes (8 rows 5120 -> 5120 7.7 us, 10.5 with pieces
+ * of K; 8 x 3004 -> 5842 5.6 and 9.0; 2 x 5120 -> 13824 13.2 and 16.3; but 32 x
+ * 13824 -> 5120 24 and 18.7). */
+template <int WAVES>
+__global__ void __launch_bounds__(WAVES * 64)
+hk_int8_narrow(hk_skinny_args g, hk_int8_out o, uint32_t groups) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t hk_lds[];
+    constexpr int D = HK_SKINNY_RING;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t row = lane & 31u, half = lane >> 5;
+    uint32_t at = blockIdx.x;
+    if (groups > 1u) at = at % 8u * (gridDim.x / 8u) + at / 8u;
+    const uint32_t n0 = at / groups * 32u, row0 = at % groups * 32u;
+    const uint32_t n = g.n, k = g.k;
+    if (n0 >= n) return;
+    const uint32_t m = min(g.m - row0, 32u), k_steps = k / 64u;
+    const uint32_t per = (k_steps + WAVES - 1u) / WAVES, base = wave * per;
+    const uint32_t steps = base < k_steps ? min(per, k_steps - base) : 0u;
+    const __amdgpu_buffer_rsrc_t xr =
+        hk_rsrc(g.x + (size_t)row0 * k, m * k * 2u);
+    const __amdgpu_buffer_rsrc_t wr = hk_rsrc(g.w, g.w_bytes);
+    uint32_t wo[4];
+#pragma unroll
+    for (int q = 0; q < 4; q++)
+        wo[q] = (min(n0 + 8u * q + (lane >> 3), n) * k + (lane & 7u) * 8u) *
+                2u;
+    const uint32_t xo = min(row, m) * k * 2u + half * 16u;
+    hk_v4i wf[D][4], xf[D][4];
+    auto load = [&](int slot, uint32_t step) {
+        const uint32_t kb = hk_skinny_k_bytes(base + step, k_steps);
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+            wf[slot][q] = __builtin_amdgcn_raw_buffer_load_b128(
+                wr, hk_skinny_lane(wo[q], step, steps), kb, HK_LOAD_ONCE);
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+            xf[slot][q] = __builtin_amdgcn_raw_buffer_load_b128(
+                xr, hk_skinny_lane(xo + q * 32u, step, steps), kb, 0);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    /* a thread makes four columns of every (8 WAVES)th row */
+    const uint32_t col = n0 + (tid & 7u) * 4u;
+    hk_int8_columns columns;
+    columns.load(o, col);
+    float sx[4 / WAVES];
+#pragma unroll
+    for (uint32_t i = 0; i < 4 / WAVES; i++)
+        sx[i] = o.xs[row0 + min(i * 8u * WAVES + (tid >> 3), m - 1u)];
+#pragma unroll
+    for (int d = 0; d + 1 < D; d++) load(d, d);
+    hk_i32x16 acc;
+#pragma unroll
+    for (int e = 0; e < 16; e++) acc[e] = 0;
+    uint8_t *own = hk_lds + wave * 4096u;
+    /* (steps past the end add zeros) */
+    for (uint32_t s0 = 0; s0 < steps; s0 += D) {
+#pragma unroll
+        for (int d = 0; d < D; d++) {
+            load((d + 3) % D, s0 + d + 3u);
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const uint32_t wrow = 8u * q + (lane >> 3);
+                *(hk_v4i *)(own + wrow * 128u +
+                            (((lane & 7u) ^ hk_swz_key(wrow)) << 4)) =
+                    wf[d][q];
+            }
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+                hk_skinny_mfma(acc,
+                               *(const hk_v4i *)(
+                                   own + row * 128u +
+                                   (((2u * q + half) ^ hk_swz_key(row)) << 4)),
+                               xf[d][q]);
+        }
+    }
+    /* rows of 128 bytes, 16-byte chunk c of row r at c ^ r % 8 */
+#pragma unroll
+    for (uint32_t q = 0; q < 4; q++)
+        *(hk_v4i *)(own + row * 128u + (((q * 2u + half) ^ (row & 7u)) << 4)) =
+            hk_v4i{acc[q * 4], acc[q * 4 + 1], acc[q * 4 + 2], acc[q * 4 + 3]};
+    __syncthreads();
+    if (col >= n) return;
+#pragma unroll
+    for (uint32_t i = 0; i < 4 / WAVES; i++) {
+        const uint32_t r = i * 8u * WAVES + (tid >> 3);
+        hk_v4i sum = {0, 0, 0, 0};
+#pragma unroll
+        for (uint32_t j = 0; j < WAVES; j++)
+            sum += *(const hk_v4i *)(hk_lds + j * 4096u + r * 128u +
+                                     (((tid & 7u) ^ (r & 7u)) << 4));
+        if (r < m) hk_int8_finish(o, row0 + r, col, sx[i], columns, sum);
+    }
 }
 
 /* Adds the pieces, as hk_skinny_reduce. */
@@ -810,19 +910,33 @@ static void hk_int8_tiles(struct h3_gpu *gpu, const hk_int8_matrix &x,
                            gpu->stream, g, o, r.splits);
 }
 
-/* The plan of the least estimated time, which it returns: a step of K takes
- * 0.18 us and 0.11 per 32 rows, what comes before and after the steps 2.4 and
- * 0.95, joining pieces 4.5; more workgroups than CUs share them, four at once,
- * and the groups' reads of W end at 6.5 TB/s.  (us by rows of a group, 32 / 64 /
- * 96 / 128: 512 x 1024 -> 1024 5.9 / 7.6 / 9.3 / 11.3, 300 x 2675 -> 1001 10.3 /
- * 11.3 / 12.6 / 14.4, 197 x 5120 -> 5120 33 / 24.1 / 20.5 / 22.5, 256 x 5120 ->
- * 13824 70 / 46 / 53 / 35.) */
+/* The plan of the least estimated time, which it returns (us): a step of K takes
+ * 0.18 and 0.11 per 32 rows, what comes before and after the steps 2.4 and 0.95,
+ * joining pieces 4.6; more workgroups than CUs share them, four at once, and the
+ * groups' reads of W end at 6.5 TB/s.  (us by rows of a group, 32 / 64 / 96 / 128:
+ * 512 x 1024 -> 1024 5.9 / 7.6 / 9.3 / 11.3, 300 x 2675 -> 1001 10.3 / 11.3 / 12.6
+ * / 14.4, 197 x 5120 -> 5120 33 / 24.1 / 20.5 / 22.5, 256 x 5120 -> 13824 70 / 46 /
+ * 53 / 35.)  Narrow: 2.5, and a step of a wave 0.2 and as much for 32 rows, or W
+ * at 6.2 TB/s and of X, for each workgroup, the part that L1 does not have; two
+ * waves where they leave no second turn of the CUs.  (us, narrow and not: 16 x
+ * 5120 -> 5120 9.0 and 10.9, 16 x 5120 -> 13824 15.9 and 16.9, 32 x 5120 -> 13824
+ * 20.1 and 18.2, 2 x 5376 -> 28672 26.9 and 24.5.) */
 static hk_int8_few_plan hk_int8_few_planned(uint32_t cus, uint32_t m,
                                             uint32_t n, uint32_t k_steps,
                                             float *us) {
     hk_int8_few_plan best = {};
+    best.groups = (m + 31u) / 32u;
+    best.columns = (n + 31u) / 32u;
+    best.narrow = best.groups * best.columns <= cus ? 2u : 1u;
+    const float lines = (float)best.groups * (float)k_steps *
+                        ((float)HK_INT8_LINE / 6.2e6f);
+    const float rows = (float)std::min(m, 32u);
+    *us = 2.5f + std::max((float)((k_steps + best.narrow - 1u) / best.narrow) *
+                              (0.2f + 0.2f / 32.0f * rows),
+                          lines * ((float)n + (0.25f + 0.0125f * rows) * rows *
+                                                  (float)best.columns));
     for (uint32_t most = 1; most <= 4; most++) {
-        hk_int8_few_plan p;
+        hk_int8_few_plan p = {};
         p.groups = (m + 32u * most - 1u) / (32u * most);
         p.mbs = ((m + p.groups - 1u) / p.groups + 31u) / 32u;
         if (p.mbs < most) continue; /* (that many groups have been tried) */
@@ -841,12 +955,13 @@ static hk_int8_few_plan hk_int8_few_planned(uint32_t cus, uint32_t m,
                 ? 1.0f
                 : 0.9f * (float)((workgroups + cus - 1u) / cus);
         const float step = 0.18f + 0.11f * (float)p.mbs;
-        float t = (2.4f + 0.95f * (float)p.mbs + step * (float)p.steps) *
-                      rounds +
-                  (p.splits > 1 ? 4.5f : 0.0f);
-        t = std::max(t, (float)p.groups * (float)n * (float)k_steps *
-                            ((float)HK_INT8_LINE / 6.5e6f));
-        if (!best.groups || t < *us) {
+        const float t =
+            std::max((2.4f + 0.95f * (float)p.mbs + step * (float)p.steps) *
+                         rounds,
+                     (float)p.groups * (float)n * (float)k_steps *
+                         ((float)HK_INT8_LINE / 6.5e6f)) +
+            (p.splits > 1 ? 4.6f : 0.0f);
+        if (t < *us) {
             best = p;
             *us = t;
         }
@@ -886,6 +1001,15 @@ static void hk_int8_few(struct h3_gpu *gpu, const hk_int8_matrix &x,
     float us;
     hk_int8_few_plan p = hk_int8_few_planned(hk_int8_cus(gpu), x.rows, o.n,
                                              x.pitch / HK_INT8_LINE, &us);
+    if (p.narrow) {
+        const uint32_t workgroups = p.columns * p.groups;
+        hipLaunchKernelGGL(
+            p.narrow == 2u ? hk_int8_narrow<2> : hk_int8_narrow<1>,
+            dim3(p.groups > 1u ? (workgroups + 7u) & ~7u : workgroups),
+            dim3(p.narrow * 64u), p.narrow * 4096u, gpu->stream, g, o,
+            p.groups);
+        return;
+    }
     g.split_steps = p.steps;
     if (p.splits > 1)
         g.partial = (float *)hk_splitk_try(
