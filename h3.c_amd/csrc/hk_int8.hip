@@ -23,7 +23,7 @@ enum {
     HK_ROWS_RMS,    /* RMS norm of it, weight, modulation */
     HK_ROWS_LAYER,  /* LayerNorm of it, weight and bias, modulation */
     HK_ROWS_F32,    /* F32 rows of `pitch` elements */
-    HK_ROWS_SWIGLU, /* silu(g) u of F32 rows [g | u] */
+    HK_ROWS_SWIGLU, /* silu(g) u of F32 rows [g | u], of the simple kernel */
 };
 
 struct hk_int8_rows_args {
@@ -149,22 +149,11 @@ hk_int8_rows_vec(hk_int8_rows_args a, uint32_t first) {
         return (threadIdx.x + (uint32_t)c * THREADS) * 8u;
     };
     float v[CHUNKS][8];
-    if (SOURCE == HK_ROWS_F32 || SOURCE == HK_ROWS_SWIGLU) {
+    if (SOURCE == HK_ROWS_F32) {
         const float *from = a.wide + (size_t)row * a.wide_pitch;
-        float u[CHUNKS][8];
 #pragma unroll
-        for (int c = 0; c < CHUNKS; c++) {
+        for (int c = 0; c < CHUNKS; c++)
             hk_int8_piece<EIGHTS>(from, column(c), a.width, v[c]);
-            if (SOURCE == HK_ROWS_SWIGLU)
-                hk_int8_piece<EIGHTS>(from + a.width, column(c), a.width, u[c]);
-        }
-        if (SOURCE == HK_ROWS_SWIGLU) {
-#pragma unroll
-            for (int c = 0; c < CHUNKS; c++)
-#pragma unroll
-                for (int i = 0; i < 8; i++)
-                    v[c][i] = hk_swiglu_f(v[c][i], u[c][i]);
-        }
         if (EIGHTS) {
 #pragma unroll
             for (int c = 0; c < CHUNKS; c++)
@@ -312,11 +301,15 @@ static hk_int8_rows_kernel hk_int8_rows_pick(bool few, uint32_t pitch) {
 template <int SOURCE>
 static void hk_int8_rows(struct h3_gpu *gpu, const hk_int8_rows_args &a) {
     const bool few = a.rows <= 512u && a.pitch > 2048u;
-    const bool any = a.pitch > 16384u || gpu->reference_kernels;
-    const hk_int8_rows_kernel kernel =
-        any                  ? hk_int8_rows_any<SOURCE>
-        : a.width % 8u == 0u ? hk_int8_rows_pick<SOURCE, true>(few, a.pitch)
-                             : hk_int8_rows_pick<SOURCE, false>(few, a.pitch);
+    const bool any = SOURCE == HK_ROWS_SWIGLU || a.pitch > 16384u ||
+                     gpu->reference_kernels;
+    hk_int8_rows_kernel kernel = hk_int8_rows_any<SOURCE>;
+    if constexpr (SOURCE != HK_ROWS_SWIGLU) {
+        if (!any)
+            kernel = a.width % 8u == 0u
+                         ? hk_int8_rows_pick<SOURCE, true>(few, a.pitch)
+                         : hk_int8_rows_pick<SOURCE, false>(few, a.pitch);
+    }
     const uint32_t threads = few && !any ? 1024u : 256u;
     hk_int8_each_rows(a.rows, [&](uint32_t first, uint32_t rows) {
         hipLaunchKernelGGL(kernel, dim3(rows), dim3(threads), 0, gpu->stream,
@@ -418,7 +411,7 @@ struct hk_int8_out {
     const float *xs, *ws;
     const uint16_t *bias;
     uint16_t *out;
-    float *wide; /* in F32 instead, padded rows */
+    float *wide; /* of the gated block: silu(g) u in F32, padded rows */
     uint32_t n;
     int gelu;
 };
@@ -451,11 +444,6 @@ __device__ __forceinline__ void hk_int8_finish(const hk_int8_out &o,
 #pragma unroll
     for (int e = 0; e < 4; e++)
         y[e] = hk_int8_made(o, sx, c.scale[e], c.bias[e], sums[e]);
-    if (o.wide) {
-        *(float4 *)(o.wide + (size_t)row * hk_int8_fours(o.n) + col) =
-            make_float4(y[0], y[1], y[2], y[3]);
-        return;
-    }
     uint16_t *to = o.out + (size_t)row * o.n + col;
     if (o.n % 4u == 0) {
         *(uint2 *)to = make_uint2(hk_pack2(y[0], y[1]), hk_pack2(y[2], y[3]));
@@ -469,6 +457,39 @@ __device__ __forceinline__ void hk_int8_finish(const hk_int8_out &o,
     }
 }
 
+/* The same, or of the gated block of a gate's sums and an up row's, whose scales
+ * stand in the place of the bias. */
+template <bool GATED>
+__device__ __forceinline__ void hk_int8_columns_load(hk_int8_columns &c,
+                                                     const hk_int8_out &o,
+                                                     uint32_t col) {
+    c.load(o, col);
+    if (GATED) {
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            c.bias[e] = col + e < o.n ? o.ws[o.n + col + e] : 0.0f;
+    }
+}
+
+template <bool GATED>
+__device__ __forceinline__ void hk_int8_leave(const hk_int8_out &o,
+                                              uint32_t row, uint32_t col,
+                                              float sx,
+                                              const hk_int8_columns &c,
+                                              hk_v4i sums, hk_v4i up) {
+    if (!GATED) {
+        hk_int8_finish(o, row, col, sx, c, sums);
+        return;
+    }
+    float y[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        y[e] = hk_swiglu_f(hk_int8_value(sums[e], sx, c.scale[e]),
+                           hk_int8_value(up[e], sx, c.bias[e]));
+    *(float4 *)(o.wide + (size_t)row * hk_int8_fours(o.n) + col) =
+        make_float4(y[0], y[1], y[2], y[3]);
+}
+
 /* One row, on the vector units: a wave takes COLUMNS rows of W, each lane 16
  * bytes of every 1024, against X's row in LDS, and adds up its lanes.  W
  * streams from HBM once, in loads of whole KiB, with no pieces of K to join in
@@ -476,20 +497,21 @@ __device__ __forceinline__ void hk_int8_finish(const hk_int8_out &o,
  * as MFMA tiles 9.7, 16.9 and 6.4; 5376 -> 28672 is level (25.4, 6.1 TB/s).  Of
  * more rows the reads of X from LDS are too many (two rows 5120 -> 5120 9.2 and
  * 9.7, 14336 -> 5376 21 and 17). */
-template <int COLUMNS>
+template <int COLUMNS, bool GATED>
 __global__ void __launch_bounds__(256)
 hk_int8_dot(hk_skinny_args g, hk_int8_out o, uint32_t pitch) {
     extern __shared__ __attribute__((aligned(16))) uint8_t xs[];
     const uint32_t tid = threadIdx.x, lane = tid & 63u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t chunks = pitch / 16u;
-    const uint32_t col0 = (blockIdx.x * 4u + wave) * COLUMNS;
+    const uint32_t col0 = (blockIdx.x * 4u + wave) * (GATED ? 1u : COLUMNS);
     constexpr int AHEAD = 4; /* loads of a row of W on their way */
     const hk_v4i *w[COLUMNS];
 #pragma unroll
     for (int c = 0; c < COLUMNS; c++)
         w[c] = (const hk_v4i *)((const uint8_t *)g.w +
-                                (size_t)min(col0 + c, g.n - 1u) * pitch);
+                                (size_t)min(GATED ? col0 + c * o.n : col0 + c,
+                                            g.n - 1u) * pitch);
     hk_v4i next[AHEAD][COLUMNS];
     auto load = [&](uint32_t at, hk_v4i (&to)[COLUMNS]) {
 #pragma unroll
@@ -523,17 +545,24 @@ hk_int8_dot(hk_skinny_args g, hk_int8_out o, uint32_t pitch) {
         }
     }
 #pragma unroll
-    for (int c = 0; c < COLUMNS; c++) {
-        int v = sum[c];
+    for (int c = 0; c < COLUMNS; c++)
 #pragma unroll
-        for (int off = 32; off; off >>= 1) v += __shfl_xor(v, off, 64);
+        for (int off = 32; off; off >>= 1)
+            sum[c] += __shfl_xor(sum[c], off, 64);
+    if constexpr (GATED) {
+        if (lane || col0 >= o.n) return;
+        o.wide[col0] = hk_swiglu_f(
+            hk_int8_value(sum[0], o.xs[0], o.ws[col0]),
+            hk_int8_value(sum[1], o.xs[0], o.ws[o.n + col0]));
+        return;
+    }
+#pragma unroll
+    for (int c = 0; c < COLUMNS; c++) {
         const uint32_t col = col0 + c;
         if (lane != (uint32_t)c || col >= g.n) continue;
-        const float y =
-            hk_int8_made(o, o.xs[0], o.ws[col],
-                         o.bias ? hk_bf2f(o.bias[col]) : -0.0f, v);
-        if (o.wide) o.wide[col] = y;
-        else o.out[col] = hk_f2bf(y);
+        o.out[col] = hk_f2bf(hk_int8_made(
+            o, o.xs[0], o.ws[col], o.bias ? hk_bf2f(o.bias[col]) : -0.0f,
+            sum[c]));
     }
 }
 
@@ -550,7 +579,7 @@ struct hk_int8_few_plan {
  * first (workgroup i runs on XCD i % 8): with the groups last in the grid 300 x
  * 1001 -> 5350 took 9.8 us, now 8.8, 256 x 5120 -> 13824 39.3 and 35.4.  A lone
  * group keeps the grid's order (128 x 5376 -> 28672: 37 us, dealt so 40). */
-template <int MB>
+template <int MB, bool GATED>
 __global__ void __launch_bounds__(256)
 hk_int8_skinny(hk_skinny_args g, hk_int8_out o, hk_int8_few_plan plan) {
     uint32_t at = blockIdx.x;
@@ -567,10 +596,12 @@ hk_int8_skinny(hk_skinny_args g, hk_int8_out o, hk_int8_few_plan plan) {
      * lane + 64: on their way during the loop */
     const uint32_t lane = threadIdx.x & 63u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    constexpr uint32_t COLS = GATED ? 16u : 32u, EACH = COLS / 4u;
+    const uint32_t col = (x * 4u + wave) * COLS + lane % EACH * 4u;
     hk_int8_columns columns;
     float sx[(MB + 1) / 2];
     if (!g.partial) {
-        columns.load(o, (x * 4u + wave) * 32u + (lane & 7u) * 4u);
+        hk_int8_columns_load<GATED>(columns, o, col);
 #pragma unroll
         for (uint32_t i = 0; i < (MB + 1) / 2; i++)
             sx[i] = o.xs[row0 + min(i * 64u + lane, g.m - 1u)];
@@ -592,7 +623,6 @@ hk_int8_skinny(hk_skinny_args g, hk_int8_out o, hk_int8_few_plan plan) {
             asm volatile("" : "+v"(columns.scale[e]), "+v"(columns.bias[e]));
 #pragma unroll
         for (int i = 0; i < (MB + 1) / 2; i++) asm volatile("" : "+v"(sx[i]));
-        const uint32_t col = n0 + (lane & 7u) * 4u;
 #pragma unroll
         for (int mb = 0; mb < MB; mb++) {
             /* through the wave's LDS, so that eight lanes write a row's 32
@@ -604,18 +634,22 @@ hk_int8_skinny(hk_skinny_args g, hk_int8_out o, hk_int8_few_plan plan) {
                     hk_v4i{acc[mb][q * 4], acc[mb][q * 4 + 1],
                            acc[mb][q * 4 + 2], acc[mb][q * 4 + 3]};
 #pragma unroll 1
-            for (uint32_t i = 0; i < 4; i++) {
-                const uint32_t r = i * 8u + (lane >> 3);
-                const hk_v4i sums = *(const hk_v4i *)(
-                    wbuf + r * 128u + (((lane & 7u) ^ (r & 7u)) << 4));
+            for (uint32_t i = 0; i < EACH / 2u; i++) {
+                const uint32_t r = i * (64u / EACH) + lane / EACH;
+                auto of = [&](uint32_t chunk) {
+                    return *(const hk_v4i *)(wbuf + r * 128u +
+                                             ((chunk ^ (r & 7u)) << 4));
+                };
+                const hk_v4i sums = of(lane % EACH);
+                const hk_v4i up = of(lane % EACH + (GATED ? EACH : 0u));
                 const float s = __shfl(sx[mb / 2], (mb & 1) * 32 + r, 64);
-                if (mb * 32u + r < g.m && col < g.n)
-                    hk_int8_finish(o, row0 + mb * 32u + r, col, s, columns,
-                                   sums);
+                if (mb * 32u + r < g.m && col < o.n)
+                    hk_int8_leave<GATED>(o, row0 + mb * 32u + r, col, s,
+                                         columns, sums, up);
             }
         }
     };
-    hk_skinny_sums<MB, 3, HK_LOAD_ONCE, hk_i32x16>(g, g.w, x, y, use);
+    hk_skinny_sums<MB, 3, HK_LOAD_ONCE, hk_i32x16, GATED>(g, g.w, x, y, use);
 }
 
 /* Narrow products: a workgroup per 32 columns and 32 rows, whose waves take a
@@ -625,7 +659,7 @@ hk_int8_skinny(hk_skinny_args g, hk_int8_out o, hk_int8_few_plan plan) {
  * latency, or by W's and X's bytes (8 rows 5120 -> 5120 7.7 us, 10.5 with pieces
  * of K; 8 x 3004 -> 5842 5.6 and 9.0; 2 x 5120 -> 13824 13.2 and 16.3; but 32 x
  * 13824 -> 5120 24 and 18.7). */
-template <int WAVES>
+template <int WAVES, bool GATED>
 __global__ void __launch_bounds__(WAVES * 64)
 hk_int8_narrow(hk_skinny_args g, hk_int8_out o, uint32_t groups) {
     extern __shared__ __attribute__((aligned(16))) uint8_t hk_lds[];
@@ -647,8 +681,9 @@ hk_int8_narrow(hk_skinny_args g, hk_int8_out o, uint32_t groups) {
     uint32_t wo[4];
 #pragma unroll
     for (int q = 0; q < 4; q++)
-        wo[q] = (min(n0 + 8u * q + (lane >> 3), n) * k + (lane & 7u) * 8u) *
-                2u;
+        wo[q] = ((GATED ? hk_skinny_gated(n0 + 8u * q + (lane >> 3), n)
+                        : min(n0 + 8u * q + (lane >> 3), n)) * k +
+                 (lane & 7u) * 8u) * 2u;
     const uint32_t xo = min(row, m) * k * 2u + half * 16u;
     hk_v4i wf[D][4], xf[D][4];
     auto load = [&](int slot, uint32_t step) {
@@ -663,14 +698,16 @@ hk_int8_narrow(hk_skinny_args g, hk_int8_out o, uint32_t groups) {
                 xr, hk_skinny_lane(xo + q * 32u, step, steps), kb, 0);
         __builtin_amdgcn_sched_barrier(0);
     };
-    /* a thread makes four columns of every (8 WAVES)th row */
-    const uint32_t col = n0 + (tid & 7u) * 4u;
+    /* a thread makes four columns of every so many rows */
+    constexpr uint32_t COLS = GATED ? 16u : 32u, EACH = COLS / 4u;
+    constexpr uint32_t AT_ONCE = 64u * WAVES / EACH, TURNS = 32u / AT_ONCE;
+    const uint32_t col = n0 / 32u * COLS + tid % EACH * 4u;
     hk_int8_columns columns;
-    columns.load(o, col);
-    float sx[4 / WAVES];
+    hk_int8_columns_load<GATED>(columns, o, col);
+    float sx[TURNS];
 #pragma unroll
-    for (uint32_t i = 0; i < 4 / WAVES; i++)
-        sx[i] = o.xs[row0 + min(i * 8u * WAVES + (tid >> 3), m - 1u)];
+    for (uint32_t i = 0; i < TURNS; i++)
+        sx[i] = o.xs[row0 + min(i * AT_ONCE + tid / EACH, m - 1u)];
 #pragma unroll
     for (int d = 0; d + 1 < D; d++) load(d, d);
     hk_i32x16 acc;
@@ -704,39 +741,52 @@ hk_int8_narrow(hk_skinny_args g, hk_int8_out o, uint32_t groups) {
         *(hk_v4i *)(own + row * 128u + (((q * 2u + half) ^ (row & 7u)) << 4)) =
             hk_v4i{acc[q * 4], acc[q * 4 + 1], acc[q * 4 + 2], acc[q * 4 + 3]};
     __syncthreads();
-    if (col >= n) return;
+    if (col >= o.n) return;
 #pragma unroll
-    for (uint32_t i = 0; i < 4 / WAVES; i++) {
-        const uint32_t r = i * 8u * WAVES + (tid >> 3);
-        hk_v4i sum = {0, 0, 0, 0};
+    for (uint32_t i = 0; i < TURNS; i++) {
+        const uint32_t r = i * AT_ONCE + tid / EACH;
+        auto of = [&](uint32_t chunk) {
+            hk_v4i sum = {0, 0, 0, 0};
 #pragma unroll
-        for (uint32_t j = 0; j < WAVES; j++)
-            sum += *(const hk_v4i *)(hk_lds + j * 4096u + r * 128u +
-                                     (((tid & 7u) ^ (r & 7u)) << 4));
-        if (r < m) hk_int8_finish(o, row0 + r, col, sx[i], columns, sum);
+            for (uint32_t j = 0; j < WAVES; j++)
+                sum += *(const hk_v4i *)(hk_lds + j * 4096u + r * 128u +
+                                         ((chunk ^ (r & 7u)) << 4));
+            return sum;
+        };
+        const hk_v4i sums = of(tid % EACH);
+        const hk_v4i up = GATED ? of(tid % EACH + EACH) : sums;
+        if (r < m)
+            hk_int8_leave<GATED>(o, row0 + r, col, sx[i], columns, sums, up);
     }
 }
 
 /* Adds the pieces, as hk_skinny_reduce. */
+template <bool GATED>
 __global__ void __launch_bounds__(256)
 hk_int8_skinny_reduce(hk_skinny_args g, hk_int8_out o, uint32_t mbs,
                       uint32_t tiles, uint32_t splits, uint32_t rows) {
     const uint32_t lane = threadIdx.x & 63u, q = threadIdx.x >> 6;
     const uint32_t tile = blockIdx.x / mbs, mb = blockIdx.x % mbs;
     const uint32_t row = mb * 32u + (lane & 31u);
-    const uint32_t col = tile * 32u + q * 8u + (lane >> 5) * 4u;
+    const uint32_t col =
+        tile * (GATED ? 16u : 32u) + q * 8u + (lane >> 5) * 4u;
     const uint32_t row0 = blockIdx.y * rows;
-    if (row >= min(g.m - row0, rows) || col >= g.n) return;
+    if (row >= min(g.m - row0, rows) || col >= o.n || (GATED && q >= 2u))
+        return;
     const size_t stride = (size_t)tiles * mbs * 256u;
     const hk_v4i *p = (const hk_v4i *)g.partial +
                       blockIdx.y * splits * stride +
                       (size_t)blockIdx.x * 256u + threadIdx.x;
     hk_int8_columns columns;
-    columns.load(o, col);
+    hk_int8_columns_load<GATED>(columns, o, col);
     const float sx = o.xs[row0 + row];
-    hk_v4i sum = *p;
-    for (uint32_t s = 1; s < splits; s++) sum += p[s * stride];
-    hk_int8_finish(o, row0 + row, col, sx, columns, sum);
+    constexpr uint32_t to_up = GATED ? 128u : 0u; /* two quarters further */
+    hk_v4i sum = *p, up = p[to_up];
+    for (uint32_t s = 1; s < splits; s++) {
+        sum += p[s * stride];
+        up += p[s * stride + to_up];
+    }
+    hk_int8_leave<GATED>(o, row0 + row, col, sx, columns, sum, up);
 }
 
 /* Adds the pieces of tiles, as hk_splitk_reduce: 4 columns a thread. */
@@ -969,42 +1019,49 @@ static hk_int8_few_plan hk_int8_few_planned(uint32_t cus, uint32_t m,
     return best;
 }
 
+template <bool GATED>
 static void hk_int8_few(struct h3_gpu *gpu, const hk_int8_matrix &x,
                         const hk_int8_matrix &w, const hk_int8_out &o) {
     hk_skinny_args g = {};
     g.x = (const uint16_t *)x.codes;
     g.w = (const uint16_t *)w.codes;
     g.m = x.rows;
-    g.n = o.n;
+    g.n = w.rows;
     g.k = x.pitch / 2u;
     g.w_bytes = w.rows * w.pitch;
     static uint64_t ready = 0;
     const uint64_t bit = 1ull << (gpu->device & 63);
     if (!(ready & bit)) {
-        (void)hipFuncSetAttribute((const void *)hk_int8_skinny<4>,
+        (void)hipFuncSetAttribute((const void *)hk_int8_skinny<4, GATED>,
                                   hipFuncAttributeMaxDynamicSharedMemorySize,
                                   4 * 4096 * 4 + 16384);
-        for (auto dot : {hk_int8_dot<1>, hk_int8_dot<2>})
+        for (auto dot : {hk_int8_dot<GATED ? 2 : 1, GATED>,
+                         hk_int8_dot<2, GATED>})
             (void)hipFuncSetAttribute(
                 (const void *)dot, hipFuncAttributeMaxDynamicSharedMemorySize,
                 HK_INT8_MOST_COLUMNS);
         ready |= bit;
     }
     if (x.rows == 1) {
-        /* two columns a wave where that leaves it eight turns of the CUs */
-        const uint32_t per = o.n > 16384u ? 2u : 1u;
-        hipLaunchKernelGGL(per == 2u ? hk_int8_dot<2> : hk_int8_dot<1>,
-                           dim3((o.n + 4u * per - 1u) / (4u * per)), dim3(256),
-                           x.pitch, gpu->stream, g, o, x.pitch);
+        /* two columns a wave where that leaves it eight turns of the CUs, or a
+         * gate and its up row */
+        const bool two = GATED || g.n > 16384u;
+        const uint32_t waves = two ? (g.n + 1u) / 2u : g.n;
+        const auto dot = two ? hk_int8_dot<2, GATED>
+                             : hk_int8_dot<GATED ? 2 : 1, GATED>;
+        hipLaunchKernelGGL(dot, dim3((waves + 3u) / 4u), dim3(256), x.pitch,
+                           gpu->stream, g, o, x.pitch);
         return;
     }
     float us;
-    hk_int8_few_plan p = hk_int8_few_planned(hk_int8_cus(gpu), x.rows, o.n,
+    hk_int8_few_plan p = hk_int8_few_planned(hk_int8_cus(gpu), x.rows, g.n,
                                              x.pitch / HK_INT8_LINE, &us);
     if (p.narrow) {
         const uint32_t workgroups = p.columns * p.groups;
+        const auto narrow = p.narrow == 2u ? hk_int8_narrow<2, GATED>
+                                           : hk_int8_narrow<1, GATED>;
         hipLaunchKernelGGL(
-            p.narrow == 2u ? hk_int8_narrow<2> : hk_int8_narrow<1>,
+            narrow,
             dim3(p.groups > 1u ? (workgroups + 7u) & ~7u : workgroups),
             dim3(p.narrow * 64u), p.narrow * 4096u, gpu->stream, g, o,
             p.groups);
@@ -1016,18 +1073,19 @@ static void hk_int8_few(struct h3_gpu *gpu, const hk_int8_matrix &x,
             gpu, (size_t)p.groups * p.splits * p.columns * 4 * p.mbs * 4096);
     if (!g.partial) p.splits = 1; /* no scratch: in one piece */
     void (*kernel)(hk_skinny_args, hk_int8_out, hk_int8_few_plan) =
-        p.mbs == 1   ? hk_int8_skinny<1>
-        : p.mbs == 2 ? hk_int8_skinny<2>
-        : p.mbs == 3 ? hk_int8_skinny<3>
-                     : hk_int8_skinny<4>;
+        p.mbs == 1   ? hk_int8_skinny<1, GATED>
+        : p.mbs == 2 ? hk_int8_skinny<2, GATED>
+        : p.mbs == 3 ? hk_int8_skinny<3, GATED>
+                     : hk_int8_skinny<4, GATED>;
     const uint32_t workgroups = p.columns * p.splits * p.groups;
     hipLaunchKernelGGL(kernel,
-                       dim3(p.groups > 1u ? (workgroups + 7u) & ~7u : workgroups),
+                       dim3(p.groups > 1u ? (workgroups + 7u) & ~7u
+                                          : workgroups),
                        dim3(256), p.mbs * 4096 * 4 + 16384, gpu->stream, g, o,
                        p);
     if (p.splits > 1)
-        hipLaunchKernelGGL(hk_int8_skinny_reduce,
-                           dim3((o.n + 31u) / 32u * p.mbs, p.groups),
+        hipLaunchKernelGGL(hk_int8_skinny_reduce<GATED>,
+                           dim3((g.n + 31u) / 32u * p.mbs, p.groups),
                            dim3(256), 0, gpu->stream, g, o, p.mbs,
                            p.columns * 4u, p.splits, 32u * p.mbs);
 }
@@ -1071,7 +1129,7 @@ static void hk_int8_linear(struct h3_gpu *gpu, hk_int8_matrix x,
     for (uint32_t left = x.rows; left; left -= x.rows) {
         x.rows = std::min(left, most);
         if (hk_int8_takes_few(gpu, x.rows, w.rows, x.pitch))
-            hk_int8_few(gpu, x, w, o);
+            hk_int8_few<false>(gpu, x, w, o);
         else
             hk_int8_tiles(gpu, x, w, w.rows, false, o,
                           {o.xs, o.ws, NULL, 0});
@@ -1081,17 +1139,8 @@ static void hk_int8_linear(struct h3_gpu *gpu, hk_int8_matrix x,
     }
 }
 
-/* Whether the gated block's first product goes over tiles, whose epilogue
- * leaves the activation; else both projections are left. */
-static bool hk_int8_gated_tiles(const struct h3_gpu *gpu,
-                                const hk_int8_matrix &x,
-                                const hk_int8_matrix &w) {
-    return hk_int8_fast(gpu, w) &&
-           !hk_int8_takes_few(gpu, x.rows, w.rows, x.pitch);
-}
-
-/* h = silu(x . gate^T) (x . up^T) in 8 bits, by way of F32 rows in `wide`, of
- * `hidden` elements over tiles and 2 hidden else, padded. */
+/* h = silu(x . gate^T) (x . up^T) in 8 bits, by way of padded F32 rows of it in
+ * `wide`, or of both projections from the simple kernel. */
 static void hk_int8_gated(struct h3_gpu *gpu, hk_int8_matrix x,
                           const hk_int8_matrix &w, uint32_t hidden,
                           float *wide, const hk_int8_matrix &h) {
@@ -1102,13 +1151,9 @@ static void hk_int8_gated(struct h3_gpu *gpu, hk_int8_matrix x,
     a.rows = x.rows;
     a.width = hidden;
     a.pitch = h.pitch;
-    if (!hk_int8_gated_tiles(gpu, x, w)) {
+    if (!hk_int8_fast(gpu, w)) {
         a.wide_pitch = hk_int8_fours(2 * hidden);
-        if (hk_int8_fast(gpu, w))
-            hk_int8_few(gpu, x, w, {x.scales, w.scales, NULL, NULL, wide,
-                                    2 * hidden, 0});
-        else
-            hk_int8_simple_run(gpu, x, w, NULL, NULL, wide, 0);
+        hk_int8_simple_run(gpu, x, w, NULL, NULL, wide, 0);
         hk_int8_rows<HK_ROWS_SWIGLU>(gpu, a);
         return;
     }
@@ -1117,7 +1162,11 @@ static void hk_int8_gated(struct h3_gpu *gpu, hk_int8_matrix x,
     hk_int8_ext e = {x.scales, w.scales, wide, a.wide_pitch};
     for (uint32_t left = x.rows; left; left -= x.rows) {
         x.rows = std::min(left, most);
-        hk_int8_tiles(gpu, x, w, hidden, true, {}, e);
+        if (hk_int8_takes_few(gpu, x.rows, w.rows, x.pitch))
+            hk_int8_few<true>(gpu, x, w,
+                              {e.xs, e.ws, NULL, NULL, e.wide, hidden, 0});
+        else
+            hk_int8_tiles(gpu, x, w, hidden, true, {}, e);
         x.codes += (size_t)x.rows * x.pitch;
         e.xs += x.rows;
         e.wide += (size_t)x.rows * e.wide_pitch;
@@ -1327,13 +1376,13 @@ int h3_hip_mlp_int8_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
         !hk_require_active(gpu))
         return 0;
     if (!rows || !output_dim) return 1;
-    /* F32 rows of the activation or, where they are few or go through the
-     * simple kernel, of both projections, then h in 8 bits */
+    /* F32 rows of the activation or, from the simple kernel, of both
+     * projections, then h in 8 bits */
     const hk_int8_matrix x = hk_int8_of(input, rows);
     const hk_int8_matrix w1 = hk_int8_of(fc1_weight, 2 * hidden_dim);
     const uint32_t pitch = fc2_weight->record.n[HK_INT8_PITCH];
     const size_t wide = hk_int8_fours(
-        hk_int8_gated_tiles(gpu, x, w1) ? hidden_dim : 2 * hidden_dim);
+        hk_int8_fast(gpu, w1) ? hidden_dim : 2 * hidden_dim);
     const size_t wide_bytes = (rows * wide * 4 + 255) & ~(size_t)255;
     const size_t code_bytes = (size_t)rows * pitch;
     uint8_t *space = (uint8_t *)hk_workspace(

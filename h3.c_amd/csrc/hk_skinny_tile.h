@@ -80,12 +80,21 @@ __device__ __forceinline__ void hk_skinny_mfma(hk_i32x16 &acc, hk_v4i w,
     acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(w, x, acc, 0, 0, 0);
 }
 
+/* The W row of column `at` where each 32 are 16 columns' gates and then their up
+ * rows, of n rows in all, gates first; n where there is none. */
+__device__ __forceinline__ uint32_t hk_skinny_gated(uint32_t at, uint32_t n) {
+    const uint32_t column = at / 32u * 16u + at % 16u;
+    return column < n / 2u ? (at & 16u ? n / 2u : 0u) + column : n;
+}
+
 /* use(acc, n0, row, half, wbuf) with the sums of piece y of workgroup x's
  * columns: acc[mb][r] = C[mb*32 + row][n0 + (r/4)*8 + half*4 + r%4], n0 = (4 x +
  * wave) 32, row and half of the lane, wbuf 4 KiB of LDS that are the wave's own.
- * Rows of bytes count K in pairs.  (With sums that a caller holds, the compiler
- * moves them about: 39 x 256 -> 10240, 5.0 us for 4.8.) */
-template <int MB, int XA, int W_POLICY, typename SUMS, typename USE>
+ * Rows of bytes count K in pairs.  GATED: columns as in hk_skinny_gated.  (With
+ * sums that a caller holds, the compiler moves them about: 39 x 256 -> 10240, 5.0
+ * us for 4.8.) */
+template <int MB, int XA, int W_POLICY, typename SUMS, bool GATED = false,
+          typename USE>
 __device__ __forceinline__ void hk_skinny_sums(const hk_skinny_args &g,
                                                const uint16_t *w, uint32_t x,
                                                uint32_t y, const USE &use) {
@@ -107,8 +116,9 @@ __device__ __forceinline__ void hk_skinny_sums(const hk_skinny_args &g,
     uint32_t wo[4];
 #pragma unroll
     for (int q = 0; q < 4; q++)
-        wo[q] = (min(n0 + 8u * q + (lane >> 3), n) * k + (lane & 7u) * 8u) *
-                2u;
+        wo[q] = ((GATED ? hk_skinny_gated(n0 + 8u * q + (lane >> 3), n)
+                        : min(n0 + 8u * q + (lane >> 3), n)) * k +
+                 (lane & 7u) * 8u) * 2u;
     /* the wave's W buffer, after the X stages */
     uint8_t *wbuf = hk_xs + (XA + 1) * XSTAGE + wave * 4096u;
     /* X staging: slot p = 256 i + tid holds row p / 8, physical chunk p % 8

@@ -405,7 +405,7 @@ int h3_hip_linear_gelu_int8_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
 /* The gated block of h3_gpu_mlp_bf16 in 8 bits: fc1 ([2 hidden][input], gate
  * rows first), h = silu(gate) up in F32, rows of h in 8 bits, fc2.  Uses the
  * context's scratch, which grows on demand: 5 bytes for each of rows x hidden,
- * 9 where the rows are few enough to run without tiles. */
+ * 9 if fc1's codes take 4 GiB or more. */
 int h3_hip_mlp_int8_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
                          const h3_gpu_tensor *input,
                          const h3_gpu_tensor *fc1_weight,

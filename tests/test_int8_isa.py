@@ -1,8 +1,9 @@
 """The 8-bit products, as compiled: the tiles' K loop is one copy, adds every
 product to the accumulator that it came from, moves none, touches no scratch
 memory, waits for its loads with vmcnt(2) only, and nothing reads a sum before
-the last products are through nor writes an operand right before its product; the loads of the kernel of few rows leave in the
-order that its waits count (test_gemm_isa.py has the same of bf16)."""
+the last products are through nor writes an operand right before its product;
+the loads of the kernel of few rows leave in the order that its waits count
+(test_gemm_isa.py has the same of bf16)."""
 import functools
 import os
 import re
@@ -86,9 +87,10 @@ def test_k_loop(epi, jb):
                 assert not registers(before.split(",")[0]) & sources, before
 
 
+@pytest.mark.parametrize("gated", [0, 1])
 @pytest.mark.parametrize("mb", [1, 2, 3, 4])
-def test_loads_of_few_rows_leave_in_the_order_its_waits_count(mb):
-    body = body_of(f"hk_int8_skinnyILi{mb}EE")
+def test_loads_of_few_rows_leave_in_the_order_its_waits_count(mb, gated):
+    body = body_of(f"hk_int8_skinnyILi{mb}ELb{gated}EE")
     loads = [(i, "X" if re.search(r"\blds\b", l) else "W")
              for i, l in enumerate(body) if "buffer_load_" in l]
     step = "X" * mb + "WWWW"
