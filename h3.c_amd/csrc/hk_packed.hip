@@ -605,8 +605,9 @@ __device__ __forceinline__ void hk_packed_item_of(const hk_packed_args &a) {
             ahead = block_scales[2u * (size_t)(tile + 1u) * a.kv_heads];
         if (more) issue_tile(tile + 1u, stage ^ 1u);
         if (live) {
-        /* what multiplies a raw score: of a block of zeros they are 0, and -inf
-         * has to stay it */
+        /* what multiplies a raw score: of a block of zeros they are 0, whatever
+         * does, and -inf, of keys past the end, has to stay it */
+        const float by = scale == 0.0f ? 0x1p-100f : scale;
         float L = a.scale_log2;
         if (SCALED) {
             L = fmaxf(L * scale, 0x1p-120f);
@@ -685,7 +686,7 @@ __device__ __forceinline__ void hk_packed_item_of(const hk_packed_args &a) {
             for (int kt = 0; kt < 2; kt++)
 #pragma unroll
                 for (int r = 0; r < 16; r++) mx = fmaxf(mx, s[kt][r]);
-            if (SCALED) mx *= scale;
+            if (SCALED) mx *= by;
             const auto sw = __builtin_amdgcn_permlane32_swap(
                 __float_as_uint(mx), __float_as_uint(mx), false, false);
             mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
@@ -699,17 +700,17 @@ __device__ __forceinline__ void hk_packed_item_of(const hk_packed_args &a) {
             neg = -(m_new * a.scale_log2);
             float less = -(ref * a.scale_log2);
             if (__builtin_amdgcn_ballot_w64(hk_packed_far(less))) {
-                const float by = hk_packed_far(less) ? ref : 0.0f;
+                const float off = hk_packed_far(less) ? ref : 0.0f;
 #pragma unroll
                 for (int kt = 0; kt < 2; kt++)
 #pragma unroll
                     for (int r = 0; r < 16; r++) {
                         if (SCALED) {
                             /* as the reference was rounded: no fused add */
-                            s[kt][r] *= scale;
+                            s[kt][r] *= by;
                             asm volatile("" : "+v"(s[kt][r]));
                         }
-                        s[kt][r] -= by;
+                        s[kt][r] -= off;
                     }
                 if (SCALED) L = a.scale_log2;
                 if (hk_packed_far(less)) less = 0.0f;

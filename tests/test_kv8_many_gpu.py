@@ -1,0 +1,42 @@
+"""Attention over the 8-bit cache by items of more than 32 rows and of fewer,
+where scores and factors lie far from zero or one, against the same in 64 bits
+at the bounds of int8_oracle."""
+import numpy as np
+import pytest
+
+import int8_oracle as io
+import requests_oracle as ro
+from test_kv8_gpu import Case, Kv
+
+pytestmark = pytest.mark.gpu
+
+FEW, ROWS = 20, 129  # query rows of items of each kind, with up to 128 keys
+
+
+def numbers(c):
+    """A case's query rows in 64 bits, [row][head][dim]."""
+    return ro.wide(c.q, c.rows, c.heads, c.dim).copy()
+
+
+def put(c, q):
+    c.q = io.bits(q.astype(np.float32)).ravel()
+
+
+@pytest.mark.parametrize("rows", [FEW, ROWS])
+@pytest.mark.parametrize("dim", [64, 96, 128])
+@pytest.mark.parametrize("stored", [False, True])
+def test_far_scores_and_a_last_block_of_zeros(gpu, rows, dim, stored):
+    """Scores to +-1e3 of one block of keys, then part of a block whose keys are
+    zeros, stored or not."""
+    c = Case(gpu, [rows], [70], 2, 2, dim)
+    c.kv = Kv(gpu, 128, 2, dim)
+
+    def change(kv):
+        kv[:64, 0] = kv[:64, dim] = 0x42c8  # 100
+        kv[64:, :2 * dim] = 0
+    c.kv.store([0], [70 if stored else 64], change=change)
+    q = numbers(c)
+    q[:, :, 0] = 0
+    q[::5, 0, 0], q[3::7, 1, 0] = 200, -200
+    put(c, q)
+    c.check()
