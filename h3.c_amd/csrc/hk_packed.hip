@@ -610,8 +610,8 @@ __device__ __forceinline__ void hk_packed_item_of(const hk_packed_args &a) {
         const float by = scale == 0.0f ? 0x1p-100f : scale;
         float L = a.scale_log2;
         if (SCALED) {
-            L = fmaxf(L * scale, 0x1p-120f);
-            if (isnan(scale)) L = scale; /* which fmaxf leaves out */
+            L *= by;
+            if (L == 0.0f) L = 0x1p-149f; /* the least there is */
         }
         hk_f32x16 s[2];
 #pragma unroll

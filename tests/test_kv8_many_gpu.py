@@ -40,3 +40,17 @@ def test_far_scores_and_a_last_block_of_zeros(gpu, rows, dim, stored):
     q[::5, 0, 0], q[3::7, 1, 0] = 200, -200
     put(c, q)
     c.check()
+
+
+@pytest.mark.parametrize("rows", [FEW, ROWS])
+@pytest.mark.parametrize("dim", [64, 80, 128])
+@pytest.mark.parametrize("size,std,scale", [
+    (1e34, 1e-31, 4.6e-5), (1e30, 1e-32, 1e-1), (1e-30, 1e30, 0.2),
+    (1e-3, 1e-33, 1e35)])
+def test_scores_of_large_and_small_factors(gpu, rows, dim, size, std, scale):
+    """Queries, keys and the scale near the ends of F32's range, scores of
+    ordinary size."""
+    c = Case(gpu, [rows], [100], 2, 2, dim, std=std)
+    put(c, numbers(c) * size)
+    c.scale = float(np.float32(scale))
+    c.check()
