@@ -700,20 +700,22 @@ __device__ __forceinline__ void hk_packed_item_of(const hk_packed_args &a) {
             neg = -(m_new * a.scale_log2);
             float less = -(ref * a.scale_log2);
             if (__builtin_amdgcn_ballot_w64(hk_packed_far(less))) {
-                const float off = hk_packed_far(less) ? ref : 0.0f;
+                const bool apart = hk_packed_far(less); /* this row's is */
 #pragma unroll
                 for (int kt = 0; kt < 2; kt++)
 #pragma unroll
                     for (int r = 0; r < 16; r++) {
                         if (SCALED) {
                             /* as the reference was rounded: no fused add */
-                            s[kt][r] *= by;
-                            asm volatile("" : "+v"(s[kt][r]));
+                            float x = s[kt][r] * by;
+                            asm volatile("" : "+v"(x));
+                            s[kt][r] = apart ? x - ref : s[kt][r];
+                        } else {
+                            s[kt][r] -= apart ? ref : 0.0f;
                         }
-                        s[kt][r] -= off;
                     }
-                if (SCALED) L = a.scale_log2;
-                if (hk_packed_far(less)) less = 0.0f;
+                if (SCALED && apart) L = a.scale_log2;
+                if (apart) less = 0.0f;
             }
             l_part *= c;
 #pragma unroll

@@ -54,3 +54,26 @@ def test_scores_of_large_and_small_factors(gpu, rows, dim, size, std, scale):
     put(c, numbers(c) * size)
     c.scale = float(np.float32(scale))
     c.check()
+
+
+@pytest.mark.parametrize("qn", [[ROWS] * 3])
+@pytest.mark.parametrize("dim", [64, 96, 128])
+def test_a_row_is_the_same_beside_any_others(gpu, qn, dim):
+    """Its bits, with rows beside it of scores far from zero, of infinities and
+    of NaN."""
+    c = Case(gpu, qn, [110] * len(qn), 2, 2, dim, share=True)
+    put(c, numbers(c) * 40)
+    want = c.check()
+    q = numbers(c)
+    other = np.arange(c.rows) % 3 > 0
+    q[other] *= 100 * np.random.default_rng(1).uniform(-1, 1,
+                                                       (other.sum(), 1, 1))
+    put(c, q)
+    got = c.check()
+    assert np.array_equal(got[~other], want[~other])
+    assert (got[other] != want[other]).any()
+    bits = c.q.reshape(c.rows, 2, dim)
+    bits[1, 0, 3], bits[4, 0, 5], bits[5, 1, 6] = 0x7f80, 0x7fc0, 0xff80
+    spoilt = c.run()
+    assert np.array_equal(spoilt[~other], want[~other])
+    assert np.isnan(ro.wide(spoilt, *spoilt.shape)[4, 0]).all()
