@@ -666,17 +666,19 @@ template <int DIMS> struct hk_kv8_wave {
             neg = -(now * L);
             float less = -(ref * L);
             if (__builtin_amdgcn_ballot_w64(hk_kv8_far(less))) {
-                /* scores as they are, rounded as the reference was, and the
-                 * reference off them first, which is exact near it */
-                const float off = hk_kv8_far(less) ? ref : 0.0f;
+                /* this row's scores as they are, rounded as the reference was,
+                 * and the reference off them first, which is exact near it */
+                const bool apart = hk_kv8_far(less);
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
                     float x = s[r] * by;
                     asm volatile("" : "+v"(x)); /* no fused add */
-                    s[r] = x - off;
+                    s[r] = apart ? x - ref : s[r];
                 }
-                own = L;
-                if (hk_kv8_far(less)) less = 0.0f;
+                if (apart) {
+                    own = L;
+                    less = 0.0f;
+                }
             }
             l *= c;
 #pragma unroll

@@ -56,7 +56,7 @@ def test_scores_of_large_and_small_factors(gpu, rows, dim, size, std, scale):
     c.check()
 
 
-@pytest.mark.parametrize("qn", [[ROWS] * 3])
+@pytest.mark.parametrize("qn", [[FEW] * 20, [ROWS] * 3])
 @pytest.mark.parametrize("dim", [64, 96, 128])
 def test_a_row_is_the_same_beside_any_others(gpu, qn, dim):
     """Its bits, with rows beside it of scores far from zero, of infinities and
