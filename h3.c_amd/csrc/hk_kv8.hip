@@ -357,10 +357,10 @@ hk_kv8_read(hk_kv8_cache c, uint16_t *key, uint16_t *value, uint32_t first,
 }
 
 /* A plan's spans of blocks as rows, [block][64][keys, values][head][dim]: the
- * keys' codes as bf16, which holds them, and the values as f16, divided by a
- * power of two that leaves the span's largest in f16's range, 2^15 at most, and
- * rounded to 11 bits (those under 2^-29 of it to fewer).  889 rows of 40 heads of
- * 128 in 9.4 us. */
+ * keys' codes, times their unit, as bf16, which holds them, and the values as
+ * f16, divided by a power of two that leaves the span's largest in f16's range,
+ * 2^15 at most, and rounded to 11 bits (those under 2^-29 of it to fewer).  889
+ * rows of 40 heads of 128 in 9.4 us. */
 __global__ void __launch_bounds__(256)
 hk_kv8_unpack(hk_kv8_cache c, const hk_packed_span *spans, uint32_t count,
               uint16_t *out, float *units, uint32_t first) {
@@ -378,8 +378,10 @@ hk_kv8_unpack(hk_kv8_cache c, const hk_packed_span *spans, uint32_t count,
     const uint32_t head = blockIdx.y, which = blockIdx.z;
     const uint64_t row0 = (uint64_t)to * HK_KV8_BLOCK;
     const size_t at = (size_t)block * c.heads + head;
-    float scale = 1.0f;
-    if (which) {
+    float scale;
+    if (which == 0) {
+        scale = hk_packed_code_unit(c.scales[at].x);
+    } else {
         uint32_t most = 0;
         for (uint32_t i = threadIdx.x; i < span.blocks; i += 256u) {
             const uint32_t s = hk_magnitude(

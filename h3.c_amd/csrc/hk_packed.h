@@ -59,6 +59,15 @@ struct hk_packed_span {
     uint32_t block, at, blocks;
 };
 
+/* What the codes of a block's keys are multiplied by among those rows: over 128
+ * dims a raw score, the query's product with the codes, would be up to 2^14
+ * times the query's largest element, past F32's range where the score, of keys
+ * of a scale under 1, is not.  A block of zeros (a scale of 0) has zeros,
+ * whatever its codes. */
+__device__ __forceinline__ float hk_packed_code_unit(float scale) {
+    return scale == 0.0f ? 0.0f : scale < 1.0f ? 0x1p-14f : 1.0f;
+}
+
 struct hk_packed_args {
     const uint16_t *q, *k, *v;
     uint16_t *o;
@@ -73,7 +82,7 @@ struct hk_packed_args {
      * (reference, sum) [part][HK_PACKED_QB] */
     float *part_o;
     float2 *part_ml;
-    /* keys that are codes (hk_packed_codes): the items' first rows, the keys'
+    /* keys that are codes times a unit (hk_packed_codes): the items' first rows, the keys'
      * scales, [block][key head][2], and what the values are divided by, of a
      * span's first block [block among the spans'][key head] */
     const uint32_t *kv_at;

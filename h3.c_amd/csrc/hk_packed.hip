@@ -450,8 +450,9 @@ __device__ __forceinline__ void hk_packed_few(const hk_packed_args &a,
 
 typedef _Float16 hk_packed_f16x8 __attribute__((ext_vector_type(8)));
 
-/* SCALED: keys are codes, whole numbers to 127 as bf16, of blocks of 64 rows
- * with a scale each, which goes into L; references are scores as they are.
+/* SCALED: keys are codes, whole numbers to 127 times hk_packed_code_unit as
+ * bf16, of blocks of 64 rows with a scale each, which goes into L; references are
+ * scores as they are.
  * Values are f16, divided by a power of two of the request's and the head's
  * (hk_kv8.hip), and so are P, times 2^7, which move at 2^15: P rounds to 11
  * bits over 2^-21 of the largest. */
@@ -607,7 +608,9 @@ __device__ __forceinline__ void hk_packed_item_of(const hk_packed_args &a) {
         if (live) {
         /* what multiplies a raw score: of a block of zeros they are 0, whatever
          * does, and -inf, of keys past the end, has to stay it */
-        const float by = scale == 0.0f ? 0x1p-100f : scale;
+        const float by = scale == 0.0f   ? 1.0f
+                         : scale < 1.0f ? scale * 0x1p14f
+                                        : scale;
         float L = a.scale_log2;
         if (SCALED) {
             L *= by;

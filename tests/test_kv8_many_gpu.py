@@ -45,14 +45,29 @@ def test_far_scores_and_a_last_block_of_zeros(gpu, rows, dim, stored):
 @pytest.mark.parametrize("rows", [FEW, ROWS])
 @pytest.mark.parametrize("dim", [64, 80, 128])
 @pytest.mark.parametrize("size,std,scale", [
-    (1e34, 1e-31, 4.6e-5), (1e30, 1e-32, 1e-1), (1e-30, 1e30, 0.2),
-    (1e-3, 1e-33, 1e35)])
+    (5e37, 1e-34, 1e-5), (1e36, 1e-33, 4.6e-5), (1e34, 1e-31, 4.6e-5),
+    (1e30, 1e-32, 1e-1), (1e-30, 1e30, 0.2), (1e-35, 1e30, 1e4),
+    (1e-30, 1.0, 1e29), (1e-3, 1e-33, 1e35)])
 def test_scores_of_large_and_small_factors(gpu, rows, dim, size, std, scale):
     """Queries, keys and the scale near the ends of F32's range, scores of
     ordinary size."""
     c = Case(gpu, [rows], [100], 2, 2, dim, std=std)
     put(c, numbers(c) * size)
     c.scale = float(np.float32(scale))
+    c.check()
+
+
+@pytest.mark.parametrize("rows", [FEW, ROWS])
+def test_rows_never_stored_are_zeros_to_large_queries(gpu, rows):
+    """In memory that held something else."""
+    c = Case(gpu, [rows], [70], 2, 2, 64)
+    old = Kv(gpu, 128, 2, 64)
+    old.store([0], [128], std=30.0)
+    gpu.free(old.t)
+    c.kv = Kv(gpu, 128, 2, 64)
+    c.kv.store([0], [64], std=1e-33)
+    put(c, numbers(c) * 1e35)
+    c.scale = float(np.float32(4.6e-4))
     c.check()
 
 
