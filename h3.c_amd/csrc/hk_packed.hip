@@ -818,8 +818,12 @@ __device__ __forceinline__ void hk_packed_item_of(const hk_packed_args &a) {
         return;
     }
     /* no keys, or none with weight: zeros (a NaN sum gives NaN) */
-    float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    if (SCALED) inv *= unit;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    /* the unit last: its product with 1 / l may be subnormal */
+    const int power = (int)(__float_as_uint(unit) >> 23) - 127;
+    auto made = [&](float x) {
+        return SCALED ? __builtin_amdgcn_ldexpf(x * inv, power) : x * inv;
+    };
     uint8_t *ow = hk_lds + wave * (32u * ROW);
 #pragma unroll
     for (int d = 0; d < ND; d++)
@@ -828,10 +832,10 @@ __device__ __forceinline__ void hk_packed_item_of(const hk_packed_args &a) {
             const uint32_t chunk = d * 4u + blk;
             *(uint2 *)(ow + col * ROW +
                        ((chunk ^ hk_packed_k_key<DP>(col)) << 4) + half * 8u) =
-                make_uint2(hk_pack2(o[d][blk * 4 + 0] * inv,
-                                    o[d][blk * 4 + 1] * inv),
-                           hk_pack2(o[d][blk * 4 + 2] * inv,
-                                    o[d][blk * 4 + 3] * inv));
+                make_uint2(hk_pack2(made(o[d][blk * 4 + 0]),
+                                    made(o[d][blk * 4 + 1])),
+                           hk_pack2(made(o[d][blk * 4 + 2]),
+                                    made(o[d][blk * 4 + 3])));
         }
     const __amdgpu_buffer_rsrc_t outr =
         hk_attn_rsrc(a.o + (((uint64_t)it.q_first + r0) * a.heads +

@@ -92,3 +92,16 @@ def test_a_row_is_the_same_beside_any_others(gpu, qn, dim):
     spoilt = c.run()
     assert np.array_equal(spoilt[~other], want[~other])
     assert np.isnan(ro.wide(spoilt, *spoilt.shape)[4, 0]).all()
+
+
+def test_values_of_the_smallest_sizes(gpu):
+    """Near 2^-113, the mean of 1475 of them."""
+    c = Case(gpu, [4096], [1475], 8, 8, 64)
+
+    def change(kv):
+        v = ro.wide(kv, *kv.shape)
+        v[:, 512:] = 1.5e-34 * (1 + 0.01 * np.tanh(v[:, 512:]))
+        kv[:] = io.bits(v.astype(np.float32)).reshape(kv.shape)
+    c.kv.store([0], [1475], change=change)
+    put(c, numbers(c) * 0)
+    c.check()
