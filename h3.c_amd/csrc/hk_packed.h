@@ -46,15 +46,15 @@ enum { HK_PACKED_HEADS, HK_PACKED_KV_HEADS, HK_PACKED_DIM,
        HK_PACKED_JOIN_ROWS, /* the most virtual rows of a join */
        HK_PACKED_PARTS,
        HK_PACKED_OFF_BLOCKS, /* a request's keys begin inside 64 rows */
-       HK_PACKED_FEW, HK_PACKED_MANY, /* items of up to 32 rows, and over */
+       HK_PACKED_FEW, HK_PACKED_MANY, /* has items of up to 32 rows, over */
        HK_PACKED_SPANS, HK_PACKED_SPAN_BLOCKS };
 #define HK_PACKED_TOO_MANY UINT32_MAX /* blocks of spans: they have no list */
 
 /* For a cache in blocks of 64 rows that is unpacked into rows for the items of
  * many rows: blocks [block, + blocks) of it, which those items read, go to
- * blocks [at, + blocks) of the rows.  Behind a plan's lists follow, if any
- * request has such items and all begin at whole blocks, a word for each item,
- * the first of its keys among those rows, and the spans. */
+ * blocks [at, + blocks) of the rows.  If any request has such items and all
+ * begin at whole blocks, the spans follow a plan's lists, in the order of block
+ * and blocks, one for each pair that a request has. */
 struct hk_packed_span {
     uint32_t block, at, blocks;
 };
@@ -82,11 +82,11 @@ struct hk_packed_args {
      * (reference, sum) [part][HK_PACKED_QB] */
     float *part_o;
     float2 *part_ml;
-    /* keys that are codes times a unit (hk_packed_codes): the items' first rows, the keys'
-     * scales, [block][key head][2], and what the values are divided by, of a
-     * span's first block [block among the spans'][key head] */
-    const uint32_t *kv_at;
+    /* keys that are codes times a unit (hk_packed_codes): where they lie among
+     * the rows, their scales, [block][key head][2], and what the values are
+     * divided by, of a span's first block [block among the spans'][key head] */
     const hk_packed_span *spans;
+    uint32_t span_count;
     const float *key_scales, *value_units;
 };
 
@@ -117,8 +117,8 @@ static inline void hk_packed_of_plan(hk_packed_args &a,
     a.rows = n[HK_PACKED_ROWS];
     a.items = (const hk_packed_item *)(a.requests + a.request_count);
     a.joins = (const hk_packed_join *)(a.items + n[HK_PACKED_ITEMS]);
-    a.kv_at = (const uint32_t *)(a.joins + n[HK_PACKED_JOINS]);
-    a.spans = (const hk_packed_span *)(a.kv_at + n[HK_PACKED_ITEMS]);
+    a.spans = (const hk_packed_span *)(a.joins + n[HK_PACKED_JOINS]);
+    a.span_count = n[HK_PACKED_SPANS];
 }
 
 /* Elements that a tensor needs for `rows` rows from `offset` on; sizes past

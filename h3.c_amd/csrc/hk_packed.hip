@@ -26,7 +26,6 @@
 
 #include <algorithm>
 #include <functional>
-#include <map>
 #include <new>
 #include <queue>
 #include <type_traits>
@@ -450,6 +449,27 @@ __device__ __forceinline__ void hk_packed_few(const hk_packed_args &a,
 
 typedef _Float16 hk_packed_f16x8 __attribute__((ext_vector_type(8)));
 
+/* The first row of the span of `blocks` blocks from `block` on.  Each lane looks
+ * at one of 64 spans, so that few requests cost a single load. */
+__device__ __forceinline__ uint32_t hk_packed_span_row(
+    const hk_packed_args &a, uint32_t block, uint32_t blocks) {
+    uint32_t low = 0, high = a.span_count;
+    while (high - low > 64u) {
+        const uint32_t mid = (low + high) / 2u;
+        const hk_packed_span s = a.spans[mid];
+        if (s.block < block || (s.block == block && s.blocks <= blocks))
+            low = mid;
+        else
+            high = mid;
+    }
+    const hk_packed_span s =
+        a.spans[min(low + (threadIdx.x & 63u), high - 1u)];
+    const uint64_t found = __builtin_amdgcn_ballot_w64(
+        s.block == block && s.blocks == blocks);
+    return (uint32_t)__builtin_amdgcn_readlane(
+               (int)s.at, __builtin_ctzll(found)) * HK_KT;
+}
+
 /* SCALED: keys are codes, whole numbers to 127 times hk_packed_code_unit as
  * bf16, of blocks of 64 rows with a scale each, which goes into L; references are
  * scores as they are.
@@ -496,10 +516,13 @@ __device__ __forceinline__ void hk_packed_item_of(const hk_packed_args &a) {
         k_off[i] = kc < dim_chunks ? row * stride + kc * 16u : 0x80000000u;
         v_off[i] = vc < dim_chunks ? row * stride + vc * 16u : 0x80000000u;
     }
-    /* (a plan of requests without keys has no list of their places) */
-    const uint32_t kv_first = !SCALED                   ? it.kv_first
-                              : it.tile_end != it.tile ? a.kv_at[blockIdx.x]
-                                                       : 0u;
+    /* (requests without keys have no span) */
+    const uint32_t kv_first =
+        !SCALED ? it.kv_first
+        : it.tile_end != it.tile
+            ? hk_packed_span_row(a, it.kv_first / HK_KT,
+                                 (it.kv_rows + HK_KT - 1u) / HK_KT)
+            : 0u;
     const uint64_t kv_base = (uint64_t)kv_first * a.kv_stride +
                              (uint64_t)it.kv_head * a.dim;
     /* the scale of the tile's block, loaded a tile ahead */
@@ -941,7 +964,6 @@ static void hk_packed_launch(struct h3_gpu *gpu, const hk_packed_args &a,
     for (uint32_t first = 0; first < n[HK_PACKED_ITEMS]; first += most) {
         hk_packed_args part = a;
         part.items = a.items + first;
-        part.kv_at = a.kv_at + first;
         hipLaunchKernelGGL(SCALED ? hk_packed_codes<DIMS>
                                   : hk_packed_flash<DIMS>,
                            dim3(std::min(n[HK_PACKED_ITEMS] - first, most)),
@@ -1005,6 +1027,7 @@ struct hk_packed_work {
     std::vector<hk_packed_item> items;
     std::vector<hk_packed_join> joins;
     uint32_t parts, join_rows;
+    uint32_t qb; /* rows of an item, but for a request's last */
 };
 
 /* Items [first, first + count) of a request: kv_head * blocks + block of its
@@ -1158,6 +1181,7 @@ static void hk_packed_lay_out(const std::vector<hk_packed_request> &list,
     std::vector<hk_packed_item> queue[8];
     double load[8] = {};
     work.parts = work.join_rows = 0;
+    work.qb = qb;
     for (const hk_packed_run &s : runs) {
         const hk_packed_request &r = list[s.request];
         for (uint64_t run = 0; run < 8; run++) {
@@ -1269,6 +1293,10 @@ h3_gpu_tensor *h3_hip_sdpa_packed_plan(h3_gpu *gpu, const uint32_t *q_first,
                           gpu->num_cus > 0 ? (uint32_t)gpu->num_cus : 256u,
                           work);
         std::vector<uint32_t> words;
+        words.reserve(1 + (list.size() * (sizeof(list[0]) +
+                                          sizeof(hk_packed_span)) +
+                           work.items.size() * sizeof(work.items[0]) +
+                           work.joins.size() * sizeof(work.joins[0])) / 4);
         auto add = [&](const void *data, size_t bytes) {
             const uint32_t *w = (const uint32_t *)data;
             words.insert(words.end(), w, w + bytes / 4);
@@ -1278,42 +1306,42 @@ h3_gpu_tensor *h3_hip_sdpa_packed_plan(h3_gpu *gpu, const uint32_t *q_first,
         add(work.joins.data(), work.joins.size() * sizeof(work.joins[0]));
         if (words.empty()) words.push_back(0);
         const size_t lists = words.size();
-        uint32_t few = 0, many = 0, span_blocks = 0;
-        /* by their first block and their number: what a request comes to does
-         * not depend on keys that only others read */
-        std::map<std::pair<uint32_t, uint32_t>, hk_packed_span> spans;
-        auto span_of = [](const hk_packed_item &item) {
-            return std::make_pair(
-                item.kv_first / HK_KT,
-                (uint32_t)(((uint64_t)item.kv_rows + HK_KT - 1) / HK_KT));
-        };
-        for (const hk_packed_item &item : work.items) {
-            if (item.row >= item.rows) continue;
-            (item.rows - item.row <= 32u ? few : many)++;
-            if (off_blocks || item.rows - item.row <= 32u || !item.kv_rows)
-                continue;
-            const auto span = span_of(item);
-            spans[span] = {span.first, 0, span.second};
+        /* which kinds of items there are, and the spans that those of many rows
+         * read: what a request comes to does not depend on keys that only
+         * others read */
+        bool few = false, many = false;
+        std::vector<hk_packed_span> spans;
+        for (const auto &r : list) {
+            const uint32_t all = r.q_rows * (heads / kv_heads);
+            const bool tall = work.qb > 32u && all > 32u;
+            many |= tall;
+            few |= !tall || (all - 1u) % work.qb < 32u;
+            if (tall && r.kv_rows && !off_blocks)
+                spans.push_back({r.kv_first / HK_KT, 0,
+                                 (r.kv_rows - 1u) / HK_KT + 1u});
         }
-        for (auto &s : spans) {
-            s.second.at = span_blocks;
+        auto before = [](const hk_packed_span &x, const hk_packed_span &y) {
+            return x.block != y.block ? x.block < y.block
+                                      : x.blocks < y.blocks;
+        };
+        std::sort(spans.begin(), spans.end(), before);
+        spans.erase(std::unique(spans.begin(), spans.end(),
+                                [&](const auto &x, const auto &y) {
+                                    return !before(x, y);
+                                }),
+                    spans.end());
+        uint32_t span_blocks = 0;
+        for (hk_packed_span &s : spans) {
+            s.at = span_blocks;
             /* their rows are numbered in 32 bits */
-            if (s.second.blocks > UINT32_MAX / HK_KT - span_blocks) {
+            if (s.blocks > UINT32_MAX / HK_KT - span_blocks) {
                 span_blocks = HK_PACKED_TOO_MANY;
                 spans.clear();
                 break;
             }
-            span_blocks += s.second.blocks;
+            span_blocks += s.blocks;
         }
-        if (!spans.empty()) {
-            for (const hk_packed_item &item : work.items) {
-                const auto s = item.row < item.rows
-                                   ? spans.find(span_of(item))
-                                   : spans.end();
-                words.push_back(s == spans.end() ? 0u : s->second.at * HK_KT);
-            }
-            for (const auto &s : spans) add(&s.second, sizeof(s.second));
-        }
+        add(spans.data(), spans.size() * sizeof(spans[0]));
         h3_gpu_tensor *plan =
             h3_gpu_tensor_from_u32(gpu, words.data(), words.size());
         if (!plan) return NULL;

@@ -105,3 +105,14 @@ def test_values_of_the_smallest_sizes(gpu):
     c.kv.store([0], [1475], change=change)
     put(c, numbers(c) * 0)
     c.check()
+
+
+@pytest.mark.parametrize("count", [63, 64, 65, 150])
+def test_many_requests(gpu, count):
+    """Each with a range of blocks of its own, or one of several of a text."""
+    kn = [1 + 37 * i % 128 for i in range(count)]
+    Case(gpu, [33 + i % 3 for i in range(count)], kn, 5, 5, 64).check()
+    c = Case(gpu, [40] * count, [700] * count, 5, 5, 64, share=True)
+    c.kf = [64 * (i % 7) for i in range(count)]
+    c.kn = [1 + 23 * i % 250 for i in range(count)]
+    c.check()
