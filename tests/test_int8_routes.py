@@ -10,6 +10,7 @@ from conftest import ROOT
 from requests_oracle import on_fake
 from test_int8_kernels_gpu import GATED, OUT, PRODUCTS
 from test_int8_no_room_gpu import BLOCKS, ROOM, WHOLE
+from test_kv8_many_gpu import FEW, MANY, ROWS
 
 RUN = """
 out = []
@@ -106,3 +107,69 @@ def test_every_kernel_is_among_them():
     found = set(re.findall(r"\bhk_int8_(\w+)\(hk_(?:skinny|gemm)_args",
                            text)) | {"gemm"}
     assert {n.split("<")[0] for n in names} == found
+
+
+ATTEND = """
+out = []
+for qn, kf, kn, heads, kv, dim in cases:
+    qf = [int(v) for v in np.cumsum([0] + qn)[:-1]]
+    if kf is None:
+        kf = [64 * int(v) for v in np.cumsum([0] + [
+            (n + 63) // 64 for n in kn])[:-1]]
+    width = heads * dim
+    made = [gpu.new_bf16(sum(qn) * width), gpu.new_bf16(sum(qn) * width),
+            gpu.kv_int8(max(f + n for f, n in zip(kf, kn)), kv, dim),
+            gpu.sdpa_packed_plan(qf, qn, kf, kn, heads, kv, dim)]
+    y, q, cache, plan = made
+    gpu.begin(); fake.fake_clear()
+    assert gpu.L.h3_hip_sdpa_packed_int8_bf16(gpu.h, y, q, 0, width, cache,
+                                              plan, 0.125), gpu.error()
+    gpu.submit()
+    out.append([l[0] for l in launches()])
+    for t in made:
+        gpu.free(t)
+"""
+
+
+def of_attention(names):
+    at = {"codes": "hk_packed_codes", "joined": "hk_packed_joined",
+          "few": "hk_kv8_few", "simple": "hk_kv8_simple"}
+    full = [n.replace(n.split("<")[0], at[n.split("<")[0]]) for n in names]
+    return ["hk_kv8_unpack"] * names[0].startswith("codes") + full
+
+
+def test_attention_of_many_rows():
+    made = on_fake(ATTEND, cases=[list(c[:-1]) for c in MANY])
+    for case, found in zip(MANY, made):
+        assert found == of_attention(case[-1]), case
+    assert {k for c in MANY for k in c[-1]} == {
+        "simple", "joined<64>", "joined<128>",
+        *(f"few<{d}>" for d in (32, 64, 96, 128)),
+        *(f"codes<{d}>" for d in (64, 96, 128))}
+
+
+@pytest.mark.parametrize("dim,padded", [(64, 64), (80, 96), (96, 96),
+                                        (128, 128)])
+def test_attention_of_the_other_cases_of_many_rows(dim, padded):
+    few, codes = f"few<{padded}>", f"codes<{padded}>"
+    cases = [([FEW], [70], [few]), ([FEW], [100], [few]),
+             ([FEW, 1], [100, 128], [few]), ([FEW] * 20, [110] * 20, [few]),
+             ([ROWS], [70], [codes, few]), ([ROWS], [100], [codes, few]),
+             ([ROWS, 1], [100, 128], [codes, few]),
+             ([ROWS] * 3, [110] * 3, [codes, few])]
+    made = on_fake(ATTEND, cases=[[q, None, k, 2, 2, dim]
+                                  for q, k, _ in cases])
+    for case, found in zip(cases, made):
+        assert found == of_attention(case[-1]), case
+
+
+def test_attention_of_many_requests_and_long_ones():
+    for count in (63, 64, 65, 150):
+        made = on_fake(ATTEND, cases=[
+            [[33 + i % 3 for i in range(count)], None,
+             [1 + 37 * i % 128 for i in range(count)], 5, 5, 64],
+            [[40] * count, [64 * (i % 7) for i in range(count)],
+             [1 + 23 * i % 250 for i in range(count)], 5, 5, 64]])
+        assert all(m == of_attention(["codes<64>"]) for m in made), count
+    made, = on_fake(ATTEND, cases=[[[4096], None, [1475], 8, 8, 64]])
+    assert made == of_attention(["codes<64>"])

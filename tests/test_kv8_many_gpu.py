@@ -1,6 +1,7 @@
-"""Attention over the 8-bit cache by items of more than 32 rows and of fewer,
-where scores and factors lie far from zero or one, against the same in 64 bits
-at the bounds of int8_oracle."""
+"""Attention over the 8-bit cache by items of more than 32 rows and of fewer
+(MANY, FEW and ROWS; test_int8_routes.py holds them to their kernels), also where
+scores and factors lie far from zero or one, against the same in 64 bits at the
+bounds of int8_oracle."""
 import numpy as np
 import pytest
 
@@ -11,6 +12,74 @@ from test_kv8_gpu import Case, Kv
 pytestmark = pytest.mark.gpu
 
 FEW, ROWS = 20, 129  # query rows of items of each kind, with up to 128 keys
+
+# query rows, first key rows (None: side by side) and key rows of each request,
+# heads, key heads, head size: the kernels between unpacking and join
+MANY = [
+    *(([129, 1, 40], None, [70, 128, 33], 4, 2, dim, kernels)
+      for dim, kernels in (
+        (8, ["codes<64>", "few<32>"]), (40, ["codes<64>", "few<64>"]),
+        (64, ["codes<64>", "few<64>"]), (72, ["codes<96>", "few<96>"]),
+        (80, ["codes<96>", "few<96>"]), (96, ["codes<96>", "few<96>"]),
+        (104, ["codes<128>", "few<128>"]),
+        (128, ["codes<128>", "few<128>"]))),
+    *(([170], None, [n], 2, 2, dim, [f"codes<{dim}>"])
+      for n in (1, 31, 32, 33, 63, 64, 65, 127, 128) for dim in (64, 128)),
+    ([1, 200, 8, 129, 40], [0, 0, 320, 448, 320], [100, 100, 65, 128, 64], 4,
+     2, 128, ["codes<128>", "few<128>"]),
+    ([2000, 1, 300, 20], [0, 0, 704, 704], [700, 500, 200, 64], 10, 10, 80,
+     ["codes<96>", "few<96>"]),
+    ([2048, 1], [0, 0], [300, 300], 16, 2, 128, ["codes<128>", "few<128>"]),
+    ([4096], None, [700], 8, 8, 96, ["codes<96>"]),
+    # in pieces
+    ([128], None, [9720], 8, 8, 128, ["codes<128>", "joined<128>"]),
+    ([256], None, [5000], 8, 2, 64, ["codes<64>", "joined<64>"]),
+    ([256], None, [5000], 8, 2, 96, ["codes<96>", "joined<128>"]),
+    ([300, 1], [0, 0], [5000, 4000], 8, 2, 128,
+     ["codes<128>", "few<128>", "joined<128>"]),
+    # what the matrix cores do not take
+    ([129, 1], None, [70, 128], 2, 2, 100, ["simple"]),
+    ([129, 1], None, [70, 128], 2, 2, 136, ["simple"]),
+]
+
+
+def many(gpu, qn, kf, kn, heads, kv_heads, dim, **more):
+    c = Case(gpu, qn, kn if not kf else [
+        max(f + n for f, n in zip(kf, kn))] * len(kn), heads, kv_heads, dim,
+        share=bool(kf), **more)
+    if kf:
+        c.kf, c.kn = kf, kn
+    return c
+
+
+@pytest.mark.parametrize("case", MANY, ids=lambda c: str(c[:6]))
+def test_many(gpu, case):
+    many(gpu, *case[:-1], pad=8, gap=2).check()
+
+
+@pytest.mark.parametrize("std", [30.0, 1e4, 1e-4])
+@pytest.mark.parametrize("rows", [FEW, ROWS])
+def test_scores_large_and_small(gpu, rows, std):
+    """One key has all the weight, or all have the same."""
+    for dim in (64, 96, 128):
+        Case(gpu, [rows, 1], [100, 128], 2, 2, dim, std=std).check()
+
+
+@pytest.mark.parametrize("powers", [[0, 9], [-9, 0], [0, 40], [-60, -70],
+                                    [30, -30]])
+def test_keys_of_unlike_scales(gpu, powers):
+    """Of the first block and the second."""
+    for rows in (FEW, ROWS):
+        c = Case(gpu, [rows], [100], 2, 2, 128)
+
+        def change(kv):
+            v = ro.wide(kv, *kv.shape)
+            for block, power in enumerate(powers):
+                v[64 * block:64 * block + 64, :256] *= 2.0 ** power
+            kv[:] = io.bits(v.astype(np.float32)).reshape(kv.shape)
+        c.kv.store([0], [100], change=change)
+        c.scale *= 2.0 ** -max(powers)
+        c.check()
 
 
 def numbers(c):
