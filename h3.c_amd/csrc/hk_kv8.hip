@@ -445,12 +445,14 @@ __device__ void hk_kv8_simple_row(const hk_kv8_args &g, uint32_t nth,
             (size_t)((r.kv_first + j0) / HK_KV8_BLOCK) * c.heads + kv_head;
         const uint8_t *codes = c.codes + at * 2u * HK_KV8_BLOCK * c.padded;
         const float2 scale = c.scales[at];
+        const float unit = hk_packed_code_unit(scale.x);
         float s = -INFINITY;
         if (lane < left) {
             s = 0.0f;
             for (uint32_t d = 0; d < a.dim; d++)
-                s = fmaf(hk_bf2f(q[d]), hk_kv8_key(c, codes, lane, d), s);
-            s *= scale.x;
+                s = fmaf(hk_bf2f(q[d]),
+                         unit * hk_kv8_key(c, codes, lane, d), s);
+            s *= hk_packed_code_scale(scale.x);
         }
         const float most = fmaxf(top, hk_wave_max(s));
         /* every score so far -inf: no weights yet */

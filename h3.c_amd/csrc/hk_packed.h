@@ -59,13 +59,18 @@ struct hk_packed_span {
     uint32_t block, at, blocks;
 };
 
-/* What the codes of a block's keys are multiplied by among those rows: over 128
- * dims a raw score, the query's product with the codes, would be up to 2^14
- * times the query's largest element, past F32's range where the score, of keys
- * of a scale under 1, is not.  A block of zeros (a scale of 0) has zeros,
- * whatever its codes. */
+/* What the codes of a block's keys are multiplied by before the products, and
+ * the products after them: over 256 dims a raw score, the query's product with
+ * the codes, would be up to 2^15 times the query's largest element, past F32's
+ * range where the score, of keys of a scale under 1, is not.  A block of zeros (a
+ * scale of 0) has zeros, whatever its codes, and what multiplies them leaves the
+ * -inf of keys past the end. */
 __device__ __forceinline__ float hk_packed_code_unit(float scale) {
-    return scale == 0.0f ? 0.0f : scale < 1.0f ? 0x1p-14f : 1.0f;
+    return scale == 0.0f ? 0.0f : scale < 1.0f ? 0x1p-15f : 1.0f;
+}
+
+__device__ __forceinline__ float hk_packed_code_scale(float scale) {
+    return scale == 0.0f ? 1.0f : scale < 1.0f ? scale * 0x1p15f : scale;
 }
 
 struct hk_packed_args {

@@ -629,11 +629,7 @@ __device__ __forceinline__ void hk_packed_item_of(const hk_packed_args &a) {
             ahead = block_scales[2u * (size_t)(tile + 1u) * a.kv_heads];
         if (more) issue_tile(tile + 1u, stage ^ 1u);
         if (live) {
-        /* what multiplies a raw score: of a block of zeros they are 0, whatever
-         * does, and -inf, of keys past the end, has to stay it */
-        const float by = scale == 0.0f   ? 1.0f
-                         : scale < 1.0f ? scale * 0x1p14f
-                                        : scale;
+        const float by = hk_packed_code_scale(scale);
         float L = a.scale_log2;
         if (SCALED) {
             L *= by;

@@ -7,6 +7,7 @@ import pytest
 
 import int8_oracle as io
 import requests_oracle as ro
+from test_int8_gpu import plain  # noqa: F401 (a fixture)
 from test_kv8_gpu import Case, Kv
 
 pytestmark = pytest.mark.gpu
@@ -111,12 +112,15 @@ def test_far_scores_and_a_last_block_of_zeros(gpu, rows, dim, stored):
     c.check()
 
 
-@pytest.mark.parametrize("rows", [FEW, ROWS])
-@pytest.mark.parametrize("dim", [64, 80, 128])
-@pytest.mark.parametrize("size,std,scale", [
+FACTORS = [
     (5e37, 1e-34, 1e-5), (1e36, 1e-33, 4.6e-5), (1e34, 1e-31, 4.6e-5),
     (1e30, 1e-32, 1e-1), (1e-30, 1e30, 0.2), (1e-35, 1e30, 1e4),
-    (1e-30, 1.0, 1e29), (1e-3, 1e-33, 1e35)])
+    (1e-30, 1.0, 1e29), (1e-3, 1e-33, 1e35)]
+
+
+@pytest.mark.parametrize("rows", [FEW, ROWS])
+@pytest.mark.parametrize("dim", [64, 80, 128])
+@pytest.mark.parametrize("size,std,scale", FACTORS)
 def test_scores_of_large_and_small_factors(gpu, rows, dim, size, std, scale):
     """Queries, keys and the scale near the ends of F32's range, scores of
     ordinary size."""
@@ -124,6 +128,13 @@ def test_scores_of_large_and_small_factors(gpu, rows, dim, size, std, scale):
     put(c, numbers(c) * size)
     c.scale = float(np.float32(scale))
     c.check()
+
+
+@pytest.mark.parametrize("dim", [64, 136, 256])
+@pytest.mark.parametrize("size,std,scale", FACTORS)
+def test_factors_in_the_simple_kernel(plain, dim, size, std,  # noqa: F811
+                                      scale):
+    test_scores_of_large_and_small_factors(plain, FEW, dim, size, std, scale)
 
 
 @pytest.mark.parametrize("rows", [FEW, ROWS])
