@@ -484,6 +484,8 @@ class Gpu:
                       key_offset, value, value_offset, kv_stride):
         """h3_hip_kv_int8_store of lists of row numbers, in an open batch."""
         n = len(rows)
+        if not n == len(cache_first) == len(source_first):
+            raise ValueError("a first row of each, for each number of rows")
         self.check(self.L.h3_hip_kv_int8_store(
             self.h, cache, *((_U32 * n)(*v) for v in (
                 cache_first, source_first, rows)),
