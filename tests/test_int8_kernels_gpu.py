@@ -84,12 +84,16 @@ def test_gated_block(gpu, m, k, h):
     rng = np.random.default_rng((m, k, h))
     x, w1 = rand_bf16(rng, m * k), rand_bf16(rng, 2 * h * k, 1.5 * k ** -0.5)
     w2 = rand_bf16(rng, OUT * h, h ** -0.5)
-    y = gpu.bf16(np.full(m * OUT + 512, MARK, np.uint16))
-    gpu.run("h3_hip_mlp_int8_bf16", y, quantize(gpu, x, m, k),
-            quantize(gpu, w1, 2 * h, k), quantize(gpu, w2, OUT, h), m, k, h,
-            OUT)
-    got = gpu.read_bf16(y)
+    sides = [quantize(gpu, x, m, k), quantize(gpu, w1, 2 * h, k),
+             quantize(gpu, w2, OUT, h)]
+
+    def run():
+        y = gpu.bf16(np.full(m * OUT + 512, MARK, np.uint16))
+        gpu.run("h3_hip_mlp_int8_bf16", y, *sides, m, k, h, OUT)
+        return gpu.read_bf16(y)
+    got = run()
     assert (got[m * OUT:] == MARK).all(), "wrote behind the last row"
+    assert np.array_equal(got, run()), "other bits the second time"
     want, bound = io.mlp(io.rows_of(ro.wide(x, m, k)),
                          io.rows_of(ro.wide(w1, 2 * h, k)),
                          io.rows_of(ro.wide(w2, OUT, h)))

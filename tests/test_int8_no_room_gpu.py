@@ -1,6 +1,6 @@
 """The 8-bit products and gated block at shapes that are cut along K, where the
-pieces' sums find no room (small_memory.cpp): the same bits, uncut.
-test_int8_routes.py holds each to its kernel."""
+pieces' sums find no room (small_memory.cpp): the same bits, uncut; and the
+attention of many rows. test_int8_routes.py holds each to its kernel."""
 import shutil
 
 import pytest
@@ -70,4 +70,36 @@ got = bare.read_bf16(y)
 assert np.array_equal(got, gpu.read_bf16(z))
 want, bound = t.io.mlp(*(t.io.rows_of(ro.wide(b, r, c)) for b, r, c in sides))
 ro.check(got.reshape(m, n), want, t.io.rounded(want, bound))
+""")
+
+
+def test_attention_of_many_rows():
+    """Items that the plan cuts run whole, in a context that has room for the
+    unpacked keys and values alone."""
+    run("""
+import test_kv8_gpu as t
+limit(0)
+bare = h3hip.Gpu()
+limit()
+a = t.Case(bare, [16384], [9720], 8, 8, 128)  # whole items
+b = t.Case(bare, [128], [9720], 8, 8, 128)
+def plan(c):
+    return bare.sdpa_packed_plan(c.qf, c.qn, c.kf, c.kn, 8, 8, 128)
+q = [bare.bf16(c.q) for c in (a, b)]
+y = [bare.new_bf16(c.rows * 1024) for c in (a, b)]
+plans = [plan(c) for c in (a, b)]
+got = []
+for i, size in ((0, -1), (1, 0), (1, -1)):
+    limit(size)
+    bare.run("h3_hip_sdpa_packed_int8_bf16", y[i], q[i], 0, 1024, (a, b)[i].kv.t,
+             plans[i], b.scale)
+    limit()
+    got.append(bare.read_bf16(y[i]))
+want, bound, _ = t.io.attention(ro.wide(b.q, 128, 8, 128), b.kv.wide,
+                                [(0, 128, 0, 9720)], 8, 8, 128,
+                                float(np.float32(b.scale)))
+for g in got[1:]:
+    ro.check(g.reshape(want.shape), want, bound)
+# another order of sums
+assert not np.array_equal(got[1], got[2])
 """)

@@ -173,3 +173,12 @@ def test_attention_of_many_requests_and_long_ones():
         assert all(m == of_attention(["codes<64>"]) for m in made), count
     made, = on_fake(ATTEND, cases=[[[4096], None, [1475], 8, 8, 64]])
     assert made == of_attention(["codes<64>"])
+
+
+def test_attention_without_scratch():
+    """As test_int8_no_room_gpu.py has it: room from a call of whole items."""
+    cases = [[[16384], None, [9720], 8, 8, 128], [[128], None, [9720], 8, 8, 128]]
+    text = ATTEND.replace("gpu.begin();", "gpu.begin(); fake.fake_largest_block("
+                          "C.c_size_t(0 if qn == [128] else 2 ** 64 - 1));")
+    assert on_fake(BARE + text, cases=cases) == [
+        of_attention(["codes<128>"])] * 2
