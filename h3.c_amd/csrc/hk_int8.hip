@@ -394,9 +394,11 @@ struct hk_int8_ext {
 };
 
 /* The tiles: the bf16 GEMM's loop over bytes, 2.2 to 2.4 PFLOP/s where 16x16x64
- * MFMAs reach 4.4 from registers (2378 x 5376 -> 21504 235 us, 6144 x 5120 ->
- * 13824 380).  Bound by the package's power, which takes the clock to about 2
- * GHz, and by a tile's start and end, 7 us of 58, in which all CUs write. */
+ * MFMAs reach 4.3 from registers (2378 x 5376 -> 21504 241 us, 6144 x 5120 ->
+ * 13824 375).  At the package's power: 1400 W and a clock of 1.9 to 2.1 GHz, 0.64
+ * pJ an operation for the MFMA's own 0.31.  MFMAs are busy 56% of the cycles: a
+ * tile's start and end take 7 us of 58, in which all CUs write, and the loop's
+ * LDS reads and loads issue between them. */
 #define HK_TRACE(p) ((void)0)
 #define HK_TRACE_CLOCK(p) ((void)0)
 #define HK_TRACE_VALUE(p, v) ((void)0)

@@ -390,7 +390,8 @@ int h3_hip_dequantize_int8(h3_gpu *gpu, h3_gpu_tensor *output,
 /* y = bf16(act(sum * (input scale * weight scale) + bias)) of 8-bit matrices,
  * [rows][input_dim] and [output_dim][input_dim]; the sums of products are
  * exact.  act is nothing or, of the F32 value, the tanh GELU.  bias (bf16) may
- * be NULL; output must be a tensor of its own. */
+ * be NULL; output must be a tensor of its own.  Weights whose codes take 4 GiB
+ * or more run without the matrix cores, a thread for each output. */
 int h3_hip_linear_int8_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
                             const h3_gpu_tensor *input,
                             const h3_gpu_tensor *weight,
@@ -448,11 +449,16 @@ int h3_hip_kv_int8_read(h3_gpu *gpu, h3_gpu_tensor *key, h3_gpu_tensor *value,
 /* h3_hip_sdpa_packed_bf16 over such a cache: the plan's key rows are rows of
  * the cache, and every request's have to begin at a multiple of 64 (requests
  * may share them).  Scores, softmax and sums are F32, of keys as the codes and
- * scales say.  P is rounded to 11 bits (f16) before P . V.  Blocks that the plan's
- * items of more than 32 query rows read are unpacked into the context's scratch,
- * which grows on demand, 4 bytes for each row, key head and dim of them; there
- * the values are rounded to 11 bits as well, those under 2^-29 of the largest of
- * the request and key head to fewer. */
+ * scales say; what a row comes to does not depend on the rows beside it.  P is
+ * rounded to 11 bits (f16) before P . V.  Blocks that the plan's items of more
+ * than 32 query rows read are unpacked into the context's scratch, which grows
+ * on demand, 4 bytes for each row, key head and dim of them; each range of blocks
+ * that requests read, by its first block and their number, is unpacked on its
+ * own, also where it shares blocks with another.  There the values are rounded to
+ * 11 bits as well, those under 2^-29 of the largest of the range and key head to
+ * fewer.  Heads over 128, and, where the plan has items of more than 32 rows,
+ * heads that are no multiple of 8, take a simple kernel, a wave for each query
+ * row. */
 int h3_hip_sdpa_packed_int8_bf16(h3_gpu *gpu, h3_gpu_tensor *output,
                                  const h3_gpu_tensor *query,
                                  size_t query_offset, uint32_t query_stride,
